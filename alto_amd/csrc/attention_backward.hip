@@ -1,0 +1,248 @@
+// Gradients of the MXFP4 attention with respect to Q, K and V (gfx950).
+//
+// With S_ij = sm_scale Q_i . K_j + bias_ij - slope |i + Sk - Sq - j| on the values that the codes stand for, and the forward's log-sum-exp:
+//   P_ij = exp(S_ij - lse_i)   (0 where the mask hides j, and in a row that sees no key),   D_i = dO_i . O_i,
+//   dV_j = sum_i P_ij dO_i,   dS_ij = P_ij (dO_i . V_j - D_i),   dQ_i = sm_scale sum_j dS_ij K_j,   dK_j = sm_scale sum_i dS_ij Q_i.
+// The roundings of Q, K, V and P to FP4 are passed straight through.  The scores are recomputed on the FP4 pipe from the forward's codes;
+// the other products have a factor that is not on the FP4 grid (P, dS, dO) and run in bf16, in which the codes' values are exact.  P and
+// dS are rounded to bf16 as factors (half a step, 2^-9 of a value at most, independent from element to element: the sums have the relative
+// error of one rounding of their result); scores, probabilities, dS before that, D and all sums are fp32.
+//
+// Three launches: this file's preparation (D and lse in the order of the tiles, the codes' values as bf16 rows), then dK and dV by blocks
+// of keys and dQ by blocks of rows.  dK and dV need a sum over rows and dQ one over keys: each has a kernel of its own that recomputes P,
+// so every gradient is summed by one wave in a fixed order and the results do not change from run to run (no atomics).
+#include <algorithm>
+#include <memory>
+#include <new>
+
+#include "attention_backward.h"
+
+namespace alto {
+namespace {
+
+struct PrepareArgs {
+  const uint8_t *q, *qs, *k, *ks, *vt, *vs;
+  const __bf16 *dout, *out;
+  const float* lse;
+  int64_t do_sb, do_sh, do_ss, o_sb, o_sh, o_ss, l_sb, l_sh, l_ss;
+  int Hq, Hk, Sq, Sk, D, Dv;
+  int64_t q_tiles;   // B Hq Sq / 32
+  float* stats;
+  uint8_t *q_scales, *k_scales;
+  __bf16 *q_rows, *k_rows, *v_rows;
+};
+
+__device__ __forceinline__ float e8m0_value(uint32_t e) { return u2f(e ? e << 23 : 0x00400000u); }
+
+// eight codes of one dword as bf16
+__device__ __forceinline__ v4i_t decode8(uint32_t codes, float scale) {
+  return v4i_t{__builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 0)), __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 1)),
+               __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 2)), __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 3))};
+}
+
+// 32 rows of Q or K: values, and the scale bytes 8 apart
+__device__ __forceinline__ void decode_rows(const uint8_t* codes, const uint8_t* scales, int64_t tile, int D, __bf16* rows, uint8_t* padded) {
+  const int tid = threadIdx.x, bands = D / 32;
+  const uint8_t* s = scales + tile * bands;
+  if (tid < 8) padded[tile * 8 + tid] = tid < bands ? s[tid] : 127;
+  const uint32_t* from = reinterpret_cast<const uint32_t*>(codes + tile * 16 * D);
+  v4i_t* to = reinterpret_cast<v4i_t*>(rows + tile * 32 * D);
+  for (int i = tid; i < 4 * D; i += 256) to[i] = decode8(from[i], e8m0_value(s[(i % (D / 8)) >> 2]));
+}
+
+// One workgroup: 32 rows of Q with their statistics, or 32 keys of K and V.
+__global__ __launch_bounds__(256) void attn_bwd_prepare_kernel(const PrepareArgs a) {
+  __shared__ __align__(16) uint32_t turned[4][32 * 20];   // one 32 x 32 block of V a wave, rows of 64 bytes 80 apart
+  const int tid = threadIdx.x;
+  int64_t tile = blockIdx.x;
+  if (tile < a.q_tiles) {
+    decode_rows(a.q, a.qs, tile, a.D, a.q_rows, a.q_scales);
+    const int64_t row = tile * 32 + (tid >> 3), bh = row / a.Sq;
+    const int64_t b = bh / a.Hq, h = bh % a.Hq, i = row % a.Sq;
+    const __bf16* go = a.dout + b * a.do_sb + h * a.do_sh + i * a.do_ss + 8 * (tid & 7);
+    const __bf16* o = a.out + b * a.o_sb + h * a.o_sh + i * a.o_ss + 8 * (tid & 7);
+    float d = 0.0f;
+    for (int c = 0; c < a.Dv; c += 64) {
+      const v4i_t x = *reinterpret_cast<const v4i_t*>(go + c), y = *reinterpret_cast<const v4i_t*>(o + c);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        d = __builtin_fmaf(bf16_lo((uint32_t)x[e]), bf16_lo((uint32_t)y[e]), d);
+        d = __builtin_fmaf(bf16_hi((uint32_t)x[e]), bf16_hi((uint32_t)y[e]), d);
+      }
+    }
+#pragma unroll
+    for (int m = 1; m < 8; m <<= 1) d += __shfl_xor(d, m, 64);
+    if ((tid & 7) == 0) {
+      const float l = a.lse[b * a.l_sb + h * a.l_sh + i * a.l_ss];
+      const bool none = l == -__builtin_inff();   // a row that sees no key: its probabilities are zeros, whatever the forward left in O
+      a.stats[tile * 64 + (tid >> 3)] = none ? __builtin_inff() : l * ATTN_RCP_LN2;
+      a.stats[tile * 64 + 32 + (tid >> 3)] = none ? 0.0f : -d;
+    }
+    return;
+  }
+  tile -= a.q_tiles;
+  decode_rows(a.k, a.ks, tile, a.D, a.k_rows, a.k_scales);
+  const int lane = tid & 63, wave = tid >> 6, bands = a.Sk / 32;
+  if (wave * 32 >= a.Dv) return;
+  const int64_t bh = tile / bands, band = tile % bands;
+  const uint8_t* column = a.vt + (bh * a.Dv + wave * 32 + (lane & 31)) * (int64_t)(a.Sk / 2) + band * 16 + 8 * (lane >> 5);
+  const uint2 w = *reinterpret_cast<const uint2*>(column);   // 16 keys of one column
+  const float scale = e8m0_value(a.vs[tile * (a.Dv / 32) + wave]);
+  uint16_t* block = reinterpret_cast<uint16_t*>(turned[wave]);
+  const v4i_t lo = decode8(w.x, scale), hi = decode8(w.y, scale);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const uint32_t v = (uint32_t)(e < 4 ? lo[e & 3] : hi[e & 3]);
+    const int key = 16 * (lane >> 5) + 2 * e;
+    block[key * 40 + (lane & 31)] = (uint16_t)v;
+    block[(key + 1) * 40 + (lane & 31)] = (uint16_t)(v >> 16);
+  }
+  wave_lds_order();
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int key = 16 * i + (lane >> 2);
+    const v4i_t v = *reinterpret_cast<const v4i_t*>(turned[wave] + key * 20 + 4 * (lane & 3));
+    *reinterpret_cast<v4i_t*>(a.v_rows + (tile * 32 + key) * a.Dv + wave * 32 + 8 * (lane & 3)) = v;
+  }
+}
+
+struct Workspace {
+  int64_t stats, q_scales, k_scales, q_rows, k_rows, v_rows, total;
+};
+Workspace workspace(int64_t B, int64_t Hq, int64_t Hk, int64_t Sq, int64_t Sk, int64_t D, int64_t Dv) {
+  Workspace w{};
+  int64_t at = 0;
+  auto take = [&](int64_t& p, int64_t n) { p = at; at += (n + 255) / 256 * 256; };
+  take(w.stats, B * Hq * Sq * 8);
+  take(w.q_scales, B * Hq * (Sq / 32) * 8);
+  take(w.k_scales, B * Hk * (Sk / 32) * 8);
+  take(w.q_rows, B * Hq * Sq * D * 2);
+  take(w.k_rows, B * Hk * Sk * D * 2);
+  take(w.v_rows, B * Hk * Sk * Dv * 2);
+  w.total = at;
+  return w;
+}
+
+int check_sizes(const alto_mxfp4_attention_bwd_t& p) {
+  const long long B = p.B, Hq = p.Hq, Hk = p.Hk, Sq = p.Sq, Sk = p.Sk, D = p.D, Dv = p.Dv;
+  ALTO_REQUIRE(B > 0 && Hq > 0 && Hk > 0 && Hq % Hk == 0, "attention_bwd: Hq=%lld must be a positive multiple of Hk=%lld", Hq, Hk);
+  ALTO_REQUIRE(Sq > 0 && Sq % 32 == 0 && Sk > 0 && Sk % 32 == 0, "attention_bwd: Sq=%lld and Sk=%lld must be positive multiples of 32", Sq, Sk);
+  ALTO_REQUIRE(D == 64 || D == 128 || D == 192 || D == 256, "attention_bwd: head dim D=%lld must be 64, 128, 192 or 256", D);
+  ALTO_REQUIRE(Dv == 64 || Dv == 128, "attention_bwd: value dim Dv=%lld must be 64 or 128", Dv);
+  ALTO_REQUIRE(B <= 65535 && Hq < (1ll << 31) && Sq <= 65535ll * 128 && Sk <= 65535ll * 128, "attention_bwd: B, Sq / 128 and Sk / 128 must fit a grid dimension");
+  ALTO_REQUIRE(product_below(1ll << 40, B * Sq, Hq, D > Dv ? D : Dv) && product_below(1ll << 40, B * Sk, Hk, D > Dv ? D : Dv), "attention_bwd: tensor too large");
+  ALTO_REQUIRE(product_below(1ll << 31, B, Hq, Sq / 32 + Sk / 32 + 1), "attention_bwd: tensor too large");
+  return ALTO_MXFP4_OK;
+}
+
+}  // namespace
+
+static int attention_bwd(const alto_mxfp4_attention_bwd_t& p, hipStream_t st) {
+  if (const int rc = check_sizes(p)) return rc;
+  ALTO_REQUIRE(p.q_codes && p.q_scales && p.k_codes && p.k_scales && p.vt_codes && p.v_scales && p.dout && p.out && p.lse && p.workspace && (p.dk || p.dq),
+               "attention_bwd: null pointer");
+  ALTO_REQUIRE(!p.dk == !p.dv, "attention_bwd: dk and dv are written together");
+  ALTO_REQUIRE(p.Sk_used > 0 && p.Sk_used <= p.Sk && p.Sk_used % 32 == 0, "attention_bwd: Sk_used=%lld must be a multiple of 32 in (0, Sk]", (long long)p.Sk_used);
+  ALTO_REQUIRE(((uintptr_t)p.q_codes | (uintptr_t)p.k_codes | (uintptr_t)p.dout | (uintptr_t)p.out) % 16 == 0 && (uintptr_t)p.vt_codes % 8 == 0,
+               "attention_bwd: Q and K codes, dout and out must be 16-byte aligned, V codes 8-byte aligned");
+  ALTO_REQUIRE(((uintptr_t)p.dq | (uintptr_t)p.dk | (uintptr_t)p.dv) % 8 == 0 && ((uintptr_t)p.lse | (uintptr_t)p.bias | (uintptr_t)p.alibi_slopes) % 4 == 0,
+               "attention_bwd: gradients must be 8-byte aligned, lse, bias and slopes 4-byte aligned");
+  for (const int64_t s : {p.dout_sb, p.dout_sh, p.dout_ss, p.out_sb, p.out_sh, p.out_ss})
+    ALTO_REQUIRE(s >= 0 && s < (1ll << 40) && s % 8 == 0, "attention_bwd: strides of dout and out must be non-negative multiples of 8 elements");
+  for (const int64_t s : {p.dq_sb, p.dq_sh, p.dq_ss, p.dk_sb, p.dk_sh, p.dk_ss, p.dv_sb, p.dv_sh, p.dv_ss})
+    ALTO_REQUIRE(s >= 0 && s < (1ll << 40) && s % 4 == 0, "attention_bwd: strides of the gradients must be non-negative multiples of 4 elements");
+  for (const int64_t s : {p.lse_sb, p.lse_sh, p.lse_ss, p.bias_sb, p.bias_sh, p.bias_sm, p.alibi_sb, p.alibi_sh})
+    ALTO_REQUIRE(s >= 0 && s < (1ll << 40), "attention_bwd: strides must be non-negative");
+  ALTO_REQUIRE(p.dout_ss < (1ll << 24), "attention_bwd: rows of dout are too far apart");
+  ALTO_REQUIRE(p.n_seqs >= 0, "attention_bwd: negative number of sequences");
+  ALTO_REQUIRE(p.causal == 0 || p.n_seqs > 0 || p.Sq <= p.Sk_used, "attention_bwd: causal attention needs Sq <= Sk (got %lld > %lld)", (long long)p.Sq, (long long)p.Sk_used);
+  if (p.n_seqs > 0) {
+    ALTO_REQUIRE(p.cu_q && p.cu_k && p.B == 1 && p.Sk_used == p.Sk && !p.bias, "attention_bwd: packed sequences need their boundaries, B = 1, all keys used and no bias");
+    ALTO_REQUIRE(p.cu_q[0] == 0 && p.cu_k[0] == 0 && p.cu_q[p.n_seqs] == p.Sq && p.cu_k[p.n_seqs] == p.Sk,
+                 "attention_bwd: the sequence boundaries must run from 0 to the token counts");
+    for (int i = 0; i < p.n_seqs; ++i) {
+      ALTO_REQUIRE(p.cu_q[i + 1] > p.cu_q[i] && p.cu_k[i + 1] > p.cu_k[i] && p.cu_q[i + 1] % 32 == 0 && p.cu_k[i + 1] % 32 == 0,
+                   "attention_bwd: sequence boundaries must be increasing multiples of 32 tokens");
+      ALTO_REQUIRE(!p.causal || p.cu_q[i + 1] - p.cu_q[i] <= p.cu_k[i + 1] - p.cu_k[i], "attention_bwd: causal attention needs Sq <= Sk (got %d > %d)",
+                   p.cu_q[i + 1] - p.cu_q[i], p.cu_k[i + 1] - p.cu_k[i]);
+    }
+  }
+  const Workspace w = workspace(p.B, p.Hq, p.Hk, p.Sq, p.Sk, p.D, p.Dv);
+  ALTO_REQUIRE(p.workspace_bytes >= w.total && (uintptr_t)p.workspace % 256 == 0, "attention_bwd: the workspace must be 256-byte aligned and hold %lld bytes", (long long)w.total);
+  std::unique_ptr<int[]> order;
+  if (p.n_seqs > 0) {
+    order.reset(new (std::nothrow) int[(size_t)p.n_seqs]);   // (no exception may leave a C entry)
+    if (!order) {
+      set_error("attention_bwd: no host memory for the order of %d sequences", p.n_seqs);
+      return ALTO_MXFP4_ELAUNCH;
+    }
+  }
+  uint8_t* ws = (uint8_t*)p.workspace;
+  PrepareArgs r{};
+  r.q = (const uint8_t*)p.q_codes; r.qs = (const uint8_t*)p.q_scales; r.k = (const uint8_t*)p.k_codes; r.ks = (const uint8_t*)p.k_scales;
+  r.vt = (const uint8_t*)p.vt_codes; r.vs = (const uint8_t*)p.v_scales;
+  r.dout = (const __bf16*)p.dout; r.out = (const __bf16*)p.out; r.lse = p.lse;
+  r.do_sb = p.dout_sb; r.do_sh = p.dout_sh; r.do_ss = p.dout_ss; r.o_sb = p.out_sb; r.o_sh = p.out_sh; r.o_ss = p.out_ss;
+  r.l_sb = p.lse_sb; r.l_sh = p.lse_sh; r.l_ss = p.lse_ss;
+  r.Hq = (int)p.Hq; r.Hk = (int)p.Hk; r.Sq = (int)p.Sq; r.Sk = (int)p.Sk; r.D = (int)p.D; r.Dv = (int)p.Dv;
+  r.q_tiles = p.B * p.Hq * (p.Sq / 32);
+  r.stats = (float*)(ws + w.stats); r.q_scales = ws + w.q_scales; r.k_scales = ws + w.k_scales;
+  r.q_rows = (__bf16*)(ws + w.q_rows); r.k_rows = (__bf16*)(ws + w.k_rows); r.v_rows = (__bf16*)(ws + w.v_rows);
+  hipLaunchKernelGGL(attn_bwd_prepare_kernel, dim3((unsigned)(r.q_tiles + p.B * p.Hk * (p.Sk / 32))), dim3(256), 0, st, r);
+  if (const int rc = check_launch("attention_bwd")) return rc;
+
+  AttnBwdArgs a{};
+  a.q = r.q; a.k = r.k; a.q_scales = r.q_scales; a.k_scales = r.k_scales; a.q_rows = r.q_rows; a.k_rows = r.k_rows; a.v_rows = r.v_rows; a.stats = r.stats;
+  a.dout = r.dout; a.do_sb = p.dout_sb; a.do_sh = p.dout_sh; a.do_ss = p.dout_ss;
+  a.dq = p.dq; a.dk = p.dk; a.dv = p.dv;
+  a.dq_sb = p.dq_sb; a.dq_sh = p.dq_sh; a.dq_ss = p.dq_ss; a.dk_sb = p.dk_sb; a.dk_sh = p.dk_sh; a.dk_ss = p.dk_ss; a.dv_sb = p.dv_sb; a.dv_sh = p.dv_sh; a.dv_ss = p.dv_ss;
+  a.B = (int)p.B; a.Hq = (int)p.Hq; a.Hk = (int)p.Hk; a.Sq = (int)p.Sq; a.Sk = (int)p.Sk; a.Sk_used = (int)p.Sk_used;
+  a.sm_scale = p.sm_scale; a.causal = p.causal ? 1 : 0;
+  a.bias = p.bias; a.bias_sb = p.bias_sb; a.bias_sh = p.bias_sh; a.bias_sm = p.bias_sm; a.alibi = p.alibi_slopes; a.alibi_sb = p.alibi_sb; a.alibi_sh = p.alibi_sh;
+  auto go = [&](const AttnBwdSeqs& s, int q_blocks, int k_blocks) {
+    switch (p.D) {
+      case 64: return launch_attn_bwd<1>(a, s, p.Dv, q_blocks, k_blocks, st);
+      case 128: return launch_attn_bwd<2>(a, s, p.Dv, q_blocks, k_blocks, st);
+      case 192: return launch_attn_bwd<3>(a, s, p.Dv, q_blocks, k_blocks, st);
+      default: return launch_attn_bwd<4>(a, s, p.Dv, q_blocks, k_blocks, st);
+    }
+  };
+  AttnBwdSeqs s;
+  s.n = 0;
+  s.zq[0] = s.zk[0] = 0;
+  if (p.n_seqs == 0) return go(s, (int)((p.Sq + 127) / 128), (int)((p.Sk + 127) / 128));
+  for (int i = 0; i < p.n_seqs; ++i) order[(size_t)i] = i;
+  std::sort(order.get(), order.get() + p.n_seqs, [&](int x, int y) {   // longest first
+    const int kx = p.cu_k[x + 1] - p.cu_k[x], ky = p.cu_k[y + 1] - p.cu_k[y];
+    return kx != ky ? kx > ky : x < y;
+  });
+  for (int at = 0; at < p.n_seqs;) {
+    s.n = 0;
+    for (; at < p.n_seqs && s.n < ATTN_MAX_SEQS; ++at) {
+      const int i = order[(size_t)at], n = s.n, qn = p.cu_q[i + 1] - p.cu_q[i], kn = p.cu_k[i + 1] - p.cu_k[i];
+      if (s.zq[n] + (qn + 127) / 128 > 65535 || s.zk[n] + (kn + 127) / 128 > 65535) break;
+      s.q0[n] = p.cu_q[i]; s.qn[n] = qn; s.k0[n] = p.cu_k[i]; s.kn[n] = kn;
+      s.zq[n + 1] = s.zq[n] + (qn + 127) / 128;
+      s.zk[n + 1] = s.zk[n] + (kn + 127) / 128;
+      ++s.n;
+    }
+    if (const int rc = go(s, s.zq[s.n], s.zk[s.n])) return rc;
+  }
+  return ALTO_MXFP4_OK;
+}
+
+}  // namespace alto
+
+extern "C" int64_t alto_mxfp4_attention_bwd_workspace_bytes(const alto_mxfp4_attention_bwd_t* p) {
+  if (!p) {
+    alto::set_error("attention_bwd_workspace_bytes: null pointer");
+    return ALTO_MXFP4_EINVAL;
+  }
+  if (const int rc = alto::check_sizes(*p)) return rc;
+  return alto::workspace(p->B, p->Hq, p->Hk, p->Sq, p->Sk, p->D, p->Dv).total;
+}
+
+extern "C" int alto_mxfp4_attention_bwd(const alto_mxfp4_attention_bwd_t* p, void* stream) {
+  ALTO_REQUIRE(p, "attention_bwd: null pointer");
+  return alto::attention_bwd(*p, (hipStream_t)stream);
+}

@@ -4,7 +4,8 @@
 ``alto/kernels/dispatch/attention.py:22`` can point at it; here it quantises K and V with one launch (2D blocks along the
 head dim, :1105-1107; V packed along the keys), read in the layout they come in, and runs one HIP kernel, which quantises
 a bf16 Q itself (an fp32 one goes through that launch as well).
-Like the reference (:1143-1145) it has no backward.  Options outside the path ALTO's dispatch layer uses
+The reference has no backward (:1143-1145); here Q, K and V that require a gradient get one: ``attention_mxfp4_backward`` recomputes the
+probabilities from the quantized operands, which is all that is kept of them (half a byte an element).  Options outside the path ALTO's dispatch layer uses
 (``alto/kernels/dispatch/attention.py:61-77``: layout "bhsd", no bias, no alibi, no dropout, fixed lengths) raise.
 """
 from __future__ import annotations
@@ -17,6 +18,28 @@ import torch
 from . import _runtime as rt
 from .._lib import check
 from .config import TrainingOpConfig
+
+
+def _additive(bias: Optional[torch.Tensor], alibi_slopes: Optional[torch.Tensor], B: int, Hq: int, Sq: int, Sk: int):
+    """``bias`` as fp32 [1 or B, 1 or Hq, Sq, Sk] with aligned rows, ``alibi_slopes`` as dense fp32 [1 or B, Hq]; None as None."""
+    b4 = sl = None
+    if bias is not None:
+        rt.require_gpu(bias)
+        b4 = bias.to(torch.float32)
+        while b4.dim() < 4:
+            b4 = b4.unsqueeze(0)
+        torch._check(b4.shape[-2] == Sq and b4.shape[-1] == Sk and b4.shape[0] in (1, B) and b4.shape[1] in (1, Hq),
+                     lambda: f"bias of shape {tuple(bias.shape)} does not broadcast to {(B, Hq, Sq, Sk)}")
+        if b4.stride(3) != 1 or b4.stride(2) % 4 or b4.data_ptr() % 16 or (b4.shape[0] > 1 and b4.stride(0) < 0) or (b4.shape[1] > 1 and b4.stride(1) < 0):
+            b4 = b4.contiguous()
+    if alibi_slopes is not None:
+        rt.require_gpu(alibi_slopes)
+        sl = alibi_slopes.to(torch.float32)
+        if sl.dim() == 1:
+            sl = sl.unsqueeze(0)
+        torch._check(sl.dim() == 2 and sl.shape[1] == Hq and sl.shape[0] in (1, B), lambda: f"alibi_slopes of shape {tuple(alibi_slopes.shape)}: [Hq] or [B, Hq]")
+        sl = sl.contiguous()
+    return b4, sl
 
 
 def attention_mxfp4_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_scale: torch.Tensor, k_scale: torch.Tensor,
@@ -43,23 +66,7 @@ def attention_mxfp4_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q
     out = torch.empty((B, Hq, Sq, Dv), dtype=torch.bfloat16, device=q.device)
     lse = torch.empty((B, Hq, Sq), dtype=torch.float32, device=q.device)
     sk_used = Sk if seqlen_k is None else int(seqlen_k)
-    b4 = sl = None
-    if bias is not None:
-        rt.require_gpu(bias)
-        b4 = bias.to(torch.float32)
-        while b4.dim() < 4:
-            b4 = b4.unsqueeze(0)
-        torch._check(b4.shape[-2] == Sq and b4.shape[-1] == sk_used and b4.shape[0] in (1, B) and b4.shape[1] in (1, Hq),
-                     lambda: f"bias of shape {tuple(bias.shape)} does not broadcast to {(B, Hq, Sq, sk_used)}")
-        if b4.stride(3) != 1 or b4.stride(2) % 4 or b4.data_ptr() % 16 or (b4.shape[0] > 1 and b4.stride(0) < 0) or (b4.shape[1] > 1 and b4.stride(1) < 0):
-            b4 = b4.contiguous()
-    if alibi_slopes is not None:
-        rt.require_gpu(alibi_slopes)
-        sl = alibi_slopes.to(torch.float32)
-        if sl.dim() == 1:
-            sl = sl.unsqueeze(0)
-        torch._check(sl.dim() == 2 and sl.shape[1] == Hq and sl.shape[0] in (1, B), lambda: f"alibi_slopes of shape {tuple(alibi_slopes.shape)}: [Hq] or [B, Hq]")
-        sl = sl.contiguous()
+    b4, sl = _additive(bias, alibi_slopes, B, Hq, Sq, sk_used)
     if b4 is None and sl is None:
         check(rt.lib().alto_mxfp4_attention_fwd(q.data_ptr(), q_scale.data_ptr(), k.data_ptr(), k_scale.data_ptr(), v.data_ptr(),
                                                 v_scale.data_ptr(), out.data_ptr(), lse.data_ptr(), B, Hq, Hk, Sq, Sk, sk_used, D, Dv,
@@ -73,6 +80,82 @@ def attention_mxfp4_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q
         rt.ptr(sl), 0 if sl is None or sl.shape[0] == 1 else sl.stride(0), 0 if sl is None else sl.stride(1),
         rt.stream_ptr(q.device)), "alto_mxfp4_attention_fwd_ex")
     return out, lse
+
+
+class _Backward(ctypes.Structure):
+    """alto_mxfp4_attention_bwd_t of include/alto_mxfp4.h."""
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("q_codes", "q_scales", "k_codes", "k_scales", "vt_codes", "v_scales", "dout", "out", "lse", "bias", "alibi_slopes",
+                                                "dq", "dk", "dv", "workspace")]
+                + [(n, ctypes.c_int64) for n in ("workspace_bytes", "B", "Hq", "Hk", "Sq", "Sk", "Sk_used", "D", "Dv")]
+                + [(f"{t}_{s}", ctypes.c_int64) for t in ("dout", "out", "lse", "dq", "dk", "dv") for s in ("sb", "sh", "ss")]
+                + [(n, ctypes.c_int64) for n in ("bias_sb", "bias_sh", "bias_sm", "alibi_sb", "alibi_sh")]
+                + [("cu_q", ctypes.POINTER(ctypes.c_int32)), ("cu_k", ctypes.POINTER(ctypes.c_int32))]
+                + [("n_seqs", ctypes.c_int), ("causal", ctypes.c_int), ("sm_scale", ctypes.c_float)])
+
+
+def _gradients(grad_out, operands, out, lse, sm_scale, causal, seqlen_k, b4, sl, cu_q, cu_k, dq, dk, dv) -> None:
+    """One backward call on [B, H, S, D] views; ``dq`` or ``dk`` and ``dv`` may be None (not wanted), ``b4`` / ``sl`` come from :func:`_additive`."""
+    q, q_scale, k, k_scale, v, v_scale = operands
+    (B, Hq, Sq), (Hk, Sk), Dv = q.shape[:3], k.shape[1:3], v.shape[2]
+    grad_out, out = _readable(grad_out), _readable(out)
+    a = _Backward(q_codes=q.data_ptr(), q_scales=q_scale.data_ptr(), k_codes=k.data_ptr(), k_scales=k_scale.data_ptr(), vt_codes=v.data_ptr(),
+                  v_scales=v_scale.data_ptr(), dout=grad_out.data_ptr(), out=out.data_ptr(), lse=lse.data_ptr(), bias=rt.ptr(b4), alibi_slopes=rt.ptr(sl),
+                  dq=rt.ptr(dq), dk=rt.ptr(dk), dv=rt.ptr(dv), B=B, Hq=Hq, Hk=Hk, Sq=Sq, Sk=Sk, Sk_used=seqlen_k, D=2 * q.shape[3], Dv=Dv, causal=int(bool(causal)),
+                  sm_scale=float(sm_scale))
+    for name, t in (("dout", grad_out), ("out", out), ("lse", lse), ("dq", dq), ("dk", dk), ("dv", dv)):
+        if t is not None:
+            for s, value in zip(("sb", "sh", "ss"), _strides(t)):
+                setattr(a, f"{name}_{s}", value)
+    if b4 is not None:
+        a.bias_sb, a.bias_sh, a.bias_sm = 0 if b4.shape[0] == 1 else b4.stride(0), 0 if b4.shape[1] == 1 else b4.stride(1), b4.stride(2)
+    if sl is not None:
+        a.alibi_sb, a.alibi_sh = 0 if sl.shape[0] == 1 else sl.stride(0), sl.stride(1)
+    if cu_q:
+        ints = ctypes.c_int32 * len(cu_q)
+        a.cu_q, a.cu_k, a.n_seqs = ints(*cu_q), ints(*cu_k), len(cu_q) - 1
+    need = rt.lib().alto_mxfp4_attention_bwd_workspace_bytes(ctypes.byref(a))
+    check(min(need, 0), "alto_mxfp4_attention_bwd_workspace_bytes")
+    with torch.cuda.device(q.device):
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+        a.workspace, a.workspace_bytes = ws.data_ptr(), need
+        check(rt.lib().alto_mxfp4_attention_bwd(ctypes.byref(a), rt.stream_ptr(q.device)), "alto_mxfp4_attention_bwd")
+
+
+def attention_mxfp4_backward(grad_out: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_scale: torch.Tensor, k_scale: torch.Tensor,
+                             v_scale: torch.Tensor, out: torch.Tensor, lse: torch.Tensor, sm_scale: float, causal: bool, seqlen_k: Optional[int] = None,
+                             bias: Optional[torch.Tensor] = None, alibi_slopes: Optional[torch.Tensor] = None, cu_seqlens_q=None,
+                             cu_seqlens_k=None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Gradients of :func:`attention_mxfp4_forward` on its operands -> (dq [B,Hq,Sq,D], dk [B,Hk,Sk,D], dv [B,Hk,Sk,Dv], all bf16).
+
+    ``grad_out`` and ``out`` bf16 [B,Hq,Sq,Dv] of any strides, ``lse`` fp32 [B,Hq,Sq]; the other arguments as the forward had them, the key dim
+    here any multiple of 32.  The probabilities are recomputed from the codes and ``lse``; the roundings of Q, K, V and of the probabilities
+    to MXFP4 are passed straight through:
+
+        P = exp(S - lse),  dV = P^T dO,  dS = P * (dO V^T - rowsum(dO * O)),  dQ = sm_scale dS K,  dK = sm_scale dS^T Q
+
+    Rows that see no key (``lse`` = -inf) give nothing to any gradient; keys from ``seqlen_k`` on get zeros.  ``bias`` gets no gradient.
+    ``cu_seqlens_q`` / ``cu_seqlens_k``: boundaries (multiples of 32, both or neither) of sequences packed along the tokens, with B = 1 and no bias.
+    Equal inputs give equal bits.
+    """
+    rt.require_gpu(grad_out, q, k, v, q_scale, k_scale, v_scale, out, lse)
+    for t in (q, k, v, q_scale, k_scale, v_scale):
+        assert t.is_contiguous() and t.dtype == torch.uint8
+    for t in (grad_out, k, v, q_scale, k_scale, v_scale, out, lse, bias, alibi_slopes):
+        assert t is None or t.device == q.device, f"tensors on {q.device} and {t.device}"
+    B, Hq, Sq, D = q.shape[0], q.shape[1], q.shape[2], q.shape[3] * 2
+    Hk, Sk, Dv = k.shape[1], k.shape[2], v.shape[2]
+    assert k.shape == (B, Hk, Sk, D // 2) and v.shape == (B, Hk, Dv, Sk // 2)
+    assert q_scale.shape == (B, Hq, Sq // 32, D // 32) and k_scale.shape == (B, Hk, Sk // 32, D // 32) and v_scale.shape == (B, Hk, Sk // 32, Dv // 32)
+    assert grad_out.shape == out.shape == (B, Hq, Sq, Dv) and grad_out.dtype == out.dtype == torch.bfloat16
+    assert lse.shape == (B, Hq, Sq) and lse.dtype == torch.float32
+    sk_used = Sk if seqlen_k is None else int(seqlen_k)
+    assert (cu_seqlens_q is None) == (cu_seqlens_k is None), "boundaries of packed sequences: for queries and keys, or for neither"
+    cu_q, cu_k = (None if c is None else [int(x) for x in (c.tolist() if isinstance(c, torch.Tensor) else c)] for c in (cu_seqlens_q, cu_seqlens_k))
+    assert cu_q is None or len(cu_q) == len(cu_k) >= 2, "cu_seqlens_q and cu_seqlens_k must describe the same number of sequences"
+    b4, sl = _additive(bias, alibi_slopes, B, Hq, Sq, sk_used)
+    dq, dk, dv = (torch.empty(shape, dtype=torch.bfloat16, device=q.device) for shape in ((B, Hq, Sq, D), (B, Hk, Sk, D), (B, Hk, Sk, Dv)))
+    _gradients(grad_out, (q, q_scale, k, k_scale, v, v_scale), out, lse, sm_scale, causal, sk_used, b4, sl, cu_q, cu_k, dq, dk, dv)
+    return dq, dk, dv
 
 
 def _strides(t: torch.Tensor) -> list:

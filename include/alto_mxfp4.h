@@ -532,6 +532,34 @@ int alto_mxfp4_attention_rows_per_workgroup(int64_t B, int64_t Hq, int64_t Sq, i
                                             int causal);
 
 /*
+ * Gradients of the attention forward with respect to Q, K and V, recomputing the probabilities: with the codes' values,
+ *   P = exp(S - lse),  dV = P^T dO,  dS = P * (dO V^T - rowsum(dO * O)),  dQ = sm_scale dS K,  dK = sm_scale dS^T Q,
+ * S and its additive terms as in alto_mxfp4_attention_fwd_ex, lse and out as that forward left them; the roundings of Q, K, V and P to
+ * MXFP4 are passed straight through.  (The reference's attention has no backward, triton_flash_attention_mxfp4.py:1143-1145.)
+ * Codes and scales dense, as alto_mxfp4_attention_fwd takes them (Sq and Sk any multiples of 32, nothing is read behind them).  dout, out and
+ * the gradients are bf16 with element strides of batch, head and row, unit stride along the head dim: dout and out 16-byte aligned
+ * with strides that are multiples of 8, the gradients 8-byte aligned with multiples of 4.  Keys from Sk_used on get zero gradients
+ * and those of a row with lse = -inf are zero.  n_seqs > 0: packed sequences as in alto_mxfp4_attention_fwd_strided (cu_q / cu_k on the host,
+ * no bias).  dq, or dk and dv together, may be NULL: not wanted.  bias: element (b, h, m, n) at b bias_sb + h bias_sh + m bias_sm + n, NULL: none; it gets no gradient.
+ * workspace: alto_mxfp4_attention_bwd_workspace_bytes() bytes (sizes alone count), 256-byte aligned, of this call until it is done.
+ * The results of equal inputs are equal bit for bit.
+ */
+typedef struct {
+  const void *q_codes, *q_scales, *k_codes, *k_scales, *vt_codes, *v_scales, *dout, *out;
+  const float *lse, *bias, *alibi_slopes;
+  void *dq, *dk, *dv, *workspace;
+  int64_t workspace_bytes, B, Hq, Hk, Sq, Sk, Sk_used, D, Dv;
+  int64_t dout_sb, dout_sh, dout_ss, out_sb, out_sh, out_ss, lse_sb, lse_sh, lse_ss;
+  int64_t dq_sb, dq_sh, dq_ss, dk_sb, dk_sh, dk_ss, dv_sb, dv_sh, dv_ss;
+  int64_t bias_sb, bias_sh, bias_sm, alibi_sb, alibi_sh;
+  const int32_t *cu_q, *cu_k;
+  int n_seqs, causal;
+  float sm_scale;
+} alto_mxfp4_attention_bwd_t;
+int64_t alto_mxfp4_attention_bwd_workspace_bytes(const alto_mxfp4_attention_bwd_t* args);
+int alto_mxfp4_attention_bwd(const alto_mxfp4_attention_bwd_t* args, void* stream);
+
+/*
  * Fills out[0 .. n) with random 32-bit words for stochastic rounding: word 4 c + j is word j of Philox4x32-10 (Salmon et
  * al., SC'11) with the 128-bit counter c + offset and the 64-bit key `seed`.  The reference draws its bits inside its
  * kernel from the same generator family (tl.randint4x, alto/kernels/fp4/fp4_common/triton_fp4_ops.py:15-18) with

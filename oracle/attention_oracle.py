@@ -25,7 +25,7 @@ an E2M1 rounding boundary: parity of the HIP kernel with this model is therefore
 """
 from __future__ import annotations
 
-from typing import Optional, Tuple
+from typing import NamedTuple, Optional, Tuple
 
 import torch
 
@@ -110,3 +110,69 @@ def attention_fp32_ref(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, cau
         masked = torch.arange(Sk)[None, :] > (torch.arange(Sq) + (Sk - Sq))[:, None]
         s = s.masked_fill(masked, float("-inf"))
     return torch.softmax(s, dim=-1) @ vf
+
+
+class AttentionGradients(NamedTuple):
+    """Gradients in 64 bits and, of the same shapes, how far a result may be from them: see :func:`attention_bwd_ref`."""
+    dq: torch.Tensor
+    dk: torch.Tensor
+    dv: torch.Tensor
+    dq_bound: torch.Tensor
+    dk_bound: torch.Tensor
+    dv_bound: torch.Tensor
+
+
+def attention_probabilities(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal: bool, sm_scale: float, bias: Optional[torch.Tensor] = None,
+                            alibi_slopes: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Softmax attention in 64 bits on values as they are -> (scores, output, log-sum-exp); a row that sees no key gets 0 and -inf."""
+    B, Hq, Sq, _ = q.shape
+    Hk, Sk = k.shape[1], k.shape[2]
+    kd, vd = (t.double().repeat_interleave(Hq // Hk, dim=1) for t in (k, v))
+    away = (torch.arange(Sq)[:, None] + (Sk - Sq) - torch.arange(Sk)[None, :])
+    s = torch.matmul(q.double(), kd.transpose(-1, -2)) * sm_scale
+    if bias is not None:
+        s = s + bias.double()
+    if alibi_slopes is not None:
+        slope = alibi_slopes.double()
+        s = s - (slope[None] if slope.dim() == 1 else slope)[..., None, None] * away.abs()
+    if causal:
+        s = s.masked_fill(away < 0, float("-inf"))
+    lse = torch.logsumexp(s, dim=-1)
+    p = torch.exp(s - lse.masked_fill(lse == float("-inf"), 0.0)[..., None])
+    return s, torch.matmul(p, vd), lse
+
+
+def attention_bwd_ref(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor, lse: torch.Tensor, *, causal: bool,
+                      sm_scale: float, bias: Optional[torch.Tensor] = None, alibi_slopes: Optional[torch.Tensor] = None) -> AttentionGradients:
+    """Gradients of attention on values (of codes) q, k, v with the forward's ``out`` and ``lse``, in 64 bits (the reference has no backward):
+
+        P = exp(S - lse),  dV = P^T dO,  dS = P (dO V^T - rowsum(dO O)),  dQ = sm_scale dS K,  dK = sm_scale dS^T Q.
+
+    The bounds allow, element by element, for the half steps of bf16 (2^-8 of a value) at P and dS as factors and at the result, and for
+    fp32 arithmetic: exponents to 2^-21 of (1 + |S| + |lse|), the inner products dO V^T and dO O to (Dv + 4) 2^-24 of the sums of their
+    terms' magnitudes, sums over rows or keys to their number times 2^-24 of the same.
+    """
+    Hq, Hk, Sq, Sk, Dv = q.shape[1], k.shape[1], q.shape[2], k.shape[2], v.shape[3]
+    s, _, _ = attention_probabilities(q, k, v, causal=causal, sm_scale=sm_scale, bias=bias, alibi_slopes=alibi_slopes)
+    qd, go, o, l = q.double(), dout.double(), out.double(), lse.double()[..., None]
+    kd, vd = (t.double().repeat_interleave(Hq // Hk, dim=1) for t in (k, v))
+    none = l == float("-inf")
+    l = l.masked_fill(none, 0.0)
+    p = torch.exp(s - l).masked_fill(none, 0.0)
+    o = o.masked_fill(none, 0.0)
+    inner = torch.matmul(go, vd.transpose(-1, -2)) - (go * o).sum(-1, keepdim=True)
+    ds = p * inner
+    dq, dk, dv = sm_scale * torch.matmul(ds, kd), sm_scale * torch.matmul(ds.transpose(-1, -2), qd), torch.matmul(p.transpose(-1, -2), go)
+
+    half, ulp = 2.0 ** -8, 2.0 ** -24
+    off_p = p * 2.0 ** -21 * (1 + s.masked_fill(s == float("-inf"), 0.0).abs() + l.abs())
+    off_inner = (Dv + 4) * ulp * (torch.matmul(go.abs(), vd.abs().transpose(-1, -2)) + (go * o).abs().sum(-1, keepdim=True))
+    off_ds = off_p * inner.abs() + p * off_inner
+    rows, keys = Sq * (Hq // Hk) * ulp, Sk * ulp
+    bq = abs(sm_scale) * torch.matmul(ds.abs() * (half + keys) + 1.01 * off_ds, kd.abs())
+    bk = abs(sm_scale) * torch.matmul((ds.abs() * (half + rows) + 1.01 * off_ds).transpose(-1, -2), qd.abs())
+    bv = torch.matmul((p * (half + rows) + 1.01 * off_p).transpose(-1, -2), go.abs())
+    group = lambda x: x.view(x.shape[0], Hk, Hq // Hk, *x.shape[2:]).sum(2)  # noqa: E731
+    dk, dv, bk, bv = group(dk), group(dv), group(bk), group(bv)
+    final = lambda x, b: b * (1 + half) + x.abs() * half + 1e-30  # noqa: E731
+    return AttentionGradients(dq, dk, dv, final(dq, bq), final(dk, bk), final(dv, bv))

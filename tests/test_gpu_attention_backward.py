@@ -1,0 +1,172 @@
+"""Gradients of the MXFP4 attention (through the C ABI) against the 64-bit formula on the values of the same codes.
+
+Tolerance: element by element what the oracle derives (half steps of bf16 at P, dS and the result, fp32 arithmetic between them)."""
+import pytest
+import torch
+
+from oracle import mxfp4_oracle as O
+from oracle.attention_oracle import attention_bwd_ref, attention_probabilities
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+@pytest.fixture(scope="module")
+def m():
+    import alto_amd.mxfp4 as mod
+    return mod
+
+
+class Operands:
+    """Quantized Q, K, V with their values, and what an exact forward leaves of them."""
+
+    def __init__(self, B, Hq, Hk, Sq, Sk, D, Dv, causal, seed, bias=None, alibi_slopes=None, magnitude=1.0, used=None):
+        g = torch.Generator().manual_seed(seed)
+        rand = lambda *shape: torch.randn(shape, generator=g)  # noqa: E731
+        q, k, v = (magnitude * rand(B, Hq, Sq, D)).bfloat16(), rand(B, Hk, Sk, D).bfloat16(), rand(B, Hk, Sk, Dv).bfloat16()
+        self.q, self.qs = O.quantize(q, axis=-1, is_2d_block=True)
+        self.k, self.ks = O.quantize(k, axis=-1, is_2d_block=True)
+        vq, self.vs = O.quantize(v, axis=-1, is_2d_block=True)
+        self.v, _ = O.quantize(v.transpose(-1, -2).contiguous(), axis=-1, is_2d_block=True)
+        back = lambda c, s: O.dequantize(c, s, torch.float32, axis=-1, is_2d_block=True)  # noqa: E731
+        used = Sk if used is None else used
+        self.values = back(self.q, self.qs), back(self.k, self.ks)[:, :, :used], back(vq, self.vs)[:, :, :used]
+        self.more = dict(causal=causal, sm_scale=D ** -0.5, bias=bias, alibi_slopes=alibi_slopes)
+        _, out, lse = attention_probabilities(*self.values, **self.more)
+        self.out, self.lse = out.bfloat16(), lse.float()
+        self.go = rand(B, Hq, Sq, Dv).bfloat16()
+
+    def expected(self):
+        return attention_bwd_ref(self.go, *self.values, self.out, self.lse, **self.more)
+
+    def call(self, m, **kw):
+        put = lambda t: None if t is None else t.to(DEV)  # noqa: E731
+        args = [put(t) for t in (self.go, self.q, self.k, self.v, self.qs, self.ks, self.vs, self.out, self.lse)]
+        return m.attention_mxfp4_backward(*args, self.more["sm_scale"], self.more["causal"], bias=put(self.more["bias"]),
+                                          alibi_slopes=put(self.more["alibi_slopes"]), **kw)
+
+
+def check(got, ref, what=""):
+    for name, x, exact, bound in zip(("dq", "dk", "dv"), got, ref[:3], ref[3:]):
+        assert x.dtype == torch.bfloat16 and x.shape == exact.shape, (what, name, x.shape, exact.shape)
+        off = (x.cpu().double() - exact).abs() / bound
+        assert float(off.max()) <= 1.0, f"{what} {name}: {int((off > 1).sum())} of {off.numel()} out of bounds, worst {float(off.max()):.3g} at {tuple((off == off.max()).nonzero()[0].tolist())}"
+
+
+CASES = [
+    # B, Hq, Hk, Sq, Sk, D, Dv, causal
+    (1, 1, 1, 32, 32, 64, 64, False),
+    (1, 1, 1, 32, 32, 64, 64, True),
+    (1, 2, 1, 64, 64, 128, 128, True),
+    (2, 4, 4, 96, 96, 64, 128, True),
+    (1, 4, 2, 128, 160, 128, 64, True),        # Sq < Sk: the mask is aligned to the bottom-right corner
+    (1, 8, 1, 256, 256, 128, 128, True),
+    (2, 2, 2, 224, 64, 64, 64, False),         # more rows than keys
+    (1, 3, 1, 32, 544, 128, 128, True),        # one tile of rows, keys over several workgroups
+    (1, 2, 2, 96, 128, 192, 128, False),
+    (1, 3, 3, 160, 320, 192, 64, True),
+    (1, 2, 1, 64, 192, 256, 128, False),
+    (1, 5, 5, 288, 288, 256, 64, True),
+]
+
+
+@pytest.mark.parametrize("case", CASES, ids=lambda c: "x".join(map(str, c)))
+def test_gradients_match_the_formula(m, case):
+    x = Operands(*case, seed=sum(case))
+    check(x.call(m), x.expected())
+
+
+@pytest.mark.parametrize("case", [(2, 4, 2, 96, 160, 128, 128, False), (2, 2, 2, 64, 64, 64, 64, True), (1, 2, 1, 64, 96, 192, 128, False), (1, 2, 1, 32, 64, 256, 64, True)],
+                         ids=lambda c: "x".join(map(str, c)))
+@pytest.mark.parametrize("extra", ["bias", "alibi", "both"])
+def test_additive_terms(m, case, extra):
+    B, Hq, Hk, Sq, Sk, D, Dv, causal = case
+    g = torch.Generator().manual_seed(5)
+    bias = alibi = None
+    if extra != "alibi":   # keys hidden here and there, one sequence's first row without any
+        bias = torch.randn(B, 1, Sq, Sk, generator=g).masked_fill(torch.rand(B, 1, Sq, Sk, generator=g) < 0.3, float("-inf"))
+        bias[-1, :, 0] = float("-inf")
+        bias[0, :, :, 0] = 0.0
+    if extra != "bias":
+        alibi = torch.rand(B, Hq, generator=g)
+    x = Operands(*case, seed=6, bias=bias, alibi_slopes=alibi)
+    got = x.call(m)
+    check(got, x.expected(), extra)
+    if bias is not None:
+        assert bool((got[0][-1, :, 0] == 0).all())
+
+
+@pytest.mark.parametrize("causal", [True, False])
+def test_packed_sequences_are_the_sequences_alone(m, causal):
+    """Lengths of one tile, of odd numbers of tiles and of more than a workgroup's block; each sequence's gradients bit for bit those of its own call."""
+    Hq, Hk, D, Dv = 4, 2, 128, 64
+    lens_q, lens_k = [32, 96, 288, 160], [32, 96, 288, 224] if causal else [64, 32, 96, 160]
+    parts = [Operands(1, Hq, Hk, a, b, D, Dv, causal, seed=a + b) for a, b in zip(lens_q, lens_k)]
+    cat = lambda name, dim: torch.cat([getattr(p, name) for p in parts], dim).contiguous()  # noqa: E731
+    whole = Operands.__new__(Operands)
+    whole.go, whole.out, whole.lse = cat("go", 2), cat("out", 2), cat("lse", 2)
+    whole.q, whole.qs, whole.k, whole.ks, whole.v, whole.vs = cat("q", 2), cat("qs", 2), cat("k", 2), cat("ks", 2), cat("v", 3), cat("vs", 2)
+    whole.more = dict(parts[0].more)
+    starts = lambda lens: [0] + torch.tensor(lens).cumsum(0).tolist()  # noqa: E731
+    cu_q, cu_k = starts(lens_q), starts(lens_k)
+    got = whole.call(m, cu_seqlens_q=cu_q, cu_seqlens_k=torch.tensor(cu_k, dtype=torch.int32))
+    for i, p in enumerate(parts):
+        rows, keys = slice(cu_q[i], cu_q[i + 1]), slice(cu_k[i], cu_k[i + 1])
+        mine = got[0][:, :, rows], got[1][:, :, keys], got[2][:, :, keys]
+        check(mine, p.expected(), f"sequence {i}")
+        for a, b in zip(mine, p.call(m)):
+            assert torch.equal(a, b)
+
+
+def test_more_sequences_than_one_launch_takes(m):
+    n, Hq, Hk, D = 67, 2, 1, 64
+    x = Operands(n, Hq, Hk, 32, 32, D, D, True, seed=11)
+    tokens = lambda t: t.transpose(0, 1).reshape(1, t.shape[1], n * t.shape[2], *t.shape[3:]).contiguous()  # noqa: E731
+    y = Operands.__new__(Operands)
+    y.go, y.out, y.lse, y.q, y.qs, y.k, y.ks = (tokens(t) for t in (x.go, x.out, x.lse, x.q, x.qs, x.k, x.ks))
+    y.v, y.vs = x.v.permute(1, 2, 0, 3).reshape(1, Hk, D, n * 16).contiguous(), tokens(x.vs)
+    y.more = x.more
+    starts = list(range(0, 32 * n + 1, 32))
+    got = y.call(m, cu_seqlens_q=starts, cu_seqlens_k=starts)
+    for a, b in zip(got, x.call(m)):
+        assert torch.equal(a, tokens(b))
+    check(x.call(m), x.expected())
+
+
+def test_keys_behind_the_used_ones_get_zeros(m):
+    """A sequence of 96 keys among 256 that are allocated: whole workgroups of keys have nothing to sum."""
+    for causal in (False, True):
+        x = Operands(1, 2, 1, 64, 256, 64, 64, causal, seed=4, used=96)
+        got = x.call(m, seqlen_k=96)
+        check((got[0], got[1][:, :, :96], got[2][:, :, :96]), x.expected())
+        assert bool((got[1][:, :, 96:] == 0).all()) and bool((got[2][:, :, 96:] == 0).all())
+
+
+def test_gradients_of_the_output_in_any_layout(m):
+    """grad_out and out as views: [B, S, H, D] memory, rows apart, one row for all (a sum's gradient), an odd offset (copied)."""
+    x = Operands(2, 4, 2, 96, 96, 64, 64, True, seed=8)
+    want = x.call(m)
+    x.out = x.out.to(DEV).transpose(1, 2).contiguous().transpose(1, 2)
+    wide = torch.full((2, 4, 96, 80), float("nan"), dtype=torch.bfloat16, device=DEV)
+    keep = x.go
+    for view in (wide[..., :64], wide[..., 8:72], wide[..., 3:67]):
+        view.copy_(keep)
+        x.go = view
+        for a, b in zip(x.call(m), want):
+            assert torch.equal(a, b)
+    x.go = torch.ones(1, 1, 1, 1, dtype=torch.bfloat16).expand(2, 4, 96, 64)
+    check(x.call(m), x.expected())
+
+
+def test_large_scores_and_probabilities_of_one(m):
+    """Scores of some hundreds: a row's probability sits on one key, the others' underflow."""
+    x = Operands(1, 2, 1, 128, 128, 128, 128, True, seed=21, magnitude=40.0)
+    check(x.call(m), x.expected())
+
+
+def test_results_do_not_change_from_run_to_run(m):
+    x = Operands(2, 8, 2, 256, 256, 128, 128, True, seed=2)
+    first = x.call(m)
+    for _ in range(3):
+        for a, b in zip(x.call(m), first):
+            assert torch.equal(a, b)
