@@ -32,8 +32,24 @@ struct AttnBwdSeqs {
   int zq[ATTN_MAX_SEQS + 1], zk[ATTN_MAX_SEQS + 1], q0[ATTN_MAX_SEQS], qn[ATTN_MAX_SEQS], k0[ATTN_MAX_SEQS], kn[ATTN_MAX_SEQS];
 };
 
+// How a launch is cut into workgroups, first those of dK and dV, then those of dQ.  A block of keys walks the tiles of 32 rows that see it, of
+// all query heads on its key head; lists longer than `chunk` are dealt out to up to `parts` workgroups, whose fp32 sums meet in a kernel of
+// their own (`partial`: one accumulator set for each part and block).
+struct AttnBwdPlan {
+  int q_blocks, k_blocks;       // over all sequences
+  int parts, chunk;
+  int key_groups, row_groups;   // workgroups of either kind (those of the keys: a multiple of 8)
+  float* partial;
+};
+
+// Keys of one wave in the dK / dV part, rows of one in the dQ part: what 512 registers a lane hold.
+constexpr int bwd_keys_sub(int) { return 1; }
+constexpr int bwd_rows_sub(int) { return 1; }
+inline int bwd_key_block(int64_t D) { return 128 * bwd_keys_sub((int)(D / 64)); }
+inline int bwd_row_block(int64_t D) { return 128 * bwd_rows_sub((int)(D / 64)); }
+
 template <int NK>
-int launch_attn_bwd(const AttnBwdArgs& a, const AttnBwdSeqs& seqs, int64_t Dv, int q_blocks, int k_blocks, hipStream_t st);
+int launch_attn_bwd(const AttnBwdArgs& a, const AttnBwdSeqs& seqs, const AttnBwdPlan& plan, int64_t Dv, hipStream_t st);
 
 #ifdef ALTO_ATTENTION_BACKWARD_KERNELS
 namespace {
@@ -116,15 +132,19 @@ __device__ __forceinline__ bf16x8_t pack8(const v16f_t& x, int c) {
 }
 
 // lane (r, h) stores row r of a transposed accumulator (registers: columns 32 n + score_row(v, h)) as bf16
-template <int N>
-__device__ __forceinline__ void store_rows(__bf16* row, const v16f_t (&acc)[N], float scale, int h) {
+__device__ __forceinline__ void store_columns(__bf16* row, const v16f_t& acc, float scale, int n, int h) {
 #pragma unroll
-  for (int n = 0; n < N; ++n)
+  for (int g = 0; g < 4; ++g) {
+    const uint2 w = make_uint2(pack_bf16x2(acc[4 * g] * scale, acc[4 * g + 1] * scale), pack_bf16x2(acc[4 * g + 2] * scale, acc[4 * g + 3] * scale));
+    *reinterpret_cast<uint2*>(row + 32 * n + 8 * g + 4 * h) = w;
+  }
+}
+
+__device__ __forceinline__ v16f_t zeros() {
+  v16f_t z;
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const uint2 w = make_uint2(pack_bf16x2(acc[n][4 * g] * scale, acc[n][4 * g + 1] * scale), pack_bf16x2(acc[n][4 * g + 2] * scale, acc[n][4 * g + 3] * scale));
-      *reinterpret_cast<uint2*>(row + 32 * n + 8 * g + 4 * h) = w;
-    }
+  for (int v = 0; v < 16; ++v) z[v] = 0.0f;
+  return z;
 }
 
 struct AttnBwdBlock {
@@ -145,6 +165,29 @@ __device__ __forceinline__ AttnBwdBlock attn_bwd_block(const AttnBwdArgs& a, con
   return w;
 }
 
+// Eight neighbouring workgroups go to the eight XCDs in turn: each XCD gets a range of consecutive (batch, head) pairs, so that a head's
+// operands come into one L2.
+__device__ __forceinline__ int head_of(int i, int heads) { return heads % 8 == 0 ? (i & 7) * (heads >> 3) + (i >> 3) : i; }
+
+// The list of a block of keys: tiles first .. all of each of the group's heads.
+struct KeyList {
+  int first, each, total, parts;
+};
+template <int KEYS>   // keys of a workgroup
+__device__ __forceinline__ KeyList key_list(const AttnBwdArgs& a, const AttnBwdBlock& w, const AttnBwdPlan& plan) {
+  KeyList l{0, 0, 0, 1};
+  const int all = w.qn / 32;
+  if (a.causal) {
+    l.first = (w.block * KEYS - (w.kn - w.qn)) / 32;
+    l.first = l.first < 0 ? 0 : l.first;
+  }
+  l.each = l.first < all && w.block * KEYS < w.kn ? all - l.first : 0;
+  l.total = l.each * (a.Hq / a.Hk);
+  l.parts = (l.total + plan.chunk - 1) / plan.chunk;
+  l.parts = l.parts < 1 ? 1 : (l.parts > plan.parts ? plan.parts : l.parts);
+  return l;
+}
+
 constexpr int BWD_RING = 3;
 
 // ---------------------------------------------------------------------------------------------------------------- dK and dV
@@ -153,54 +196,59 @@ struct KeysTile {
   static constexpr int CODES = CodeTile<NK>::BYTES, ROWS = RowTile<64 * NK>::BYTES, GRAD = RowTile<64 * NV>::BYTES;
   static constexpr int O_ROWS = CODES, O_GRAD = O_ROWS + ROWS, O_STATS = O_GRAD + GRAD, SLOT = O_STATS + 256;
   static constexpr int LOADS = 1 + NK + NV + (NK == 4 ? 1 : 0);   // of a wave, for one tile
+  static constexpr int SUB = bwd_keys_sub(NK), KEYS = 128 * SUB;
+  static constexpr int ACC = 2 * NK + 2 * NV;                                     // accumulators of 32 keys
+  static constexpr int64_t PARTIAL = (int64_t)4 * SUB * ACC * 16 * 64;            // floats of a workgroup's sums
 };
 
-// Four waves own 128 consecutive keys of one key head, 32 each, and walk the query rows of the head's group in tiles of 32.
+// Four waves own 128 SUB consecutive keys of one key head, 32 SUB each, and walk their part of the list in tiles of 32 rows.
 template <int NK, int NV, bool BIASED>
-__device__ __forceinline__ void attn_bwd_keys_body(const AttnBwdArgs& a, const AttnBwdSeqs& seqs, __bf16* __restrict__ dk_out, __bf16* __restrict__ dv_out, uint8_t* ring) {
+__device__ __forceinline__ void attn_bwd_keys_body(const AttnBwdArgs& a, const AttnBwdSeqs& seqs, const AttnBwdPlan& plan, int item, __bf16* __restrict__ dk_out,
+                                                   __bf16* __restrict__ dv_out, float* __restrict__ partial, uint8_t* ring) {
   using T = KeysTile<NK, NV>;
   using QT = RowTile<64 * NK>;
   using GT = RowTile<64 * NV>;
-  constexpr int D = 64 * NK, DV = 64 * NV;
+  constexpr int D = 64 * NK, DV = 64 * NV, SUB = T::SUB;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 31, h = lane >> 5;
-  const AttnBwdBlock w = attn_bwd_block<true>(a, seqs, (int)blockIdx.z);
-  const int hk = blockIdx.x, b = blockIdx.y, group = a.Hq / a.Hk;
-  const int shift = w.kn - w.qn, key0 = w.block * 128 + wave * 32;
-  const bool live = key0 < w.kn;
-  const bool stored = seqs.n ? live : key0 < a.Sk;   // keys behind the used ones get zeros
-  const int64_t k_base = ((int64_t)b * a.Hk + hk) * a.Sk + w.k_first + (live ? key0 : 0);   // row of the wave's first key
+  const int heads = a.B * a.Hk, bh = head_of(item % heads, heads);
+  const int part = (item / heads) % plan.parts, z = item / heads / plan.parts;
+  if (z >= plan.k_blocks) return;
+  const AttnBwdBlock w = attn_bwd_block<true>(a, seqs, z);
+  const KeyList list = key_list<T::KEYS>(a, w, plan);
+  if (part >= list.parts) return;
+  const int begin = (int)((int64_t)list.total * part / list.parts), total = (int)((int64_t)list.total * (part + 1) / list.parts) - begin;
+  const int hk = bh % a.Hk, b = bh / a.Hk, group = a.Hq / a.Hk;
+  const int shift = w.kn - w.qn, key0 = w.block * T::KEYS + wave * 32 * SUB;
+  const int64_t k_base = (int64_t)bh * a.Sk + w.k_first;
 
   // the wave's keys and values stay in registers
-  v8i_t kf[NK];
-  int ksc[NK];
-  bf16x8_t vf[4 * NV];
+  v8i_t kf[SUB][NK];
+  int ksc[SUB][NK];
+  bf16x8_t vf[SUB][4 * NV];
 #pragma unroll
-  for (int s = 0; s < NK; ++s) {
-    kf[s] = frag16(a.k + (k_base + r) * (D / 2) + s * 32 + h * 16);
-    ksc[s] = a.k_scales[(k_base / 32) * 8 + 2 * s + h];
+  for (int u = 0; u < SUB; ++u) {
+    const int64_t row = k_base + (key0 + 32 * u < w.kn ? key0 + 32 * u : 0);
+#pragma unroll
+    for (int s = 0; s < NK; ++s) {
+      kf[u][s] = frag16(a.k + (row + r) * (D / 2) + s * 32 + h * 16);
+      ksc[u][s] = a.k_scales[(row / 32) * 8 + 2 * s + h];
+    }
+#pragma unroll
+    for (int i = 0; i < 4 * NV; ++i) vf[u][i] = *reinterpret_cast<const bf16x8_t*>(a.v_rows + (row + r) * DV + 16 * i + 8 * h);
   }
-#pragma unroll
-  for (int i = 0; i < 4 * NV; ++i) vf[i] = *reinterpret_cast<const bf16x8_t*>(a.v_rows + (k_base + r) * DV + 16 * i + 8 * h);
 
-  v16f_t dk[2 * NK], dv[2 * NV];
+  v16f_t dk[SUB][2 * NK], dv[SUB][2 * NV];
 #pragma unroll
-  for (int n = 0; n < 2 * NK; ++n)
+  for (int u = 0; u < SUB; ++u) {
 #pragma unroll
-    for (int v = 0; v < 16; ++v) dk[n][v] = 0.0f;
+    for (int n = 0; n < 2 * NK; ++n) dk[u][n] = zeros();
 #pragma unroll
-  for (int n = 0; n < 2 * NV; ++n)
-#pragma unroll
-    for (int v = 0; v < 16; ++v) dv[n][v] = 0.0f;
+    for (int n = 0; n < 2 * NV; ++n) dv[u][n] = zeros();
+  }
 
-  // query tiles: those that see the workgroup's first key, of every head of the group
   const int all = w.qn / 32;
-  int first = 0;
-  if (a.causal) {
-    first = (w.block * 128 - shift) / 32;
-    first = first < 0 ? 0 : first;
-  }
-  const int each = first < all && w.block * 128 < w.kn ? all - first : 0, total = each * group;
-  const int own_first = a.causal ? (key0 - shift) / 32 : 0;   // the tile whose diagonal the wave's keys are on (maybe below zero)
+  const int own_first = a.causal ? (key0 - shift) / 32 : 0;   // the tile whose diagonal the wave's first keys are on (maybe below zero)
+  const int own_whole = a.causal ? own_first + SUB : 0;       // from here on all of the wave's keys are seen
   const float c2 = a.sm_scale * ATTN_RCP_LN2;
 
   // each lane's part of a tile's loads
@@ -211,7 +259,9 @@ __device__ __forceinline__ void attn_bwd_keys_body(const AttnBwdArgs& a, const A
   const int go_pitch = (int)(a.do_ss * 2);
 #pragma unroll
   for (int j = 0; j < NV; ++j) o_grad[j] = GT::source(64 * (4 * j + wave) + lane, go_pitch);
-  int next_head = 0, next_tile = first;   // of the next load
+  int head = 0, tile = list.first;
+  if (begin > 0) { head = begin / list.each; tile += begin % list.each; }
+  int next_head = head, next_tile = tile;   // of the next load
   auto fetch = [&](int slot) {
     const int hq = hk * group + next_head;
     const int64_t row = ((int64_t)b * a.Hq + hq) * a.Sq + w.q_first + 32 * next_tile;
@@ -225,7 +275,7 @@ __device__ __forceinline__ void attn_bwd_keys_body(const AttnBwdArgs& a, const A
     const __amdgpu_buffer_rsrc_t grad = buffer(a.dout + b * a.do_sb + hq * a.do_sh + (int64_t)(w.q_first + 32 * next_tile) * a.do_ss, (int64_t)31 * go_pitch + 2 * DV);
 #pragma unroll
     for (int j = 0; j < NV; ++j) load_piece(grad, to + T::O_GRAD + 1024 * (4 * j + wave), o_grad[j]);
-    if (++next_tile == all) { next_tile = first; ++next_head; }
+    if (++next_tile == all) { next_tile = list.first; ++next_head; }
   };
   auto wait = [](bool one_in_flight) {
     if (one_in_flight) __builtin_amdgcn_s_waitcnt(0x0070 | 0x0F00 | (T::LOADS & 15));
@@ -237,81 +287,156 @@ __device__ __forceinline__ void attn_bwd_keys_body(const AttnBwdArgs& a, const A
   asm volatile("s_barrier" ::: "memory");
 
   const int row_base = GT::row_base(lane), q_col = QT::column_base(lane), g_col = GT::column_base(lane);
-  int slot = 0, tile = first, head = 0;
+  int slot = 0;
+  const bool live = key0 < w.kn;
+  auto compute = [&](const uint8_t* at, int hq, uint32_t qs0, uint32_t qs1) {
+    v16f_t S[SUB], dp[SUB];
+#pragma unroll
+    for (int u = 0; u < SUB; ++u) S[u] = zeros();
+    static_for<NK>([&](auto sc) {
+      constexpr int s = decltype(sc)::value;
+      const v8i_t qf = CodeTile<NK>::frag(at, lane, s);
+      const int qs = (int)((s < 2 ? qs0 : qs1) >> (8 * h));
+#pragma unroll
+      for (int u = 0; u < SUB; ++u) S[u] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(qf, kf[u][s], S[u], 4, 4, (2 * s) % 4, qs, 0, ksc[u][s]);
+    });
+    const float* stats = reinterpret_cast<const float*>(at + T::O_STATS);
+    v16f_t lse2, nd;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const v4f_t x = *reinterpret_cast<const v4f_t*>(stats + 8 * g + 4 * h), y = *reinterpret_cast<const v4f_t*>(stats + 32 + 8 * g + 4 * h);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) { lse2[4 * g + i] = x[i]; nd[4 * g + i] = y[i]; }
+    }
+#pragma unroll
+    for (int u = 0; u < SUB; ++u) dp[u] = nd;
+#pragma unroll
+    for (int kc = 0; kc < 4 * NV; ++kc) {
+      const bf16x8_t gf = GT::row_frag(at + T::O_GRAD, row_base, kc);
+#pragma unroll
+      for (int u = 0; u < SUB; ++u) dp[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(gf, vf[u][kc], dp[u], 0, 0, 0);
+    }
+#pragma unroll
+    for (int u = 0; u < SUB; ++u)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) {
+        float y = S[u][v] * c2;
+        const int row = 32 * tile + score_row(v, h), key = key0 + 32 * u + r;
+        if constexpr (BIASED) {
+          if (a.bias) y = __builtin_fmaf(a.bias[b * a.bias_sb + hq * a.bias_sh + row * a.bias_sm + (key < w.kn ? key : 0)], ATTN_RCP_LN2, y);
+          if (a.alibi) y = __builtin_fmaf(-a.alibi[b * a.alibi_sb + hq * a.alibi_sh] * ATTN_RCP_LN2, __builtin_fabsf((float)(row + shift - key)), y);
+        }
+        S[u][v] = y - lse2[v];
+      }
+    if (tile < own_whole) {
+      asm volatile("" ::: "memory");   // keep this a branch: most tiles skip it
+#pragma unroll
+      for (int u = 0; u < SUB; ++u)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) S[u][v] = key0 + 32 * u + r > 32 * tile + score_row(v, h) + shift ? -__builtin_inff() : S[u][v];
+    }
+#pragma unroll
+    for (int u = 0; u < SUB; ++u)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) S[u][v] = __builtin_amdgcn_exp2f(S[u][v]);
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      bf16x8_t p[SUB];
+#pragma unroll
+      for (int u = 0; u < SUB; ++u) p[u] = pack8(S[u], c);
+#pragma unroll
+      for (int n = 0; n < 2 * NV; ++n) {
+        const bf16x8_t gf = GT::column_frag(at + T::O_GRAD, g_col, n, c);
+#pragma unroll
+        for (int u = 0; u < SUB; ++u) dv[u][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(gf, p[u], dv[u][n], 0, 0, 0);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < SUB; ++u)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) dp[u][v] *= S[u][v];
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      bf16x8_t ds[SUB];
+#pragma unroll
+      for (int u = 0; u < SUB; ++u) ds[u] = pack8(dp[u], c);
+#pragma unroll
+      for (int n = 0; n < 2 * NK; ++n) {
+        const bf16x8_t qf = QT::column_frag(at + T::O_ROWS, q_col, n, c);
+#pragma unroll
+        for (int u = 0; u < SUB; ++u) dk[u][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(qf, ds[u], dk[u][n], 0, 0, 0);
+      }
+    }
+  };
   for (int t = 0; t < total; ++t) {
     const uint8_t* at = ring + slot * T::SLOT;
     const int hq = hk * group + head;
     const scalar_u32 qsp = scalar_ptr(a.q_scales + ((((int64_t)b * a.Hq + hq) * a.Sq + w.q_first) / 32 + tile) * 8);
-    uint32_t qs[2] = {qsp[0], NK > 2 ? qsp[1] : 0};
+    const uint32_t qs0 = qsp[0], qs1 = NK > 2 ? qsp[1] : 0;
     if (t + 2 < total) fetch(slot == 0 ? BWD_RING - 1 : slot - 1);
-    if (live && tile >= own_first) {
-      v16f_t S, P;
-#pragma unroll
-      for (int v = 0; v < 16; ++v) S[v] = 0.0f;
-      static_for<NK>([&](auto sc) {
-        constexpr int s = decltype(sc)::value;
-        S = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(CodeTile<NK>::frag(at, lane, s), kf[s], S, 4, 4, (2 * s) % 4, (int)(qs[s >> 1] >> (8 * h)), 0, ksc[s]);
-      });
-      const float* stats = reinterpret_cast<const float*>(at + T::O_STATS);
-      v16f_t dp;
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const v4f_t x = *reinterpret_cast<const v4f_t*>(stats + 32 + 8 * g + 4 * h);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) dp[4 * g + i] = x[i];
-      }
-#pragma unroll
-      for (int kc = 0; kc < 4 * NV; ++kc) dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(GT::row_frag(at + T::O_GRAD, row_base, kc), vf[kc], dp, 0, 0, 0);
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const v4f_t x = *reinterpret_cast<const v4f_t*>(stats + 8 * g + 4 * h);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float y = S[4 * g + i] * c2;
-          if constexpr (BIASED) {
-            const int row = 32 * tile + 8 * g + 4 * h + i;
-            if (a.bias) y = __builtin_fmaf(a.bias[b * a.bias_sb + hq * a.bias_sh + row * a.bias_sm + key0 + r], ATTN_RCP_LN2, y);
-            if (a.alibi) y = __builtin_fmaf(-a.alibi[b * a.alibi_sb + hq * a.alibi_sh] * ATTN_RCP_LN2, __builtin_fabsf((float)(row + shift - key0 - r)), y);
-          }
-          S[4 * g + i] = y - x[i];
-        }
-      }
-      if (a.causal && tile == own_first) {   // on the diagonal: key r is hidden from the rows before it
-#pragma unroll
-        for (int v = 0; v < 16; ++v) S[v] = score_row(v, h) < r ? -__builtin_inff() : S[v];
-      }
-#pragma unroll
-      for (int v = 0; v < 16; ++v) P[v] = __builtin_amdgcn_exp2f(S[v]);
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const bf16x8_t p = pack8(P, c);
-#pragma unroll
-        for (int n = 0; n < 2 * NV; ++n) dv[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(GT::column_frag(at + T::O_GRAD, g_col, n, c), p, dv[n], 0, 0, 0);
-      }
-#pragma unroll
-      for (int v = 0; v < 16; ++v) dp[v] *= P[v];
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const bf16x8_t ds = pack8(dp, c);
-#pragma unroll
-        for (int n = 0; n < 2 * NK; ++n) dk[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(QT::column_frag(at + T::O_ROWS, q_col, n, c), ds, dk[n], 0, 0, 0);
-      }
-    }
+    if (live && tile >= own_first) compute(at, hq, qs0, qs1);
     wait(t + 2 < total);
     asm volatile("s_barrier" ::: "memory");
     slot = slot == BWD_RING - 1 ? 0 : slot + 1;
-    if (++tile == all) { tile = first; ++head; }
+    if (++tile == all) { tile = list.first; ++head; }
   }
-  if (!stored) return;
-  const int64_t key = w.k_first + key0 + r;
-  store_rows(dk_out + b * a.dk_sb + hk * a.dk_sh + key * a.dk_ss, dk, a.sm_scale, h);
-  store_rows(dv_out + b * a.dv_sb + hk * a.dv_sh + key * a.dv_ss, dv, 1.0f, h);
+  if (list.parts > 1) {
+    v4f_t* to = reinterpret_cast<v4f_t*>(partial + (((int64_t)z * plan.parts + part) * heads + bh) * T::PARTIAL) + wave * (SUB * T::ACC * 4 * 64) + lane;
+#pragma unroll
+    for (int u = 0; u < SUB; ++u)
+#pragma unroll
+      for (int n = 0; n < T::ACC; ++n)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const v16f_t& x = n < 2 * NK ? dk[u][n < 2 * NK ? n : 0] : dv[u][n < 2 * NK ? 0 : n - 2 * NK];
+          to[((u * T::ACC + n) * 4 + g) * 64] = v4f_t{x[4 * g], x[4 * g + 1], x[4 * g + 2], x[4 * g + 3]};
+        }
+    return;
+  }
+#pragma unroll
+  for (int u = 0; u < SUB; ++u) {
+    const int key = key0 + 32 * u;
+    if (key >= (seqs.n ? w.kn : a.Sk)) continue;
+    const bool used = key < w.kn;   // keys behind the used ones get zeros
+    const int64_t at = w.k_first + key + r;
+#pragma unroll
+    for (int n = 0; n < 2 * NK; ++n) store_columns(dk_out + b * a.dk_sb + hk * a.dk_sh + at * a.dk_ss, used ? dk[u][n] : zeros(), a.sm_scale, n, h);
+#pragma unroll
+    for (int n = 0; n < 2 * NV; ++n) store_columns(dv_out + b * a.dv_sb + hk * a.dv_sh + at * a.dv_ss, used ? dv[u][n] : zeros(), 1.0f, n, h);
+  }
 }
 
-template <int NK, int NV, bool BIASED>
-__global__ __launch_bounds__(256, NK > 2 ? 1 : 2) void attn_bwd_keys_kernel(AttnBwdArgs a, AttnBwdSeqs seqs) {
-  extern __shared__ __attribute__((aligned(256))) uint8_t ring[];
-  attn_bwd_keys_body<NK, NV, BIASED>(a, seqs, reinterpret_cast<__bf16*>(a.dk), reinterpret_cast<__bf16*>(a.dv), ring);
+// Sums of the parts, in their order.  Grid: (heads, key blocks, accumulators of 32 keys); a wave has the keys that it has in the kernel above.
+template <int NK, int NV>
+__global__ __launch_bounds__(256) void attn_bwd_sum_kernel(AttnBwdArgs a, AttnBwdSeqs seqs, AttnBwdPlan plan) {
+  using T = KeysTile<NK, NV>;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 31, h = lane >> 5;
+  const int heads = a.B * a.Hk, bh = blockIdx.x, z = blockIdx.y, n = blockIdx.z;
+  const AttnBwdBlock w = attn_bwd_block<true>(a, seqs, z);
+  const KeyList list = key_list<T::KEYS>(a, w, plan);
+  if (list.parts == 1) return;
+  const int hk = bh % a.Hk, b = bh / a.Hk;
+#pragma unroll
+  for (int u = 0; u < T::SUB; ++u) {
+    const int key = w.block * T::KEYS + (wave * T::SUB + u) * 32;
+    if (key >= (seqs.n ? w.kn : a.Sk)) continue;
+    v16f_t sum = zeros();
+    if (key < w.kn) {
+      for (int part = 0; part < list.parts; ++part) {
+        const v4f_t* from = reinterpret_cast<const v4f_t*>(plan.partial + (((int64_t)z * plan.parts + part) * heads + bh) * T::PARTIAL) + wave * (T::SUB * T::ACC * 4 * 64) +
+                            (u * T::ACC + n) * 4 * 64 + lane;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const v4f_t x = from[g * 64];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sum[4 * g + i] += x[i];
+        }
+      }
+    }
+    const int64_t at = w.k_first + key + r;
+    if (n < 2 * NK) store_columns(reinterpret_cast<__bf16*>(a.dk) + b * a.dk_sb + hk * a.dk_sh + at * a.dk_ss, sum, a.sm_scale, n, h);
+    else store_columns(reinterpret_cast<__bf16*>(a.dv) + b * a.dv_sb + hk * a.dv_sh + at * a.dv_ss, sum, 1.0f, n - 2 * NK, h);
+  }
 }
 
 // ---------------------------------------------------------------------------------------------------------------------- dQ
@@ -320,52 +445,60 @@ struct RowsTile {
   static constexpr int CODES = CodeTile<NK>::BYTES, ROWS = RowTile<64 * NK>::BYTES, VALUES = RowTile<64 * NV>::BYTES;
   static constexpr int O_ROWS = CODES, O_VALUES = O_ROWS + ROWS, SLOT = O_VALUES + VALUES;
   static constexpr int LOADS = 1 + NK + NV;
+  static constexpr int SUB = bwd_rows_sub(NK), ROWS_WG = 128 * SUB;
 };
 
-// Four waves own 128 consecutive query rows of one head, 32 each, and walk the keys in tiles of 32.
+// Four waves own 128 SUB consecutive query rows of one head, 32 SUB each, and walk the keys in tiles of 32.
 template <int NK, int NV, bool BIASED>
-__device__ __forceinline__ void attn_bwd_rows_body(const AttnBwdArgs& a, const AttnBwdSeqs& seqs, __bf16* __restrict__ dq_out, uint8_t* ring) {
+__device__ __forceinline__ void attn_bwd_rows_body(const AttnBwdArgs& a, const AttnBwdSeqs& seqs, const AttnBwdPlan& plan, int item, __bf16* __restrict__ dq_out, uint8_t* ring) {
   using T = RowsTile<NK, NV>;
   using KT = RowTile<64 * NK>;
   using VT = RowTile<64 * NV>;
-  constexpr int D = 64 * NK, DV = 64 * NV;
+  constexpr int D = 64 * NK, DV = 64 * NV, SUB = T::SUB;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 31, h = lane >> 5;
-  const int z = a.causal && !seqs.n ? (int)(gridDim.z - 1 - blockIdx.z) : (int)blockIdx.z;
-  const AttnBwdBlock w = attn_bwd_block<false>(a, seqs, z);
-  const int hq = blockIdx.x, b = blockIdx.y, hk = hq / (a.Hq / a.Hk);
-  const int shift = w.kn - w.qn, row0 = w.block * 128 + wave * 32;
-  const bool live = row0 < w.qn;
-  const int64_t q_base = ((int64_t)b * a.Hq + hq) * a.Sq + w.q_first + (live ? row0 : 0);
+  const int heads = a.B * a.Hq, bh = head_of(item % heads, heads), zi = item / heads;
+  const AttnBwdBlock w = attn_bwd_block<false>(a, seqs, a.causal && !seqs.n ? plan.q_blocks - 1 - zi : zi);
+  const int hq = bh % a.Hq, b = bh / a.Hq, hk = hq / (a.Hq / a.Hk);
+  const int shift = w.kn - w.qn, row0 = w.block * T::ROWS_WG + wave * 32 * SUB;
+  const int64_t q_base = (int64_t)bh * a.Sq + w.q_first;
   const int64_t k_base = ((int64_t)b * a.Hk + hk) * a.Sk + w.k_first;
 
-  v8i_t qf[NK];
-  int qsc[NK];
-  bf16x8_t gf[4 * NV];
+  v8i_t qf[SUB][NK];
+  int qsc[SUB][NK];
+  bf16x8_t gf[SUB][4 * NV];
+  float lse2[SUB], nd[SUB];
 #pragma unroll
-  for (int s = 0; s < NK; ++s) {
-    qf[s] = frag16(a.q + (q_base + r) * (D / 2) + s * 32 + h * 16);
-    qsc[s] = a.q_scales[(q_base / 32) * 8 + 2 * s + h];
+  for (int u = 0; u < SUB; ++u) {
+    const int first = row0 + 32 * u < w.qn ? row0 + 32 * u : 0;
+    const int64_t row = q_base + first;
+#pragma unroll
+    for (int s = 0; s < NK; ++s) {
+      qf[u][s] = frag16(a.q + (row + r) * (D / 2) + s * 32 + h * 16);
+      qsc[u][s] = a.q_scales[(row / 32) * 8 + 2 * s + h];
+    }
+    const __bf16* g_row = a.dout + b * a.do_sb + hq * a.do_sh + (int64_t)(w.q_first + first + r) * a.do_ss;
+#pragma unroll
+    for (int i = 0; i < 4 * NV; ++i) gf[u][i] = *reinterpret_cast<const bf16x8_t*>(g_row + 16 * i + 8 * h);
+    lse2[u] = a.stats[row * 2 + r];
+    nd[u] = a.stats[row * 2 + 32 + r];
   }
-  const __bf16* g_row = a.dout + b * a.do_sb + hq * a.do_sh + (int64_t)(w.q_first + (live ? row0 : 0) + r) * a.do_ss;
-#pragma unroll
-  for (int i = 0; i < 4 * NV; ++i) gf[i] = *reinterpret_cast<const bf16x8_t*>(g_row + 16 * i + 8 * h);
-  const float lse2 = a.stats[q_base * 2 + r], nd = a.stats[q_base * 2 + 32 + r];
 
-  v16f_t dq[2 * NK];
+  v16f_t dq[SUB][2 * NK];
 #pragma unroll
-  for (int n = 0; n < 2 * NK; ++n)
+  for (int u = 0; u < SUB; ++u)
 #pragma unroll
-    for (int v = 0; v < 16; ++v) dq[n][v] = 0.0f;
+    for (int n = 0; n < 2 * NK; ++n) dq[u][n] = zeros();
 
-  // key tiles that the wave's and the workgroup's rows see
+  // key tiles that the wave's and the workgroup's rows see, and those that all of the wave's rows see
   const int all = w.kn / 32;
-  int own = all, total = all;
+  int own = all, whole = all, total = all;
   if (a.causal) {
-    own = (row0 + shift) / 32 + 1;
-    const int last = w.block * 128 + 96 < w.qn - 32 ? w.block * 128 + 96 : w.qn - 32;
-    total = (last + shift) / 32 + 1;
+    whole = (row0 + shift) / 32;
+    own = whole + SUB < all ? whole + SUB : all;
+    const int end = (w.block + 1) * T::ROWS_WG < w.qn ? (w.block + 1) * T::ROWS_WG : w.qn;
+    total = (end + shift) / 32;
   }
-  if (!live) own = 0;
+  if (row0 >= w.qn) own = 0;
   const float c2 = a.sm_scale * ATTN_RCP_LN2;
   const float slope2 = BIASED && a.alibi ? a.alibi[b * a.alibi_sb + hq * a.alibi_sh] * ATTN_RCP_LN2 : 0.0f;
 
@@ -395,82 +528,110 @@ __device__ __forceinline__ void attn_bwd_rows_body(const AttnBwdArgs& a, const A
   asm volatile("s_barrier" ::: "memory");
 
   const int v_row = VT::row_base(lane), k_col = KT::column_base(lane);
+  auto compute = [&](const uint8_t* at, int t, uint32_t ks0, uint32_t ks1) {
+    v16f_t S[SUB], dp[SUB];
+#pragma unroll
+    for (int u = 0; u < SUB; ++u) S[u] = zeros();
+    static_for<NK>([&](auto sc) {
+      constexpr int s = decltype(sc)::value;
+      const v8i_t kf = CodeTile<NK>::frag(at, lane, s);
+      const int ks = (int)((s < 2 ? ks0 : ks1) >> (8 * h));
+#pragma unroll
+      for (int u = 0; u < SUB; ++u) S[u] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(kf, qf[u][s], S[u], 4, 4, (2 * s) % 4, ks, 0, qsc[u][s]);
+    });
+#pragma unroll
+    for (int u = 0; u < SUB; ++u)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) dp[u][v] = nd[u];
+#pragma unroll
+    for (int kc = 0; kc < 4 * NV; ++kc) {
+      const bf16x8_t vf = VT::row_frag(at + T::O_VALUES, v_row, kc);
+#pragma unroll
+      for (int u = 0; u < SUB; ++u) dp[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, gf[u][kc], dp[u], 0, 0, 0);
+    }
+#pragma unroll
+    for (int u = 0; u < SUB; ++u)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) {
+        float y = __builtin_fmaf(S[u][v], c2, -lse2[u]);
+        const int key = 32 * t + score_row(v, h), row = row0 + 32 * u + r;
+        if constexpr (BIASED) {
+          if (a.bias) y = __builtin_fmaf(a.bias[b * a.bias_sb + hq * a.bias_sh + (row < w.qn ? row : 0) * a.bias_sm + key], ATTN_RCP_LN2, y);
+          y = __builtin_fmaf(-slope2, __builtin_fabsf((float)(row + shift - key)), y);
+        }
+        S[u][v] = y;
+      }
+    if (t >= whole) {
+      asm volatile("" ::: "memory");   // keep this a branch: most tiles skip it
+#pragma unroll
+      for (int u = 0; u < SUB; ++u)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) S[u][v] = 32 * t + score_row(v, h) > row0 + 32 * u + r + shift ? -__builtin_inff() : S[u][v];
+    }
+#pragma unroll
+    for (int u = 0; u < SUB; ++u)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) dp[u][v] *= __builtin_amdgcn_exp2f(S[u][v]);
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      bf16x8_t ds[SUB];
+#pragma unroll
+      for (int u = 0; u < SUB; ++u) ds[u] = pack8(dp[u], c);
+#pragma unroll
+      for (int n = 0; n < 2 * NK; ++n) {
+        const bf16x8_t kf = KT::column_frag(at + T::O_ROWS, k_col, n, c);
+#pragma unroll
+        for (int u = 0; u < SUB; ++u) dq[u][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, ds[u], dq[u][n], 0, 0, 0);
+      }
+    }
+  };
   int slot = 0;
   for (int t = 0; t < total; ++t) {
     const uint8_t* at = ring + slot * T::SLOT;
     const scalar_u32 ksp = scalar_ptr(a.k_scales + (k_base / 32 + t) * 8);
-    uint32_t ks[2] = {ksp[0], NK > 2 ? ksp[1] : 0};
+    const uint32_t ks0 = ksp[0], ks1 = NK > 2 ? ksp[1] : 0;
     if (t + 2 < total) fetch(t + 2, slot == 0 ? BWD_RING - 1 : slot - 1);
-    if (t < own) {
-      v16f_t S, dp;
-#pragma unroll
-      for (int v = 0; v < 16; ++v) S[v] = 0.0f;
-      static_for<NK>([&](auto sc) {
-        constexpr int s = decltype(sc)::value;
-        S = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(CodeTile<NK>::frag(at, lane, s), qf[s], S, 4, 4, (2 * s) % 4, (int)(ks[s >> 1] >> (8 * h)), 0, qsc[s]);
-      });
-#pragma unroll
-      for (int v = 0; v < 16; ++v) dp[v] = nd;
-#pragma unroll
-      for (int kc = 0; kc < 4 * NV; ++kc) dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(VT::row_frag(at + T::O_VALUES, v_row, kc), gf[kc], dp, 0, 0, 0);
-#pragma unroll
-      for (int v = 0; v < 16; ++v) {
-        float y = __builtin_fmaf(S[v], c2, -lse2);
-        if constexpr (BIASED) {
-          const int key = 32 * t + score_row(v, h), row = row0 + r;
-          if (a.bias) y = __builtin_fmaf(a.bias[b * a.bias_sb + hq * a.bias_sh + row * a.bias_sm + key], ATTN_RCP_LN2, y);
-          y = __builtin_fmaf(-slope2, __builtin_fabsf((float)(row + shift - key)), y);
-        }
-        S[v] = y;
-      }
-      if (a.causal && t == own - 1) {
-#pragma unroll
-        for (int v = 0; v < 16; ++v) S[v] = score_row(v, h) > r ? -__builtin_inff() : S[v];
-      }
-#pragma unroll
-      for (int v = 0; v < 16; ++v) dp[v] *= __builtin_amdgcn_exp2f(S[v]);
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const bf16x8_t ds = pack8(dp, c);
-#pragma unroll
-        for (int n = 0; n < 2 * NK; ++n) dq[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(KT::column_frag(at + T::O_ROWS, k_col, n, c), ds, dq[n], 0, 0, 0);
-      }
-    }
+    if (t < own) compute(at, t, ks0, ks1);
     wait(t + 2 < total);
     asm volatile("s_barrier" ::: "memory");
     slot = slot == BWD_RING - 1 ? 0 : slot + 1;
   }
-  if (!live) return;
-  store_rows(dq_out + b * a.dq_sb + hq * a.dq_sh + (int64_t)(w.q_first + row0 + r) * a.dq_ss, dq, a.sm_scale, h);
-}
-
-template <int NK, int NV, bool BIASED>
-__global__ __launch_bounds__(256, 2) void attn_bwd_rows_kernel(AttnBwdArgs a, AttnBwdSeqs seqs) {
-  extern __shared__ __attribute__((aligned(256))) uint8_t ring[];
-  attn_bwd_rows_body<NK, NV, BIASED>(a, seqs, reinterpret_cast<__bf16*>(a.dq), ring);
-}
-
-template <int NK, int NV, bool BIASED>
-int launch_one(const AttnBwdArgs& a, const AttnBwdSeqs& seqs, int q_blocks, int k_blocks, hipStream_t st) {
-  constexpr int keys_lds = BWD_RING * KeysTile<NK, NV>::SLOT, rows_lds = BWD_RING * RowsTile<NK, NV>::SLOT;
-  static LdsLimit keys_limit, rows_limit;
-  if (const int rc = keys_limit.raise((const void*)attn_bwd_keys_kernel<NK, NV, BIASED>, keys_lds, "attention_bwd")) return rc;
-  if (const int rc = rows_limit.raise((const void*)attn_bwd_rows_kernel<NK, NV, BIASED>, rows_lds, "attention_bwd")) return rc;
-  if (a.dk) {
-    hipLaunchKernelGGL((attn_bwd_keys_kernel<NK, NV, BIASED>), dim3((unsigned)a.Hk, (unsigned)a.B, (unsigned)k_blocks), dim3(256), keys_lds, st, a, seqs);
-    if (const int rc = check_launch("attention_bwd")) return rc;
+#pragma unroll
+  for (int u = 0; u < SUB; ++u) {
+    if (row0 + 32 * u >= w.qn) continue;
+    __bf16* row = dq_out + b * a.dq_sb + hq * a.dq_sh + (int64_t)(w.q_first + row0 + 32 * u + r) * a.dq_ss;
+#pragma unroll
+    for (int n = 0; n < 2 * NK; ++n) store_columns(row, dq[u][n], a.sm_scale, n, h);
   }
-  if (a.dq) hipLaunchKernelGGL((attn_bwd_rows_kernel<NK, NV, BIASED>), dim3((unsigned)a.Hq, (unsigned)a.B, (unsigned)q_blocks), dim3(256), rows_lds, st, a, seqs);
+}
+
+template <int NK, int NV, bool BIASED>
+__global__ __launch_bounds__(256, NK > 2 ? 1 : 2) void attn_bwd_kernel(AttnBwdArgs a, AttnBwdSeqs seqs, AttnBwdPlan plan) {
+  extern __shared__ __attribute__((aligned(256))) uint8_t ring[];
+  const int item = (int)blockIdx.x;
+  if (item < plan.key_groups) attn_bwd_keys_body<NK, NV, BIASED>(a, seqs, plan, item, reinterpret_cast<__bf16*>(a.dk), reinterpret_cast<__bf16*>(a.dv), plan.partial, ring);
+  else attn_bwd_rows_body<NK, NV, BIASED>(a, seqs, plan, item - plan.key_groups, reinterpret_cast<__bf16*>(a.dq), ring);
+}
+
+template <int NK, int NV, bool BIASED>
+int launch_one(const AttnBwdArgs& a, const AttnBwdSeqs& seqs, const AttnBwdPlan& plan, hipStream_t st) {
+  constexpr int slot = KeysTile<NK, NV>::SLOT > RowsTile<NK, NV>::SLOT ? KeysTile<NK, NV>::SLOT : RowsTile<NK, NV>::SLOT;
+  static LdsLimit limit;
+  if (const int rc = limit.raise((const void*)attn_bwd_kernel<NK, NV, BIASED>, BWD_RING * slot, "attention_bwd")) return rc;
+  hipLaunchKernelGGL((attn_bwd_kernel<NK, NV, BIASED>), dim3((unsigned)(plan.key_groups + plan.row_groups)), dim3(256), BWD_RING * slot, st, a, seqs, plan);
+  if (const int rc = check_launch("attention_bwd")) return rc;
+  if (!a.dk || plan.parts == 1) return ALTO_MXFP4_OK;
+  hipLaunchKernelGGL((attn_bwd_sum_kernel<NK, NV>), dim3((unsigned)(a.B * a.Hk), (unsigned)plan.k_blocks, KeysTile<NK, NV>::ACC), dim3(256), 0, st, a, seqs, plan);
   return check_launch("attention_bwd");
 }
 
 }  // namespace
 
 template <int NK>
-int launch_attn_bwd(const AttnBwdArgs& a, const AttnBwdSeqs& seqs, int64_t Dv, int q_blocks, int k_blocks, hipStream_t st) {
+int launch_attn_bwd(const AttnBwdArgs& a, const AttnBwdSeqs& seqs, const AttnBwdPlan& plan, int64_t Dv, hipStream_t st) {
   const bool biased = a.bias || a.alibi;
-  if (Dv == 64) return biased ? launch_one<NK, 1, true>(a, seqs, q_blocks, k_blocks, st) : launch_one<NK, 1, false>(a, seqs, q_blocks, k_blocks, st);
-  return biased ? launch_one<NK, 2, true>(a, seqs, q_blocks, k_blocks, st) : launch_one<NK, 2, false>(a, seqs, q_blocks, k_blocks, st);
+  if (Dv == 64) return biased ? launch_one<NK, 1, true>(a, seqs, plan, st) : launch_one<NK, 1, false>(a, seqs, plan, st);
+  return biased ? launch_one<NK, 2, true>(a, seqs, plan, st) : launch_one<NK, 2, false>(a, seqs, plan, st);
 }
 #endif
 

@@ -106,10 +106,44 @@ __global__ __launch_bounds__(256) void attn_bwd_prepare_kernel(const PrepareArgs
   }
 }
 
-struct Workspace {
-  int64_t stats, q_scales, k_scales, q_rows, k_rows, v_rows, total;
+// Cuts of the key blocks' lists: see AttnBwdPlan.  Counted in tiles of one workgroup; what a tile of the dQ part takes is `row_cost` of one of the dK /
+// dV part (matrix cycles of 32 x 32 scores: D / 64 products on FP4, then D and 3 D or 2 D columns' worth in bf16).
+struct Cuts {
+  int parts, chunk;
 };
-Workspace workspace(int64_t B, int64_t Hq, int64_t Hk, int64_t Sq, int64_t Sk, int64_t D, int64_t Dv) {
+int64_t count_tiles(int64_t qn, int64_t kn, int64_t block_keys, int causal, int64_t heads, int64_t& longest) {   // of one key head
+  const int64_t blocks = (kn + block_keys - 1) / block_keys, tiles = qn / 32;
+  int64_t sum = 0;
+  for (int64_t b = 0; b < blocks; ++b) {
+    int64_t first = causal ? (b * block_keys - (kn - qn)) / 32 : 0;
+    first = first < 0 ? 0 : first;
+    const int64_t n = first < tiles ? (tiles - first) * heads : 0;
+    sum += n;
+    longest = n > longest ? n : longest;
+  }
+  return sum;
+}
+Cuts cut(const alto_mxfp4_attention_bwd_t& p) {
+  const int64_t block = bwd_key_block(p.D), heads = p.Hq / p.Hk;
+  int64_t longest = 0, sum = 0;
+  if (p.n_seqs > 0 && p.cu_q && p.cu_k) {
+    for (int i = 0; i < p.n_seqs; ++i) sum += count_tiles(p.cu_q[i + 1] - p.cu_q[i], p.cu_k[i + 1] - p.cu_k[i], block, p.causal, heads, longest);
+  } else {
+    sum = count_tiles(p.Sq, p.Sk_used, block, p.causal, heads, longest);
+  }
+  const int64_t share = sum * p.B * p.Hk / 256;   // tiles of a compute unit
+  int64_t chunk = share < 16 ? 16 : share;
+  int64_t parts = (longest + chunk - 1) / chunk;
+  parts = parts < 1 ? 1 : (parts > 16 ? 16 : parts);
+  if (parts == 16) chunk = (longest + 15) / 16;
+  return {(int)parts, (int)(chunk < (1 << 30) ? chunk : 1 << 30)};
+}
+
+struct Workspace {
+  int64_t stats, q_scales, k_scales, q_rows, k_rows, v_rows, partial, total;
+};
+Workspace workspace(const alto_mxfp4_attention_bwd_t& p, const Cuts& cuts) {
+  const int64_t B = p.B, Hq = p.Hq, Hk = p.Hk, Sq = p.Sq, Sk = p.Sk, D = p.D, Dv = p.Dv;
   Workspace w{};
   int64_t at = 0;
   auto take = [&](int64_t& p, int64_t n) { p = at; at += (n + 255) / 256 * 256; };
@@ -119,6 +153,8 @@ Workspace workspace(int64_t B, int64_t Hq, int64_t Hk, int64_t Sq, int64_t Sk, i
   take(w.q_rows, B * Hq * Sq * D * 2);
   take(w.k_rows, B * Hk * Sk * D * 2);
   take(w.v_rows, B * Hk * Sk * Dv * 2);
+  const int64_t block = bwd_key_block(D), blocks = Sk / block + (p.n_seqs > 0 ? (p.n_seqs < ATTN_MAX_SEQS ? p.n_seqs : ATTN_MAX_SEQS) : 1);   // (at least those of any launch)
+  take(w.partial, cuts.parts > 1 ? B * Hk * blocks * cuts.parts * block * (D + Dv) * 4 : 0);
   w.total = at;
   return w;
 }
@@ -129,7 +165,7 @@ int check_sizes(const alto_mxfp4_attention_bwd_t& p) {
   ALTO_REQUIRE(Sq > 0 && Sq % 32 == 0 && Sk > 0 && Sk % 32 == 0, "attention_bwd: Sq=%lld and Sk=%lld must be positive multiples of 32", Sq, Sk);
   ALTO_REQUIRE(D == 64 || D == 128 || D == 192 || D == 256, "attention_bwd: head dim D=%lld must be 64, 128, 192 or 256", D);
   ALTO_REQUIRE(Dv == 64 || Dv == 128, "attention_bwd: value dim Dv=%lld must be 64 or 128", Dv);
-  ALTO_REQUIRE(B <= 65535 && Hq < (1ll << 31) && Sq <= 65535ll * 128 && Sk <= 65535ll * 128, "attention_bwd: B, Sq / 128 and Sk / 128 must fit a grid dimension");
+  ALTO_REQUIRE(B <= 65535 && Hq < (1ll << 31) && Sq <= 65535ll * 128 && Sk <= 65535ll * 128, "attention_bwd: B, Sq / 128 and Sk / 128 must stay below 65536");
   ALTO_REQUIRE(product_below(1ll << 40, B * Sq, Hq, D > Dv ? D : Dv) && product_below(1ll << 40, B * Sk, Hk, D > Dv ? D : Dv), "attention_bwd: tensor too large");
   ALTO_REQUIRE(product_below(1ll << 31, B, Hq, Sq / 32 + Sk / 32 + 1), "attention_bwd: tensor too large");
   return ALTO_MXFP4_OK;
@@ -167,7 +203,8 @@ static int attention_bwd(const alto_mxfp4_attention_bwd_t& p, hipStream_t st) {
                    p.cu_q[i + 1] - p.cu_q[i], p.cu_k[i + 1] - p.cu_k[i]);
     }
   }
-  const Workspace w = workspace(p.B, p.Hq, p.Hk, p.Sq, p.Sk, p.D, p.Dv);
+  const Cuts cuts = cut(p);
+  const Workspace w = workspace(p, cuts);
   ALTO_REQUIRE(p.workspace_bytes >= w.total && (uintptr_t)p.workspace % 256 == 0, "attention_bwd: the workspace must be 256-byte aligned and hold %lld bytes", (long long)w.total);
   std::unique_ptr<int[]> order;
   if (p.n_seqs > 0) {
@@ -199,18 +236,24 @@ static int attention_bwd(const alto_mxfp4_attention_bwd_t& p, hipStream_t st) {
   a.B = (int)p.B; a.Hq = (int)p.Hq; a.Hk = (int)p.Hk; a.Sq = (int)p.Sq; a.Sk = (int)p.Sk; a.Sk_used = (int)p.Sk_used;
   a.sm_scale = p.sm_scale; a.causal = p.causal ? 1 : 0;
   a.bias = p.bias; a.bias_sb = p.bias_sb; a.bias_sh = p.bias_sh; a.bias_sm = p.bias_sm; a.alibi = p.alibi_slopes; a.alibi_sb = p.alibi_sb; a.alibi_sh = p.alibi_sh;
+  const int row_block = bwd_row_block(p.D), key_block = bwd_key_block(p.D);
   auto go = [&](const AttnBwdSeqs& s, int q_blocks, int k_blocks) {
+    AttnBwdPlan plan{q_blocks, k_blocks, cuts.parts, cuts.chunk, 0, 0, (float*)(ws + w.partial)};
+    const int64_t keys = p.dk ? (p.B * p.Hk * cuts.parts * k_blocks + 7) / 8 * 8 : 0, rows = p.dq ? p.B * p.Hq * q_blocks : 0;
+    ALTO_REQUIRE(keys + rows < (1ll << 31), "attention_bwd: too many workgroups");
+    plan.key_groups = (int)keys;
+    plan.row_groups = (int)rows;
     switch (p.D) {
-      case 64: return launch_attn_bwd<1>(a, s, p.Dv, q_blocks, k_blocks, st);
-      case 128: return launch_attn_bwd<2>(a, s, p.Dv, q_blocks, k_blocks, st);
-      case 192: return launch_attn_bwd<3>(a, s, p.Dv, q_blocks, k_blocks, st);
-      default: return launch_attn_bwd<4>(a, s, p.Dv, q_blocks, k_blocks, st);
+      case 64: return launch_attn_bwd<1>(a, s, plan, p.Dv, st);
+      case 128: return launch_attn_bwd<2>(a, s, plan, p.Dv, st);
+      case 192: return launch_attn_bwd<3>(a, s, plan, p.Dv, st);
+      default: return launch_attn_bwd<4>(a, s, plan, p.Dv, st);
     }
   };
   AttnBwdSeqs s;
   s.n = 0;
   s.zq[0] = s.zk[0] = 0;
-  if (p.n_seqs == 0) return go(s, (int)((p.Sq + 127) / 128), (int)((p.Sk + 127) / 128));
+  if (p.n_seqs == 0) return go(s, (int)((p.Sq + row_block - 1) / row_block), (int)((p.Sk + key_block - 1) / key_block));
   for (int i = 0; i < p.n_seqs; ++i) order[(size_t)i] = i;
   std::sort(order.get(), order.get() + p.n_seqs, [&](int x, int y) {   // longest first
     const int kx = p.cu_k[x + 1] - p.cu_k[x], ky = p.cu_k[y + 1] - p.cu_k[y];
@@ -220,10 +263,9 @@ static int attention_bwd(const alto_mxfp4_attention_bwd_t& p, hipStream_t st) {
     s.n = 0;
     for (; at < p.n_seqs && s.n < ATTN_MAX_SEQS; ++at) {
       const int i = order[(size_t)at], n = s.n, qn = p.cu_q[i + 1] - p.cu_q[i], kn = p.cu_k[i + 1] - p.cu_k[i];
-      if (s.zq[n] + (qn + 127) / 128 > 65535 || s.zk[n] + (kn + 127) / 128 > 65535) break;
       s.q0[n] = p.cu_q[i]; s.qn[n] = qn; s.k0[n] = p.cu_k[i]; s.kn[n] = kn;
-      s.zq[n + 1] = s.zq[n] + (qn + 127) / 128;
-      s.zk[n + 1] = s.zk[n] + (kn + 127) / 128;
+      s.zq[n + 1] = s.zq[n] + (qn + row_block - 1) / row_block;
+      s.zk[n + 1] = s.zk[n] + (kn + key_block - 1) / key_block;
       ++s.n;
     }
     if (const int rc = go(s, s.zq[s.n], s.zk[s.n])) return rc;
@@ -239,7 +281,9 @@ extern "C" int64_t alto_mxfp4_attention_bwd_workspace_bytes(const alto_mxfp4_att
     return ALTO_MXFP4_EINVAL;
   }
   if (const int rc = alto::check_sizes(*p)) return rc;
-  return alto::workspace(p->B, p->Hq, p->Hk, p->Sq, p->Sk, p->D, p->Dv).total;
+  ALTO_REQUIRE(p->Sk_used > 0 && p->Sk_used <= p->Sk && p->n_seqs >= 0, "attention_bwd_workspace_bytes: Sk_used or n_seqs out of range");
+  ALTO_REQUIRE(p->n_seqs == 0 || (p->cu_q && p->cu_k), "attention_bwd_workspace_bytes: packed sequences need their boundaries");
+  return alto::workspace(*p, alto::cut(*p)).total;
 }
 
 extern "C" int alto_mxfp4_attention_bwd(const alto_mxfp4_attention_bwd_t* p, void* stream) {

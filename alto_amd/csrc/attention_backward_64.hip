@@ -3,5 +3,5 @@
 #include "attention_backward.h"
 
 namespace alto {
-template int launch_attn_bwd<1>(const AttnBwdArgs&, const AttnBwdSeqs&, int64_t, int, int, hipStream_t);
+template int launch_attn_bwd<1>(const AttnBwdArgs&, const AttnBwdSeqs&, const AttnBwdPlan&, int64_t, hipStream_t);
 }  // namespace alto

@@ -541,7 +541,7 @@ int alto_mxfp4_attention_rows_per_workgroup(int64_t B, int64_t Hq, int64_t Sq, i
  * with strides that are multiples of 8, the gradients 8-byte aligned with multiples of 4.  Keys from Sk_used on get zero gradients
  * and those of a row with lse = -inf are zero.  n_seqs > 0: packed sequences as in alto_mxfp4_attention_fwd_strided (cu_q / cu_k on the host,
  * no bias).  dq, or dk and dv together, may be NULL: not wanted.  bias: element (b, h, m, n) at b bias_sb + h bias_sh + m bias_sm + n, NULL: none; it gets no gradient.
- * workspace: alto_mxfp4_attention_bwd_workspace_bytes() bytes (sizes alone count), 256-byte aligned, of this call until it is done.
+ * workspace: alto_mxfp4_attention_bwd_workspace_bytes() bytes (sizes, the mask and the boundaries count, pointers do not), 256-byte aligned, of this call until it is done.
  * The results of equal inputs are equal bit for bit.
  */
 typedef struct {

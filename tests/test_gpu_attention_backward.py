@@ -37,7 +37,7 @@ class Operands:
         self.go = rand(B, Hq, Sq, Dv).bfloat16()
 
     def expected(self):
-        return attention_bwd_ref(self.go, *self.values, self.out, self.lse, **self.more)
+        return attention_bwd_ref(self.go.cpu(), *self.values, self.out.cpu(), self.lse, **self.more)
 
     def call(self, m, **kw):
         put = lambda t: None if t is None else t.to(DEV)  # noqa: E731
