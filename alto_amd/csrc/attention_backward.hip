@@ -26,10 +26,10 @@ struct PrepareArgs {
   const float* lse;
   int64_t do_sb, do_sh, do_ss, o_sb, o_sh, o_ss, l_sb, l_sh, l_ss;
   int Hq, Hk, Sq, Sk, D, Dv;
-  int64_t q_tiles;   // B Hq Sq / 32
+  int q_tiles;   // B Hq Sq / 32
   float* stats;
   uint8_t *q_scales, *k_scales;
-  __bf16 *q_rows, *k_rows, *v_rows;
+  v4i_t *q_rows, *k_rows, *v_rows, *g_rows;
 };
 
 __device__ __forceinline__ float e8m0_value(uint32_t e) { return u2f(e ? e << 23 : 0x00400000u); }
@@ -40,30 +40,39 @@ __device__ __forceinline__ v4i_t decode8(uint32_t codes, float scale) {
                __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 2)), __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 3))};
 }
 
-// 32 rows of Q or K: values, and the scale bytes 8 apart
-__device__ __forceinline__ void decode_rows(const uint8_t* codes, const uint8_t* scales, int64_t tile, int D, __bf16* rows, uint8_t* padded) {
+// A tile of Q or K: values, and the scale bytes in the order of the score products
+__device__ __forceinline__ void decode_tile(const uint8_t* codes, const uint8_t* scales, int64_t tile, int D, v4i_t* rows, uint8_t* ordered) {
   const int tid = threadIdx.x, bands = D / 32;
   const uint8_t* s = scales + tile * bands;
-  if (tid < 8) padded[tile * 8 + tid] = tid < bands ? s[tid] : 127;
+  if (tid < 8) {
+    const int c = 2 * (tid & 3) + (tid >> 2);
+    ordered[tile * 8 + tid] = c < bands ? s[c] : 127;
+  }
   const uint32_t* from = reinterpret_cast<const uint32_t*>(codes + tile * 16 * D);
-  v4i_t* to = reinterpret_cast<v4i_t*>(rows + tile * 32 * D);
-  for (int i = tid; i < 4 * D; i += 256) to[i] = decode8(from[i], e8m0_value(s[(i % (D / 8)) >> 2]));
+  v4i_t* to = rows + tile * 4 * D;
+  for (int i = tid; i < 4 * D; i += 256) {
+    const int p = i >> 5, row = (i & 31) ^ ((p & 3) << 2);   // piece i of the tile
+    to[i] = decode8(from[row * (D / 8) + p], e8m0_value(s[p >> 2]));
+  }
 }
 
-// One workgroup: 32 rows of Q with their statistics, or 32 keys of K and V.
+// One workgroup: 32 rows of Q with dO and their statistics, or 32 keys of K and V.
 __global__ __launch_bounds__(256) void attn_bwd_prepare_kernel(const PrepareArgs a) {
-  __shared__ __align__(16) uint32_t turned[4][32 * 20];   // one 32 x 32 block of V a wave, rows of 64 bytes 80 apart
+  __shared__ __align__(16) uint32_t turned[4][32 * 20];   // one 32 x 32 block of V a wave, rows of 64 bytes 80 apart; or a tile of dO
   const int tid = threadIdx.x;
   int64_t tile = blockIdx.x;
   if (tile < a.q_tiles) {
-    decode_rows(a.q, a.qs, tile, a.D, a.q_rows, a.q_scales);
-    const int64_t row = tile * 32 + (tid >> 3), bh = row / a.Sq;
+    decode_tile(a.q, a.qs, tile, a.D, a.q_rows, a.q_scales);
+    v4i_t* const grad = reinterpret_cast<v4i_t*>(turned);
+    const int r = tid >> 3, c = tid & 7;
+    const int64_t row = tile * 32 + r, bh = row / a.Sq;
     const int64_t b = bh / a.Hq, h = bh % a.Hq, i = row % a.Sq;
-    const __bf16* go = a.dout + b * a.do_sb + h * a.do_sh + i * a.do_ss + 8 * (tid & 7);
-    const __bf16* o = a.out + b * a.o_sb + h * a.o_sh + i * a.o_ss + 8 * (tid & 7);
+    const v4i_t* go = reinterpret_cast<const v4i_t*>(a.dout + b * a.do_sb + h * a.do_sh + i * a.do_ss);
+    const v4i_t* o = reinterpret_cast<const v4i_t*>(a.out + b * a.o_sb + h * a.o_sh + i * a.o_ss);
     float d = 0.0f;
-    for (int c = 0; c < a.Dv; c += 64) {
-      const v4i_t x = *reinterpret_cast<const v4i_t*>(go + c), y = *reinterpret_cast<const v4i_t*>(o + c);
+    for (int p = c; p < a.Dv / 8; p += 8) {
+      const v4i_t x = go[p], y = o[p];
+      grad[tile_piece(r, p)] = x;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         d = __builtin_fmaf(bf16_lo((uint32_t)x[e]), bf16_lo((uint32_t)y[e]), d);
@@ -72,16 +81,18 @@ __global__ __launch_bounds__(256) void attn_bwd_prepare_kernel(const PrepareArgs
     }
 #pragma unroll
     for (int m = 1; m < 8; m <<= 1) d += __shfl_xor(d, m, 64);
-    if ((tid & 7) == 0) {
+    if (c == 0) {
       const float l = a.lse[b * a.l_sb + h * a.l_sh + i * a.l_ss];
       const bool none = l == -__builtin_inff();   // a row that sees no key: its probabilities are zeros, whatever the forward left in O
-      a.stats[tile * 64 + (tid >> 3)] = none ? __builtin_inff() : l * ATTN_RCP_LN2;
-      a.stats[tile * 64 + 32 + (tid >> 3)] = none ? 0.0f : -d;
+      a.stats[tile * 64 + r] = none ? __builtin_inff() : l * ATTN_RCP_LN2;
+      a.stats[tile * 64 + 32 + r] = none ? 0.0f : -d;
     }
+    __syncthreads();
+    for (int k = tid; k < 4 * a.Dv; k += 256) a.g_rows[tile * 4 * a.Dv + k] = grad[k];
     return;
   }
   tile -= a.q_tiles;
-  decode_rows(a.k, a.ks, tile, a.D, a.k_rows, a.k_scales);
+  decode_tile(a.k, a.ks, tile, a.D, a.k_rows, a.k_scales);
   const int lane = tid & 63, wave = tid >> 6, bands = a.Sk / 32;
   if (wave * 32 >= a.Dv) return;
   const int64_t bh = tile / bands, band = tile % bands;
@@ -99,10 +110,9 @@ __global__ __launch_bounds__(256) void attn_bwd_prepare_kernel(const PrepareArgs
   }
   wave_lds_order();
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int key = 16 * i + (lane >> 2);
-    const v4i_t v = *reinterpret_cast<const v4i_t*>(turned[wave] + key * 20 + 4 * (lane & 3));
-    *reinterpret_cast<v4i_t*>(a.v_rows + (tile * 32 + key) * a.Dv + wave * 32 + 8 * (lane & 3)) = v;
+  for (int k = 0; k < 2; ++k) {   // the wave's four pieces of the 32 keys
+    const int i = 64 * k + lane, p = i >> 5, key = (i & 31) ^ (p << 2);
+    a.v_rows[tile * 4 * a.Dv + wave * 128 + i] = *reinterpret_cast<const v4i_t*>(turned[wave] + key * 20 + 4 * p);
   }
 }
 
@@ -124,7 +134,7 @@ int64_t count_tiles(int64_t qn, int64_t kn, int64_t block_keys, int causal, int6
   return sum;
 }
 Cuts cut(const alto_mxfp4_attention_bwd_t& p) {
-  const int64_t block = bwd_key_block(p.D), heads = p.Hq / p.Hk;
+  const int64_t block = ATTN_BWD_BLOCK, heads = p.Hq / p.Hk;
   int64_t longest = 0, sum = 0;
   if (p.n_seqs > 0 && p.cu_q && p.cu_k) {
     for (int i = 0; i < p.n_seqs; ++i) sum += count_tiles(p.cu_q[i + 1] - p.cu_q[i], p.cu_k[i + 1] - p.cu_k[i], block, p.causal, heads, longest);
@@ -140,7 +150,7 @@ Cuts cut(const alto_mxfp4_attention_bwd_t& p) {
 }
 
 struct Workspace {
-  int64_t stats, q_scales, k_scales, q_rows, k_rows, v_rows, partial, total;
+  int64_t stats, q_scales, k_scales, q_rows, k_rows, v_rows, g_rows, partial, total;
 };
 Workspace workspace(const alto_mxfp4_attention_bwd_t& p, const Cuts& cuts) {
   const int64_t B = p.B, Hq = p.Hq, Hk = p.Hk, Sq = p.Sq, Sk = p.Sk, D = p.D, Dv = p.Dv;
@@ -153,7 +163,8 @@ Workspace workspace(const alto_mxfp4_attention_bwd_t& p, const Cuts& cuts) {
   take(w.q_rows, B * Hq * Sq * D * 2);
   take(w.k_rows, B * Hk * Sk * D * 2);
   take(w.v_rows, B * Hk * Sk * Dv * 2);
-  const int64_t block = bwd_key_block(D), blocks = Sk / block + (p.n_seqs > 0 ? (p.n_seqs < ATTN_MAX_SEQS ? p.n_seqs : ATTN_MAX_SEQS) : 1);   // (at least those of any launch)
+  take(w.g_rows, B * Hq * Sq * Dv * 2);
+  const int64_t block = ATTN_BWD_BLOCK, blocks = Sk / block + (p.n_seqs > 0 ? (p.n_seqs < ATTN_MAX_SEQS ? p.n_seqs : ATTN_MAX_SEQS) : 1);   // (at least those of any launch)
   take(w.partial, cuts.parts > 1 ? B * Hk * blocks * cuts.parts * block * (D + Dv) * 4 : 0);
   w.total = at;
   return w;
@@ -189,7 +200,6 @@ static int attention_bwd(const alto_mxfp4_attention_bwd_t& p, hipStream_t st) {
     ALTO_REQUIRE(s >= 0 && s < (1ll << 40) && s % 4 == 0, "attention_bwd: strides of the gradients must be non-negative multiples of 4 elements");
   for (const int64_t s : {p.lse_sb, p.lse_sh, p.lse_ss, p.bias_sb, p.bias_sh, p.bias_sm, p.alibi_sb, p.alibi_sh})
     ALTO_REQUIRE(s >= 0 && s < (1ll << 40), "attention_bwd: strides must be non-negative");
-  ALTO_REQUIRE(p.dout_ss < (1ll << 24), "attention_bwd: rows of dout are too far apart");
   ALTO_REQUIRE(p.n_seqs >= 0, "attention_bwd: negative number of sequences");
   ALTO_REQUIRE(p.causal == 0 || p.n_seqs > 0 || p.Sq <= p.Sk_used, "attention_bwd: causal attention needs Sq <= Sk (got %lld > %lld)", (long long)p.Sq, (long long)p.Sk_used);
   if (p.n_seqs > 0) {
@@ -222,25 +232,25 @@ static int attention_bwd(const alto_mxfp4_attention_bwd_t& p, hipStream_t st) {
   r.do_sb = p.dout_sb; r.do_sh = p.dout_sh; r.do_ss = p.dout_ss; r.o_sb = p.out_sb; r.o_sh = p.out_sh; r.o_ss = p.out_ss;
   r.l_sb = p.lse_sb; r.l_sh = p.lse_sh; r.l_ss = p.lse_ss;
   r.Hq = (int)p.Hq; r.Hk = (int)p.Hk; r.Sq = (int)p.Sq; r.Sk = (int)p.Sk; r.D = (int)p.D; r.Dv = (int)p.Dv;
-  r.q_tiles = p.B * p.Hq * (p.Sq / 32);
+  r.q_tiles = (int)(p.B * p.Hq * (p.Sq / 32));
   r.stats = (float*)(ws + w.stats); r.q_scales = ws + w.q_scales; r.k_scales = ws + w.k_scales;
-  r.q_rows = (__bf16*)(ws + w.q_rows); r.k_rows = (__bf16*)(ws + w.k_rows); r.v_rows = (__bf16*)(ws + w.v_rows);
-  hipLaunchKernelGGL(attn_bwd_prepare_kernel, dim3((unsigned)(r.q_tiles + p.B * p.Hk * (p.Sk / 32))), dim3(256), 0, st, r);
+  r.q_rows = (v4i_t*)(ws + w.q_rows); r.k_rows = (v4i_t*)(ws + w.k_rows); r.v_rows = (v4i_t*)(ws + w.v_rows); r.g_rows = (v4i_t*)(ws + w.g_rows);
+  hipLaunchKernelGGL(attn_bwd_prepare_kernel, dim3((unsigned)(r.q_tiles + (int)(p.B * p.Hk * (p.Sk / 32)))), dim3(256), 0, st, r);
   if (const int rc = check_launch("attention_bwd")) return rc;
 
   AttnBwdArgs a{};
-  a.q = r.q; a.k = r.k; a.q_scales = r.q_scales; a.k_scales = r.k_scales; a.q_rows = r.q_rows; a.k_rows = r.k_rows; a.v_rows = r.v_rows; a.stats = r.stats;
-  a.dout = r.dout; a.do_sb = p.dout_sb; a.do_sh = p.dout_sh; a.do_ss = p.dout_ss;
+  a.q = r.q; a.k = r.k; a.q_scales = r.q_scales; a.k_scales = r.k_scales; a.stats = r.stats;
+  a.q_tiles = (const __bf16*)r.q_rows; a.k_tiles = (const __bf16*)r.k_rows; a.v_tiles = (const __bf16*)r.v_rows; a.g_tiles = (const __bf16*)r.g_rows;
   a.dq = p.dq; a.dk = p.dk; a.dv = p.dv;
   a.dq_sb = p.dq_sb; a.dq_sh = p.dq_sh; a.dq_ss = p.dq_ss; a.dk_sb = p.dk_sb; a.dk_sh = p.dk_sh; a.dk_ss = p.dk_ss; a.dv_sb = p.dv_sb; a.dv_sh = p.dv_sh; a.dv_ss = p.dv_ss;
   a.B = (int)p.B; a.Hq = (int)p.Hq; a.Hk = (int)p.Hk; a.Sq = (int)p.Sq; a.Sk = (int)p.Sk; a.Sk_used = (int)p.Sk_used;
   a.sm_scale = p.sm_scale; a.causal = p.causal ? 1 : 0;
   a.bias = p.bias; a.bias_sb = p.bias_sb; a.bias_sh = p.bias_sh; a.bias_sm = p.bias_sm; a.alibi = p.alibi_slopes; a.alibi_sb = p.alibi_sb; a.alibi_sh = p.alibi_sh;
-  const int row_block = bwd_row_block(p.D), key_block = bwd_key_block(p.D);
+  const int row_block = ATTN_BWD_BLOCK, key_block = ATTN_BWD_BLOCK;
   auto go = [&](const AttnBwdSeqs& s, int q_blocks, int k_blocks) {
     AttnBwdPlan plan{q_blocks, k_blocks, cuts.parts, cuts.chunk, 0, 0, (float*)(ws + w.partial)};
     const int64_t keys = p.dk ? (p.B * p.Hk * cuts.parts * k_blocks + 7) / 8 * 8 : 0, rows = p.dq ? p.B * p.Hq * q_blocks : 0;
-    ALTO_REQUIRE(keys + rows < (1ll << 31), "attention_bwd: too many workgroups");
+    ALTO_REQUIRE(2 * keys + rows < (1ll << 31), "attention_bwd: too many workgroups");
     plan.key_groups = (int)keys;
     plan.row_groups = (int)rows;
     switch (p.D) {
