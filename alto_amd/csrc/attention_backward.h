@@ -11,7 +11,7 @@ struct AttnBwdArgs {
   const uint8_t* k;             // codes [B, Hk, Sk, D/2]
   const uint8_t* q_scales;      // workspace: 8 bytes a tile, that of columns 64 s + 32 h .. + 32 at 4 h + s
   const uint8_t* k_scales;
-  const __bf16 *q_tiles, *k_tiles, *v_tiles, *g_tiles;   // workspace: bf16 tiles (RowTile) of Q, K, V as their codes have them, and of dO
+  const __bf16 *k_tiles, *v_tiles, *g_tiles;   // workspace: bf16 tiles (RowTile) of K and V as their codes have them, and of dO
   const float* stats;           // workspace: of every tile of Q, 32 times lse log2(e) (+inf for a row that sees no key), then 32 times -dO . O
   void *dq, *dk, *dv;           // bf16, element (b, h, row, column) at these strides, unit stride along the head dim; dq, or dk and dv, may be NULL: not wanted
   int64_t dq_sb, dq_sh, dq_ss, dk_sb, dk_sh, dk_ss, dv_sb, dv_sh, dv_ss;
@@ -34,19 +34,29 @@ struct AttnBwdSeqs {
   int zq[ATTN_MAX_SEQS + 1], zk[ATTN_MAX_SEQS + 1], q0[ATTN_MAX_SEQS], qn[ATTN_MAX_SEQS], k0[ATTN_MAX_SEQS], kn[ATTN_MAX_SEQS];
 };
 
-// How a launch is cut into workgroups: first those of dK, then those of dV, then those of dQ.  A block of keys walks the tiles of 32 rows that see
-// it, of all query heads on its key head; lists longer than `chunk` are dealt out to up to `parts` workgroups, whose fp32 sums meet in a
-// kernel of their own (`partial`: one set of accumulators for each gradient, part and block).
+// How a launch is cut into workgroups, first those of dK and dV, then those of dQ.  A block of keys walks the tiles of 32 rows that see it, of
+// all query heads on its key head; lists longer than `chunk` are dealt out to up to `parts` workgroups, whose fp32 sums meet in a kernel of
+// their own (`partial`: one set of accumulators for each part and block).
 struct AttnBwdPlan {
   int q_blocks, k_blocks;       // over all sequences
   int parts, chunk;
-  int key_groups, row_groups;   // workgroups of dK (and as many of dV; a multiple of 8), of dQ
+  int key_groups, row_groups;   // workgroups of either kind (those of the keys: a multiple of 8)
   float* partial;
 };
-constexpr int ATTN_BWD_BLOCK = 128;   // keys or query rows of a workgroup
+// Waves of a workgroup, each with 32 keys or query rows; two workgroups share a compute unit where 256 registers a lane do.  (One of 8 waves reads each
+// tile half as often, but its two waves on a SIMD keep step and wait together: 4 x 2048 tokens, 64 / 8 heads of 128, 988 us for 889.)
+constexpr int BWD_WAVES = 4, BWD_BLOCK = 32 * BWD_WAVES;
 
 template <int NK>
 int launch_attn_bwd(const AttnBwdArgs& a, const AttnBwdSeqs& seqs, const AttnBwdPlan& plan, int64_t Dv, hipStream_t st);
+
+__device__ __forceinline__ float e8m0_value(uint32_t e) { return u2f(e ? e << 23 : 0x00400000u); }
+
+// eight codes of one dword as bf16
+__device__ __forceinline__ v4i_t decode8(uint32_t codes, float scale) {
+  return v4i_t{__builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 0)), __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 1)),
+               __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 2)), __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 3))};
+}
 
 #ifdef ALTO_ATTENTION_BACKWARD_KERNELS
 namespace {
@@ -91,6 +101,10 @@ __device__ __forceinline__ void load_piece(__amdgpu_buffer_rsrc_t src, const uin
   __builtin_amdgcn_raw_ptr_buffer_load_lds(src, (__attribute__((address_space(3))) void*)to, 16, lane_offset, offset, 0, 0);
 }
 
+__device__ __forceinline__ void load_dwords(__amdgpu_buffer_rsrc_t src, const uint8_t* to, int lane_offset) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(src, (__attribute__((address_space(3))) void*)to, 4, lane_offset, 0, 0, 0);
+}
+
 // score register v of half h <-> row 8 (v / 4) + 4 h + v % 4 of the tile
 __device__ __forceinline__ int score_row(int v, int h) { return 8 * (v >> 2) + 4 * h + (v & 3); }
 
@@ -128,9 +142,16 @@ __device__ __forceinline__ AttnBwdBlock attn_bwd_block(const AttnBwdArgs& a, con
   return w;
 }
 
-// Eight neighbouring workgroups go to the eight XCDs in turn: each XCD gets a range of consecutive (batch, head) pairs, so that a head's
-// operands come into one L2.
-__device__ __forceinline__ int head_of(int i, int heads) { return heads % 8 == 0 ? (i & 7) * (heads >> 3) + (i >> 3) : i; }
+// Workgroup `item` of heads x each: its (batch, head) pair and its place among that pair's, the longest of all pairs first.  Eight neighbouring
+// workgroups go to the eight XCDs in turn: each XCD gets a range of consecutive pairs, so that a head's operands come into one L2.  (One pair after the
+// other in each XCD misses less in the L2 while it lasts, but ends with the last pair's longest: 4 x 2048 tokens, 64 / 8 heads of 128, 943 us for 889.)
+struct HeadItem {
+  int head, index;
+};
+__device__ __forceinline__ HeadItem head_item(int item, int heads) {
+  const int o = item % heads;
+  return {heads % 8 == 0 ? (o & 7) * (heads >> 3) + (o >> 3) : o, item / heads};
+}
 
 // The list of a block of keys: tiles first .. all of each of the group's heads.
 struct KeyList {
@@ -140,380 +161,321 @@ __device__ __forceinline__ KeyList key_list(const AttnBwdArgs& a, const AttnBwdB
   KeyList l{0, 0, 0, 1};
   const int all = w.qn / 32;
   if (a.causal) {
-    l.first = (w.block * ATTN_BWD_BLOCK - (w.kn - w.qn)) / 32;
+    l.first = (w.block * BWD_BLOCK - (w.kn - w.qn)) / 32;
     l.first = l.first < 0 ? 0 : l.first;
   }
-  l.each = l.first < all && w.block * ATTN_BWD_BLOCK < w.kn ? all - l.first : 0;
+  l.each = l.first < all && w.block * BWD_BLOCK < w.kn ? all - l.first : 0;
   l.total = l.each * (a.Hq / a.Hk);
   l.parts = (l.total + plan.chunk - 1) / plan.chunk;
   l.parts = l.parts < 1 ? 1 : (l.parts > plan.parts ? plan.parts : l.parts);
   return l;
 }
 
-// The three gradients have one shape.  A wave holds 32 rows (of K for dK and dV, of Q for dQ: "its own side") and walks tiles of 32 rows of the
-// other side, from which it takes
-//   the codes, for the scores        S = codes x own codes                 (rows of the tile in registers, its own in lanes),
-//   bf16 rows, for dP                V or dO x own dO or V                 (dK, dQ),
-//   bf16 rows by columns, the factor of its sums   dK += dS^T Q, dQ += dS K, dV += P^T dO.
-enum AttnBwdKind { BWD_DQ, BWD_DK, BWD_DV };
+// What the two kinds of workgroup share.  A wave holds 32 rows of its own side (keys for dK and dV, query rows for dQ) and walks tiles of 32 rows of
+// the other side, from which it takes
+//   the codes, for the scores        S = codes x own codes                  (rows of the tile in registers, its own in lanes),
+//   bf16 rows, for dP                dO x own V, or V x own dO,
+//   bf16 rows by columns, as the factor of its sums   dV += P^T dO and dK += dS^T Q, or dQ += dS K.
+// A tile comes into the LDS by loads without registers in between, 1 KB each, dealt out to the waves.
+template <int NK, int NV>
+struct BwdShape {
+  static constexpr int CODES = CodeTile<NK>::BYTES, ROWS_D = RowTile<64 * NK>::BYTES, ROWS_V = RowTile<64 * NV>::BYTES;
+  static constexpr int ACC = 2 * NK + 2 * NV;                                 // accumulators of 32 keys
+  static constexpr int64_t PARTIAL = (int64_t)BWD_WAVES * ACC * 16 * 64;      // floats of a workgroup's sums
+};
 
-template <int KIND, int NK, int NV>
-struct BwdTile {
-  static constexpr int NA = KIND == BWD_DV ? NV : NK;   // width of the gradient / 64
-  static constexpr int CODES = CodeTile<NK>::BYTES, INNER = KIND == BWD_DV ? 0 : RowTile<64 * NV>::BYTES, FACTOR = RowTile<64 * NA>::BYTES;
-  // three slots of each, four of the statistics
-  static constexpr int O_INNER = 3 * CODES, O_FACTOR = O_INNER + 3 * INNER, O_STATS = O_FACTOR + 3 * FACTOR, LDS = O_STATS + (KIND == BWD_DQ ? 0 : 4 * 256);
-  static constexpr int SCORE_LOADS = 1 + (KIND != BWD_DQ && NK == 4 ? 1 : 0) + (KIND == BWD_DV ? 0 : NV), LOADS = SCORE_LOADS + NA;   // of a wave, each step
-  static constexpr int64_t PARTIAL = (int64_t)4 * 2 * NA * 16 * 64;   // floats of a workgroup's sums
+struct BwdPlace {
+  int tile, at;   // a tile's number in its sequence, and among all of its side
+};
 
-  // The products of a step, in order: those of the scores, then by turns one of dP and one of the sums.
-  static constexpr int NS = NK, NI = KIND == BWD_DV ? 0 : 4 * NV, NF = 4 * NA, PRODUCTS = NS + NI + NF;
-  struct Op {
-    int kind, j;   // 0: S, 1: dP, 2: sums
-  };
-  static constexpr Op op(int i) {
-    if (i < NS) return {0, i};
-    int inner = 0, factor = 0;
-    for (int k = NS;; ++k) {
-      const bool take_inner = inner < NI && (factor == NF || inner * NF <= factor * NI);
-      if (k == i) return take_inner ? Op{1, inner} : Op{2, factor};
-      if (take_inner) ++inner; else ++factor;
+// A tile's codes, statistics (keys) and scales; SMALL loads of each wave, the last waves' repeat the scales
+template <bool KEYS, int NK>
+struct BwdSmall {
+  static constexpr int LOADS = (NK + (KEYS ? 2 : 1) + BWD_WAVES - 1) / BWD_WAVES, CODES = CodeTile<NK>::BYTES;
+  const uint8_t *codes, *scales;
+  const float* stats;
+  __device__ __forceinline__ void operator()(uint8_t* to_codes, uint8_t* to_record, const BwdPlace& p, int wave, int lane) const {
+#pragma unroll
+    for (int l = 0; l < LOADS; ++l) {
+      const int i = BWD_WAVES * l + wave;
+      if (i < NK) load_piece(buffer(codes + (int64_t)p.at * CODES, CODES), to_codes + 1024 * i, CodeTile<NK>::source(64 * i + lane), 0);
+      else if (KEYS && i == NK) load_dwords(buffer(stats + (int64_t)p.at * 64, 256), to_record, lane * 4);
+      else load_dwords(buffer(scales + (int64_t)p.at * 8, 8), to_record + 256, (lane & 1) * 4);
     }
   }
 };
+// Load `l` of a tile of bf16 rows (as many of each wave as it is wide / 64)
+template <int W>
+__device__ __forceinline__ void load_rows(const uint8_t* tiles, uint8_t* to, const BwdPlace& p, int l, int wave, int lane) {
+  const int piece = BWD_WAVES * l + wave;
+  load_piece(buffer(tiles + (int64_t)p.at * RowTile<W>::BYTES, RowTile<W>::BYTES), to + 1024 * piece, lane * 16 + 1024 * wave, 1024 * BWD_WAVES * l);
+}
+template <int N>
+__device__ __forceinline__ void wait_all_but() { __builtin_amdgcn_s_waitcnt(0x0070 | 0x0F00 | (N & 15)); }
 
-template <int KIND, int NK, int NV, bool BIASED>
-__device__ __forceinline__ void attn_bwd_body(const AttnBwdArgs& a, const AttnBwdSeqs& seqs, const AttnBwdPlan& plan, int item, __bf16* __restrict__ grad_out,
-                                              float* __restrict__ partial, uint8_t* lds) {
-  using T = BwdTile<KIND, NK, NV>;
-  using IT = RowTile<64 * NV>;
-  using FT = RowTile<64 * T::NA>;
-  constexpr bool KEYS = KIND != BWD_DQ;
-  constexpr int D = 64 * NK, DV = 64 * NV, NA = T::NA;
+// Which steps' products are issued where, and what lies between them: a fixed order (sched_barrier).  The read of an operand runs AHEAD products
+// before its use, vector work lies behind each product.  Left to itself the compiler puts every read right in front of its product and waits there.
+constexpr int BWD_AHEAD = 2;
+
+// ---------------------------------------------------------------------------------------------------------------- dK and dV
+// Four slots of codes, statistics and scales, three of dO, two of Q's values, which the workgroup makes from the codes one step ahead (a quarter of the
+// bytes to fetch).
+template <int NK, int NV>
+struct KeysLds {
+  using T = BwdShape<NK, NV>;
+  static constexpr int O_V = 4 * T::CODES, O_D = O_V + 3 * T::ROWS_V, O_STATS = O_D + 2 * T::ROWS_D, BYTES = O_STATS + 4 * 512;
+};
+// One step: S and dP of a tile, its probabilities, and its part of the sums.  P is taken from S behind the products of dP, dS behind those of dV.
+template <int NK, int NV, bool BIASED>
+__device__ __forceinline__ void attn_bwd_keys_body(const AttnBwdArgs& a, const AttnBwdSeqs& seqs, const AttnBwdPlan& plan, int item, __bf16* __restrict__ dk_out,
+                                                   __bf16* __restrict__ dv_out, float* __restrict__ partial, uint8_t* lds) {
+  using T = BwdShape<NK, NV>;
+  using VT = RowTile<64 * NV>;
+  using DT = RowTile<64 * NK>;
+  using L = KeysLds<NK, NV>;
+  using Small = BwdSmall<true, NK>;
+  constexpr int D = 64 * NK;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 31, h = lane >> 5;
+  const int heads = a.B * a.Hk, group = a.Hq / a.Hk;
+  const HeadItem it = head_item(item, heads);
+  const int bh = it.head, part = it.index % plan.parts, z = it.index / plan.parts;
+  if (z >= plan.k_blocks) return;   // (the last few of a number that is no multiple of 8)
+  const AttnBwdBlock w = attn_bwd_block<true>(a, seqs, z);
+  const KeyList list = key_list(a, w, plan);
+  if (part >= list.parts) return;
+  const int begin = (int)((int64_t)list.total * part / list.parts), total = (int)((int64_t)list.total * (part + 1) / list.parts) - begin;
+  const int b = bh / a.Hk, hk = bh % a.Hk;
+  const int shift = w.kn - w.qn, key0 = w.block * BWD_BLOCK + wave * 32;
+  const bool live = key0 < w.kn;
+  const int own_tile = bh * (a.Sk / 32) + w.k_first / 32 + (live ? key0 / 32 : 0);
 
-  // ---- what this workgroup works on
-  const int heads = a.B * (KEYS ? a.Hk : a.Hq), bh = head_of(item % heads, heads), group = a.Hq / a.Hk;
-  const int part = KEYS ? (item / heads) % plan.parts : 0;
-  int z = KEYS ? item / heads / plan.parts : item / heads;
-  if (KEYS && z >= plan.k_blocks) return;
-  if (!KEYS && a.causal && !seqs.n) z = plan.q_blocks - 1 - z;
-  const AttnBwdBlock w = attn_bwd_block<KEYS>(a, seqs, z);
-  const int b = bh / (KEYS ? a.Hk : a.Hq), head = bh % (KEYS ? a.Hk : a.Hq);
-  const int shift = w.kn - w.qn, own0 = w.block * ATTN_BWD_BLOCK + wave * 32;   // the wave's first row in its sequence
-  const bool live = own0 < (KEYS ? w.kn : w.qn);
-  int first = 0, last, begin = 0, total, parts = 1;   // the other side's tiles first .. last (of each head), and this workgroup's part of the list
-  if constexpr (KEYS) {
-    const KeyList list = key_list(a, w, plan);
-    if (part >= list.parts) return;
-    parts = list.parts;
-    first = list.first;
-    last = w.qn / 32;
-    begin = (int)((int64_t)list.total * part / parts);
-    total = (int)((int64_t)list.total * (part + 1) / parts) - begin;
-  } else {
-    last = w.kn / 32;
-    if (a.causal) {
-      const int end = (w.block + 1) * ATTN_BWD_BLOCK < w.qn ? (w.block + 1) * ATTN_BWD_BLOCK : w.qn;
-      last = (end + shift) / 32;
-    }
-    total = last;
-  }
-  const int own_tile = (KEYS ? bh * (a.Sk / 32) + w.k_first / 32 : bh * (a.Sq / 32) + w.q_first / 32) + (live ? own0 / 32 : 0);   // among all tiles of its side
-
-  v16f_t acc[2 * NA];
+  v16f_t dk[2 * NK], dv[2 * NV];
 #pragma unroll
-  for (int n = 0; n < 2 * NA; ++n) acc[n] = zeros();
+  for (int n = 0; n < 2 * NK; ++n) dk[n] = zeros();
+#pragma unroll
+  for (int n = 0; n < 2 * NV; ++n) dv[n] = zeros();
 
   if (total > 0) {
-    // ---- its own side, in registers
     v8i_t xf[NK];
-    bf16x8_t yf[KIND == BWD_DV ? 1 : 4 * NV];
-    float lse2 = 0.0f;
-    v16f_t nd;
+    bf16x8_t yf[4 * NV];
 #pragma unroll
-    for (int s = 0; s < NK; ++s) xf[s] = frag16((KEYS ? a.k : a.q) + ((int64_t)own_tile * 32 + r) * (D / 2) + s * 32 + h * 16);
-    const uint32_t x_scales = *reinterpret_cast<const uint32_t*>((KEYS ? a.k_scales : a.q_scales) + (int64_t)own_tile * 8 + 4 * h);
-    if constexpr (KIND != BWD_DV) {
-      const uint8_t* y = reinterpret_cast<const uint8_t*>(KEYS ? a.v_tiles : a.g_tiles) + (int64_t)own_tile * IT::BYTES;
+    for (int s = 0; s < NK; ++s) xf[s] = frag16(a.k + ((int64_t)own_tile * 32 + r) * (D / 2) + s * 32 + h * 16);
+    const uint32_t x_scales = *reinterpret_cast<const uint32_t*>(a.k_scales + (int64_t)own_tile * 8 + 4 * h);
+    const uint8_t* y = reinterpret_cast<const uint8_t*>(a.v_tiles) + (int64_t)own_tile * T::ROWS_V;
 #pragma unroll
-      for (int i = 0; i < 4 * NV; ++i) yf[i] = IT::row_frag(y + IT::row_base(lane, i & 1), i);
-    }
-    if constexpr (!KEYS) {
-      lse2 = a.stats[(int64_t)own_tile * 64 + r];
-      const float x = a.stats[(int64_t)own_tile * 64 + 32 + r];
-#pragma unroll
-      for (int v = 0; v < 16; ++v) nd[v] = x;
-    }
+    for (int i = 0; i < 4 * NV; ++i) yf[i] = VT::row_frag(y + VT::row_base(lane, i & 1), i);
 
-    // ---- the other side's tiles
-    struct Place {
-      int tile, at;   // in its sequence, among all
-    };
-    const int tiles = KEYS ? a.Sq / 32 : a.Sk / 32;   // of a head
-    int next_tile = first, left = total, next_base = KEYS ? (b * a.Hq + head * group) * tiles + w.q_first / 32 : (b * a.Hk + head / group) * tiles + w.k_first / 32;
-    if (KEYS && begin > 0) {
-      next_base += begin / (last - first) * tiles;
-      next_tile += begin % (last - first);
+    const int tiles = a.Sq / 32, last = w.qn / 32;
+    int next_tile = list.first, left = total, next_base = (b * a.Hq + hk * group) * tiles + w.q_first / 32;
+    if (begin > 0) {
+      next_base += begin / list.each * tiles;
+      next_tile += begin % list.each;
     }
     auto next = [&]() {   // (past the end: the last tile again)
-      const Place p{next_tile, next_base + next_tile};
+      const BwdPlace p{next_tile, next_base + next_tile};
       if (--left > 0 && ++next_tile == last) {
-        next_tile = first;
+        next_tile = list.first;
         next_base += tiles;
       }
       return p;
     };
-    const int o_codes = CodeTile<NK>::source(64 * (wave % NK) + lane), o_linear = wave * 1024 + lane * 16;
-    const uint8_t* const codes = KEYS ? a.q : a.k;
-    const uint8_t* const inner = reinterpret_cast<const uint8_t*>(KEYS ? a.g_tiles : a.v_tiles);
-    const uint8_t* const factor = reinterpret_cast<const uint8_t*>(KIND == BWD_DV ? a.g_tiles : (KEYS ? a.q_tiles : a.k_tiles));
-    const uint8_t* const scales = (KEYS ? a.q_scales : a.k_scales) + 4 * h;
-    auto load_scores = [&](const Place& p, int slot, int t) {   // what S and dP need, and the statistics
-      if (!KEYS || NK == 4 || wave < NK) load_piece(buffer(codes + (int64_t)p.at * T::CODES, T::CODES), lds + slot * T::CODES + 1024 * (wave % NK), o_codes, 0);   // (dQ: waves past the last piece repeat one)
-      if constexpr (KEYS) {
-        if (NK == 4 || wave >= NK)
-          __builtin_amdgcn_raw_ptr_buffer_load_lds(buffer(a.stats + (int64_t)p.at * 64, 256), (__attribute__((address_space(3))) void*)(lds + T::O_STATS + (t & 3) * 256), 4, lane * 4, 0, 0, 0);
-      }
-      if constexpr (KIND != BWD_DV) {
-        const __amdgpu_buffer_rsrc_t from = buffer(inner + (int64_t)p.at * T::INNER, T::INNER);
-#pragma unroll
-        for (int j = 0; j < NV; ++j) load_piece(from, lds + T::O_INNER + slot * T::INNER + 1024 * (4 * j + wave), o_linear, 4096 * j);
-      }
-    };
-    auto load_factor = [&](const Place& p, int slot) {
-      const __amdgpu_buffer_rsrc_t from = buffer(factor + (int64_t)p.at * T::FACTOR, T::FACTOR);
-#pragma unroll
-      for (int j = 0; j < NA; ++j) load_piece(from, lds + T::O_FACTOR + slot * T::FACTOR + 1024 * (4 * j + wave), o_linear, 4096 * j);
-    };
-    auto scales_of = [&](const Place& p) { return *reinterpret_cast<const uint32_t*>(scales + (int64_t)p.at * 8); };
-    auto wait_all_but = [](auto n) { __builtin_amdgcn_s_waitcnt(0x0070 | 0x0F00 | (decltype(n)::value & 15)); };
-
-    const int code_base = lane * 16, row_base[2] = {IT::row_base(lane, 0), IT::row_base(lane, 1)}, column_base[2] = {FT::column_base(lane, 0), FT::column_base(lane, 1)};
+    const Small small{a.q, a.q_scales, a.stats};
+    const uint8_t* const grads = reinterpret_cast<const uint8_t*>(a.g_tiles);
+    const int code_base = lane * 16, row_base[2] = {VT::row_base(lane, 0), VT::row_base(lane, 1)}, column_base[2] = {VT::column_base(lane, 0), VT::column_base(lane, 1)};
     const float c2 = a.sm_scale * ATTN_RCP_LN2;
-
-    // Which rows of the tile the lane sees, in the bits of the packed pairs: most tiles are seen whole (state 2), the diagonal's in part (1), a tile
-    // before its diagonal not at all (0: another wave of the workgroup needs it).
-    uint32_t seen[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) seen[i] = ~0u;
-    int state = 2;
-    auto look = [&](const Place& p) {
-      if (!a.causal) return;
-      const int away = KEYS ? 32 * p.tile + shift - own0 : own0 + shift - 32 * p.tile;   // a multiple of 32
-      const int now = away > 0 ? 2 : (away == 0 ? 1 : 0);
-      if (now == state) return;
-      state = now;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int x = score_row(2 * i, h);   // the pair's first row; the second is the next one
-        const bool lo = KEYS ? x >= r : x <= r, hi = KEYS ? x + 1 >= r : x + 1 <= r;
-        seen[i] = now == 2 ? ~0u : (now == 1 ? (lo ? 0xFFFFu : 0u) | (hi ? 0xFFFF0000u : 0u) : 0u);
-      }
+    // Eight columns of one row of tile `i`'s values, from its codes: dword `j` of row tid % 32, j = tid / 32 + 8 u
+    uint32_t eight = 0;
+    float eight_scale = 0.0f;
+    auto read_codes = [&](int i, int u) {
+      const int row = tid & 31, j = (tid >> 5) + 8 * u, block = j >> 2;
+      eight = *reinterpret_cast<const uint32_t*>(lds + (i & 3) * T::CODES + (block * 32 + row) * 16 + 4 * (j & 3));
+      const uint32_t e = (reinterpret_cast<const uint32_t*>(lds + L::O_STATS + (i & 3) * 512 + 256)[block & 1] >> (8 * (block >> 1))) & 0xFFu;
+      eight_scale = e8m0_value(e);
     };
-
-    // ---- Three stages in one step: S and dP of tile t + 1 and the sums' product with tile t - 1 on the matrix pipe, the probabilities of tile t
-    // on the vector pipe.  Loads go out two steps before they are used: a step starts those of the scores of t + 3 and the factor of t + 1, and
-    // ends with a wait for everything that earlier steps started.  The products are issued in a fixed order (sched_barrier): the read of
-    // an operand AHEAD products before its use, a sixteenth of the vector work behind each.  Left to itself the compiler puts every read right
-    // in front of its product and waits there.
-    constexpr int AHEAD = 4, HALVES = 16;
-    struct Scores {
-      v16f_t S, dp;
+    auto write_values = [&](int i, int u) {
+      const int row = tid & 31, j = (tid >> 5) + 8 * u;
+      *reinterpret_cast<v4i_t*>(lds + L::O_D + (i & 1) * T::ROWS_D + tile_piece(row, j) * 16) = decode8(eight, eight_scale);
     };
-    // (RUN: the first step only has scores to compute)
-    auto step = [&](auto run, int t, int slot, const Place& p, uint32_t sc, const Scores& from, const bf16x8_t (&f)[2], Scores& to, bf16x8_t (&f_next)[2]) {
-      constexpr bool RUN = decltype(run)::value;
-      const int after = slot == 2 ? 0 : slot + 1, before = slot == 0 ? 2 : slot - 1;
-      const uint8_t* const at_codes = lds + after * T::CODES + code_base;
-      const uint8_t* at_rows[2];
-      const uint8_t* at_columns[2];
+    auto load_small = [&](const BwdPlace& p, int i) { small(lds + (i & 3) * T::CODES, lds + L::O_STATS + (i & 3) * 512, p, wave, lane); };
+
+    BwdPlace p0 = next(), p1 = next(), p2 = next();
+    load_small(p0, 0);
+    load_small(p1, 1);
+#pragma unroll
+    for (int l = 0; l < NV; ++l) load_rows<64 * NV>(grads, lds + L::O_V, p0, l, wave, lane);
+#pragma unroll
+    for (int l = 0; l < NV; ++l) load_rows<64 * NV>(grads, lds + L::O_V + T::ROWS_V, p1, l, wave, lane);
+    load_small(p2, 2);
+    wait_all_but<NV + Small::LOADS>();
+    asm volatile("s_barrier" ::: "memory");
+#pragma unroll
+    for (int u = 0; u < NK; ++u) {
+      read_codes(0, u);
+      write_values(0, u);
+    }
+    __builtin_amdgcn_s_waitcnt(0xC07F);   // lgkmcnt(0)
+    asm volatile("s_barrier" ::: "memory");
+
+    constexpr int NS = NK, NI = 4 * NV, NF = 4 * NV, NG = 4 * NK, N = NS + NI + NF + NG, AHEAD = BWD_AHEAD;
+    int slot = 0;
+    for (int t = 0; t < total; ++t) {
+      const int two_on = slot == 0 ? 2 : slot - 1;
+      const BwdPlace p3 = next();
+      const uint8_t* const at_codes = lds + (t & 3) * T::CODES + code_base;
+      const uint8_t *at_rows[2], *at_v[2], *at_d[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        at_rows[i] = lds + T::O_INNER + after * T::INNER + row_base[i];
-        at_columns[i] = lds + T::O_FACTOR + before * T::FACTOR + column_base[i];
+        at_rows[i] = lds + L::O_V + slot * T::ROWS_V + row_base[i];
+        at_v[i] = lds + L::O_V + slot * T::ROWS_V + column_base[i];
+        at_d[i] = lds + L::O_D + (t & 1) * T::ROWS_D + column_base[i];
       }
-      const float* const stats = reinterpret_cast<const float*>(lds + T::O_STATS + (t & 3) * 256) + 4 * h;
-      const float* const stats_next = reinterpret_cast<const float*>(lds + T::O_STATS + ((t + 1) & 3) * 256) + 4 * h;
-      constexpr int N = RUN ? T::PRODUCTS : T::NS + T::NI;
-      auto op = [](int i) constexpr { return RUN ? T::op(i) : typename T::Op{i < T::NS ? 0 : 1, i < T::NS ? i : i - T::NS}; };
+      const float* const stats = reinterpret_cast<const float*>(lds + L::O_STATS + (t & 3) * 512) + 4 * h;
+      v16f_t S, dp;
+      v4f_t l4[2];
       bf16x8_t frag[AHEAD + 1];
+      uint32_t pk[8], dsk[8];
       auto read = [&](auto ic) {
         constexpr int i = decltype(ic)::value;
         if constexpr (i < N) {
-          constexpr typename T::Op o = op(i);
           bf16x8_t& x = frag[i % (AHEAD + 1)];
-          if constexpr (o.kind == 0) x = *reinterpret_cast<const bf16x8_t*>(at_codes + o.j * 1024);
-          else if constexpr (o.kind == 1) x = IT::row_frag(at_rows[o.j & 1], o.j);
-          else x = FT::column_frag(at_columns[0], at_columns[1], o.j % (2 * NA), o.j / (2 * NA));
+          if constexpr (i < NS) x = *reinterpret_cast<const bf16x8_t*>(at_codes + i * 1024);
+          else if constexpr (i < NS + NI) x = VT::row_frag(at_rows[(i - NS) & 1], i - NS);
+          else if constexpr (i < NS + NI + NF) x = VT::column_frag(at_v[0], at_v[1], (i - NS - NI) % (2 * NV), (i - NS - NI) / (2 * NV));
+          else x = DT::column_frag(at_d[0], at_d[1], (i - NS - NI - NF) % (2 * NK), (i - NS - NI - NF) / (2 * NK));
         }
       };
+      auto four = [](const uint32_t (&o)[8], int c) { return __builtin_bit_cast(bf16x8_t, v4i_t{(int)o[4 * c], (int)o[4 * c + 1], (int)o[4 * c + 2], (int)o[4 * c + 3]}); };
+      const uint32_t sc = reinterpret_cast<const uint32_t*>(lds + L::O_STATS + (t & 3) * 512 + 256)[h];
       auto product = [&](auto ic) {
         constexpr int i = decltype(ic)::value;
-        constexpr typename T::Op o = op(i);
         const bf16x8_t& x = frag[i % (AHEAD + 1)];
-        if constexpr (o.kind == 0) {
+        if constexpr (i < NS) {
           const v4i_t q = __builtin_bit_cast(v4i_t, x);
-          to.S = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(v8i_t{q[0], q[1], q[2], q[3], 0, 0, 0, 0}, xf[o.j], o.j == 0 ? zeros() : to.S, 4, 4, o.j, (int)sc, o.j, (int)x_scales);
-        } else if constexpr (o.kind == 1) {
-          if constexpr (!KEYS && o.j == 0) to.dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, yf[o.j], nd, 0, 0, 0);
-          else to.dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, yf[o.j], to.dp, 0, 0, 0);
+          S = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(v8i_t{q[0], q[1], q[2], q[3], 0, 0, 0, 0}, xf[i], i == 0 ? zeros() : S, 4, 4, i, (int)sc, i, (int)x_scales);
+        } else if constexpr (i < NS + NI) {
+          dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, yf[i - NS], dp, 0, 0, 0);
+        } else if constexpr (i < NS + NI + NF) {
+          constexpr int j = i - NS - NI, n = j % (2 * NV), c = j / (2 * NV);
+          dv[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, four(pk, c), dv[n], 0, 0, 0);
         } else {
-          acc[o.j % (2 * NA)] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, f[o.j / (2 * NA)], acc[o.j % (2 * NA)], 0, 0, 0);
+          constexpr int j = i - NS - NI - NF, n = j % (2 * NK), c = j / (2 * NK);
+          dk[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, four(dsk, c), dk[n], 0, 0, 0);
         }
       };
-      // P or dS of tile t, a pair of rows at a time, in two halves
-      v4f_t l4[2];
-      float e[8][2];
-      uint32_t out[8];
-      auto read_stats = [&](int g) {
-        if constexpr (KEYS) l4[g & 1] = *reinterpret_cast<const v4f_t*>(stats + 8 * g);
-      };
-      auto half = [&](auto uc) {
-        constexpr int u = decltype(uc)::value, i = u >> 1;
-        if constexpr ((u & 1) == 0) {
+      auto read_stats = [&](int g) { l4[g & 1] = *reinterpret_cast<const v4f_t*>(stats + 8 * g); };
+      auto probability = [&](int i) {   // of the pair of rows i
 #pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const int v = 2 * i + k;
-            float y = __builtin_fmaf(from.S[v], c2, -(KEYS ? l4[(v >> 2) & 1][v & 3] : lse2));
-            if constexpr (BIASED) {
-              const int there = 32 * p.tile + score_row(v, h), here = live ? own0 + r : 0;
-              const int row = KEYS ? there : here, key = KEYS ? here : there;
-              const int64_t hq = KEYS ? p.at / tiles - b * a.Hq : head;
-              if (a.bias) y = __builtin_fmaf(a.bias[b * a.bias_sb + hq * a.bias_sh + row * a.bias_sm + key], ATTN_RCP_LN2, y);
-              if (a.alibi) y = __builtin_fmaf(-a.alibi[b * a.alibi_sb + hq * a.alibi_sh] * ATTN_RCP_LN2, __builtin_fabsf((float)(row + shift - key)), y);
-            }
-            e[i][k] = __builtin_amdgcn_exp2f(y);
-          }
-          if constexpr (KEYS && (i & 1) == 1 && i / 2 + 2 < 4) read_stats(i / 2 + 2);   // (the group's last use is behind us)
-        } else {
-          if constexpr (KIND != BWD_DV) {
-            e[i][0] *= from.dp[2 * i];
-            e[i][1] *= from.dp[2 * i + 1];
-          }
-          out[i] = pack_bf16x2(e[i][0], e[i][1]) & seen[i];
-          asm volatile("" : "+v"(out[i]));   // (here: otherwise it is moved behind the step, to where it is used)
+        for (int k = 0; k < 2; ++k) {
+          const int v = 2 * i + k;
+          float x = BIASED ? S[v] - l4[(v >> 2) & 1][v & 3] : __builtin_fmaf(S[v], c2, -l4[(v >> 2) & 1][v & 3]);
+          S[v] = __builtin_amdgcn_exp2f(x);
         }
+        if ((i & 1) == 1 && i / 2 + 2 < 4) read_stats(i / 2 + 2);   // (the group's last use is behind us)
       };
+      auto pack_p = [&](int i) { pk[i] = pack_bf16x2(S[2 * i], S[2 * i + 1]); };
+      auto pack_ds = [&](int i) { dsk[i] = pack_bf16x2(S[2 * i] * dp[2 * i], S[2 * i + 1] * dp[2 * i + 1]); };
       __builtin_amdgcn_sched_barrier(0);
-      if constexpr (RUN) {
-        read_stats(0);
-        read_stats(1);
-      }
-      if constexpr (KIND == BWD_DK) {
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const v4f_t x = *reinterpret_cast<const v4f_t*>(stats_next + 32 + 8 * g);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) to.dp[4 * g + i] = x[i];
-        }
-      }
       static_for<AHEAD>([&](auto ic) { read(ic); });
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const v4f_t x = *reinterpret_cast<const v4f_t*>(stats + 32 + 8 * g);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) dp[4 * g + i] = x[i];
+      }
+      read_stats(0);
+      read_stats(1);
       __builtin_amdgcn_sched_barrier(0);
       static_for<N>([&](auto ic) {
         constexpr int i = decltype(ic)::value;
         read(std::integral_constant<int, i + AHEAD>{});
         product(ic);
-        if constexpr (RUN) {
-          constexpr int u0 = HALVES * i / N, u1 = HALVES * (i + 1) / N;
-          static_for<u1 - u0>([&](auto uc) { half(std::integral_constant<int, u0 + decltype(uc)::value>{}); });
+        if constexpr (i == NS - 1) {
+          if constexpr (BIASED) {   // scores into the base-2 domain with their additive terms
+#pragma unroll
+            for (int v = 0; v < 16; ++v) {
+              const int row = 32 * p0.tile + score_row(v, h), key = live ? key0 + r : 0;
+              const int64_t hq = p0.at / tiles - b * a.Hq;
+              float x = S[v] * c2;
+              if (a.bias) x = __builtin_fmaf(a.bias[b * a.bias_sb + hq * a.bias_sh + row * a.bias_sm + key], ATTN_RCP_LN2, x);
+              if (a.alibi) x = __builtin_fmaf(-a.alibi[b * a.alibi_sb + hq * a.alibi_sh] * ATTN_RCP_LN2, __builtin_fabsf((float)(row + shift - key)), x);
+              S[v] = x;
+            }
+          }
+          if (a.causal && 32 * p0.tile + shift <= key0) {   // the diagonal's tile, or one before it, that another wave of the workgroup needs
+            asm volatile("" ::: "memory");   // keep this a branch: most tiles skip it
+            const int hidden = key0 + r - 32 * p0.tile - shift;
+#pragma unroll
+            for (int v = 0; v < 16; ++v) S[v] = score_row(v, h) < hidden ? -__builtin_inff() : S[v];
+          }
+        }
+        // vector work
+        if constexpr (i >= NS && i < NS + NI) {
+          constexpr int j = i - NS, u0 = 8 * j / NI, u1 = 8 * (j + 1) / NI;
+#pragma unroll
+          for (int u = u0; u < u1; ++u) probability(u);
+#pragma unroll
+          for (int u = u0; u < u1; ++u)
+            if (u > 0) pack_p(u - 1);
+          if constexpr (j == NI - 1) pack_p(7);
+        }
+        if constexpr (i >= NS + NI && i < NS + NI + NF) {
+          constexpr int j = i - NS - NI, first = NF / 4, u0 = j < first ? 0 : 8 * (j - first) / (NF - first), u1 = j < first ? 0 : 8 * (j - first + 1) / (NF - first);
+#pragma unroll
+          for (int u = u0; u < u1; ++u) pack_ds(u);
+        }
+        if constexpr (i >= NS + NI + NF) {   // the loads for later tiles, the next one's values
+          constexpr int j = i - NS - NI - NF;
+          if constexpr (j == 0) load_small(p3, t + 3);
+          if constexpr (j >= 1 && j <= NV) load_rows<64 * NV>(grads, lds + L::O_V + two_on * T::ROWS_V, p2, j - 1, wave, lane);
+          if constexpr (j % 4 == 0) read_codes(t + 1, j / 4);
+          if constexpr (j % 4 == 3) write_values(t + 1, j / 4);
         }
         __builtin_amdgcn_sched_barrier(0);
       });
-      if constexpr (RUN) {
-#pragma unroll
-        for (int c = 0; c < 2; ++c) f_next[c] = __builtin_bit_cast(bf16x8_t, v4i_t{(int)out[4 * c], (int)out[4 * c + 1], (int)out[4 * c + 2], (int)out[4 * c + 3]});
-      }
-    };
-
-    Place p0 = next();
-    load_scores(p0, 0, 0);
-    load_factor(p0, 0);
-    load_factor(p0, 2);   // (what the first step multiplies with zeros)
-    Place p1 = next();
-    load_scores(p1, 1, 1);
-    Place p2 = next();
-    uint32_t sc = scales_of(p0), sc1 = scales_of(p1);
-    load_scores(p2, 2, 2);
-    wait_all_but(std::integral_constant<int, T::SCORE_LOADS>{});
-    asm volatile("s_barrier" ::: "memory");
-    Scores x, y;
-    bf16x8_t f[2], g[2];
-    f[0] = f[1] = __builtin_bit_cast(bf16x8_t, v4i_t{0, 0, 0, 0});
-    step(std::false_type{}, -1, 2, p0, sc, x, f, x, f);
-    int slot = 0;   // of tile t
-    auto whole_step = [&](int t, const Scores& from, const bf16x8_t (&f_now)[2], Scores& to, bf16x8_t (&f_next)[2]) {
-      const int after = slot == 2 ? 0 : slot + 1;
-      sc = sc1;
-      sc1 = scales_of(p2);
-      const Place p3 = next();
-      load_scores(p3, slot, t + 3);
-      load_factor(p1, after);
-      look(p0);
-      step(std::true_type{}, t, slot, p0, sc, from, f_now, to, f_next);
       p0 = p1;
       p1 = p2;
       p2 = p3;
-      slot = after;
-      wait_all_but(std::integral_constant<int, T::LOADS>{});
+      slot = slot == 2 ? 0 : slot + 1;
+      __builtin_amdgcn_s_waitcnt(0x0070 | ((Small::LOADS + NV) & 15));   // all but this step's loads, and lgkmcnt(0): the values are written
       asm volatile("s_barrier" ::: "memory");
-    };
-    auto final_sums = [&](const bf16x8_t (&f_now)[2]) {
-      const uint8_t* at = lds + T::O_FACTOR + (slot == 0 ? 2 : slot - 1) * T::FACTOR;
-#pragma unroll
-      for (int c = 0; c < 2; ++c)
-#pragma unroll
-        for (int n = 0; n < 2 * NA; ++n) acc[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(FT::column_frag(at + column_base[0], at + column_base[1], n, c), f_now[c], acc[n], 0, 0, 0);
-    };
-    int t = 0;
-    for (; t + 1 < total; t += 2) {
-      whole_step(t, x, f, y, g);
-      whole_step(t + 1, y, g, x, f);
     }
-    if (t < total) {
-      whole_step(t, x, f, y, g);
-      f[0] = g[0];
-      f[1] = g[1];
-    }
-    final_sums(f);
-    wait_all_but(std::integral_constant<int, 0>{});   // (the last loads into the LDS, which nobody reads, before it is given back)
+    wait_all_but<0>();   // (the last loads into the LDS, which nobody reads, before it is given back)
   }
 
-  // ---- results
-  if (KEYS && parts > 1) {
-    v4f_t* to = reinterpret_cast<v4f_t*>(partial + (((int64_t)z * plan.parts + part) * heads + bh) * T::PARTIAL) + wave * (2 * NA * 4 * 64) + lane;
+  if (list.parts > 1) {
+    v4f_t* to = reinterpret_cast<v4f_t*>(partial + (((int64_t)z * plan.parts + part) * heads + bh) * T::PARTIAL) + wave * (T::ACC * 4 * 64) + lane;
 #pragma unroll
-    for (int n = 0; n < 2 * NA; ++n)
+    for (int n = 0; n < T::ACC; ++n)
 #pragma unroll
-      for (int g = 0; g < 4; ++g) to[(n * 4 + g) * 64] = v4f_t{acc[n][4 * g], acc[n][4 * g + 1], acc[n][4 * g + 2], acc[n][4 * g + 3]};
+      for (int g = 0; g < 4; ++g) {
+        const v16f_t& x = n < 2 * NK ? dk[n < 2 * NK ? n : 0] : dv[n < 2 * NK ? 0 : n - 2 * NK];
+        to[(n * 4 + g) * 64] = v4f_t{x[4 * g], x[4 * g + 1], x[4 * g + 2], x[4 * g + 3]};
+      }
     return;
   }
-  if (own0 >= (KEYS ? (seqs.n ? w.kn : a.Sk) : w.qn)) return;
-  const int64_t sb = KIND == BWD_DQ ? a.dq_sb : (KIND == BWD_DK ? a.dk_sb : a.dv_sb), sh = KIND == BWD_DQ ? a.dq_sh : (KIND == BWD_DK ? a.dk_sh : a.dv_sh),
-                ss = KIND == BWD_DQ ? a.dq_ss : (KIND == BWD_DK ? a.dk_ss : a.dv_ss);
-  __bf16* row = grad_out + b * sb + head * sh + (int64_t)((KEYS ? w.k_first : w.q_first) + own0 + r) * ss;
+  if (key0 >= (seqs.n ? w.kn : a.Sk)) return;
+  const int64_t at = w.k_first + key0 + r;   // (keys behind the used ones: zeros)
 #pragma unroll
-  for (int n = 0; n < 2 * NA; ++n) store_columns(row, live ? acc[n] : zeros(), KIND == BWD_DV ? 1.0f : a.sm_scale, n, h);   // (keys behind the used ones: zeros)
+  for (int n = 0; n < 2 * NK; ++n) store_columns(dk_out + b * a.dk_sb + hk * a.dk_sh + at * a.dk_ss, live ? dk[n] : zeros(), a.sm_scale, n, h);
+#pragma unroll
+  for (int n = 0; n < 2 * NV; ++n) store_columns(dv_out + b * a.dv_sb + hk * a.dv_sh + at * a.dv_ss, live ? dv[n] : zeros(), 1.0f, n, h);
 }
 
 // Sums of the parts, in their order.  Grid: (heads, key blocks, blocks of 32 columns of dK, then of dV).
 template <int NK, int NV>
-__global__ __launch_bounds__(256) void attn_bwd_sum_kernel(AttnBwdArgs a, AttnBwdSeqs seqs, AttnBwdPlan plan) {
+__global__ __launch_bounds__(64 * BWD_WAVES) void attn_bwd_sum_kernel(AttnBwdArgs a, AttnBwdSeqs seqs, AttnBwdPlan plan) {
+  using T = BwdShape<NK, NV>;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 31, h = lane >> 5;
-  const int heads = a.B * a.Hk, bh = blockIdx.x, z = blockIdx.y;
-  const bool is_k = blockIdx.z < 2 * NK;
-  const int n = is_k ? blockIdx.z : blockIdx.z - 2 * NK, width = is_k ? 2 * NK : 2 * NV;
+  const int heads = a.B * a.Hk, bh = blockIdx.x, z = blockIdx.y, n = blockIdx.z;
   const AttnBwdBlock w = attn_bwd_block<true>(a, seqs, z);
   const KeyList list = key_list(a, w, plan);
-  const int key = w.block * ATTN_BWD_BLOCK + wave * 32;
+  const int key = w.block * BWD_BLOCK + wave * 32;
   if (list.parts == 1 || key >= (seqs.n ? w.kn : a.Sk)) return;
   const int hk = bh % a.Hk, b = bh / a.Hk;
-  const int64_t one = is_k ? BwdTile<BWD_DK, NK, NV>::PARTIAL : BwdTile<BWD_DV, NK, NV>::PARTIAL;
-  const float* sums = plan.partial + (is_k ? 0 : (int64_t)plan.k_blocks * plan.parts * heads * BwdTile<BWD_DK, NK, NV>::PARTIAL);
   v16f_t sum = zeros();
   if (key < w.kn) {
     for (int part = 0; part < list.parts; ++part) {
-      const v4f_t* from = reinterpret_cast<const v4f_t*>(sums + (((int64_t)z * plan.parts + part) * heads + bh) * one) + (wave * width + n) * 4 * 64 + lane;
+      const v4f_t* from = reinterpret_cast<const v4f_t*>(plan.partial + (((int64_t)z * plan.parts + part) * heads + bh) * T::PARTIAL) + (wave * T::ACC + n) * 4 * 64 + lane;
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         const v4f_t x = from[g * 64];
@@ -523,30 +485,251 @@ __global__ __launch_bounds__(256) void attn_bwd_sum_kernel(AttnBwdArgs a, AttnBw
     }
   }
   const int64_t at = w.k_first + key + r;
-  if (is_k) store_columns(reinterpret_cast<__bf16*>(a.dk) + b * a.dk_sb + hk * a.dk_sh + at * a.dk_ss, sum, a.sm_scale, n, h);
-  else store_columns(reinterpret_cast<__bf16*>(a.dv) + b * a.dv_sb + hk * a.dv_sh + at * a.dv_ss, sum, 1.0f, n, h);
+  if (n < 2 * NK) store_columns(reinterpret_cast<__bf16*>(a.dk) + b * a.dk_sb + hk * a.dk_sh + at * a.dk_ss, sum, a.sm_scale, n, h);
+  else store_columns(reinterpret_cast<__bf16*>(a.dv) + b * a.dv_sb + hk * a.dv_sh + at * a.dv_ss, sum, 1.0f, n - 2 * NK, h);
+}
+
+// ---------------------------------------------------------------------------------------------------------------------- dQ
+template <int NK, int NV>
+struct RowsLds {   // three slots of codes, V and K, four of scales
+  using T = BwdShape<NK, NV>;
+  static constexpr int O_V = 3 * T::CODES, O_D = O_V + 3 * T::ROWS_V, O_STATS = O_D + 3 * T::ROWS_D, BYTES = O_STATS + 4 * 512;
+};
+// Three stages in one step: S and dP of tile t + 1 and the sums' product with tile t - 1 on the matrix pipe, dS of tile t on the vector pipe.
+template <int NK, int NV, bool BIASED>
+__device__ __forceinline__ void attn_bwd_rows_body(const AttnBwdArgs& a, const AttnBwdSeqs& seqs, const AttnBwdPlan& plan, int item, __bf16* __restrict__ dq_out, uint8_t* lds) {
+  using T = BwdShape<NK, NV>;
+  using VT = RowTile<64 * NV>;
+  using DT = RowTile<64 * NK>;
+  constexpr int D = 64 * NK;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 31, h = lane >> 5;
+  using L = RowsLds<NK, NV>;
+  using Small = BwdSmall<false, NK>;
+  const int heads = a.B * a.Hq;
+  const HeadItem it = head_item(item, heads);
+  const int bh = it.head, b = bh / a.Hq, hq = bh % a.Hq, hk = hq / (a.Hq / a.Hk);
+  const AttnBwdBlock w = attn_bwd_block<false>(a, seqs, a.causal && !seqs.n ? plan.q_blocks - 1 - it.index : it.index);
+  const int shift = w.kn - w.qn, row0 = w.block * BWD_BLOCK + wave * 32;
+  const bool live = row0 < w.qn;
+  int total = w.kn / 32;
+  if (a.causal) {
+    const int end = (w.block + 1) * BWD_BLOCK < w.qn ? (w.block + 1) * BWD_BLOCK : w.qn;
+    total = (end + shift) / 32;
+  }
+  const int own_tile = bh * (a.Sq / 32) + w.q_first / 32 + (live ? row0 / 32 : 0), first_at = (b * a.Hk + hk) * (a.Sk / 32) + w.k_first / 32;
+
+  v16f_t acc[2 * NK];
+#pragma unroll
+  for (int n = 0; n < 2 * NK; ++n) acc[n] = zeros();
+  v8i_t xf[NK];
+  bf16x8_t yf[4 * NV];
+  v16f_t nd;
+#pragma unroll
+  for (int s = 0; s < NK; ++s) xf[s] = frag16(a.q + ((int64_t)own_tile * 32 + r) * (D / 2) + s * 32 + h * 16);
+  const uint32_t x_scales = *reinterpret_cast<const uint32_t*>(a.q_scales + (int64_t)own_tile * 8 + 4 * h);
+  const uint8_t* y0 = reinterpret_cast<const uint8_t*>(a.g_tiles) + (int64_t)own_tile * T::ROWS_V;
+#pragma unroll
+  for (int i = 0; i < 4 * NV; ++i) yf[i] = VT::row_frag(y0 + VT::row_base(lane, i & 1), i);
+  const float lse2 = a.stats[(int64_t)own_tile * 64 + r], minus_d = a.stats[(int64_t)own_tile * 64 + 32 + r];
+#pragma unroll
+  for (int v = 0; v < 16; ++v) nd[v] = minus_d;
+  const float c2 = a.sm_scale * ATTN_RCP_LN2, slope2 = BIASED && a.alibi ? a.alibi[b * a.alibi_sb + hq * a.alibi_sh] * ATTN_RCP_LN2 : 0.0f;
+
+  const Small small{a.k, a.k_scales, nullptr};
+  const int code_base = lane * 16, row_base[2] = {VT::row_base(lane, 0), VT::row_base(lane, 1)}, column_base[2] = {DT::column_base(lane, 0), DT::column_base(lane, 1)};
+  auto place = [&](int t) { t = t < total ? t : total - 1; return BwdPlace{t, first_at + t}; };   // (past the end: the last tile again)
+
+  // Which keys of the tile the lane's row sees, in the bits of the packed pairs: most tiles are seen whole (state 2), the diagonal's in part (1), a
+  // tile behind it not at all (0: another wave of the workgroup needs it).
+  uint32_t seen[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) seen[i] = ~0u;
+  int state = 2;
+  auto look = [&](int tile) {
+    if (!a.causal) return;
+    const int away = row0 + shift - 32 * tile;   // a multiple of 32
+    const int now = away > 0 ? 2 : (away == 0 ? 1 : 0);
+    if (now == state) return;
+    state = now;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int x = score_row(2 * i, h);   // the pair's first key; the second is the next one
+      seen[i] = now == 2 ? ~0u : (now == 1 ? (x <= r ? 0xFFFFu : 0u) | (x + 1 <= r ? 0xFFFF0000u : 0u) : 0u);
+    }
+  };
+
+  // The products in order: those of the scores, then by turns one of dP and one of the sums.
+  constexpr int NS = NK, NI = 4 * NV, NF = 4 * NK, AHEAD = BWD_AHEAD, HALVES = 16;
+  struct Op {
+    int kind, j;   // 0: S, 1: dP, 2: sums
+  };
+  struct Scores {
+    v16f_t S, dp;
+  };
+  // (RUN: the first step only has scores to compute)
+  auto step = [&](auto run, int t, int slot, const Scores& from, const bf16x8_t (&f)[2], Scores& to, bf16x8_t (&f_next)[2]) {
+    constexpr bool RUN = decltype(run)::value;
+    const int after = slot == 2 ? 0 : slot + 1, before = slot == 0 ? 2 : slot - 1;
+    const uint8_t* const at_codes = lds + after * T::CODES + code_base;
+    const uint8_t *at_rows[2], *at_columns[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      at_rows[i] = lds + L::O_V + after * T::ROWS_V + row_base[i];
+      at_columns[i] = lds + L::O_D + before * T::ROWS_D + column_base[i];
+    }
+    constexpr int N = RUN ? NS + NI + NF : NS + NI;
+    auto op = [](int i) constexpr {
+      if (i < NS) return Op{0, i};
+      if (!RUN) return Op{1, i - NS};
+      int inner = 0, factor = 0;
+      for (int k = NS;; ++k) {
+        const bool take_inner = inner < NI && (factor == NF || inner * NF <= factor * NI);
+        if (k == i) return take_inner ? Op{1, inner} : Op{2, factor};
+        if (take_inner) ++inner; else ++factor;
+      }
+    };
+    const uint32_t sc = reinterpret_cast<const uint32_t*>(lds + L::O_STATS + ((t + 1) & 3) * 512 + 256)[h];
+    bf16x8_t frag[AHEAD + 1];
+    auto read = [&](auto ic) {
+      constexpr int i = decltype(ic)::value;
+      if constexpr (i < N) {
+        constexpr Op o = op(i);
+        bf16x8_t& x = frag[i % (AHEAD + 1)];
+        if constexpr (o.kind == 0) x = *reinterpret_cast<const bf16x8_t*>(at_codes + o.j * 1024);
+        else if constexpr (o.kind == 1) x = VT::row_frag(at_rows[o.j & 1], o.j);
+        else x = DT::column_frag(at_columns[0], at_columns[1], o.j % (2 * NK), o.j / (2 * NK));
+      }
+    };
+    auto product = [&](auto ic) {
+      constexpr int i = decltype(ic)::value;
+      constexpr Op o = op(i);
+      const bf16x8_t& x = frag[i % (AHEAD + 1)];
+      if constexpr (o.kind == 0) {
+        const v4i_t q = __builtin_bit_cast(v4i_t, x);
+        to.S = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(v8i_t{q[0], q[1], q[2], q[3], 0, 0, 0, 0}, xf[o.j], o.j == 0 ? zeros() : to.S, 4, 4, o.j, (int)sc, o.j, (int)x_scales);
+      } else if constexpr (o.kind == 1) {
+        to.dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, yf[o.j], o.j == 0 ? nd : to.dp, 0, 0, 0);
+      } else {
+        acc[o.j % (2 * NK)] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, f[o.j / (2 * NK)], acc[o.j % (2 * NK)], 0, 0, 0);
+      }
+    };
+    // dS of tile t, a pair of keys at a time, in two halves
+    float e[8][2];
+    uint32_t out[8];
+    auto half = [&](auto uc) {
+      constexpr int u = decltype(uc)::value, i = u >> 1;
+      if constexpr ((u & 1) == 0) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const int v = 2 * i + k;
+          float x = __builtin_fmaf(from.S[v], c2, -lse2);
+          if constexpr (BIASED) {
+            const int key = 32 * t + score_row(v, h), row = live ? row0 + r : 0;
+            if (a.bias) x = __builtin_fmaf(a.bias[b * a.bias_sb + hq * a.bias_sh + row * a.bias_sm + key], ATTN_RCP_LN2, x);
+            x = __builtin_fmaf(-slope2, __builtin_fabsf((float)(row + shift - key)), x);
+          }
+          e[i][k] = __builtin_amdgcn_exp2f(x);
+        }
+      } else {
+        out[i] = pack_bf16x2(e[i][0] * from.dp[2 * i], e[i][1] * from.dp[2 * i + 1]) & seen[i];
+        asm volatile("" : "+v"(out[i]));   // (here: otherwise it is moved behind the step, to where it is used)
+      }
+    };
+    __builtin_amdgcn_sched_barrier(0);
+    static_for<AHEAD>([&](auto ic) { read(ic); });
+    __builtin_amdgcn_sched_barrier(0);
+    static_for<N>([&](auto ic) {
+      constexpr int i = decltype(ic)::value;
+      read(std::integral_constant<int, i + AHEAD>{});
+      product(ic);
+      if constexpr (RUN) {
+        constexpr int u0 = HALVES * i / N, u1 = HALVES * (i + 1) / N;
+        static_for<u1 - u0>([&](auto uc) { half(std::integral_constant<int, u0 + decltype(uc)::value>{}); });
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    });
+    if constexpr (RUN) {
+#pragma unroll
+      for (int c = 0; c < 2; ++c) f_next[c] = __builtin_bit_cast(bf16x8_t, v4i_t{(int)out[4 * c], (int)out[4 * c + 1], (int)out[4 * c + 2], (int)out[4 * c + 3]});
+    }
+  };
+
+  // Loads go out two steps before they are used: a step starts those of the scores of t + 3 and the factor of t + 1, and ends with a wait for
+  // everything that earlier steps started.
+  auto load_scores = [&](int i, int slot) {
+    const BwdPlace p = place(i);
+    small(lds + slot * T::CODES, lds + L::O_STATS + (i & 3) * 512, p, wave, lane);
+#pragma unroll
+    for (int l = 0; l < NV; ++l) load_rows<64 * NV>(reinterpret_cast<const uint8_t*>(a.v_tiles), lds + L::O_V + slot * T::ROWS_V, p, l, wave, lane);
+  };
+  auto load_factor = [&](int i, int slot) {
+#pragma unroll
+    for (int l = 0; l < NK; ++l) load_rows<64 * NK>(reinterpret_cast<const uint8_t*>(a.k_tiles), lds + L::O_D + slot * T::ROWS_D, place(i), l, wave, lane);
+  };
+  load_scores(0, 0);
+  load_factor(0, 0);
+  load_factor(0, 2);   // (what the first step multiplies with zeros)
+  load_scores(1, 1);
+  load_scores(2, 2);
+  wait_all_but<Small::LOADS + NV>();
+  asm volatile("s_barrier" ::: "memory");
+  Scores x, y;
+  bf16x8_t f[2], g[2];
+  f[0] = f[1] = __builtin_bit_cast(bf16x8_t, v4i_t{0, 0, 0, 0});
+  step(std::false_type{}, -1, 2, x, f, x, f);
+  int slot = 0;   // of tile t
+  auto whole_step = [&](int t, const Scores& from, const bf16x8_t (&f_now)[2], Scores& to, bf16x8_t (&f_next)[2]) {
+    const int after = slot == 2 ? 0 : slot + 1;
+    load_scores(t + 3, slot);
+    load_factor(t + 1, after);
+    look(t);
+    step(std::true_type{}, t, slot, from, f_now, to, f_next);
+    slot = after;
+    wait_all_but<Small::LOADS + NV + NK>();
+    asm volatile("s_barrier" ::: "memory");
+  };
+  int t = 0;
+  for (; t + 1 < total; t += 2) {
+    whole_step(t, x, f, y, g);
+    whole_step(t + 1, y, g, x, f);
+  }
+  if (t < total) {
+    whole_step(t, x, f, y, g);
+    f[0] = g[0];
+    f[1] = g[1];
+  }
+  {   // the last tile's sums
+    const uint8_t* at = lds + L::O_D + (slot == 0 ? 2 : slot - 1) * T::ROWS_D;
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int n = 0; n < 2 * NK; ++n) acc[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(DT::column_frag(at + column_base[0], at + column_base[1], n, c), f[c], acc[n], 0, 0, 0);
+  }
+  wait_all_but<0>();   // (the last loads into the LDS, which nobody reads, before it is given back)
+  if (!live) return;
+  __bf16* row = dq_out + b * a.dq_sb + hq * a.dq_sh + (int64_t)(w.q_first + row0 + r) * a.dq_ss;
+#pragma unroll
+  for (int n = 0; n < 2 * NK; ++n) store_columns(row, acc[n], a.sm_scale, n, h);
 }
 
 template <int NK, int NV, bool BIASED>
-__global__ __launch_bounds__(256, NK > 2 ? 1 : 2) void attn_bwd_kernel(AttnBwdArgs a, AttnBwdSeqs seqs, AttnBwdPlan plan) {
+__global__ __launch_bounds__(64 * BWD_WAVES, NK > 2 ? 1 : 2) void attn_bwd_kernel(AttnBwdArgs a, AttnBwdSeqs seqs, AttnBwdPlan plan) {
   extern __shared__ __attribute__((aligned(256))) uint8_t lds[];
-  const int item = (int)blockIdx.x, keys = plan.key_groups;
-  if (item < keys) attn_bwd_body<BWD_DK, NK, NV, BIASED>(a, seqs, plan, item, reinterpret_cast<__bf16*>(a.dk), plan.partial, lds);
-  else if (item < 2 * keys)
-    attn_bwd_body<BWD_DV, NK, NV, BIASED>(a, seqs, plan, item - keys, reinterpret_cast<__bf16*>(a.dv),
-                                          plan.partial + (int64_t)plan.k_blocks * plan.parts * a.B * a.Hk * BwdTile<BWD_DK, NK, NV>::PARTIAL, lds);
-  else attn_bwd_body<BWD_DQ, NK, NV, BIASED>(a, seqs, plan, item - 2 * keys, reinterpret_cast<__bf16*>(a.dq), nullptr, lds);
+  const int item = (int)blockIdx.x;
+  if (item < plan.key_groups) attn_bwd_keys_body<NK, NV, BIASED>(a, seqs, plan, item, reinterpret_cast<__bf16*>(a.dk), reinterpret_cast<__bf16*>(a.dv), plan.partial, lds);
+  else attn_bwd_rows_body<NK, NV, BIASED>(a, seqs, plan, item - plan.key_groups, reinterpret_cast<__bf16*>(a.dq), lds);
 }
 
 template <int NK, int NV, bool BIASED>
 int launch_one(const AttnBwdArgs& a, const AttnBwdSeqs& seqs, const AttnBwdPlan& plan, hipStream_t st) {
-  constexpr int lds = BwdTile<BWD_DK, NK, NV>::LDS;   // the largest of the three
+  using T = BwdShape<NK, NV>;
+  constexpr int lds = KeysLds<NK, NV>::BYTES > RowsLds<NK, NV>::BYTES ? KeysLds<NK, NV>::BYTES : RowsLds<NK, NV>::BYTES;
   static LdsLimit limit;
   if (const int rc = limit.raise((const void*)attn_bwd_kernel<NK, NV, BIASED>, lds, "attention_bwd")) return rc;
-  hipLaunchKernelGGL((attn_bwd_kernel<NK, NV, BIASED>), dim3((unsigned)(2 * plan.key_groups + plan.row_groups)), dim3(256), lds, st, a, seqs, plan);
+  hipLaunchKernelGGL((attn_bwd_kernel<NK, NV, BIASED>), dim3((unsigned)(plan.key_groups + plan.row_groups)), dim3(64 * BWD_WAVES), lds, st, a, seqs, plan);
   if (const int rc = check_launch("attention_bwd")) return rc;
   if (!a.dk || plan.parts == 1) return ALTO_MXFP4_OK;
-  hipLaunchKernelGGL((attn_bwd_sum_kernel<NK, NV>), dim3((unsigned)(a.B * a.Hk), (unsigned)plan.k_blocks, 2 * NK + 2 * NV), dim3(256), 0, st, a, seqs, plan);
+  hipLaunchKernelGGL((attn_bwd_sum_kernel<NK, NV>), dim3((unsigned)(a.B * a.Hk), (unsigned)plan.k_blocks, T::ACC), dim3(64 * BWD_WAVES), 0, st, a, seqs, plan);
   return check_launch("attention_bwd");
 }
 

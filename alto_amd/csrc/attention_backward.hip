@@ -21,7 +21,7 @@ namespace alto {
 namespace {
 
 struct PrepareArgs {
-  const uint8_t *q, *qs, *k, *ks, *vt, *vs;
+  const uint8_t *qs, *k, *ks, *vt, *vs;
   const __bf16 *dout, *out;
   const float* lse;
   int64_t do_sb, do_sh, do_ss, o_sb, o_sh, o_ss, l_sb, l_sh, l_ss;
@@ -29,25 +29,19 @@ struct PrepareArgs {
   int q_tiles;   // B Hq Sq / 32
   float* stats;
   uint8_t *q_scales, *k_scales;
-  v4i_t *q_rows, *k_rows, *v_rows, *g_rows;
+  v4i_t *k_rows, *v_rows, *g_rows;
 };
 
-__device__ __forceinline__ float e8m0_value(uint32_t e) { return u2f(e ? e << 23 : 0x00400000u); }
-
-// eight codes of one dword as bf16
-__device__ __forceinline__ v4i_t decode8(uint32_t codes, float scale) {
-  return v4i_t{__builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 0)), __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 1)),
-               __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 2)), __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 3))};
+// The scale bytes of a tile of Q or K in the order of the score products
+__device__ __forceinline__ void order_scales(const uint8_t* scales, int64_t tile, int bands, uint8_t* ordered) {
+  const int tid = threadIdx.x, c = 2 * (tid & 3) + (tid >> 2);
+  if (tid < 8) ordered[tile * 8 + tid] = c < bands ? scales[tile * bands + c] : 127;
 }
 
-// A tile of Q or K: values, and the scale bytes in the order of the score products
-__device__ __forceinline__ void decode_tile(const uint8_t* codes, const uint8_t* scales, int64_t tile, int D, v4i_t* rows, uint8_t* ordered) {
-  const int tid = threadIdx.x, bands = D / 32;
-  const uint8_t* s = scales + tile * bands;
-  if (tid < 8) {
-    const int c = 2 * (tid & 3) + (tid >> 2);
-    ordered[tile * 8 + tid] = c < bands ? s[c] : 127;
-  }
+// The values of a tile of K
+__device__ __forceinline__ void decode_tile(const uint8_t* codes, const uint8_t* scales, int64_t tile, int D, v4i_t* rows) {
+  const int tid = threadIdx.x;
+  const uint8_t* s = scales + tile * (D / 32);
   const uint32_t* from = reinterpret_cast<const uint32_t*>(codes + tile * 16 * D);
   v4i_t* to = rows + tile * 4 * D;
   for (int i = tid; i < 4 * D; i += 256) {
@@ -56,13 +50,13 @@ __device__ __forceinline__ void decode_tile(const uint8_t* codes, const uint8_t*
   }
 }
 
-// One workgroup: 32 rows of Q with dO and their statistics, or 32 keys of K and V.
+// One workgroup: 32 query rows (dO, their statistics, the scales of Q), or 32 keys of K and V.
 __global__ __launch_bounds__(256) void attn_bwd_prepare_kernel(const PrepareArgs a) {
   __shared__ __align__(16) uint32_t turned[4][32 * 20];   // one 32 x 32 block of V a wave, rows of 64 bytes 80 apart; or a tile of dO
   const int tid = threadIdx.x;
   int64_t tile = blockIdx.x;
   if (tile < a.q_tiles) {
-    decode_tile(a.q, a.qs, tile, a.D, a.q_rows, a.q_scales);
+    order_scales(a.qs, tile, a.D / 32, a.q_scales);
     v4i_t* const grad = reinterpret_cast<v4i_t*>(turned);
     const int r = tid >> 3, c = tid & 7;
     const int64_t row = tile * 32 + r, bh = row / a.Sq;
@@ -92,7 +86,8 @@ __global__ __launch_bounds__(256) void attn_bwd_prepare_kernel(const PrepareArgs
     return;
   }
   tile -= a.q_tiles;
-  decode_tile(a.k, a.ks, tile, a.D, a.k_rows, a.k_scales);
+  order_scales(a.ks, tile, a.D / 32, a.k_scales);
+  decode_tile(a.k, a.ks, tile, a.D, a.k_rows);
   const int lane = tid & 63, wave = tid >> 6, bands = a.Sk / 32;
   if (wave * 32 >= a.Dv) return;
   const int64_t bh = tile / bands, band = tile % bands;
@@ -134,14 +129,16 @@ int64_t count_tiles(int64_t qn, int64_t kn, int64_t block_keys, int causal, int6
   return sum;
 }
 Cuts cut(const alto_mxfp4_attention_bwd_t& p) {
-  const int64_t block = ATTN_BWD_BLOCK, heads = p.Hq / p.Hk;
+  const int64_t block = BWD_BLOCK, heads = p.Hq / p.Hk;
   int64_t longest = 0, sum = 0;
   if (p.n_seqs > 0 && p.cu_q && p.cu_k) {
     for (int i = 0; i < p.n_seqs; ++i) sum += count_tiles(p.cu_q[i + 1] - p.cu_q[i], p.cu_k[i + 1] - p.cu_k[i], block, p.causal, heads, longest);
   } else {
     sum = count_tiles(p.Sq, p.Sk_used, block, p.causal, heads, longest);
   }
-  const int64_t share = sum * p.B * p.Hk / 256;   // tiles of a compute unit
+  // A tile of dQ takes about .62 of one of dK and dV (products: 18 to 26 with D = Dv = 128).  The compute units hold 512 workgroups; a list longer than
+  // an equal share of the whole would end alone.
+  const int64_t share = (int64_t)(0.85 * 1.62 * (double)(sum * p.B * p.Hk) / 512.0);
   int64_t chunk = share < 16 ? 16 : share;
   int64_t parts = (longest + chunk - 1) / chunk;
   parts = parts < 1 ? 1 : (parts > 16 ? 16 : parts);
@@ -150,7 +147,7 @@ Cuts cut(const alto_mxfp4_attention_bwd_t& p) {
 }
 
 struct Workspace {
-  int64_t stats, q_scales, k_scales, q_rows, k_rows, v_rows, g_rows, partial, total;
+  int64_t stats, q_scales, k_scales, k_rows, v_rows, g_rows, partial, total;
 };
 Workspace workspace(const alto_mxfp4_attention_bwd_t& p, const Cuts& cuts) {
   const int64_t B = p.B, Hq = p.Hq, Hk = p.Hk, Sq = p.Sq, Sk = p.Sk, D = p.D, Dv = p.Dv;
@@ -160,11 +157,10 @@ Workspace workspace(const alto_mxfp4_attention_bwd_t& p, const Cuts& cuts) {
   take(w.stats, B * Hq * Sq * 8);
   take(w.q_scales, B * Hq * (Sq / 32) * 8);
   take(w.k_scales, B * Hk * (Sk / 32) * 8);
-  take(w.q_rows, B * Hq * Sq * D * 2);
   take(w.k_rows, B * Hk * Sk * D * 2);
   take(w.v_rows, B * Hk * Sk * Dv * 2);
   take(w.g_rows, B * Hq * Sq * Dv * 2);
-  const int64_t block = ATTN_BWD_BLOCK, blocks = Sk / block + (p.n_seqs > 0 ? (p.n_seqs < ATTN_MAX_SEQS ? p.n_seqs : ATTN_MAX_SEQS) : 1);   // (at least those of any launch)
+  const int64_t block = BWD_BLOCK, blocks = Sk / block + (p.n_seqs > 0 ? (p.n_seqs < ATTN_MAX_SEQS ? p.n_seqs : ATTN_MAX_SEQS) : 1);   // (at least those of any launch)
   take(w.partial, cuts.parts > 1 ? B * Hk * blocks * cuts.parts * block * (D + Dv) * 4 : 0);
   w.total = at;
   return w;
@@ -200,6 +196,7 @@ static int attention_bwd(const alto_mxfp4_attention_bwd_t& p, hipStream_t st) {
     ALTO_REQUIRE(s >= 0 && s < (1ll << 40) && s % 4 == 0, "attention_bwd: strides of the gradients must be non-negative multiples of 4 elements");
   for (const int64_t s : {p.lse_sb, p.lse_sh, p.lse_ss, p.bias_sb, p.bias_sh, p.bias_sm, p.alibi_sb, p.alibi_sh})
     ALTO_REQUIRE(s >= 0 && s < (1ll << 40), "attention_bwd: strides must be non-negative");
+  ALTO_REQUIRE(p.sm_scale > 0.0f && p.sm_scale < __builtin_inff(), "attention_bwd: sm_scale must be positive and finite");
   ALTO_REQUIRE(p.n_seqs >= 0, "attention_bwd: negative number of sequences");
   ALTO_REQUIRE(p.causal == 0 || p.n_seqs > 0 || p.Sq <= p.Sk_used, "attention_bwd: causal attention needs Sq <= Sk (got %lld > %lld)", (long long)p.Sq, (long long)p.Sk_used);
   if (p.n_seqs > 0) {
@@ -226,7 +223,7 @@ static int attention_bwd(const alto_mxfp4_attention_bwd_t& p, hipStream_t st) {
   }
   uint8_t* ws = (uint8_t*)p.workspace;
   PrepareArgs r{};
-  r.q = (const uint8_t*)p.q_codes; r.qs = (const uint8_t*)p.q_scales; r.k = (const uint8_t*)p.k_codes; r.ks = (const uint8_t*)p.k_scales;
+  r.qs = (const uint8_t*)p.q_scales; r.k = (const uint8_t*)p.k_codes; r.ks = (const uint8_t*)p.k_scales;
   r.vt = (const uint8_t*)p.vt_codes; r.vs = (const uint8_t*)p.v_scales;
   r.dout = (const __bf16*)p.dout; r.out = (const __bf16*)p.out; r.lse = p.lse;
   r.do_sb = p.dout_sb; r.do_sh = p.dout_sh; r.do_ss = p.dout_ss; r.o_sb = p.out_sb; r.o_sh = p.out_sh; r.o_ss = p.out_ss;
@@ -234,23 +231,23 @@ static int attention_bwd(const alto_mxfp4_attention_bwd_t& p, hipStream_t st) {
   r.Hq = (int)p.Hq; r.Hk = (int)p.Hk; r.Sq = (int)p.Sq; r.Sk = (int)p.Sk; r.D = (int)p.D; r.Dv = (int)p.Dv;
   r.q_tiles = (int)(p.B * p.Hq * (p.Sq / 32));
   r.stats = (float*)(ws + w.stats); r.q_scales = ws + w.q_scales; r.k_scales = ws + w.k_scales;
-  r.q_rows = (v4i_t*)(ws + w.q_rows); r.k_rows = (v4i_t*)(ws + w.k_rows); r.v_rows = (v4i_t*)(ws + w.v_rows); r.g_rows = (v4i_t*)(ws + w.g_rows);
+  r.k_rows = (v4i_t*)(ws + w.k_rows); r.v_rows = (v4i_t*)(ws + w.v_rows); r.g_rows = (v4i_t*)(ws + w.g_rows);
   hipLaunchKernelGGL(attn_bwd_prepare_kernel, dim3((unsigned)(r.q_tiles + (int)(p.B * p.Hk * (p.Sk / 32)))), dim3(256), 0, st, r);
   if (const int rc = check_launch("attention_bwd")) return rc;
 
   AttnBwdArgs a{};
-  a.q = r.q; a.k = r.k; a.q_scales = r.q_scales; a.k_scales = r.k_scales; a.stats = r.stats;
-  a.q_tiles = (const __bf16*)r.q_rows; a.k_tiles = (const __bf16*)r.k_rows; a.v_tiles = (const __bf16*)r.v_rows; a.g_tiles = (const __bf16*)r.g_rows;
+  a.q = (const uint8_t*)p.q_codes; a.k = r.k; a.q_scales = r.q_scales; a.k_scales = r.k_scales; a.stats = r.stats;
+  a.k_tiles = (const __bf16*)r.k_rows; a.v_tiles = (const __bf16*)r.v_rows; a.g_tiles = (const __bf16*)r.g_rows;
   a.dq = p.dq; a.dk = p.dk; a.dv = p.dv;
   a.dq_sb = p.dq_sb; a.dq_sh = p.dq_sh; a.dq_ss = p.dq_ss; a.dk_sb = p.dk_sb; a.dk_sh = p.dk_sh; a.dk_ss = p.dk_ss; a.dv_sb = p.dv_sb; a.dv_sh = p.dv_sh; a.dv_ss = p.dv_ss;
   a.B = (int)p.B; a.Hq = (int)p.Hq; a.Hk = (int)p.Hk; a.Sq = (int)p.Sq; a.Sk = (int)p.Sk; a.Sk_used = (int)p.Sk_used;
   a.sm_scale = p.sm_scale; a.causal = p.causal ? 1 : 0;
   a.bias = p.bias; a.bias_sb = p.bias_sb; a.bias_sh = p.bias_sh; a.bias_sm = p.bias_sm; a.alibi = p.alibi_slopes; a.alibi_sb = p.alibi_sb; a.alibi_sh = p.alibi_sh;
-  const int row_block = ATTN_BWD_BLOCK, key_block = ATTN_BWD_BLOCK;
+  const int row_block = BWD_BLOCK, key_block = row_block;
   auto go = [&](const AttnBwdSeqs& s, int q_blocks, int k_blocks) {
     AttnBwdPlan plan{q_blocks, k_blocks, cuts.parts, cuts.chunk, 0, 0, (float*)(ws + w.partial)};
     const int64_t keys = p.dk ? (p.B * p.Hk * cuts.parts * k_blocks + 7) / 8 * 8 : 0, rows = p.dq ? p.B * p.Hq * q_blocks : 0;
-    ALTO_REQUIRE(2 * keys + rows < (1ll << 31), "attention_bwd: too many workgroups");
+    ALTO_REQUIRE(keys + rows < (1ll << 31), "attention_bwd: too many workgroups");
     plan.key_groups = (int)keys;
     plan.row_groups = (int)rows;
     switch (p.D) {
