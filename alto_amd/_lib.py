@@ -88,6 +88,7 @@ SIGNATURES = {
     "alto_mxfp4_attention_fwd_strided": (c_int, [c_vp] * 8 + [c_i64] * 13 + [c_int, c_vp, c_vp, c_f32, c_int, c_vp, c_i64, c_i64, c_vp]),
     "alto_mxfp4_attention_bwd_workspace_bytes": (c_i64, [c_vp]),
     "alto_mxfp4_attention_bwd": (c_int, [c_vp, c_vp]),
+    "alto_mxfp4_rotary": (c_int, [c_vp, c_vp]),
     "alto_mxfp4_gemm_two": (c_int, [c_vp, c_vp, c_vp]),
     "alto_mxfp4_gemm_two_tile": (c_int, [c_vp, c_vp]),
     "alto_mxfp4_attention_rows_per_workgroup": (c_int, [c_i64] * 5 + [c_int, c_vp, c_vp, c_int]),

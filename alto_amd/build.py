@@ -21,7 +21,7 @@ HOSTSRC = os.path.join(CSRC, "host.cpp")
 HEADER = os.path.join(HERE, "..", "include", "alto_mxfp4.h")
 
 SOURCES = ["capi.hip", "quantize.hip", "dequantize.hip", "gemm.hip", "gemm_tiled.hip", "gemm_mid.hip", "gemm_skinny.hip", "grouped_gemm.hip", "probe.hip", "qdq.hip", "attention.hip", "attention_split.hip", "attention_quantize.hip", "attention_backward.hip", "attention_backward_64.hip", "attention_backward_128.hip", "attention_backward_192.hip",
-           "attention_backward_256.hip", "quantize_dynamic.hip", "random.hip"]
+           "attention_backward_256.hip", "rotary.hip", "quantize_dynamic.hip", "random.hip"]
 
 HIPCC_FLAGS = [
     "--offload-arch=gfx950",

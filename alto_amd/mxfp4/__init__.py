@@ -10,6 +10,7 @@ from .linear import (MXFP4LinearFunction, _to_mxfp4_then_scaled_mm, blockwise_mx
 from .ops import register_torch_ops
 from .qdq import _make_qdq_fn_for, quantize_dequantize
 from .quantization import BLOCK_SIZE_DEFAULT, convert_from_mxfp4, convert_to_mxfp4, hadamard_left, quantize_rowcol
+from .rotary import Rotary, apply_rotary, rotary_frequencies
 from ._runtime import enable_device_philox_state, set_rand_bits_source, use_hardware_stochastic_rounding
 from .tensor import MXFP4TrainingWeightWrapperTensor, TrainingWeightWrapperBaseTensor, swap_params
 
@@ -51,5 +52,8 @@ __all__ = (
     "attention_mxfp4_backward",
     "quantize_qkv",
     "LPScaledDotProductAttention",
+    "apply_rotary",
+    "rotary_frequencies",
+    "Rotary",
     "register_torch_ops",
 )

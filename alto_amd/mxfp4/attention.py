@@ -14,10 +14,12 @@ import ctypes
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _runtime as rt
 from .._lib import check
 from .config import TrainingOpConfig
+from .rotary import Rotary, apply_rotary
 
 
 def _additive(bias: Optional[torch.Tensor], alibi_slopes: Optional[torch.Tensor], B: int, Hq: int, Sq: int, Sk: int):
@@ -202,21 +204,85 @@ def _attend(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, sm_scale: float, 
     caller's results in whatever layout they have.  ``cu_q`` / ``cu_k``: boundaries (host ints) of sequences packed along S."""
     if alibi_slopes is None and rt.host().attend(q, k, v, sm_scale, bool(causal), out, lse, cu_q or [], cu_k or [], rt.stream_ptr(q.device)):
         return
-    qq, qs, kq, ks, vq, vs = quantize_qkv(q, k, v)
-    (B, Hq, Sq, D), (_, Hk, Sk, Dv) = q.shape, v.shape
-    sl = None
-    if alibi_slopes is not None:
-        rt.require_gpu(alibi_slopes)
-        sl = alibi_slopes.to(torch.float32)
-        sl = (sl.unsqueeze(0) if sl.dim() == 1 else sl).contiguous()
-        torch._check(sl.dim() == 2 and sl.shape[1] == Hq and sl.shape[0] in (1, B), lambda: f"alibi_slopes of shape {tuple(alibi_slopes.shape)}: [Hq] or [B, Hq]")
+    operands = quantize_qkv(q, k, v)
+    _attend_quantized(operands, sm_scale, causal, out, lse, _additive(None, alibi_slopes, q.shape[0], q.shape[1], q.shape[2], k.shape[2])[1], cu_q, cu_k)
+
+
+def _attend_quantized(operands, sm_scale: float, causal: bool, out: torch.Tensor, lse: torch.Tensor, sl: Optional[torch.Tensor], cu_q, cu_k) -> None:
+    """The attention kernel on what :func:`quantize_qkv` gives; ``sl``: slopes as :func:`_additive` gives them."""
+    qq, qs, kq, ks, vq, vs = operands
+    (B, Hq, Sq), (Hk, Sk), D, Dv = qq.shape[:3], kq.shape[1:3], 2 * qq.shape[3], vq.shape[2]
     n = 0 if cu_q is None else len(cu_q) - 1
     ints = ctypes.c_int32 * (n + 1)
     check(rt.lib().alto_mxfp4_attention_fwd_strided(
         qq.data_ptr(), qs.data_ptr(), kq.data_ptr(), ks.data_ptr(), vq.data_ptr(), vs.data_ptr(), out.data_ptr(), lse.data_ptr(), B, Hq, Hk, Sq, Sk, D, Dv,
         *out.stride()[:3], *lse.stride(), n, ints(*cu_q) if n else None, ints(*cu_k) if n else None, float(sm_scale), int(bool(causal)),
-        rt.ptr(sl), 0 if sl is None or sl.shape[0] == 1 else sl.stride(0), 0 if sl is None else sl.stride(1), rt.stream_ptr(q.device)),
+        rt.ptr(sl), 0 if sl is None or sl.shape[0] == 1 else sl.stride(0), 0 if sl is None else sl.stride(1), rt.stream_ptr(qq.device)),
         "alto_mxfp4_attention_fwd_strided")
+
+
+@torch.compiler.allow_in_graph
+class MXFP4AttentionFunction(torch.autograd.Function):
+    """The attention of :func:`_attend` (or with a ``bias``, of :func:`attention_mxfp4_forward`) on [B, H, S, D] views, with its backward.  Kept from
+    one to the other: Q, K and V as codes and scales, the output and the log-sum-exp."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, sm_scale, causal, rows_outer, bias, alibi_slopes, cu_q, cu_k):
+        torch._check(0.0 < sm_scale < float("inf"), lambda: f"sm_scale {sm_scale}: the backward needs a positive one")
+        (B, Hq, Sq, D), (_, Hk, Sk, Dv) = q.shape, v.shape
+        ctx.dtypes, ctx.sizes = (q.dtype, k.dtype, v.dtype), (D, Sk, Dv)
+        pad = 32 if bias is not None and Sk % 64 == 32 else 0   # (as in _fixed_length)
+        if pad:
+            k, v = (torch.nn.functional.pad(t, (0, 0, 0, pad)) for t in (k, v))
+        qq, qs, kq, ks, vq, vs = quantize_qkv(q, k, v)
+        b4, sl = _additive(bias, alibi_slopes, B, Hq, Sq, Sk)
+        if bias is None:
+            out, lse = _results(q, Dv, rows_outer, cu_q is not None)
+            _attend_quantized((qq, qs, kq, ks, vq, vs), sm_scale, causal, out, lse, sl, cu_q, cu_k)
+        else:
+            out, lse = attention_mxfp4_forward(qq, kq, vq, qs, ks, vs, sm_scale, causal, seqlen_k=Sk, bias=b4, alibi_slopes=sl)
+        ctx.save_for_backward(qq, qs, kq, ks, vq, vs, out, lse, b4, sl)
+        ctx.more = sm_scale, causal, rows_outer, cu_q, cu_k
+        ctx.mark_non_differentiable(lse)
+        return out, lse
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_out, _):
+        qq, qs, kq, ks, vq, vs, out, lse, b4, sl = ctx.saved_tensors
+        sm_scale, causal, rows_outer, cu_q, cu_k = ctx.more
+        D, Sk, Dv = ctx.sizes
+        want_q, want_kv = ctx.needs_input_grad[0], ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
+
+        def empty(like, columns):
+            B, H, S = like.shape[:3]
+            if rows_outer:
+                return torch.empty((B, S, H, columns), dtype=torch.bfloat16, device=like.device).transpose(1, 2)
+            return torch.empty((B, H, S, columns), dtype=torch.bfloat16, device=like.device)
+
+        dq = empty(qq, D) if want_q else None
+        dk, dv = (empty(kq, D), empty(kq, Dv)) if want_kv else (None, None)
+        if want_q or want_kv:
+            _gradients(grad_out, (qq, qs, kq, ks, vq, vs), out, lse, sm_scale, causal, Sk, b4, sl, cu_q, cu_k, dq, dk, dv)
+        grads = [None if g is None or not need else g[:, :, :n].to(dt) for g, need, n, dt in
+                 zip((dq, dk, dv), ctx.needs_input_grad, (qq.shape[2], Sk, Sk), ctx.dtypes)]
+        return (*grads, None, None, None, None, None, None, None)
+
+
+def _results(q: torch.Tensor, Dv: int, rows_outer: bool, lse_rows_outer: bool) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Room for [B, Hq, Sq, Dv] and [B, Hq, Sq]; ``rows_outer``: as views of memory with the rows outside the heads."""
+    B, Hq, Sq = q.shape[:3]
+    if rows_outer:
+        out = torch.empty((B, Sq, Hq, Dv), dtype=torch.bfloat16, device=q.device).transpose(1, 2)
+    else:
+        out = torch.empty((B, Hq, Sq, Dv), dtype=torch.bfloat16, device=q.device)
+    if lse_rows_outer:
+        return out, torch.empty((B, Sq, Hq), dtype=torch.float32, device=q.device).transpose(1, 2)
+    return out, torch.empty((B, Hq, Sq), dtype=torch.float32, device=q.device)
+
+
+def _differentiated(*tensors: torch.Tensor) -> bool:
+    return torch.is_grad_enabled() and any(t.requires_grad for t in tensors)
 
 
 def triton_attention_mxfp4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, alibi_slopes: Optional[torch.Tensor] = None,
@@ -256,6 +322,10 @@ def triton_attention_mxfp4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, al
         torch._check(all(a < b for a, b in zip(cq, cq[1:])) and all(a < b for a, b in zip(ck, ck[1:])), lambda: "empty sequences are not supported")
         _check_options(dropout_p, return_scores)
         rt.require_gpu(q, k, v)
+        if _differentiated(q, k, v):
+            q4, k4, v4 = (t.transpose(0, 1).unsqueeze(0) for t in (q, k, v))
+            out, lse = MXFP4AttentionFunction.apply(q4, k4, v4, q.shape[-1] ** -0.5 if sm_scale is None else float(sm_scale), bool(causal), True, None, alibi_slopes, cq, ck)
+            return out.squeeze(0).transpose(0, 1), lse.squeeze(0).transpose(0, 1), torch.empty([], device=q.device, dtype=torch.float32)
         out = torch.empty((q.shape[0], q.shape[1], v.shape[2]), dtype=torch.bfloat16, device=q.device)
         lse = torch.empty((q.shape[0], q.shape[1]), dtype=torch.float32, device=q.device)
         q4, k4, v4, o4 = (t.transpose(0, 1).unsqueeze(0) for t in (q, k, v, out))
@@ -276,13 +346,12 @@ def _fixed_length(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, alibi_slope
     assert max_seqlens_q in (None, q.shape[2]) and max_seqlens_k in (None, k.shape[2]), "variable lengths are not implemented"
     if sm_scale is None:
         sm_scale = q.shape[-1] ** -0.5
-    if bias is None:
-        (B, Hq, Sq, _), Dv = q.shape, v.shape[3]
-        if rows_outer:
-            out = torch.empty((B, Sq, Hq, Dv), dtype=torch.bfloat16, device=q.device).transpose(1, 2)
-        else:
-            out = torch.empty((B, Hq, Sq, Dv), dtype=torch.bfloat16, device=q.device)
-        lse = torch.empty((B, Hq, Sq), dtype=torch.float32, device=q.device)
+    if _differentiated(q, k, v):
+        if bias is not None and bias.requires_grad:
+            raise NotImplementedError("a bias that requires a gradient is not implemented: detach it")
+        out, lse = MXFP4AttentionFunction.apply(q, k, v, float(sm_scale), bool(causal), rows_outer, bias, alibi_slopes, None, None)
+    elif bias is None:
+        out, lse = _results(q, v.shape[3], rows_outer, False)
         _attend(q, k, v, sm_scale, causal, out, lse, alibi_slopes)
     else:
         seqlen_k = k.shape[2]
@@ -311,7 +380,8 @@ class LPScaledDotProductAttention(torch.nn.Module):
         self.config = config
 
     def forward(self, q_BLNH, k_BLNH, v_BLNH, *, attention_masks=None, scale: Optional[float] = None, enable_gqa: bool = False,
-                is_causal: bool = True, **kwargs):
+                is_causal: bool = True, rotary: Optional[Rotary] = None, **kwargs):
+        """``rotary``: Q and K come unrotated, and are rotated first (``apply_rotary``)."""
         if attention_masks is not None:
             raise ValueError("ScaledDotProductAttention does not support attention_masks; it only supports causal/non-causal "
                              "attention via is_causal.")
@@ -319,4 +389,6 @@ class LPScaledDotProductAttention(torch.nn.Module):
         assert q.shape[0] == k.shape[0] == v.shape[0] and k.shape[2] == v.shape[2]
         assert q.shape[3] == k.shape[3] and k.shape[1] == v.shape[1]
         sm_scale = q.shape[3] ** -0.5 if scale is None else scale
+        if rotary is not None:
+            q, k = apply_rotary(q, k, rotary.inv_freq, rotary.positions, interleaved=rotary.interleaved, factor=rotary.factor, layout="bshd")
         return triton_attention_mxfp4(q, k, v, sm_scale=sm_scale, causal=is_causal, max_seqlens_q=q.shape[1], max_seqlens_k=k.shape[1], layout="bshd")[0]

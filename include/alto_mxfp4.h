@@ -560,6 +560,26 @@ int64_t alto_mxfp4_attention_bwd_workspace_bytes(const alto_mxfp4_attention_bwd_
 int alto_mxfp4_attention_bwd(const alto_mxfp4_attention_bwd_t* args, void* stream);
 
 /*
+ * Rotary positions: of every head's D columns of Q and K the first R are rotated in pairs -- columns i and i + R/2, or 2i and 2i + 1 with
+ * `interleaved` -- by position * inv_freq[i] radians, cosine and sine multiplied with `factor`; the others are copied.  `inverse` rotates
+ * back (the transpose: its backward).  q [B][S][Hq][D] and k [B][S][Hk][D] (Hk = 0: none) at element strides of batch, head and row, unit
+ * stride along D, bf16 or f32, outputs alike; an output is no input.  inv_freq: R/2 doubles on the device; angles, cosines and sines are taken
+ * in 64 bits, products in 32, rounded once.  positions: int64 (or int32 with positions_are_32), element (b, s) at b pos_sb + s pos_ss, any
+ * sign; NULL: s.  R even, at most 2048.
+ */
+typedef struct {
+  const void *q, *k;
+  void *q_out, *k_out;
+  const double* inv_freq;
+  const void* positions;
+  int64_t B, S, Hq, Hk, D, R;
+  int64_t q_sb, q_sh, q_ss, k_sb, k_sh, k_ss, qo_sb, qo_sh, qo_ss, ko_sb, ko_sh, ko_ss, pos_sb, pos_ss;
+  double factor;
+  int dtype, interleaved, inverse, positions_are_32;
+} alto_mxfp4_rotary_t;
+int alto_mxfp4_rotary(const alto_mxfp4_rotary_t* args, void* stream);
+
+/*
  * Fills out[0 .. n) with random 32-bit words for stochastic rounding: word 4 c + j is word j of Philox4x32-10 (Salmon et
  * al., SC'11) with the 128-bit counter c + offset and the 64-bit key `seed`.  The reference draws its bits inside its
  * kernel from the same generator family (tl.randint4x, alto/kernels/fp4/fp4_common/triton_fp4_ops.py:15-18) with
