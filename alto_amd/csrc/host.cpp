@@ -13,6 +13,7 @@
 
 #include <ATen/ATen.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
+#include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -52,6 +53,9 @@ struct Api {
   ALTO_FN(grouped_gemm_plan_ends);
   ALTO_FN(quantize_operands);
   ALTO_FN(gemm_two);
+  ALTO_FN(attention_bwd);
+  ALTO_FN(attention_bwd_workspace_bytes);
+  ALTO_FN(rotary);
 #undef ALTO_FN
 } api;
 py::object* check_fn = nullptr;   // _lib.check(rc, name): raises for rc != 0 (never freed: the interpreter may be gone by then)
@@ -76,6 +80,9 @@ void bind(const py::dict& address, py::object check) {
   ALTO_FN(grouped_gemm_plan_ends);
   ALTO_FN(quantize_operands);
   ALTO_FN(gemm_two);
+  ALTO_FN(attention_bwd);
+  ALTO_FN(attention_bwd_workspace_bytes);
+  ALTO_FN(rotary);
 #undef ALTO_FN
   delete check_fn;
   check_fn = new py::object(std::move(check));
@@ -291,6 +298,67 @@ bool attend(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in, double s
   call("alto_mxfp4_attention_fwd_strided", api.attention_fwd_strided, qq, qs, kq, ks, vq, vs, out.data_ptr(), lse_p, B, Hq, Hk, Sq, Sk, D, Dv, out.stride(0), out.stride(1),
        out.stride(2), lse.stride(0), lse.stride(1), lse.stride(2), n, cq, ck, (float)sm_scale, (int)causal, static_cast<const float*>(nullptr), (int64_t)0, (int64_t)0, s);
   return true;
+}
+
+// attention.py:attention_mxfp4_backward on dense operands -> (dq, dk, dv)
+bool on_current_device(const Tensor& t) { return on_gpu(t) && t.get_device() == c10::hip::current_device(); }
+py::object attention_gradients(const Tensor& go_in, const Tensor& q, const Tensor& q_scale, const Tensor& k, const Tensor& k_scale, const Tensor& v, const Tensor& v_scale,
+                               const Tensor& out_in, const Tensor& lse, double sm_scale, bool causal, int64_t seqlen_k, const OptTensor& bias, const OptTensor& slopes,
+                               const std::vector<int32_t>& cu_q, const std::vector<int32_t>& cu_k, bool rows_outer, bool want_q, bool want_kv) {
+  for (const Tensor* t : {&q, &q_scale, &k, &k_scale, &v, &v_scale})
+    if (!on_current_device(*t) || t->scalar_type() != at::kByte || t->dim() != 4 || !t->is_contiguous()) return py::none();
+  for (const Tensor* t : {&go_in, &out_in})
+    if (!on_current_device(*t) || t->scalar_type() != at::kBFloat16 || t->dim() != 4) return py::none();
+  const int64_t B = q.size(0), Hq = q.size(1), Sq = q.size(2), D = 2 * q.size(3), Hk = k.size(1), Sk = k.size(2), Dv = v.size(2);
+  auto is = [](const Tensor& t, at::IntArrayRef size) { return t.sizes() == size; };
+  if (!is(k, {B, Hk, Sk, D / 2}) || !is(v, {B, Hk, Dv, Sk / 2}) || !is(q_scale, {B, Hq, Sq / 32, D / 32}) || !is(k_scale, {B, Hk, Sk / 32, D / 32}) ||
+      !is(v_scale, {B, Hk, Sk / 32, Dv / 32}) || !is(go_in, {B, Hq, Sq, Dv}) || !is(out_in, {B, Hq, Sq, Dv}))
+    return py::none();
+  if (!on_current_device(lse) || lse.scalar_type() != at::kFloat || !is(lse, {B, Hq, Sq}) || cu_q.size() != cu_k.size() || cu_q.size() == 1) return py::none();
+  for (const OptTensor* t : {&bias, &slopes})   // (as _additive gives them)
+    if (t->has_value() && (!on_current_device(**t) || (*t)->scalar_type() != at::kFloat)) return py::none();
+  auto readable = [](const Tensor& t) {
+    return t.stride(3) == 1 && aligned16(t) && stride_of(t, 0) % 8 == 0 && stride_of(t, 1) % 8 == 0 && stride_of(t, 2) % 8 == 0 ? t : t.contiguous();
+  };
+  const Tensor go = readable(go_in), out = readable(out_in);
+  const auto opts = at::TensorOptions().dtype(at::kBFloat16).device(q.device());
+  auto grad = [&](bool want, int64_t H, int64_t S, int64_t n) {
+    if (!want) return Tensor();
+    return rows_outer ? at::empty({B, S, H, n}, opts).transpose(1, 2) : at::empty({B, H, S, n}, opts);
+  };
+  const Tensor dq = grad(want_q, Hq, Sq, D), dk = grad(want_kv, Hk, Sk, D), dv = grad(want_kv, Hk, Sk, Dv);
+  alto_mxfp4_attention_bwd_t a{};
+  a.q_codes = bytes(q); a.q_scales = bytes(q_scale); a.k_codes = bytes(k); a.k_scales = bytes(k_scale); a.vt_codes = bytes(v); a.v_scales = bytes(v_scale);
+  a.dout = bytes(go); a.out = bytes(out); a.lse = static_cast<const float*>(lse.data_ptr());
+  a.dq = bytes(dq); a.dk = bytes(dk); a.dv = bytes(dv);
+  a.B = B; a.Hq = Hq; a.Hk = Hk; a.Sq = Sq; a.Sk = Sk; a.Sk_used = seqlen_k; a.D = D; a.Dv = Dv;
+  auto strides = [](const Tensor& t, int64_t& sb, int64_t& sh, int64_t& ss) {
+    if (!t.defined()) return;
+    sb = stride_of(t, 0); sh = stride_of(t, 1); ss = stride_of(t, 2);
+  };
+  strides(go, a.dout_sb, a.dout_sh, a.dout_ss);
+  strides(out, a.out_sb, a.out_sh, a.out_ss);
+  strides(lse, a.lse_sb, a.lse_sh, a.lse_ss);
+  strides(dq, a.dq_sb, a.dq_sh, a.dq_ss);
+  strides(dk, a.dk_sb, a.dk_sh, a.dk_ss);
+  strides(dv, a.dv_sb, a.dv_sh, a.dv_ss);
+  if (bias.has_value()) {
+    a.bias = static_cast<const float*>(bias->data_ptr());
+    a.bias_sb = stride_of(*bias, 0); a.bias_sh = stride_of(*bias, 1); a.bias_sm = bias->stride(2);
+  }
+  if (slopes.has_value()) {
+    a.alibi_slopes = static_cast<const float*>(slopes->data_ptr());
+    a.alibi_sb = stride_of(*slopes, 0); a.alibi_sh = slopes->stride(1);
+  }
+  if (!cu_q.empty()) { a.cu_q = cu_q.data(); a.cu_k = cu_k.data(); a.n_seqs = (int)cu_q.size() - 1; }
+  a.causal = causal; a.sm_scale = (float)sm_scale;
+  a.workspace_bytes = api.attention_bwd_workspace_bytes(&a);
+  if (a.workspace_bytes < 0) return py::none();   // (the general path words the error)
+  const Tensor ws = Alloc(q).dense({a.workspace_bytes});
+  a.workspace = ws.data_ptr();
+  call("alto_mxfp4_attention_bwd", api.attention_bwd, &a, c10::hip::getCurrentHIPStream(q.device().index()).stream());
+  auto opt = [](const Tensor& t) -> py::object { return t.defined() ? py::cast(t) : py::none(); };
+  return py::make_tuple(opt(dq), opt(dk), opt(dv));
 }
 
 // ------------------------------------------------------------------------------------------------- whole training directions
@@ -752,6 +820,129 @@ py::tuple draw_hadamard(const std::optional<at::Generator>& gen, at::ScalarType 
   return py::make_tuple(signs, perm);
 }
 
+// ------------------------------------------------------------------------------------------------------------ rotary positions
+// rotary.py:apply_rotary and its backward.  As Python functions around one native call each a forward took 21 us and a training step 145
+// (10 and 55 here).
+struct RotaryOperands {
+  Tensor inv_freq, positions;   // (positions undefined: 0, 1, ...)
+  bool interleaved = false, inverse = false;
+  double factor = 1.0;
+  int64_t layout = 0;           // 0: [B, H, S, D], 1: [B, S, H, D], 2: [T, H, D]
+  int64_t batch() const { return layout == 2 ? -1 : 0; }
+  int64_t head() const { return layout == 0 ? 1 : layout == 1 ? 2 : 1; }
+  int64_t row() const { return layout == 0 ? 2 : layout == 1 ? 1 : 0; }
+};
+
+// q and k rotated (either may be undefined: not wanted), of whatever strides
+variable_list rotate(Failure& f, const Tensor& q_in, const Tensor& k_in, const RotaryOperands& op) {
+  auto readable = [](const Tensor& t) { return !t.defined() || t.stride(-1) == 1 ? t : t.contiguous(); };
+  Tensor q = readable(q_in), k = readable(k_in);
+  if (!q.defined()) std::swap(q, k);
+  variable_list out(2);
+  Tensor q2 = at::empty(q.sizes(), q.options()), k2 = k.defined() ? at::empty(k.sizes(), k.options()) : Tensor();
+  alto_mxfp4_rotary_t a{};
+  a.q = q.data_ptr(); a.q_out = q2.data_ptr();
+  if (k.defined()) { a.k = k.data_ptr(); a.k_out = k2.data_ptr(); a.Hk = k.size(op.head()); }
+  a.inv_freq = static_cast<const double*>(op.inv_freq.data_ptr());
+  a.B = op.batch() < 0 ? 1 : q.size(op.batch()); a.S = q.size(op.row()); a.Hq = q.size(op.head()); a.D = q.size(-1); a.R = 2 * op.inv_freq.size(0);
+  auto strides = [&](const Tensor& t, int64_t& sb, int64_t& sh, int64_t& ss) {
+    if (!t.defined()) return;
+    sb = op.batch() < 0 ? 0 : stride_of(t, op.batch()); sh = stride_of(t, op.head()); ss = stride_of(t, op.row());
+  };
+  strides(q, a.q_sb, a.q_sh, a.q_ss);
+  strides(k, a.k_sb, a.k_sh, a.k_ss);
+  strides(q2, a.qo_sb, a.qo_sh, a.qo_ss);
+  strides(k2, a.ko_sb, a.ko_sh, a.ko_ss);
+  if (op.positions.defined()) {
+    const Tensor& p = op.positions;
+    a.positions = p.data_ptr();
+    a.positions_are_32 = p.scalar_type() == at::kInt;
+    a.pos_sb = p.dim() == 1 ? 0 : stride_of(p, 0); a.pos_ss = stride_of(p, p.dim() - 1);
+  }
+  a.factor = op.factor; a.dtype = dtype_code(q.scalar_type()); a.interleaved = op.interleaved; a.inverse = op.inverse;
+  f.ok("alto_mxfp4_rotary", api.rotary(&a, current_stream(q)));
+  out[q_in.defined() ? 0 : 1] = q2;
+  if (k.defined()) out[1] = k2;
+  return out;
+}
+
+struct RotaryNode : torch::autograd::Function<RotaryNode> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const RotaryOperands& op) {
+    Failure f;
+    variable_list out = rotate(f, q, k, op);
+    if (f.rc != 0) throw Refused{f};
+    ctx->save_for_backward({op.inv_freq, op.positions});
+    ctx->saved_data["interleaved"] = op.interleaved;
+    ctx->saved_data["inverse"] = op.inverse;
+    ctx->saved_data["factor"] = op.factor;
+    ctx->saved_data["layout"] = op.layout;
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list saved = ctx->get_saved_variables();
+    RotaryOperands op;
+    op.inv_freq = saved[0];
+    op.positions = saved[1];
+    op.interleaved = ctx->saved_data["interleaved"].toBool();
+    op.inverse = !ctx->saved_data["inverse"].toBool();
+    op.factor = ctx->saved_data["factor"].toDouble();
+    op.layout = ctx->saved_data["layout"].toInt();
+    variable_list out(3);   // q, k, the operands
+    Failure f;
+    if (at::GradMode::is_enabled() && (grads[0].requires_grad() || grads[1].requires_grad())) {   // (the rotation is linear: its gradient is one)
+      try {
+        const variable_list both = apply(grads[0], grads[1], op);
+        out[0] = both[0];
+        out[1] = both[1];
+      } catch (const Refused& r) {
+        f = r.failure;
+      }
+    } else {
+      const variable_list both = rotate(f, ctx->needs_input_grad(0) ? grads[0] : Tensor(), ctx->needs_input_grad(1) ? grads[1] : Tensor(), op);
+      out[0] = both[0];
+      out[1] = both[1];
+    }
+    raise_in_engine(f);
+    return out;
+  }
+};
+
+// q and k of everyday calls -> (q, k) rotated, with their graph where they need one
+py::object rotary(const Tensor& q, const Tensor& k, const Tensor& inv_freq, const OptTensor& positions, bool interleaved, double factor, int64_t layout) {
+  const int64_t dims = layout == 2 ? 3 : 4;
+  RotaryOperands op{inv_freq, positions.has_value() ? *positions : Tensor(), interleaved, false, factor, layout};
+  for (const Tensor* t : {&q, &k})
+    if (!on_current_device(*t) || !is_float(*t) || t->dim() != dims) return py::none();
+  if (q.scalar_type() != k.scalar_type() || q.numel() == 0 || k.numel() == 0) return py::none();
+  for (int64_t d = 0; d < dims; ++d)
+    if (d != op.head() && q.size(d) != k.size(d)) return py::none();
+  if (!on_current_device(inv_freq) || inv_freq.scalar_type() != at::kDouble || inv_freq.dim() != 1 || !inv_freq.is_contiguous() || inv_freq.requires_grad()) return py::none();
+  if (inv_freq.size(0) < 1 || inv_freq.size(0) > 1024 || 2 * inv_freq.size(0) > q.size(-1)) return py::none();
+  if (positions.has_value()) {
+    const Tensor& p = *positions;
+    if (!on_current_device(p) || (p.scalar_type() != at::kInt && p.scalar_type() != at::kLong)) return py::none();
+    const int64_t S = q.size(op.row());
+    if (!(p.dim() == 1 && p.size(0) == S) && !(layout != 2 && p.dim() == 2 && (p.size(0) == 1 || p.size(0) == q.size(0)) && p.size(1) == S)) return py::none();
+  }
+  if (!node_serves(q, k)) return py::none();
+  variable_list out;
+  Failure f;
+  {
+    py::gil_scoped_release nogil;
+    if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad())) {
+      try {
+        out = RotaryNode::apply(q, k, op);
+      } catch (const Refused& r) {
+        f = r.failure;
+      }
+    } else {
+      out = rotate(f, q, k, op);
+    }
+  }
+  f.raise();
+  return py::make_tuple(out[0], out[1]);
+}
+
 // A node as the interpreter sees it (y.grad_fn): torch's own attributes, with the name and the saved tensors that a Python function's node has.
 template <typename Step>
 PyObject* node_saved_tensors(PyObject* self, void*) {
@@ -784,6 +975,7 @@ void introduce_node(const char* name) {
 PYBIND11_MODULE(alto_mxfp4_host, m) {
   introduce_node<LinearNode>("MXFP4LinearStepBackward");
   introduce_node<GroupedNode>("MXFP4GroupedStepBackward");
+  introduce_node<RotaryNode>("RotaryBackward");
   m.def("bind", &bind);
   m.def("quantize", &quantize);
   m.def("dequantize", &dequantize);
@@ -792,6 +984,8 @@ PYBIND11_MODULE(alto_mxfp4_host, m) {
   m.def("grouped_packed", &grouped_packed);
   m.def("grouped_dw_packed", &grouped_dw_packed);
   m.def("attend", &attend);
+  m.def("attention_gradients", &attention_gradients);
+  m.def("rotary", &rotary);
   m.def("linear_step", &linear_step);
   m.def("linear_saved", &linear_saved);
   m.def("grouped_step", &grouped_step);

@@ -95,14 +95,28 @@ class _Backward(ctypes.Structure):
                 + [("n_seqs", ctypes.c_int), ("causal", ctypes.c_int), ("sm_scale", ctypes.c_float)])
 
 
-def _gradients(grad_out, operands, out, lse, sm_scale, causal, seqlen_k, b4, sl, cu_q, cu_k, dq, dk, dv) -> None:
-    """One backward call on [B, H, S, D] views; ``dq`` or ``dk`` and ``dv`` may be None (not wanted), ``b4`` / ``sl`` come from :func:`_additive`."""
+def _gradients(grad_out, operands, out, lse, sm_scale, causal, seqlen_k, b4, sl, cu_q, cu_k, rows_outer, want_q, want_kv):
+    """(dq, dk, dv) of one backward call on [B, H, S, D] views, None where not wanted; ``rows_outer``: as views of memory with the rows outside the
+    heads.  ``b4`` / ``sl`` come from :func:`_additive`."""
     q, q_scale, k, k_scale, v, v_scale = operands
-    (B, Hq, Sq), (Hk, Sk), Dv = q.shape[:3], k.shape[1:3], v.shape[2]
+    native = rt.host().attention_gradients(grad_out, q, q_scale, k, k_scale, v, v_scale, out, lse, sm_scale, causal, seqlen_k, b4, sl, cu_q or [], cu_k or [], rows_outer,
+                                           want_q, want_kv)
+    if native is not None:
+        return native
+    (B, Hq, Sq), (Hk, Sk), D, Dv = q.shape[:3], k.shape[1:3], 2 * q.shape[3], v.shape[2]
+
+    def empty(want, heads, rows, columns):
+        if not want:
+            return None
+        if rows_outer:
+            return torch.empty((B, rows, heads, columns), dtype=torch.bfloat16, device=q.device).transpose(1, 2)
+        return torch.empty((B, heads, rows, columns), dtype=torch.bfloat16, device=q.device)
+
+    dq, dk, dv = empty(want_q, Hq, Sq, D), empty(want_kv, Hk, Sk, D), empty(want_kv, Hk, Sk, Dv)
     grad_out, out = _readable(grad_out), _readable(out)
     a = _Backward(q_codes=q.data_ptr(), q_scales=q_scale.data_ptr(), k_codes=k.data_ptr(), k_scales=k_scale.data_ptr(), vt_codes=v.data_ptr(),
                   v_scales=v_scale.data_ptr(), dout=grad_out.data_ptr(), out=out.data_ptr(), lse=lse.data_ptr(), bias=rt.ptr(b4), alibi_slopes=rt.ptr(sl),
-                  dq=rt.ptr(dq), dk=rt.ptr(dk), dv=rt.ptr(dv), B=B, Hq=Hq, Hk=Hk, Sq=Sq, Sk=Sk, Sk_used=seqlen_k, D=2 * q.shape[3], Dv=Dv, causal=int(bool(causal)),
+                  dq=rt.ptr(dq), dk=rt.ptr(dk), dv=rt.ptr(dv), B=B, Hq=Hq, Hk=Hk, Sq=Sq, Sk=Sk, Sk_used=seqlen_k, D=D, Dv=Dv, causal=int(bool(causal)),
                   sm_scale=float(sm_scale))
     for name, t in (("dout", grad_out), ("out", out), ("lse", lse), ("dq", dq), ("dk", dk), ("dv", dv)):
         if t is not None:
@@ -121,6 +135,7 @@ def _gradients(grad_out, operands, out, lse, sm_scale, causal, seqlen_k, b4, sl,
         ws = torch.empty(need, dtype=torch.uint8, device=q.device)
         a.workspace, a.workspace_bytes = ws.data_ptr(), need
         check(rt.lib().alto_mxfp4_attention_bwd(ctypes.byref(a), rt.stream_ptr(q.device)), "alto_mxfp4_attention_bwd")
+    return dq, dk, dv
 
 
 def attention_mxfp4_backward(grad_out: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_scale: torch.Tensor, k_scale: torch.Tensor,
@@ -155,9 +170,7 @@ def attention_mxfp4_backward(grad_out: torch.Tensor, q: torch.Tensor, k: torch.T
     cu_q, cu_k = (None if c is None else [int(x) for x in (c.tolist() if isinstance(c, torch.Tensor) else c)] for c in (cu_seqlens_q, cu_seqlens_k))
     assert cu_q is None or len(cu_q) == len(cu_k) >= 2, "cu_seqlens_q and cu_seqlens_k must describe the same number of sequences"
     b4, sl = _additive(bias, alibi_slopes, B, Hq, Sq, sk_used)
-    dq, dk, dv = (torch.empty(shape, dtype=torch.bfloat16, device=q.device) for shape in ((B, Hq, Sq, D), (B, Hk, Sk, D), (B, Hk, Sk, Dv)))
-    _gradients(grad_out, (q, q_scale, k, k_scale, v, v_scale), out, lse, sm_scale, causal, sk_used, b4, sl, cu_q, cu_k, dq, dk, dv)
-    return dq, dk, dv
+    return _gradients(grad_out, (q, q_scale, k, k_scale, v, v_scale), out, lse, sm_scale, causal, sk_used, b4, sl, cu_q, cu_k, False, True, True)
 
 
 def _strides(t: torch.Tensor) -> list:
@@ -230,7 +243,7 @@ class MXFP4AttentionFunction(torch.autograd.Function):
     def forward(ctx, q, k, v, sm_scale, causal, rows_outer, bias, alibi_slopes, cu_q, cu_k):
         torch._check(0.0 < sm_scale < float("inf"), lambda: f"sm_scale {sm_scale}: the backward needs a positive one")
         (B, Hq, Sq, D), (_, Hk, Sk, Dv) = q.shape, v.shape
-        ctx.dtypes, ctx.sizes = (q.dtype, k.dtype, v.dtype), (D, Sk, Dv)
+        ctx.dtypes, ctx.keys = (q.dtype, k.dtype, v.dtype), Sk
         pad = 32 if bias is not None and Sk % 64 == 32 else 0   # (as in _fixed_length)
         if pad:
             k, v = (torch.nn.functional.pad(t, (0, 0, 0, pad)) for t in (k, v))
@@ -251,21 +264,10 @@ class MXFP4AttentionFunction(torch.autograd.Function):
     def backward(ctx, grad_out, _):
         qq, qs, kq, ks, vq, vs, out, lse, b4, sl = ctx.saved_tensors
         sm_scale, causal, rows_outer, cu_q, cu_k = ctx.more
-        D, Sk, Dv = ctx.sizes
         want_q, want_kv = ctx.needs_input_grad[0], ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
-
-        def empty(like, columns):
-            B, H, S = like.shape[:3]
-            if rows_outer:
-                return torch.empty((B, S, H, columns), dtype=torch.bfloat16, device=like.device).transpose(1, 2)
-            return torch.empty((B, H, S, columns), dtype=torch.bfloat16, device=like.device)
-
-        dq = empty(qq, D) if want_q else None
-        dk, dv = (empty(kq, D), empty(kq, Dv)) if want_kv else (None, None)
-        if want_q or want_kv:
-            _gradients(grad_out, (qq, qs, kq, ks, vq, vs), out, lse, sm_scale, causal, Sk, b4, sl, cu_q, cu_k, dq, dk, dv)
+        dq, dk, dv = _gradients(grad_out, (qq, qs, kq, ks, vq, vs), out, lse, sm_scale, causal, ctx.keys, b4, sl, cu_q, cu_k, rows_outer, want_q, want_kv)
         grads = [None if g is None or not need else g[:, :, :n].to(dt) for g, need, n, dt in
-                 zip((dq, dk, dv), ctx.needs_input_grad, (qq.shape[2], Sk, Sk), ctx.dtypes)]
+                 zip((dq, dk, dv), ctx.needs_input_grad, (qq.shape[2], ctx.keys, ctx.keys), ctx.dtypes)]
         return (*grads, None, None, None, None, None, None, None)
 
 

@@ -10,7 +10,6 @@ import math
 from typing import NamedTuple, Optional, Tuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _runtime as rt
 from .._lib import check
@@ -78,6 +77,7 @@ class _Args(ctypes.Structure):
 
 # dims of batch, head and row in each layout (None: there is none)
 _DIMS = {"bhsd": (0, 1, 2), "bshd": (0, 2, 1), "thd": (None, 1, 0)}
+_NATIVE = {"bhsd": 0, "bshd": 1, "thd": 2}
 
 
 def _strides(t: torch.Tensor, layout: str):
@@ -114,24 +114,18 @@ class RotaryFunction(torch.autograd.Function):
     """(q, k) rotated; the backward rotates their gradients back with the same kernel and keeps neither Q nor K."""
 
     @staticmethod
-    def forward(ctx, q, k, inv_freq, positions, interleaved, factor, layout):
+    def forward(ctx, q, k, inv_freq, positions, interleaved, factor, layout, inverse):
         ctx.save_for_backward(inv_freq, positions)
-        ctx.more = interleaved, factor, layout
-        return tuple(_rotate(q, k, inv_freq, positions, interleaved, factor, layout, False)) if k is not None else _rotate(q, None, inv_freq, positions, interleaved, factor, layout, False)[0]
+        ctx.more = interleaved, factor, layout, inverse
+        out = _rotate(q, k, inv_freq, positions, *ctx.more)
+        return tuple(out) if k is not None else out[0]
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dq, dk=None):
         inv_freq, positions = ctx.saved_tensors
-        interleaved, factor, layout = ctx.more
-        want_q, want_k = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
-        if want_q and want_k:
-            dq, dk = _rotate(dq, dk, inv_freq, positions, interleaved, factor, layout, True)
-        elif want_q:
-            dq, dk = _rotate(dq, None, inv_freq, positions, interleaved, factor, layout, True)
-        else:
-            dq, dk = None, _rotate(dk, None, inv_freq, positions, interleaved, factor, layout, True)[0]
-        return dq, dk, None, None, None, None, None
+        interleaved, factor, layout, inverse = ctx.more
+        back = RotaryFunction.apply(dq, dk, inv_freq, positions, interleaved, factor, layout, not inverse)   # (linear: its gradient is one)
+        return (*(back if dk is not None else (back, None)), None, None, None, None, None, None)
 
 
 def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], inv_freq: torch.Tensor, positions: Optional[torch.Tensor] = None, *, interleaved: bool = False,
@@ -145,6 +139,10 @@ def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], inv_freq: torch.Ten
     """
     if layout not in _DIMS:
         raise NotImplementedError(f"layout {layout!r}: 'bhsd', 'bshd' and 'thd' are implemented")
+    if k is not None and q.is_cuda and not torch.compiler.is_compiling():   # one native call; what it declines goes on here
+        out = rt.host().rotary(q, k, inv_freq, positions, bool(interleaved), float(factor), _NATIVE[layout])
+        if out is not None:
+            return out
     rt.require_gpu(q, k, inv_freq, positions)
     dims = 3 if layout == "thd" else 4
     batch, head, row = _DIMS[layout]
@@ -160,6 +158,6 @@ def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], inv_freq: torch.Ten
     for t in (k, inv_freq, positions):
         assert t is None or t.device == q.device, f"tensors on {q.device} and {t.device}"
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
-        return RotaryFunction.apply(q, k, inv_freq, positions, bool(interleaved), float(factor), layout)
+        return RotaryFunction.apply(q, k, inv_freq, positions, bool(interleaved), float(factor), layout, False)
     out = _rotate(q, k, inv_freq, positions, bool(interleaved), float(factor), layout, False)
     return tuple(out) if k is not None else out[0]

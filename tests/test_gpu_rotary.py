@@ -204,3 +204,33 @@ def test_refusals(m):
         m.apply_rotary(q, None, freq, layout="sbhd")
     with pytest.raises(RuntimeError):
         m.apply_rotary(q, None, freq.cpu())
+
+
+def test_native_call_and_python_function_are_the_same(m, monkeypatch):
+    """What the native call declines takes the Python function's way, with the same bits; the second derivative through either is the rotation."""
+    from alto_amd.mxfp4 import _runtime as rt
+    q, k = (t.to(DEV) for t in tensors("bshd", 2, 9, 4, 2, 64, torch.bfloat16))
+    g, h = (t.to(DEV) for t in tensors("bshd", 2, 9, 4, 2, 64, torch.bfloat16, seed=1))
+    freq, positions = m.rotary_frequencies(32)[0].to(DEV), torch.arange(9, 18, device=DEV)
+
+    def everything():
+        x, y = q.clone().requires_grad_(True), k.clone().requires_grad_(True)
+        a, b = m.apply_rotary(x, y, freq, positions, interleaved=True, factor=0.5, layout="bshd")
+        u = g.clone().requires_grad_(True)
+        dx, dy = torch.autograd.grad((a, b), (x, y), (u, h), create_graph=True)
+        (du,) = torch.autograd.grad(dx, u, q)
+        return a.detach(), b.detach(), dx.detach(), dy, du, a.grad_fn.name()
+
+    native = everything()
+    calls = rt.host()
+
+    class Declines:
+        def __getattr__(self, name):
+            return (lambda *a: None) if name == "rotary" else getattr(calls, name)
+
+    monkeypatch.setattr(rt, "host", lambda: Declines())
+    general = everything()
+    assert native[-1] != general[-1]
+    for a, b in zip(native[:-1], general[:-1]):
+        assert torch.equal(a, b)
+    assert torch.equal(native[4], native[0])   # d<R^T u, q>/du = R q
