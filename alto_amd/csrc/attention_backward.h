@@ -461,12 +461,12 @@ __device__ __forceinline__ void attn_bwd_keys_body(const AttnBwdArgs& a, const A
   for (int n = 0; n < 2 * NV; ++n) store_columns(dv_out + b * a.dv_sb + hk * a.dv_sh + at * a.dv_ss, live ? dv[n] : zeros(), 1.0f, n, h);
 }
 
-// Sums of the parts, in their order.  Grid: (heads, key blocks, blocks of 32 columns of dK, then of dV).
+// Sums of the parts, in their order.  Grid: (key blocks by heads, blocks of 32 columns of dK, then of dV).
 template <int NK, int NV>
 __global__ __launch_bounds__(64 * BWD_WAVES) void attn_bwd_sum_kernel(AttnBwdArgs a, AttnBwdSeqs seqs, AttnBwdPlan plan) {
   using T = BwdShape<NK, NV>;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 31, h = lane >> 5;
-  const int heads = a.B * a.Hk, bh = blockIdx.x, z = blockIdx.y, n = blockIdx.z;
+  const int heads = a.B * a.Hk, bh = blockIdx.x % heads, z = blockIdx.x / heads, n = blockIdx.y;
   const AttnBwdBlock w = attn_bwd_block<true>(a, seqs, z);
   const KeyList list = key_list(a, w, plan);
   const int key = w.block * BWD_BLOCK + wave * 32;
@@ -729,7 +729,7 @@ int launch_one(const AttnBwdArgs& a, const AttnBwdSeqs& seqs, const AttnBwdPlan&
   hipLaunchKernelGGL((attn_bwd_kernel<NK, NV, BIASED>), dim3((unsigned)(plan.key_groups + plan.row_groups)), dim3(64 * BWD_WAVES), lds, st, a, seqs, plan);
   if (const int rc = check_launch("attention_bwd")) return rc;
   if (!a.dk || plan.parts == 1) return ALTO_MXFP4_OK;
-  hipLaunchKernelGGL((attn_bwd_sum_kernel<NK, NV>), dim3((unsigned)(a.B * a.Hk), (unsigned)plan.k_blocks, T::ACC), dim3(64 * BWD_WAVES), 0, st, a, seqs, plan);
+  hipLaunchKernelGGL((attn_bwd_sum_kernel<NK, NV>), dim3((unsigned)(a.B * a.Hk * plan.k_blocks), T::ACC), dim3(64 * BWD_WAVES), 0, st, a, seqs, plan);
   return check_launch("attention_bwd");
 }
 
