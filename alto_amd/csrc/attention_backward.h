@@ -9,8 +9,8 @@ namespace alto {
 struct AttnBwdArgs {
   const uint8_t* q;             // codes [B, Hq, Sq, D/2]
   const uint8_t* k;             // codes [B, Hk, Sk, D/2]
-  const uint8_t* q_scales;      // workspace: 8 bytes a tile, that of columns 64 s + 32 h .. + 32 at 4 h + s
-  const uint8_t* k_scales;
+  const uint8_t* q_scales;      // workspace: records of 16 bytes a tile, the scale of columns 64 s + 32 h .. + 32 at 4 h + s, behind them -slope / sm_scale of the head
+  const uint8_t* k_scales;      // workspace: 8 bytes a tile, as Q's
   const __bf16 *k_tiles, *v_tiles, *g_tiles;   // workspace: bf16 tiles (RowTile) of K and V as their codes have them, and of dO
   const float* stats;           // workspace: of every tile of Q, 32 times lse log2(e) (+inf for a row that sees no key), then 32 times -dO . O
   void *dq, *dk, *dv;           // bf16, element (b, h, row, column) at these strides, unit stride along the head dim; dq, or dk and dv, may be NULL: not wanted
@@ -18,8 +18,8 @@ struct AttnBwdArgs {
   int B, Hq, Hk, Sq, Sk, Sk_used;
   float sm_scale;
   int causal;
-  const float* bias;  int64_t bias_sb, bias_sh, bias_sm;
-  const float* alibi; int64_t alibi_sb, alibi_sh;
+  const float* bias;  int64_t bias_sb, bias_sh, bias_sm;   // bias_sm below 2^24
+  int distances;                // the records' slopes count
 };
 
 // Where 16-byte piece `p` of row `row` (columns 8 p .. 8 p + 7) sits in a tile of bf16 rows: the 32 rows' pieces of the same columns side by side,
@@ -101,8 +101,8 @@ __device__ __forceinline__ void load_piece(__amdgpu_buffer_rsrc_t src, const uin
   __builtin_amdgcn_raw_ptr_buffer_load_lds(src, (__attribute__((address_space(3))) void*)to, 16, lane_offset, offset, 0, 0);
 }
 
-__device__ __forceinline__ void load_dwords(__amdgpu_buffer_rsrc_t src, const uint8_t* to, int lane_offset) {
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(src, (__attribute__((address_space(3))) void*)to, 4, lane_offset, 0, 0, 0);
+__device__ __forceinline__ void load_dword(__amdgpu_buffer_rsrc_t src, const uint8_t* to, int lane_offset, int offset) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(src, (__attribute__((address_space(3))) void*)to, 4, lane_offset, offset, 0, 0);
 }
 
 // score register v of half h <-> row 8 (v / 4) + 4 h + v % 4 of the tile
@@ -191,7 +191,7 @@ struct BwdPlace {
 // A tile's codes, statistics (keys) and scales; SMALL loads of each wave, the last waves' repeat the scales
 template <bool KEYS, int NK>
 struct BwdSmall {
-  static constexpr int LOADS = (NK + (KEYS ? 2 : 1) + BWD_WAVES - 1) / BWD_WAVES, CODES = CodeTile<NK>::BYTES;
+  static constexpr int LOADS = (NK + (KEYS ? 2 : 1) + BWD_WAVES - 1) / BWD_WAVES, CODES = CodeTile<NK>::BYTES, RECORD = KEYS ? 16 : 8;
   const uint8_t *codes, *scales;
   const float* stats;
   __device__ __forceinline__ void operator()(uint8_t* to_codes, uint8_t* to_record, const BwdPlace& p, int wave, int lane) const {
@@ -199,8 +199,8 @@ struct BwdSmall {
     for (int l = 0; l < LOADS; ++l) {
       const int i = BWD_WAVES * l + wave;
       if (i < NK) load_piece(buffer(codes + (int64_t)p.at * CODES, CODES), to_codes + 1024 * i, CodeTile<NK>::source(64 * i + lane), 0);
-      else if (KEYS && i == NK) load_dwords(buffer(stats + (int64_t)p.at * 64, 256), to_record, lane * 4);
-      else load_dwords(buffer(scales + (int64_t)p.at * 8, 8), to_record + 256, (lane & 1) * 4);
+      else if (KEYS && i == NK) load_dword(buffer(stats + (int64_t)p.at * 64, 256), to_record, lane * 4, 0);
+      else load_dword(buffer(scales + (int64_t)p.at * RECORD, RECORD), to_record + 256, (lane & (RECORD / 4 - 1)) * 4, 0);
     }
   }
 };
@@ -210,8 +210,48 @@ __device__ __forceinline__ void load_rows(const uint8_t* tiles, uint8_t* to, con
   const int piece = BWD_WAVES * l + wave;
   load_piece(buffer(tiles + (int64_t)p.at * RowTile<W>::BYTES, RowTile<W>::BYTES), to + 1024 * piece, lane * 16 + 1024 * wave, 1024 * BWD_WAVES * l);
 }
-template <int N>
-__device__ __forceinline__ void wait_all_but() { __builtin_amdgcn_s_waitcnt(0x0070 | 0x0F00 | (N & 15)); }
+template <int N>   // loads that may stay under way
+__device__ __forceinline__ void wait_all_but() { __builtin_amdgcn_s_waitcnt(0x0070 | 0x0F00 | (N & 15) | (N >> 4) << 14); }
+template <int N>   // ... but no read or write of the LDS
+__device__ __forceinline__ void wait_lds_and_all_but() { __builtin_amdgcn_s_waitcnt(0x0070 | (N & 15) | (N >> 4) << 14); }
+
+// What is added to the scores: nothing; slopes times distances; a bias, and distances (of slope 0 where there are none).  A score tile's additive terms,
+// over sm_scale, are what its accumulators start with: the rest of a step does not know of them.
+enum { ADD_NOTHING, ADD_DISTANCES, ADD_BIAS };
+
+// A wave's 32 x 32 block of the bias in the LDS, 4 KB of its own: one dword a lane and load straight from memory, which asks nothing of the bias'
+// alignment and needs no register on the way.  (Read element by element where it is used, the same bias made the whole backward of 3 x 8 heads, 480
+// rows, 1056 keys of 192 / 128 three times as long: 181 us for 61 without it.)  Register 4 g + e of lane (r, h) takes the element 8 g + 4 h + e of
+// the side that is in the registers and r of the other.
+template <bool KEYS>
+struct BiasBlock {
+  static constexpr int LOADS = 16, BYTES = 4096;
+  // in: the block's first element
+  __device__ static __forceinline__ void load(const float* in, int64_t row_stride, const uint8_t* to, int lane) {
+    const int stride = 4 * (int)row_stride;
+    const __amdgpu_buffer_rsrc_t src = buffer(in, 0x7FFFFFFF);
+#pragma unroll
+    for (int l = 0; l < LOADS; ++l) {
+      if constexpr (KEYS) {   // 4 rows x 16 keys, in the order of the reading lanes
+        load_dword(src, to + 256 * l, (lane & 3) * stride + (lane >> 2) * 4, (4 * (l >> 1)) * stride + 64 * (l & 1));
+      } else {                // 2 rows x 32 keys, pieces of four keys in an order that changes with the row
+        load_dword(src, to + 256 * l, (lane >> 5) * stride + ((4 * (lane & 31)) ^ ((l & 7) << 4)), 2 * l * stride);
+      }
+    }
+  }
+  __device__ static __forceinline__ v4f_t read(const uint8_t* at, int lane, int g) {
+    if constexpr (KEYS) return *reinterpret_cast<const v4f_t*>(at + 1024 * g + 16 * lane);
+    const int r = lane & 31, h = lane >> 5;
+    return *reinterpret_cast<const v4f_t*>(at + 128 * r + 16 * ((2 * g + h) ^ ((r >> 1) & 7)));
+  }
+};
+
+// A probability.  None is above 1; where the bias is so large that lse has no bits left for the scores, a rounding could say so.
+template <int ADD>
+__device__ __forceinline__ float probability_of(float x, std::integral_constant<int, ADD>) {
+  const float p = __builtin_amdgcn_exp2f(x);
+  return ADD == ADD_BIAS ? __builtin_amdgcn_fmed3f(p, 0.0f, 1.0f) : p;
+}
 
 // Which steps' products are issued where, and what lies between them: a fixed order (sched_barrier).  The read of an operand runs AHEAD products
 // before its use, vector work lies behind each product.  Left to itself the compiler puts every read right in front of its product and waits there.
@@ -223,10 +263,10 @@ constexpr int BWD_AHEAD = 2;
 template <int NK, int NV>
 struct KeysLds {
   using T = BwdShape<NK, NV>;
-  static constexpr int O_V = 4 * T::CODES, O_D = O_V + 3 * T::ROWS_V, O_STATS = O_D + 2 * T::ROWS_D, BYTES = O_STATS + 4 * 512;
+  static constexpr int O_V = 4 * T::CODES, O_D = O_V + 3 * T::ROWS_V, O_STATS = O_D + 2 * T::ROWS_D, O_BIAS = O_STATS + 4 * 512;
 };
 // One step: S and dP of a tile, its probabilities, and its part of the sums.  P is taken from S behind the products of dP, dS behind those of dV.
-template <int NK, int NV, bool BIASED>
+template <int NK, int NV, int ADD>
 __device__ __forceinline__ void attn_bwd_keys_body(const AttnBwdArgs& a, const AttnBwdSeqs& seqs, const AttnBwdPlan& plan, int item, __bf16* __restrict__ dk_out,
                                                    __bf16* __restrict__ dv_out, float* __restrict__ partial, uint8_t* lds) {
   using T = BwdShape<NK, NV>;
@@ -234,6 +274,7 @@ __device__ __forceinline__ void attn_bwd_keys_body(const AttnBwdArgs& a, const A
   using DT = RowTile<64 * NK>;
   using L = KeysLds<NK, NV>;
   using Small = BwdSmall<true, NK>;
+  using Bias = BiasBlock<true>;
   constexpr int D = 64 * NK;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 31, h = lane >> 5;
   const int heads = a.B * a.Hk, group = a.Hq / a.Hk;
@@ -282,7 +323,27 @@ __device__ __forceinline__ void attn_bwd_keys_body(const AttnBwdArgs& a, const A
     const Small small{a.q, a.q_scales, a.stats};
     const uint8_t* const grads = reinterpret_cast<const uint8_t*>(a.g_tiles);
     const int code_base = lane * 16, row_base[2] = {VT::row_base(lane, 0), VT::row_base(lane, 1)}, column_base[2] = {VT::column_base(lane, 0), VT::column_base(lane, 1)};
-    const float c2 = a.sm_scale * ATTN_RCP_LN2;
+    const float c2 = a.sm_scale * ATTN_RCP_LN2, inverse_scale = 1.0f / a.sm_scale;
+    // The additive terms of tile `i`
+    v16f_t S;
+    uint8_t* const at_bias = lds + L::O_BIAS + wave * Bias::BYTES;
+    auto load_bias = [&](const BwdPlace& p) {
+      const int hq = p.at / tiles - b * a.Hq;
+      Bias::load(a.bias + b * a.bias_sb + hq * a.bias_sh + (int64_t)(32 * p.tile) * a.bias_sm + (live ? key0 : 0), a.bias_sm, at_bias, lane);
+    };
+    auto read_bias = [&](int g) {
+      const v4f_t x = Bias::read(at_bias, lane, g);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) S[4 * g + e] = x[e];
+    };
+    auto add = [&](const BwdPlace& p, int i, int g) {
+      const float slope = reinterpret_cast<const float*>(lds + L::O_STATS + (i & 3) * 512 + 256)[2], away = (float)(32 * p.tile + 4 * h + shift - key0 - r);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float x = slope * __builtin_fabsf(away + (float)(8 * g + e));
+        S[4 * g + e] = ADD == ADD_BIAS ? __builtin_fmaf(S[4 * g + e], inverse_scale, x) : x;
+      }
+    };
     // Eight columns of one row of tile `i`'s values, from its codes: dword `j` of row tid % 32, j = tid / 32 + 8 u
     uint32_t eight = 0;
     float eight_scale = 0.0f;
@@ -299,6 +360,7 @@ __device__ __forceinline__ void attn_bwd_keys_body(const AttnBwdArgs& a, const A
     auto load_small = [&](const BwdPlace& p, int i) { small(lds + (i & 3) * T::CODES, lds + L::O_STATS + (i & 3) * 512, p, wave, lane); };
 
     BwdPlace p0 = next(), p1 = next(), p2 = next();
+    if constexpr (ADD == ADD_BIAS) load_bias(p0);
     load_small(p0, 0);
     load_small(p1, 1);
 #pragma unroll
@@ -313,8 +375,16 @@ __device__ __forceinline__ void attn_bwd_keys_body(const AttnBwdArgs& a, const A
       read_codes(0, u);
       write_values(0, u);
     }
+    if constexpr (ADD != ADD_NOTHING) {
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        if constexpr (ADD == ADD_BIAS) read_bias(g);
+        add(p0, 0, g);
+      }
+    }
     __builtin_amdgcn_s_waitcnt(0xC07F);   // lgkmcnt(0)
     asm volatile("s_barrier" ::: "memory");
+    if constexpr (ADD == ADD_BIAS) load_bias(p1);
 
     constexpr int NS = NK, NI = 4 * NV, NF = 4 * NV, NG = 4 * NK, N = NS + NI + NF + NG, AHEAD = BWD_AHEAD;
     int slot = 0;
@@ -330,7 +400,8 @@ __device__ __forceinline__ void attn_bwd_keys_body(const AttnBwdArgs& a, const A
         at_d[i] = lds + L::O_D + (t & 1) * T::ROWS_D + column_base[i];
       }
       const float* const stats = reinterpret_cast<const float*>(lds + L::O_STATS + (t & 3) * 512) + 4 * h;
-      v16f_t S, dp;
+      if constexpr (ADD == ADD_NOTHING) S = zeros();
+      v16f_t dp;
       v4f_t l4[2];
       bf16x8_t frag[AHEAD + 1];
       uint32_t pk[8], dsk[8];
@@ -351,7 +422,7 @@ __device__ __forceinline__ void attn_bwd_keys_body(const AttnBwdArgs& a, const A
         const bf16x8_t& x = frag[i % (AHEAD + 1)];
         if constexpr (i < NS) {
           const v4i_t q = __builtin_bit_cast(v4i_t, x);
-          S = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(v8i_t{q[0], q[1], q[2], q[3], 0, 0, 0, 0}, xf[i], i == 0 ? zeros() : S, 4, 4, i, (int)sc, i, (int)x_scales);
+          S = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(v8i_t{q[0], q[1], q[2], q[3], 0, 0, 0, 0}, xf[i], S, 4, 4, i, (int)sc, i, (int)x_scales);
         } else if constexpr (i < NS + NI) {
           dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, yf[i - NS], dp, 0, 0, 0);
         } else if constexpr (i < NS + NI + NF) {
@@ -367,8 +438,7 @@ __device__ __forceinline__ void attn_bwd_keys_body(const AttnBwdArgs& a, const A
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           const int v = 2 * i + k;
-          float x = BIASED ? S[v] - l4[(v >> 2) & 1][v & 3] : __builtin_fmaf(S[v], c2, -l4[(v >> 2) & 1][v & 3]);
-          S[v] = __builtin_amdgcn_exp2f(x);
+          S[v] = probability_of(__builtin_fmaf(S[v], c2, -l4[(v >> 2) & 1][v & 3]), std::integral_constant<int, ADD>{});
         }
         if ((i & 1) == 1 && i / 2 + 2 < 4) read_stats(i / 2 + 2);   // (the group's last use is behind us)
       };
@@ -388,19 +458,9 @@ __device__ __forceinline__ void attn_bwd_keys_body(const AttnBwdArgs& a, const A
       static_for<N>([&](auto ic) {
         constexpr int i = decltype(ic)::value;
         read(std::integral_constant<int, i + AHEAD>{});
+        if constexpr (ADD == ADD_BIAS && i == NS + NI + NF) wait_all_but<0>();   // the last step's loads, the bias of the next tile among them
         product(ic);
         if constexpr (i == NS - 1) {
-          if constexpr (BIASED) {   // scores into the base-2 domain with their additive terms
-#pragma unroll
-            for (int v = 0; v < 16; ++v) {
-              const int row = 32 * p0.tile + score_row(v, h), key = live ? key0 + r : 0;
-              const int64_t hq = p0.at / tiles - b * a.Hq;
-              float x = S[v] * c2;
-              if (a.bias) x = __builtin_fmaf(a.bias[b * a.bias_sb + hq * a.bias_sh + row * a.bias_sm + key], ATTN_RCP_LN2, x);
-              if (a.alibi) x = __builtin_fmaf(-a.alibi[b * a.alibi_sb + hq * a.alibi_sh] * ATTN_RCP_LN2, __builtin_fabsf((float)(row + shift - key)), x);
-              S[v] = x;
-            }
-          }
           if (a.causal && 32 * p0.tile + shift <= key0) {   // the diagonal's tile, or one before it, that another wave of the workgroup needs
             asm volatile("" ::: "memory");   // keep this a branch: most tiles skip it
             const int hidden = key0 + r - 32 * p0.tile - shift;
@@ -429,6 +489,15 @@ __device__ __forceinline__ void attn_bwd_keys_body(const AttnBwdArgs& a, const A
           if constexpr (j >= 1 && j <= NV) load_rows<64 * NV>(grads, lds + L::O_V + two_on * T::ROWS_V, p2, j - 1, wave, lane);
           if constexpr (j % 4 == 0) read_codes(t + 1, j / 4);
           if constexpr (j % 4 == 3) write_values(t + 1, j / 4);
+          if constexpr (ADD == ADD_BIAS && j < 2) {
+            read_bias(2 * j);
+            read_bias(2 * j + 1);
+          }
+          if constexpr (ADD != ADD_NOTHING && (j == 2 || j == 3)) {
+            add(p1, t + 1, 2 * (j - 2));
+            add(p1, t + 1, 2 * (j - 2) + 1);
+            if constexpr (ADD == ADD_BIAS && j == 3) load_bias(p2);   // (where the block lay that has just been read)
+          }
         }
         __builtin_amdgcn_sched_barrier(0);
       });
@@ -436,7 +505,7 @@ __device__ __forceinline__ void attn_bwd_keys_body(const AttnBwdArgs& a, const A
       p1 = p2;
       p2 = p3;
       slot = slot == 2 ? 0 : slot + 1;
-      __builtin_amdgcn_s_waitcnt(0x0070 | ((Small::LOADS + NV) & 15));   // all but this step's loads, and lgkmcnt(0): the values are written
+      wait_lds_and_all_but<Small::LOADS + NV + (ADD == ADD_BIAS ? Bias::LOADS : 0)>();   // all but this step's loads; the values are written
       asm volatile("s_barrier" ::: "memory");
     }
     wait_all_but<0>();   // (the last loads into the LDS, which nobody reads, before it is given back)
@@ -493,10 +562,10 @@ __global__ __launch_bounds__(64 * BWD_WAVES) void attn_bwd_sum_kernel(AttnBwdArg
 template <int NK, int NV>
 struct RowsLds {   // three slots of codes, V and K, four of scales
   using T = BwdShape<NK, NV>;
-  static constexpr int O_V = 3 * T::CODES, O_D = O_V + 3 * T::ROWS_V, O_STATS = O_D + 3 * T::ROWS_D, BYTES = O_STATS + 4 * 512;
+  static constexpr int O_V = 3 * T::CODES, O_D = O_V + 3 * T::ROWS_V, O_STATS = O_D + 3 * T::ROWS_D, O_BIAS = O_STATS + 4 * 512;
 };
 // Three stages in one step: S and dP of tile t + 1 and the sums' product with tile t - 1 on the matrix pipe, dS of tile t on the vector pipe.
-template <int NK, int NV, bool BIASED>
+template <int NK, int NV, int ADD>
 __device__ __forceinline__ void attn_bwd_rows_body(const AttnBwdArgs& a, const AttnBwdSeqs& seqs, const AttnBwdPlan& plan, int item, __bf16* __restrict__ dq_out, uint8_t* lds) {
   using T = BwdShape<NK, NV>;
   using VT = RowTile<64 * NV>;
@@ -505,6 +574,7 @@ __device__ __forceinline__ void attn_bwd_rows_body(const AttnBwdArgs& a, const A
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 31, h = lane >> 5;
   using L = RowsLds<NK, NV>;
   using Small = BwdSmall<false, NK>;
+  using Bias = BiasBlock<false>;
   const int heads = a.B * a.Hq;
   const HeadItem it = head_item(item, heads);
   const int bh = it.head, b = bh / a.Hq, hq = bh % a.Hq, hk = hq / (a.Hq / a.Hk);
@@ -526,14 +596,15 @@ __device__ __forceinline__ void attn_bwd_rows_body(const AttnBwdArgs& a, const A
   v16f_t nd;
 #pragma unroll
   for (int s = 0; s < NK; ++s) xf[s] = frag16(a.q + ((int64_t)own_tile * 32 + r) * (D / 2) + s * 32 + h * 16);
-  const uint32_t x_scales = *reinterpret_cast<const uint32_t*>(a.q_scales + (int64_t)own_tile * 8 + 4 * h);
+  const uint32_t x_scales = *reinterpret_cast<const uint32_t*>(a.q_scales + (int64_t)own_tile * 16 + 4 * h);
   const uint8_t* y0 = reinterpret_cast<const uint8_t*>(a.g_tiles) + (int64_t)own_tile * T::ROWS_V;
 #pragma unroll
   for (int i = 0; i < 4 * NV; ++i) yf[i] = VT::row_frag(y0 + VT::row_base(lane, i & 1), i);
   const float lse2 = a.stats[(int64_t)own_tile * 64 + r], minus_d = a.stats[(int64_t)own_tile * 64 + 32 + r];
 #pragma unroll
   for (int v = 0; v < 16; ++v) nd[v] = minus_d;
-  const float c2 = a.sm_scale * ATTN_RCP_LN2, slope2 = BIASED && a.alibi ? a.alibi[b * a.alibi_sb + hq * a.alibi_sh] * ATTN_RCP_LN2 : 0.0f;
+  const float c2 = a.sm_scale * ATTN_RCP_LN2, inverse_scale = 1.0f / a.sm_scale;
+  const float slope = ADD == ADD_NOTHING ? 0.0f : *reinterpret_cast<const float*>(a.q_scales + (int64_t)own_tile * 16 + 8);
 
   const Small small{a.k, a.k_scales, nullptr};
   const int code_base = lane * 16, row_base[2] = {VT::row_base(lane, 0), VT::row_base(lane, 1)}, column_base[2] = {DT::column_base(lane, 0), DT::column_base(lane, 1)};
@@ -559,15 +630,30 @@ __device__ __forceinline__ void attn_bwd_rows_body(const AttnBwdArgs& a, const A
   };
 
   // The products in order: those of the scores, then by turns one of dP and one of the sums.
-  constexpr int NS = NK, NI = 4 * NV, NF = 4 * NK, AHEAD = BWD_AHEAD, HALVES = 16;
+  constexpr int NS = NK, NI = 4 * NV, NF = 4 * NK, AHEAD = BWD_AHEAD, HALVES = 16, STEP_LOADS = Small::LOADS + NV + NK;
   struct Op {
     int kind, j;   // 0: S, 1: dP, 2: sums
   };
   struct Scores {
     v16f_t S, dp;
   };
+  // The additive terms of tile `i`, in the registers where its scores will be
+  uint8_t* const at_bias = lds + L::O_BIAS + wave * Bias::BYTES;
+  auto load_bias = [&](int i) {
+    Bias::load(a.bias + b * a.bias_sb + hq * a.bias_sh + (int64_t)(live ? row0 : 0) * a.bias_sm + 32 * place(i).tile, a.bias_sm, at_bias, lane);
+  };
+  auto add = [&](int i, int g, v16f_t& S) {
+    const float away = (float)(row0 + r + shift - 32 * i - 4 * h);
+    v4f_t x;
+    if constexpr (ADD == ADD_BIAS) x = Bias::read(at_bias, lane, g);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float y = slope * __builtin_fabsf(away - (float)(8 * g + e));
+      S[4 * g + e] = ADD == ADD_BIAS ? __builtin_fmaf(x[e], inverse_scale, y) : y;
+    }
+  };
   // (RUN: the first step only has scores to compute)
-  auto step = [&](auto run, int t, int slot, const Scores& from, const bf16x8_t (&f)[2], Scores& to, bf16x8_t (&f_next)[2]) {
+  auto step = [&](auto run, int t, int slot, Scores& from, const bf16x8_t (&f)[2], Scores& to, bf16x8_t (&f_next)[2]) {
     constexpr bool RUN = decltype(run)::value;
     const int after = slot == 2 ? 0 : slot + 1, before = slot == 0 ? 2 : slot - 1;
     const uint8_t* const at_codes = lds + after * T::CODES + code_base;
@@ -606,7 +692,7 @@ __device__ __forceinline__ void attn_bwd_rows_body(const AttnBwdArgs& a, const A
       const bf16x8_t& x = frag[i % (AHEAD + 1)];
       if constexpr (o.kind == 0) {
         const v4i_t q = __builtin_bit_cast(v4i_t, x);
-        to.S = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(v8i_t{q[0], q[1], q[2], q[3], 0, 0, 0, 0}, xf[o.j], o.j == 0 ? zeros() : to.S, 4, 4, o.j, (int)sc, o.j, (int)x_scales);
+        to.S = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(v8i_t{q[0], q[1], q[2], q[3], 0, 0, 0, 0}, xf[o.j], ADD == ADD_NOTHING && o.j == 0 ? zeros() : to.S, 4, 4, o.j, (int)sc, o.j, (int)x_scales);
       } else if constexpr (o.kind == 1) {
         to.dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, yf[o.j], o.j == 0 ? nd : to.dp, 0, 0, 0);
       } else {
@@ -622,17 +708,15 @@ __device__ __forceinline__ void attn_bwd_rows_body(const AttnBwdArgs& a, const A
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           const int v = 2 * i + k;
-          float x = __builtin_fmaf(from.S[v], c2, -lse2);
-          if constexpr (BIASED) {
-            const int key = 32 * t + score_row(v, h), row = live ? row0 + r : 0;
-            if (a.bias) x = __builtin_fmaf(a.bias[b * a.bias_sb + hq * a.bias_sh + row * a.bias_sm + key], ATTN_RCP_LN2, x);
-            x = __builtin_fmaf(-slope2, __builtin_fabsf((float)(row + shift - key)), x);
-          }
-          e[i][k] = __builtin_amdgcn_exp2f(x);
+          e[i][k] = probability_of(__builtin_fmaf(from.S[v], c2, -lse2), std::integral_constant<int, ADD>{});
         }
       } else {
         out[i] = pack_bf16x2(e[i][0] * from.dp[2 * i], e[i][1] * from.dp[2 * i + 1]) & seen[i];
         asm volatile("" : "+v"(out[i]));   // (here: otherwise it is moved behind the step, to where it is used)
+        if constexpr (ADD != ADD_NOTHING && (i & 1) == 1) {
+          if constexpr (ADD == ADD_BIAS && i == 1) wait_all_but<STEP_LOADS>();   // the last step's loads, the bias of tile t + 2 among them
+          add(t + 2, i >> 1, from.S);
+        }
       }
     };
     __builtin_amdgcn_sched_barrier(0);
@@ -666,6 +750,28 @@ __device__ __forceinline__ void attn_bwd_rows_body(const AttnBwdArgs& a, const A
 #pragma unroll
     for (int l = 0; l < NK; ++l) load_rows<64 * NK>(reinterpret_cast<const uint8_t*>(a.k_tiles), lds + L::O_D + slot * T::ROWS_D, place(i), l, wave, lane);
   };
+  Scores x, y;
+  if constexpr (ADD == ADD_BIAS) {
+    load_bias(0);
+    wait_all_but<0>();
+  }
+  if constexpr (ADD != ADD_NOTHING) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g) add(0, g, x.S);
+  }
+  if constexpr (ADD == ADD_BIAS) {
+    __builtin_amdgcn_s_waitcnt(0xC07F);   // lgkmcnt(0): the block is read
+    load_bias(1);
+    wait_all_but<0>();
+  }
+  if constexpr (ADD != ADD_NOTHING) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g) add(1, g, y.S);
+  }
+  if constexpr (ADD == ADD_BIAS) {
+    __builtin_amdgcn_s_waitcnt(0xC07F);
+    load_bias(2);
+  }
   load_scores(0, 0);
   load_factor(0, 0);
   load_factor(0, 2);   // (what the first step multiplies with zeros)
@@ -673,19 +779,22 @@ __device__ __forceinline__ void attn_bwd_rows_body(const AttnBwdArgs& a, const A
   load_scores(2, 2);
   wait_all_but<Small::LOADS + NV>();
   asm volatile("s_barrier" ::: "memory");
-  Scores x, y;
   bf16x8_t f[2], g[2];
   f[0] = f[1] = __builtin_bit_cast(bf16x8_t, v4i_t{0, 0, 0, 0});
   step(std::false_type{}, -1, 2, x, f, x, f);
   int slot = 0;   // of tile t
-  auto whole_step = [&](int t, const Scores& from, const bf16x8_t (&f_now)[2], Scores& to, bf16x8_t (&f_next)[2]) {
+  auto whole_step = [&](int t, Scores& from, const bf16x8_t (&f_now)[2], Scores& to, bf16x8_t (&f_next)[2]) {
     const int after = slot == 2 ? 0 : slot + 1;
     load_scores(t + 3, slot);
     load_factor(t + 1, after);
     look(t);
     step(std::true_type{}, t, slot, from, f_now, to, f_next);
     slot = after;
-    wait_all_but<Small::LOADS + NV + NK>();
+    if constexpr (ADD == ADD_BIAS) {
+      __builtin_amdgcn_s_waitcnt(0xC07F);
+      load_bias(t + 3);   // (where the block lay that has just been read)
+    }
+    wait_all_but<STEP_LOADS + (ADD == ADD_BIAS ? Bias::LOADS : 0)>();
     asm volatile("s_barrier" ::: "memory");
   };
   int t = 0;
@@ -712,21 +821,21 @@ __device__ __forceinline__ void attn_bwd_rows_body(const AttnBwdArgs& a, const A
   for (int n = 0; n < 2 * NK; ++n) store_columns(row, acc[n], a.sm_scale, n, h);
 }
 
-template <int NK, int NV, bool BIASED>
+template <int NK, int NV, int ADD>
 __global__ __launch_bounds__(64 * BWD_WAVES, NK > 2 ? 1 : 2) void attn_bwd_kernel(AttnBwdArgs a, AttnBwdSeqs seqs, AttnBwdPlan plan) {
   extern __shared__ __attribute__((aligned(256))) uint8_t lds[];
   const int item = (int)blockIdx.x;
-  if (item < plan.key_groups) attn_bwd_keys_body<NK, NV, BIASED>(a, seqs, plan, item, reinterpret_cast<__bf16*>(a.dk), reinterpret_cast<__bf16*>(a.dv), plan.partial, lds);
-  else attn_bwd_rows_body<NK, NV, BIASED>(a, seqs, plan, item - plan.key_groups, reinterpret_cast<__bf16*>(a.dq), lds);
+  if (item < plan.key_groups) attn_bwd_keys_body<NK, NV, ADD>(a, seqs, plan, item, reinterpret_cast<__bf16*>(a.dk), reinterpret_cast<__bf16*>(a.dv), plan.partial, lds);
+  else attn_bwd_rows_body<NK, NV, ADD>(a, seqs, plan, item - plan.key_groups, reinterpret_cast<__bf16*>(a.dq), lds);
 }
 
-template <int NK, int NV, bool BIASED>
+template <int NK, int NV, int ADD>
 int launch_one(const AttnBwdArgs& a, const AttnBwdSeqs& seqs, const AttnBwdPlan& plan, hipStream_t st) {
   using T = BwdShape<NK, NV>;
-  constexpr int lds = KeysLds<NK, NV>::BYTES > RowsLds<NK, NV>::BYTES ? KeysLds<NK, NV>::BYTES : RowsLds<NK, NV>::BYTES;
+  constexpr int keys = KeysLds<NK, NV>::O_BIAS, rows = RowsLds<NK, NV>::O_BIAS, lds = (keys > rows ? keys : rows) + (ADD == ADD_BIAS ? BWD_WAVES * 4096 : 0);
   static LdsLimit limit;
-  if (const int rc = limit.raise((const void*)attn_bwd_kernel<NK, NV, BIASED>, lds, "attention_bwd")) return rc;
-  hipLaunchKernelGGL((attn_bwd_kernel<NK, NV, BIASED>), dim3((unsigned)(plan.key_groups + plan.row_groups)), dim3(64 * BWD_WAVES), lds, st, a, seqs, plan);
+  if (const int rc = limit.raise((const void*)attn_bwd_kernel<NK, NV, ADD>, lds, "attention_bwd")) return rc;
+  hipLaunchKernelGGL((attn_bwd_kernel<NK, NV, ADD>), dim3((unsigned)(plan.key_groups + plan.row_groups)), dim3(64 * BWD_WAVES), lds, st, a, seqs, plan);
   if (const int rc = check_launch("attention_bwd")) return rc;
   if (!a.dk || plan.parts == 1) return ALTO_MXFP4_OK;
   hipLaunchKernelGGL((attn_bwd_sum_kernel<NK, NV>), dim3((unsigned)(a.B * a.Hk * plan.k_blocks), T::ACC), dim3(64 * BWD_WAVES), 0, st, a, seqs, plan);
@@ -737,9 +846,16 @@ int launch_one(const AttnBwdArgs& a, const AttnBwdSeqs& seqs, const AttnBwdPlan&
 
 template <int NK>
 int launch_attn_bwd(const AttnBwdArgs& a, const AttnBwdSeqs& seqs, const AttnBwdPlan& plan, int64_t Dv, hipStream_t st) {
-  const bool biased = a.bias || a.alibi;
-  if (Dv == 64) return biased ? launch_one<NK, 1, true>(a, seqs, plan, st) : launch_one<NK, 1, false>(a, seqs, plan, st);
-  return biased ? launch_one<NK, 2, true>(a, seqs, plan, st) : launch_one<NK, 2, false>(a, seqs, plan, st);
+  const int add = a.bias ? ADD_BIAS : (a.distances ? ADD_DISTANCES : ADD_NOTHING);
+  auto one = [&](auto nv) {
+    constexpr int NV = decltype(nv)::value;
+    switch (add) {
+      case ADD_BIAS: return launch_one<NK, NV, ADD_BIAS>(a, seqs, plan, st);
+      case ADD_DISTANCES: return launch_one<NK, NV, ADD_DISTANCES>(a, seqs, plan, st);
+      default: return launch_one<NK, NV, ADD_NOTHING>(a, seqs, plan, st);
+    }
+  };
+  return Dv == 64 ? one(std::integral_constant<int, 1>{}) : one(std::integral_constant<int, 2>{});
 }
 #endif
 

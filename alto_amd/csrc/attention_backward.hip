@@ -28,8 +28,9 @@ namespace {
 struct PrepareArgs {
   const uint8_t *qs, *k, *ks, *vt, *vs;
   const __bf16 *dout, *out;
-  const float* lse;
-  int64_t do_sb, do_sh, do_ss, o_sb, o_sh, o_ss, l_sb, l_sh, l_ss;
+  const float *lse, *alibi;
+  float sm_scale;
+  int64_t alibi_sb, alibi_sh, do_sb, do_sh, do_ss, o_sb, o_sh, o_ss, l_sb, l_sh, l_ss;
   int Hq, Hk, Sq, Sk, D, Dv;
   int q_tiles;   // B Hq Sq / 32
   float* stats;
@@ -38,9 +39,9 @@ struct PrepareArgs {
 };
 
 // The scale bytes of a tile of Q or K in the order of the score products
-__device__ __forceinline__ void order_scales(const uint8_t* scales, int64_t tile, int bands, uint8_t* ordered) {
+__device__ __forceinline__ void order_scales(const uint8_t* scales, int64_t tile, int bands, uint8_t* record) {
   const int tid = threadIdx.x, c = 2 * (tid & 3) + (tid >> 2);
-  if (tid < 8) ordered[tile * 8 + tid] = c < bands ? scales[tile * bands + c] : 127;
+  if (tid < 8) record[tid] = c < bands ? scales[tile * bands + c] : 127;
 }
 
 // The values of a tile of K
@@ -61,11 +62,12 @@ __global__ __launch_bounds__(256) void attn_bwd_prepare_kernel(const PrepareArgs
   const int tid = threadIdx.x;
   int64_t tile = blockIdx.x;
   if (tile < a.q_tiles) {
-    order_scales(a.qs, tile, a.D / 32, a.q_scales);
+    order_scales(a.qs, tile, a.D / 32, a.q_scales + tile * 16);
     v4i_t* const grad = reinterpret_cast<v4i_t*>(turned);
     const int r = tid >> 3, c = tid & 7;
     const int64_t row = tile * 32 + r, bh = row / a.Sq;
     const int64_t b = bh / a.Hq, h = bh % a.Hq, i = row % a.Sq;
+    if (tid == 0) *reinterpret_cast<float*>(a.q_scales + tile * 16 + 8) = a.alibi ? -a.alibi[b * a.alibi_sb + h * a.alibi_sh] / a.sm_scale : 0.0f;
     const v4i_t* go = reinterpret_cast<const v4i_t*>(a.dout + b * a.do_sb + h * a.do_sh + i * a.do_ss);
     const v4i_t* o = reinterpret_cast<const v4i_t*>(a.out + b * a.o_sb + h * a.o_sh + i * a.o_ss);
     float d = 0.0f;
@@ -91,7 +93,7 @@ __global__ __launch_bounds__(256) void attn_bwd_prepare_kernel(const PrepareArgs
     return;
   }
   tile -= a.q_tiles;
-  order_scales(a.ks, tile, a.D / 32, a.k_scales);
+  order_scales(a.ks, tile, a.D / 32, a.k_scales + tile * 8);
   decode_tile(a.k, a.ks, tile, a.D, a.k_rows);
   const int lane = tid & 63, wave = tid >> 6, bands = a.Sk / 32;
   if (wave * 32 >= a.Dv) return;
@@ -159,7 +161,7 @@ Workspace workspace(const alto_mxfp4_attention_bwd_t& p, const Cuts& cuts) {
   int64_t at = 0;
   auto take = [&](int64_t& p, int64_t n) { p = at; at += (n + 255) / 256 * 256; };
   take(w.stats, B * Hq * Sq * 8);
-  take(w.q_scales, B * Hq * (Sq / 32) * 8);
+  take(w.q_scales, B * Hq * (Sq / 32) * 16);
   take(w.k_scales, B * Hk * (Sk / 32) * 8);
   take(w.k_rows, B * Hk * Sk * D * 2);
   take(w.v_rows, B * Hk * Sk * Dv * 2);
@@ -214,6 +216,8 @@ static int attention_bwd(const alto_mxfp4_attention_bwd_t& p, hipStream_t st) {
   for (const int64_t s : {p.lse_sb, p.lse_sh, p.lse_ss, p.bias_sb, p.bias_sh, p.bias_sm, p.alibi_sb, p.alibi_sh})
     ALTO_REQUIRE(s >= 0 && s < (1ll << 40), "attention_bwd: strides must be non-negative");
   ALTO_REQUIRE(p.sm_scale > 0.0f && p.sm_scale < __builtin_inff(), "attention_bwd: sm_scale must be positive and finite");
+  ALTO_REQUIRE(p.sm_scale >= 0x1p-64f || (!p.bias && !p.alibi_slopes), "attention_bwd: sm_scale must be at least 2^-64 with a bias or slopes");
+  ALTO_REQUIRE(!p.bias || p.bias_sm < (1 << 24), "attention_bwd: rows of the bias must be less than 2^24 elements apart");
   const Cuts cuts = cut(p);
   const Workspace w = workspace(p, cuts);
   ALTO_REQUIRE(p.workspace_bytes >= w.total && (uintptr_t)p.workspace % 256 == 0, "attention_bwd: the workspace must be 256-byte aligned and hold %lld bytes", (long long)w.total);
@@ -229,7 +233,7 @@ static int attention_bwd(const alto_mxfp4_attention_bwd_t& p, hipStream_t st) {
   PrepareArgs r{};
   r.qs = (const uint8_t*)p.q_scales; r.k = (const uint8_t*)p.k_codes; r.ks = (const uint8_t*)p.k_scales;
   r.vt = (const uint8_t*)p.vt_codes; r.vs = (const uint8_t*)p.v_scales;
-  r.dout = (const __bf16*)p.dout; r.out = (const __bf16*)p.out; r.lse = p.lse;
+  r.dout = (const __bf16*)p.dout; r.out = (const __bf16*)p.out; r.lse = p.lse; r.alibi = p.alibi_slopes; r.alibi_sb = p.alibi_sb; r.alibi_sh = p.alibi_sh; r.sm_scale = p.sm_scale;
   r.do_sb = p.dout_sb; r.do_sh = p.dout_sh; r.do_ss = p.dout_ss; r.o_sb = p.out_sb; r.o_sh = p.out_sh; r.o_ss = p.out_ss;
   r.l_sb = p.lse_sb; r.l_sh = p.lse_sh; r.l_ss = p.lse_ss;
   r.Hq = (int)p.Hq; r.Hk = (int)p.Hk; r.Sq = (int)p.Sq; r.Sk = (int)p.Sk; r.D = (int)p.D; r.Dv = (int)p.Dv;
@@ -246,7 +250,7 @@ static int attention_bwd(const alto_mxfp4_attention_bwd_t& p, hipStream_t st) {
   a.dq_sb = p.dq_sb; a.dq_sh = p.dq_sh; a.dq_ss = p.dq_ss; a.dk_sb = p.dk_sb; a.dk_sh = p.dk_sh; a.dk_ss = p.dk_ss; a.dv_sb = p.dv_sb; a.dv_sh = p.dv_sh; a.dv_ss = p.dv_ss;
   a.B = (int)p.B; a.Hq = (int)p.Hq; a.Hk = (int)p.Hk; a.Sq = (int)p.Sq; a.Sk = (int)p.Sk; a.Sk_used = (int)p.Sk_used;
   a.sm_scale = p.sm_scale; a.causal = p.causal ? 1 : 0;
-  a.bias = p.bias; a.bias_sb = p.bias_sb; a.bias_sh = p.bias_sh; a.bias_sm = p.bias_sm; a.alibi = p.alibi_slopes; a.alibi_sb = p.alibi_sb; a.alibi_sh = p.alibi_sh;
+  a.bias = p.bias; a.bias_sb = p.bias_sb; a.bias_sh = p.bias_sh; a.bias_sm = p.bias_sm; a.distances = p.alibi_slopes != nullptr;
   const int row_block = BWD_BLOCK, key_block = row_block;
   auto go = [&](const AttnBwdSeqs& s, int q_blocks, int k_blocks) {
     AttnBwdPlan plan{q_blocks, k_blocks, cuts.parts, cuts.chunk, 0, 0, (float*)(ws + w.partial)};
