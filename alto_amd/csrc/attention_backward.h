@@ -9,10 +9,9 @@ namespace alto {
 struct AttnBwdArgs {
   const uint8_t* q;             // codes [B, Hq, Sq, D/2]
   const uint8_t* k;             // codes [B, Hk, Sk, D/2]
-  const uint8_t* q_scales;      // workspace: records of 16 bytes a tile, the scale of columns 64 s + 32 h .. + 32 at 4 h + s, behind them -slope / sm_scale of the head
-  const uint8_t* k_scales;      // workspace: 8 bytes a tile, as Q's
+  const struct QRecord* q_records;   // workspace: one of every tile
+  const struct KRecord* k_records;
   const __bf16 *k_tiles, *v_tiles, *g_tiles;   // workspace: bf16 tiles (RowTile) of K and V as their codes have them, and of dO
-  const float* stats;           // workspace: of every tile of Q, 32 times lse log2(e) (+inf for a row that sees no key), then 32 times -dO . O
   void *dq, *dk, *dv;           // bf16, element (b, h, row, column) at these strides, unit stride along the head dim; dq, or dk and dv, may be NULL: not wanted
   int64_t dq_sb, dq_sh, dq_ss, dk_sb, dk_sh, dk_ss, dv_sb, dv_sh, dv_ss;
   int B, Hq, Hk, Sq, Sk, Sk_used;
@@ -27,6 +26,17 @@ struct AttnBwdArgs {
 // consecutive rows at one piece) and transposed ones (4 rows x 64 bytes); either meets all banks of the LDS once, and all of a tile's
 // fragments sit at constant distances from one or two addresses a lane.
 __host__ __device__ __forceinline__ constexpr int tile_piece(int row, int p) { return p * 32 + (row ^ ((p & 3) << 2)); }
+
+// What a tile has besides its rows.  The scale byte of columns 64 s + 32 h .. + 32 is at 4 h + s, the order of the score products.
+struct KRecord {
+  uint8_t scales[8], unused[8];
+};
+struct QRecord {
+  float lse2[32], minus_d[32];   // lse log2(e) (+inf for a row that sees no key), -dO . O
+  uint8_t scales[8];
+  float slope;                   // -slope / sm_scale of the head
+  float unused;
+};
 
 // Sequences as AttnSeqs has them, the blocks of queries (dQ) and of keys (dK, dV) of sequence i at zq[i] and zk[i]; n = 0: B sequences of one length.
 struct AttnBwdSeqs {
@@ -188,20 +198,25 @@ struct BwdPlace {
   int tile, at;   // a tile's number in its sequence, and among all of its side
 };
 
-// A tile's codes, statistics (keys) and scales; SMALL loads of each wave, the last waves' repeat the scales
+// A tile's codes and its record (in a slot of 1 KB), one load of 64 pieces of 16 bytes a wave; with D = 256 two.  Waves behind the codes' pieces all take
+// the record: where a wave loads from and to is settled before the loop, and no step has a branch for it.
 template <bool KEYS, int NK>
 struct BwdSmall {
-  static constexpr int LOADS = (NK + (KEYS ? 2 : 1) + BWD_WAVES - 1) / BWD_WAVES, CODES = CodeTile<NK>::BYTES, RECORD = KEYS ? 16 : 8;
-  const uint8_t *codes, *scales;
-  const float* stats;
-  __device__ __forceinline__ void operator()(uint8_t* to_codes, uint8_t* to_record, const BwdPlace& p, int wave, int lane) const {
-#pragma unroll
-    for (int l = 0; l < LOADS; ++l) {
-      const int i = BWD_WAVES * l + wave;
-      if (i < NK) load_piece(buffer(codes + (int64_t)p.at * CODES, CODES), to_codes + 1024 * i, CodeTile<NK>::source(64 * i + lane), 0);
-      else if (KEYS && i == NK) load_dword(buffer(stats + (int64_t)p.at * 64, 256), to_record, lane * 4, 0);
-      else load_dword(buffer(scales + (int64_t)p.at * RECORD, RECORD), to_record + 256, (lane & (RECORD / 4 - 1)) * 4, 0);
-    }
+  static constexpr int LOADS = NK == 4 ? 2 : 1, CODES = CodeTile<NK>::BYTES, RECORD = KEYS ? sizeof(QRecord) : sizeof(KRecord);
+  const uint8_t *codes, *records, *from;
+  int bytes, offset;      // of what this wave loads first: a tile's, and this lane's in it
+  bool takes_codes;
+  int at;
+  __device__ __forceinline__ BwdSmall(const uint8_t* codes, const void* all_records, int wave, int lane) : codes(codes), records(reinterpret_cast<const uint8_t*>(all_records)) {
+    takes_codes = wave < NK;
+    from = takes_codes ? codes : records;
+    bytes = takes_codes ? CODES : RECORD;
+    offset = takes_codes ? CodeTile<NK>::source(64 * wave + lane) : 16 * lane;
+    at = takes_codes ? 1024 * wave : 0;
+  }
+  __device__ __forceinline__ void operator()(const uint8_t* to_codes, const uint8_t* to_record, const BwdPlace& p, int lane) const {
+    load_piece(buffer(from + (int64_t)p.at * bytes, bytes), (takes_codes ? to_codes : to_record) + at, offset, 0);
+    if constexpr (LOADS == 2) load_piece(buffer(records + (int64_t)p.at * RECORD, RECORD), to_record, 16 * lane, 0);
   }
 };
 // Load `l` of a tile of bf16 rows (as many of each wave as it is wide / 64)
@@ -263,7 +278,7 @@ constexpr int BWD_AHEAD = 2;
 template <int NK, int NV>
 struct KeysLds {
   using T = BwdShape<NK, NV>;
-  static constexpr int O_V = 4 * T::CODES, O_D = O_V + 3 * T::ROWS_V, O_STATS = O_D + 2 * T::ROWS_D, O_BIAS = O_STATS + 4 * 512;
+  static constexpr int O_V = 4 * T::CODES, O_D = O_V + 3 * T::ROWS_V, O_RECORD = O_D + 2 * T::ROWS_D, O_BIAS = O_RECORD + 4 * 1024;
 };
 // One step: S and dP of a tile, its probabilities, and its part of the sums.  P is taken from S behind the products of dP, dS behind those of dV.
 template <int NK, int NV, int ADD>
@@ -301,7 +316,7 @@ __device__ __forceinline__ void attn_bwd_keys_body(const AttnBwdArgs& a, const A
     bf16x8_t yf[4 * NV];
 #pragma unroll
     for (int s = 0; s < NK; ++s) xf[s] = frag16(a.k + ((int64_t)own_tile * 32 + r) * (D / 2) + s * 32 + h * 16);
-    const uint32_t x_scales = *reinterpret_cast<const uint32_t*>(a.k_scales + (int64_t)own_tile * 8 + 4 * h);
+    const uint32_t x_scales = *reinterpret_cast<const uint32_t*>(a.k_records[own_tile].scales + 4 * h);
     const uint8_t* y = reinterpret_cast<const uint8_t*>(a.v_tiles) + (int64_t)own_tile * T::ROWS_V;
 #pragma unroll
     for (int i = 0; i < 4 * NV; ++i) yf[i] = VT::row_frag(y + VT::row_base(lane, i & 1), i);
@@ -314,13 +329,16 @@ __device__ __forceinline__ void attn_bwd_keys_body(const AttnBwdArgs& a, const A
     }
     auto next = [&]() {   // (past the end: the last tile again)
       const BwdPlace p{next_tile, next_base + next_tile};
-      if (--left > 0 && ++next_tile == last) {
-        next_tile = list.first;
-        next_base += tiles;
-      }
+      const int more = left > 1 ? 1 : 0;
+      left -= more;
+      next_tile += more;
+      const int wrap = next_tile == last ? -1 : 0;
+      next_tile += wrap & (list.first - last);
+      next_base += wrap & tiles;
       return p;
     };
-    const Small small{a.q, a.q_scales, a.stats};
+    const Small small(a.q, a.q_records, wave, lane);
+    auto record = [&](int i) { return reinterpret_cast<const QRecord*>(lds + L::O_RECORD + (i & 3) * 1024); };
     const uint8_t* const grads = reinterpret_cast<const uint8_t*>(a.g_tiles);
     const int code_base = lane * 16, row_base[2] = {VT::row_base(lane, 0), VT::row_base(lane, 1)}, column_base[2] = {VT::column_base(lane, 0), VT::column_base(lane, 1)};
     const float c2 = a.sm_scale * ATTN_RCP_LN2, inverse_scale = 1.0f / a.sm_scale;
@@ -337,7 +355,7 @@ __device__ __forceinline__ void attn_bwd_keys_body(const AttnBwdArgs& a, const A
       for (int e = 0; e < 4; ++e) S[4 * g + e] = x[e];
     };
     auto add = [&](const BwdPlace& p, int i, int g) {
-      const float slope = reinterpret_cast<const float*>(lds + L::O_STATS + (i & 3) * 512 + 256)[2], away = (float)(32 * p.tile + 4 * h + shift - key0 - r);
+      const float slope = record(i)->slope, away = (float)(32 * p.tile + 4 * h + shift - key0 - r);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float x = slope * __builtin_fabsf(away + (float)(8 * g + e));
@@ -345,19 +363,17 @@ __device__ __forceinline__ void attn_bwd_keys_body(const AttnBwdArgs& a, const A
       }
     };
     // Eight columns of one row of tile `i`'s values, from its codes: dword `j` of row tid % 32, j = tid / 32 + 8 u
-    uint32_t eight = 0;
-    float eight_scale = 0.0f;
+    uint32_t eight = 0, eight_scales = 0;
     auto read_codes = [&](int i, int u) {
       const int row = tid & 31, j = (tid >> 5) + 8 * u, block = j >> 2;
       eight = *reinterpret_cast<const uint32_t*>(lds + (i & 3) * T::CODES + (block * 32 + row) * 16 + 4 * (j & 3));
-      const uint32_t e = (reinterpret_cast<const uint32_t*>(lds + L::O_STATS + (i & 3) * 512 + 256)[block & 1] >> (8 * (block >> 1))) & 0xFFu;
-      eight_scale = e8m0_value(e);
+      eight_scales = reinterpret_cast<const uint32_t*>(record(i)->scales)[block & 1];
     };
     auto write_values = [&](int i, int u) {
       const int row = tid & 31, j = (tid >> 5) + 8 * u;
-      *reinterpret_cast<v4i_t*>(lds + L::O_D + (i & 1) * T::ROWS_D + tile_piece(row, j) * 16) = decode8(eight, eight_scale);
+      *reinterpret_cast<v4i_t*>(lds + L::O_D + (i & 1) * T::ROWS_D + tile_piece(row, j) * 16) = decode8(eight, e8m0_value((eight_scales >> (8 * (j >> 3))) & 0xFFu));
     };
-    auto load_small = [&](const BwdPlace& p, int i) { small(lds + (i & 3) * T::CODES, lds + L::O_STATS + (i & 3) * 512, p, wave, lane); };
+    auto load_small = [&](const BwdPlace& p, int i) { small(lds + (i & 3) * T::CODES, lds + L::O_RECORD + (i & 3) * 1024, p, lane); };
 
     BwdPlace p0 = next(), p1 = next(), p2 = next();
     if constexpr (ADD == ADD_BIAS) load_bias(p0);
@@ -399,7 +415,7 @@ __device__ __forceinline__ void attn_bwd_keys_body(const AttnBwdArgs& a, const A
         at_v[i] = lds + L::O_V + slot * T::ROWS_V + column_base[i];
         at_d[i] = lds + L::O_D + (t & 1) * T::ROWS_D + column_base[i];
       }
-      const float* const stats = reinterpret_cast<const float*>(lds + L::O_STATS + (t & 3) * 512) + 4 * h;
+      const QRecord* const rec = record(t);
       if constexpr (ADD == ADD_NOTHING) S = zeros();
       v16f_t dp;
       v4f_t l4[2];
@@ -416,7 +432,7 @@ __device__ __forceinline__ void attn_bwd_keys_body(const AttnBwdArgs& a, const A
         }
       };
       auto four = [](const uint32_t (&o)[8], int c) { return __builtin_bit_cast(bf16x8_t, v4i_t{(int)o[4 * c], (int)o[4 * c + 1], (int)o[4 * c + 2], (int)o[4 * c + 3]}); };
-      const uint32_t sc = reinterpret_cast<const uint32_t*>(lds + L::O_STATS + (t & 3) * 512 + 256)[h];
+      const uint32_t sc = reinterpret_cast<const uint32_t*>(rec->scales)[h];
       auto product = [&](auto ic) {
         constexpr int i = decltype(ic)::value;
         const bf16x8_t& x = frag[i % (AHEAD + 1)];
@@ -433,7 +449,7 @@ __device__ __forceinline__ void attn_bwd_keys_body(const AttnBwdArgs& a, const A
           dk[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, four(dsk, c), dk[n], 0, 0, 0);
         }
       };
-      auto read_stats = [&](int g) { l4[g & 1] = *reinterpret_cast<const v4f_t*>(stats + 8 * g); };
+      auto read_stats = [&](int g) { l4[g & 1] = *reinterpret_cast<const v4f_t*>(rec->lse2 + 8 * g + 4 * h); };
       auto probability = [&](int i) {   // of the pair of rows i
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
@@ -448,7 +464,7 @@ __device__ __forceinline__ void attn_bwd_keys_body(const AttnBwdArgs& a, const A
       static_for<AHEAD>([&](auto ic) { read(ic); });
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        const v4f_t x = *reinterpret_cast<const v4f_t*>(stats + 32 + 8 * g);
+        const v4f_t x = *reinterpret_cast<const v4f_t*>(rec->minus_d + 8 * g + 4 * h);
 #pragma unroll
         for (int i = 0; i < 4; ++i) dp[4 * g + i] = x[i];
       }
@@ -562,7 +578,7 @@ __global__ __launch_bounds__(64 * BWD_WAVES) void attn_bwd_sum_kernel(AttnBwdArg
 template <int NK, int NV>
 struct RowsLds {   // three slots of codes, V and K, four of scales
   using T = BwdShape<NK, NV>;
-  static constexpr int O_V = 3 * T::CODES, O_D = O_V + 3 * T::ROWS_V, O_STATS = O_D + 3 * T::ROWS_D, O_BIAS = O_STATS + 4 * 512;
+  static constexpr int O_V = 3 * T::CODES, O_D = O_V + 3 * T::ROWS_V, O_RECORD = O_D + 3 * T::ROWS_D, O_BIAS = O_RECORD + 4 * 1024;
 };
 // Three stages in one step: S and dP of tile t + 1 and the sums' product with tile t - 1 on the matrix pipe, dS of tile t on the vector pipe.
 template <int NK, int NV, int ADD>
@@ -596,17 +612,18 @@ __device__ __forceinline__ void attn_bwd_rows_body(const AttnBwdArgs& a, const A
   v16f_t nd;
 #pragma unroll
   for (int s = 0; s < NK; ++s) xf[s] = frag16(a.q + ((int64_t)own_tile * 32 + r) * (D / 2) + s * 32 + h * 16);
-  const uint32_t x_scales = *reinterpret_cast<const uint32_t*>(a.q_scales + (int64_t)own_tile * 16 + 4 * h);
+  const QRecord* const own_record = a.q_records + own_tile;
+  const uint32_t x_scales = *reinterpret_cast<const uint32_t*>(own_record->scales + 4 * h);
   const uint8_t* y0 = reinterpret_cast<const uint8_t*>(a.g_tiles) + (int64_t)own_tile * T::ROWS_V;
 #pragma unroll
   for (int i = 0; i < 4 * NV; ++i) yf[i] = VT::row_frag(y0 + VT::row_base(lane, i & 1), i);
-  const float lse2 = a.stats[(int64_t)own_tile * 64 + r], minus_d = a.stats[(int64_t)own_tile * 64 + 32 + r];
+  const float lse2 = own_record->lse2[r], minus_d = own_record->minus_d[r];
 #pragma unroll
   for (int v = 0; v < 16; ++v) nd[v] = minus_d;
   const float c2 = a.sm_scale * ATTN_RCP_LN2, inverse_scale = 1.0f / a.sm_scale;
-  const float slope = ADD == ADD_NOTHING ? 0.0f : *reinterpret_cast<const float*>(a.q_scales + (int64_t)own_tile * 16 + 8);
+  const float slope = ADD == ADD_NOTHING ? 0.0f : own_record->slope;
 
-  const Small small{a.k, a.k_scales, nullptr};
+  const Small small(a.k, a.k_records, wave, lane);
   const int code_base = lane * 16, row_base[2] = {VT::row_base(lane, 0), VT::row_base(lane, 1)}, column_base[2] = {DT::column_base(lane, 0), DT::column_base(lane, 1)};
   auto place = [&](int t) { t = t < total ? t : total - 1; return BwdPlace{t, first_at + t}; };   // (past the end: the last tile again)
 
@@ -674,7 +691,7 @@ __device__ __forceinline__ void attn_bwd_rows_body(const AttnBwdArgs& a, const A
         if (take_inner) ++inner; else ++factor;
       }
     };
-    const uint32_t sc = reinterpret_cast<const uint32_t*>(lds + L::O_STATS + ((t + 1) & 3) * 512 + 256)[h];
+    const uint32_t sc = reinterpret_cast<const uint32_t*>(lds + L::O_RECORD + ((t + 1) & 3) * 1024)[h];
     bf16x8_t frag[AHEAD + 1];
     auto read = [&](auto ic) {
       constexpr int i = decltype(ic)::value;
@@ -742,7 +759,7 @@ __device__ __forceinline__ void attn_bwd_rows_body(const AttnBwdArgs& a, const A
   // everything that earlier steps started.
   auto load_scores = [&](int i, int slot) {
     const BwdPlace p = place(i);
-    small(lds + slot * T::CODES, lds + L::O_STATS + (i & 3) * 512, p, wave, lane);
+    small(lds + slot * T::CODES, lds + L::O_RECORD + (i & 3) * 1024, p, lane);
 #pragma unroll
     for (int l = 0; l < NV; ++l) load_rows<64 * NV>(reinterpret_cast<const uint8_t*>(a.v_tiles), lds + L::O_V + slot * T::ROWS_V, p, l, wave, lane);
   };

@@ -33,15 +33,15 @@ struct PrepareArgs {
   int64_t alibi_sb, alibi_sh, do_sb, do_sh, do_ss, o_sb, o_sh, o_ss, l_sb, l_sh, l_ss;
   int Hq, Hk, Sq, Sk, D, Dv;
   int q_tiles;   // B Hq Sq / 32
-  float* stats;
-  uint8_t *q_scales, *k_scales;
+  QRecord* q_records;
+  KRecord* k_records;
   v4i_t *k_rows, *v_rows, *g_rows;
 };
 
 // The scale bytes of a tile of Q or K in the order of the score products
-__device__ __forceinline__ void order_scales(const uint8_t* scales, int64_t tile, int bands, uint8_t* record) {
+__device__ __forceinline__ void order_scales(const uint8_t* scales, int64_t tile, int bands, uint8_t* ordered) {
   const int tid = threadIdx.x, c = 2 * (tid & 3) + (tid >> 2);
-  if (tid < 8) record[tid] = c < bands ? scales[tile * bands + c] : 127;
+  if (tid < 8) ordered[tid] = c < bands ? scales[tile * bands + c] : 127;
 }
 
 // The values of a tile of K
@@ -62,12 +62,12 @@ __global__ __launch_bounds__(256) void attn_bwd_prepare_kernel(const PrepareArgs
   const int tid = threadIdx.x;
   int64_t tile = blockIdx.x;
   if (tile < a.q_tiles) {
-    order_scales(a.qs, tile, a.D / 32, a.q_scales + tile * 16);
+    order_scales(a.qs, tile, a.D / 32, a.q_records[tile].scales);
     v4i_t* const grad = reinterpret_cast<v4i_t*>(turned);
     const int r = tid >> 3, c = tid & 7;
     const int64_t row = tile * 32 + r, bh = row / a.Sq;
     const int64_t b = bh / a.Hq, h = bh % a.Hq, i = row % a.Sq;
-    if (tid == 0) *reinterpret_cast<float*>(a.q_scales + tile * 16 + 8) = a.alibi ? -a.alibi[b * a.alibi_sb + h * a.alibi_sh] / a.sm_scale : 0.0f;
+    if (tid == 0) a.q_records[tile].slope = a.alibi ? -a.alibi[b * a.alibi_sb + h * a.alibi_sh] / a.sm_scale : 0.0f;
     const v4i_t* go = reinterpret_cast<const v4i_t*>(a.dout + b * a.do_sb + h * a.do_sh + i * a.do_ss);
     const v4i_t* o = reinterpret_cast<const v4i_t*>(a.out + b * a.o_sb + h * a.o_sh + i * a.o_ss);
     float d = 0.0f;
@@ -85,15 +85,15 @@ __global__ __launch_bounds__(256) void attn_bwd_prepare_kernel(const PrepareArgs
     if (c == 0) {
       const float l = a.lse[b * a.l_sb + h * a.l_sh + i * a.l_ss];
       const bool none = l == -__builtin_inff();   // a row that sees no key: its probabilities are zeros, whatever the forward left in O
-      a.stats[tile * 64 + r] = none ? __builtin_inff() : l * ATTN_RCP_LN2;
-      a.stats[tile * 64 + 32 + r] = none ? 0.0f : -d;
+      a.q_records[tile].lse2[r] = none ? __builtin_inff() : l * ATTN_RCP_LN2;
+      a.q_records[tile].minus_d[r] = none ? 0.0f : -d;
     }
     __syncthreads();
     for (int k = tid; k < 4 * a.Dv; k += 256) a.g_rows[tile * 4 * a.Dv + k] = grad[k];
     return;
   }
   tile -= a.q_tiles;
-  order_scales(a.ks, tile, a.D / 32, a.k_scales + tile * 8);
+  order_scales(a.ks, tile, a.D / 32, a.k_records[tile].scales);
   decode_tile(a.k, a.ks, tile, a.D, a.k_rows);
   const int lane = tid & 63, wave = tid >> 6, bands = a.Sk / 32;
   if (wave * 32 >= a.Dv) return;
@@ -153,16 +153,15 @@ Cuts cut(const alto_mxfp4_attention_bwd_t& p) {
 }
 
 struct Workspace {
-  int64_t stats, q_scales, k_scales, k_rows, v_rows, g_rows, partial, total;
+  int64_t q_records, k_records, k_rows, v_rows, g_rows, partial, total;
 };
 Workspace workspace(const alto_mxfp4_attention_bwd_t& p, const Cuts& cuts) {
   const int64_t B = p.B, Hq = p.Hq, Hk = p.Hk, Sq = p.Sq, Sk = p.Sk, D = p.D, Dv = p.Dv;
   Workspace w{};
   int64_t at = 0;
   auto take = [&](int64_t& p, int64_t n) { p = at; at += (n + 255) / 256 * 256; };
-  take(w.stats, B * Hq * Sq * 8);
-  take(w.q_scales, B * Hq * (Sq / 32) * 16);
-  take(w.k_scales, B * Hk * (Sk / 32) * 8);
+  take(w.q_records, B * Hq * (Sq / 32) * (int64_t)sizeof(QRecord));
+  take(w.k_records, B * Hk * (Sk / 32) * (int64_t)sizeof(KRecord));
   take(w.k_rows, B * Hk * Sk * D * 2);
   take(w.v_rows, B * Hk * Sk * Dv * 2);
   take(w.g_rows, B * Hq * Sq * Dv * 2);
@@ -238,13 +237,13 @@ static int attention_bwd(const alto_mxfp4_attention_bwd_t& p, hipStream_t st) {
   r.l_sb = p.lse_sb; r.l_sh = p.lse_sh; r.l_ss = p.lse_ss;
   r.Hq = (int)p.Hq; r.Hk = (int)p.Hk; r.Sq = (int)p.Sq; r.Sk = (int)p.Sk; r.D = (int)p.D; r.Dv = (int)p.Dv;
   r.q_tiles = (int)(p.B * p.Hq * (p.Sq / 32));
-  r.stats = (float*)(ws + w.stats); r.q_scales = ws + w.q_scales; r.k_scales = ws + w.k_scales;
+  r.q_records = (QRecord*)(ws + w.q_records); r.k_records = (KRecord*)(ws + w.k_records);
   r.k_rows = (v4i_t*)(ws + w.k_rows); r.v_rows = (v4i_t*)(ws + w.v_rows); r.g_rows = (v4i_t*)(ws + w.g_rows);
   hipLaunchKernelGGL(attn_bwd_prepare_kernel, dim3((unsigned)(r.q_tiles + (int)(p.B * p.Hk * (p.Sk / 32)))), dim3(256), 0, st, r);
   if (const int rc = check_launch("attention_bwd")) return rc;
 
   AttnBwdArgs a{};
-  a.q = (const uint8_t*)p.q_codes; a.k = r.k; a.q_scales = r.q_scales; a.k_scales = r.k_scales; a.stats = r.stats;
+  a.q = (const uint8_t*)p.q_codes; a.k = r.k; a.q_records = r.q_records; a.k_records = r.k_records;
   a.k_tiles = (const __bf16*)r.k_rows; a.v_tiles = (const __bf16*)r.v_rows; a.g_tiles = (const __bf16*)r.g_rows;
   a.dq = p.dq; a.dk = p.dk; a.dv = p.dv;
   a.dq_sb = p.dq_sb; a.dq_sh = p.dq_sh; a.dq_ss = p.dq_ss; a.dk_sb = p.dk_sb; a.dk_sh = p.dk_sh; a.dk_ss = p.dk_ss; a.dv_sb = p.dv_sb; a.dv_sh = p.dv_sh; a.dv_ss = p.dv_ss;

@@ -69,12 +69,12 @@ def test_attention_workspace():
         return -(-n // 256) * 256
 
     # one key block of 3 tiles by 2 heads: nothing to cut
-    tiles = up(4 * 96 * 8) + up(4 * 3 * 8) + up(2 * 4 * 8) + 2 * 128 * (128 + 64) * 2 + 4 * 96 * 64 * 2
+    tiles = up(4 * 3 * 272) + up(2 * 4 * 16) + 2 * 128 * (128 + 64) * 2 + 4 * 96 * 64 * 2
     assert size(ctypes.byref(attention())) == tiles
     assert size(ctypes.byref(attention(n_seqs=1, cu_q=ints(0, 96), cu_k=ints(0, 128)))) == tiles
     # one head with one block of keys and 1024 tiles of rows: 16 parts
     long = dict(Hq=1, Hk=1, Sq=32768, causal=0)
-    assert size(ctypes.byref(attention(**long))) == up(32768 * 8) + up(1024 * 8) + up(4 * 8) + 128 * 192 * 2 + 32768 * 64 * 2 + 2 * 16 * 128 * 192 * 4
+    assert size(ctypes.byref(attention(**long))) == up(1024 * 272) + up(4 * 16) + 128 * 192 * 2 + 32768 * 64 * 2 + 2 * 16 * 128 * 192 * 4
 
 
 @pytest.mark.parametrize("changes,text", [
