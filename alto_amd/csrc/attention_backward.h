@@ -127,6 +127,28 @@ __device__ __forceinline__ void store_columns(__bf16* row, const v16f_t& acc, fl
   }
 }
 
+// A wave's 32 rows of W columns of transposed accumulators as bf16 to memory, by way of `lds` (64 W bytes of the wave's own, idle): written straight from
+// the registers they would be 16 bytes a row and store, and a store passes one line of the cache at a time.  The 16-byte pieces of a row change
+// places with the row, so that the writes of 32 rows meet all banks.
+template <int W>
+__device__ __forceinline__ void store_rows(const v16f_t* acc, float scale, bool live, uint8_t* lds, __bf16* to, int64_t stride, int lane) {
+  const int r = lane & 31, h = lane >> 5;
+#pragma unroll
+  for (int n = 0; n < W / 32; ++n)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const uint2 w = make_uint2(pack_bf16x2(acc[n][4 * g] * scale, acc[n][4 * g + 1] * scale), pack_bf16x2(acc[n][4 * g + 2] * scale, acc[n][4 * g + 3] * scale));
+      *reinterpret_cast<uint2*>(lds + r * 2 * W + ((4 * n + g) ^ (r & 7)) * 16 + 8 * h) = live ? w : make_uint2(0, 0);
+    }
+  wave_lds_order();
+#pragma unroll
+  for (int k = 0; k < W / 16; ++k) {
+    const int i = 64 * k + lane, row = i / (W / 8), piece = i % (W / 8);
+    *reinterpret_cast<v4i_t*>(to + row * stride + 8 * piece) = *reinterpret_cast<const v4i_t*>(lds + row * 2 * W + (piece ^ (row & 7)) * 16);
+  }
+  wave_lds_order();
+}
+
 __device__ __forceinline__ v16f_t zeros() {
   v16f_t z;
 #pragma unroll
@@ -538,12 +560,12 @@ __device__ __forceinline__ void attn_bwd_keys_body(const AttnBwdArgs& a, const A
       }
     return;
   }
+  asm volatile("s_barrier" ::: "memory");   // (no wave's loads or reads are under way any more)
   if (key0 >= (seqs.n ? w.kn : a.Sk)) return;
-  const int64_t at = w.k_first + key0 + r;   // (keys behind the used ones: zeros)
-#pragma unroll
-  for (int n = 0; n < 2 * NK; ++n) store_columns(dk_out + b * a.dk_sb + hk * a.dk_sh + at * a.dk_ss, live ? dk[n] : zeros(), a.sm_scale, n, h);
-#pragma unroll
-  for (int n = 0; n < 2 * NV; ++n) store_columns(dv_out + b * a.dv_sb + hk * a.dv_sh + at * a.dv_ss, live ? dv[n] : zeros(), 1.0f, n, h);
+  const int64_t at = w.k_first + key0;   // (keys behind the used ones: zeros)
+  uint8_t* const own = lds + wave * (64 * 64 * (NK > NV ? NK : NV));
+  store_rows<64 * NK>(dk, a.sm_scale, live, own, dk_out + b * a.dk_sb + hk * a.dk_sh + at * a.dk_ss, a.dk_ss, lane);
+  store_rows<64 * NV>(dv, 1.0f, live, own, dv_out + b * a.dv_sb + hk * a.dv_sh + at * a.dv_ss, a.dv_ss, lane);
 }
 
 // Sums of the parts, in their order.  Grid: (key blocks by heads, blocks of 32 columns of dK, then of dV).
@@ -559,7 +581,8 @@ __global__ __launch_bounds__(64 * BWD_WAVES) void attn_bwd_sum_kernel(AttnBwdArg
   const int hk = bh % a.Hk, b = bh / a.Hk;
   v16f_t sum = zeros();
   if (key < w.kn) {
-    for (int part = 0; part < list.parts; ++part) {
+#pragma unroll 4
+    for (int part = 0; part < list.parts; ++part) {   // (the loads of four parts at a time under way)
       const v4f_t* from = reinterpret_cast<const v4f_t*>(plan.partial + (((int64_t)z * plan.parts + part) * heads + bh) * T::PARTIAL) + (wave * T::ACC + n) * 4 * 64 + lane;
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
@@ -832,10 +855,9 @@ __device__ __forceinline__ void attn_bwd_rows_body(const AttnBwdArgs& a, const A
       for (int n = 0; n < 2 * NK; ++n) acc[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(DT::column_frag(at + column_base[0], at + column_base[1], n, c), f[c], acc[n], 0, 0, 0);
   }
   wait_all_but<0>();   // (the last loads into the LDS, which nobody reads, before it is given back)
+  asm volatile("s_barrier" ::: "memory");   // (no wave's loads or reads are under way any more)
   if (!live) return;
-  __bf16* row = dq_out + b * a.dq_sb + hq * a.dq_sh + (int64_t)(w.q_first + row0 + r) * a.dq_ss;
-#pragma unroll
-  for (int n = 0; n < 2 * NK; ++n) store_columns(row, acc[n], a.sm_scale, n, h);
+  store_rows<64 * NK>(acc, a.sm_scale, true, lds + wave * (64 * 64 * NK), dq_out + b * a.dq_sb + hq * a.dq_sh + (int64_t)(w.q_first + row0) * a.dq_ss, a.dq_ss, lane);
 }
 
 template <int NK, int NV, int ADD>

@@ -145,7 +145,7 @@ Cuts cut(const alto_mxfp4_attention_bwd_t& p) {
   // A tile of dQ takes about .62 of one of dK and dV (products: 18 to 26 with D = Dv = 128).  The compute units hold 512 workgroups; a list longer than
   // an equal share of the whole would end alone.
   const int64_t share = (int64_t)(0.85 * 1.62 * (double)(sum * p.B * p.Hk) / 512.0);
-  int64_t chunk = share < 16 ? 16 : share;
+  int64_t chunk = share < 24 ? 24 : share;
   int64_t parts = (longest + chunk - 1) / chunk;
   parts = parts < 1 ? 1 : (parts > 16 ? 16 : parts);
   if (parts == 16) chunk = (longest + 15) / 16;
@@ -204,14 +204,11 @@ static int attention_bwd(const alto_mxfp4_attention_bwd_t& p, hipStream_t st) {
   ALTO_REQUIRE(p.q_codes && p.q_scales && p.k_codes && p.k_scales && p.vt_codes && p.v_scales && p.dout && p.out && p.lse && p.workspace && (p.dk || p.dq),
                "attention_bwd: null pointer");
   ALTO_REQUIRE(!p.dk == !p.dv, "attention_bwd: dk and dv are written together");
-  ALTO_REQUIRE(((uintptr_t)p.q_codes | (uintptr_t)p.k_codes | (uintptr_t)p.dout | (uintptr_t)p.out) % 16 == 0 && (uintptr_t)p.vt_codes % 8 == 0,
-               "attention_bwd: Q and K codes, dout and out must be 16-byte aligned, V codes 8-byte aligned");
-  ALTO_REQUIRE(((uintptr_t)p.dq | (uintptr_t)p.dk | (uintptr_t)p.dv) % 8 == 0 && ((uintptr_t)p.lse | (uintptr_t)p.bias | (uintptr_t)p.alibi_slopes) % 4 == 0,
-               "attention_bwd: gradients must be 8-byte aligned, lse, bias and slopes 4-byte aligned");
-  for (const int64_t s : {p.dout_sb, p.dout_sh, p.dout_ss, p.out_sb, p.out_sh, p.out_ss})
-    ALTO_REQUIRE(s >= 0 && s < (1ll << 40) && s % 8 == 0, "attention_bwd: strides of dout and out must be non-negative multiples of 8 elements");
-  for (const int64_t s : {p.dq_sb, p.dq_sh, p.dq_ss, p.dk_sb, p.dk_sh, p.dk_ss, p.dv_sb, p.dv_sh, p.dv_ss})
-    ALTO_REQUIRE(s >= 0 && s < (1ll << 40) && s % 4 == 0, "attention_bwd: strides of the gradients must be non-negative multiples of 4 elements");
+  ALTO_REQUIRE(((uintptr_t)p.q_codes | (uintptr_t)p.k_codes | (uintptr_t)p.dout | (uintptr_t)p.out | (uintptr_t)p.dq | (uintptr_t)p.dk | (uintptr_t)p.dv) % 16 == 0 &&
+               (uintptr_t)p.vt_codes % 8 == 0, "attention_bwd: Q and K codes, dout, out and the gradients must be 16-byte aligned, V codes 8-byte aligned");
+  ALTO_REQUIRE(((uintptr_t)p.lse | (uintptr_t)p.bias | (uintptr_t)p.alibi_slopes) % 4 == 0, "attention_bwd: lse, bias and slopes must be 4-byte aligned");
+  for (const int64_t s : {p.dout_sb, p.dout_sh, p.dout_ss, p.out_sb, p.out_sh, p.out_ss, p.dq_sb, p.dq_sh, p.dq_ss, p.dk_sb, p.dk_sh, p.dk_ss, p.dv_sb, p.dv_sh, p.dv_ss})
+    ALTO_REQUIRE(s >= 0 && s < (1ll << 40) && s % 8 == 0, "attention_bwd: strides of dout, out and the gradients must be non-negative multiples of 8 elements");
   for (const int64_t s : {p.lse_sb, p.lse_sh, p.lse_ss, p.bias_sb, p.bias_sh, p.bias_sm, p.alibi_sb, p.alibi_sh})
     ALTO_REQUIRE(s >= 0 && s < (1ll << 40), "attention_bwd: strides must be non-negative");
   ALTO_REQUIRE(p.sm_scale > 0.0f && p.sm_scale < __builtin_inff(), "attention_bwd: sm_scale must be positive and finite");

@@ -52,8 +52,8 @@ def test_attention_sizes(changes, text):
 @pytest.mark.parametrize("changes,text", [
     *[(dict([(name, None)]), "null pointer") for name in ("q_codes", "q_scales", "k_codes", "k_scales", "vt_codes", "v_scales", "dout", "out", "lse", "workspace")],
     (dict(dq=None, dk=None, dv=None), "null pointer"), (dict(dk=None), "together"), (dict(dv=None), "together"), (dict(q_codes=P + 8), "aligned"), (dict(dout=P + 8), "aligned"),
-    (dict(vt_codes=P + 4), "aligned"), (dict(dk=P + 4), "aligned"), (dict(lse=P + 2), "aligned"), (dict(bias=P + 2), "aligned"), (dict(dout_ss=12), "multiples of 8"),
-    (dict(out_sb=-8), "multiples of 8"), (dict(dq_sh=6), "multiples of 4"), (dict(dv_ss=-4), "multiples of 4"), (dict(bias_sm=-1), "non-negative"), (dict(lse_sb=1 << 50), "non-negative"),
+    (dict(vt_codes=P + 4), "aligned"), (dict(dk=P + 8), "aligned"), (dict(lse=P + 2), "aligned"), (dict(bias=P + 2), "aligned"), (dict(dout_ss=12), "multiples of 8"),
+    (dict(out_sb=-8), "multiples of 8"), (dict(dq_sh=12), "multiples of 8"), (dict(dv_ss=-8), "multiples of 8"), (dict(bias=P, bias_sm=1 << 24), "2^24"), (dict(bias=P, sm_scale=1e-20), "2^-64"), (dict(alibi_slopes=P, sm_scale=1e-20), "2^-64"), (dict(bias_sm=-1), "non-negative"), (dict(lse_sb=1 << 50), "non-negative"),
     (dict(sm_scale=0.0), "sm_scale"), (dict(sm_scale=-1.0), "sm_scale"), (dict(sm_scale=float("inf")), "sm_scale"), (dict(sm_scale=float("nan")), "sm_scale"),
     (dict(workspace_bytes=1024), "workspace"), (dict(workspace=P + 128), "workspace"),
 ])
