@@ -32,7 +32,7 @@ def _additive(bias: Optional[torch.Tensor], alibi_slopes: Optional[torch.Tensor]
             b4 = b4.unsqueeze(0)
         torch._check(b4.shape[-2] == Sq and b4.shape[-1] == Sk and b4.shape[0] in (1, B) and b4.shape[1] in (1, Hq),
                      lambda: f"bias of shape {tuple(bias.shape)} does not broadcast to {(B, Hq, Sq, Sk)}")
-        if b4.stride(3) != 1 or b4.stride(2) % 4 or b4.data_ptr() % 16 or (b4.shape[0] > 1 and b4.stride(0) < 0) or (b4.shape[1] > 1 and b4.stride(1) < 0):
+        if b4.stride(3) != 1 or b4.stride(2) % 4 or b4.stride(2) >= 1 << 24 or b4.data_ptr() % 16 or (b4.shape[0] > 1 and b4.stride(0) < 0) or (b4.shape[1] > 1 and b4.stride(1) < 0):
             b4 = b4.contiguous()
     if alibi_slopes is not None:
         rt.require_gpu(alibi_slopes)

@@ -96,6 +96,55 @@ def test_additive_terms(m, case, extra):
         assert bool((got[0][-1, :, 0] == 0).all())
 
 
+@pytest.mark.parametrize("case", [(2, 4, 2, 96, 160, 128, 64, True), (2, 2, 2, 160, 192, 192, 128, False)], ids=lambda c: "x".join(map(str, c)))
+def test_a_bias_of_any_layout(m, case):
+    """Broadcast rows, batches and heads, a part of something larger at an odd place with rows an odd number of elements apart: the bits of its dense copy."""
+    B, Hq, _, Sq, Sk, *_ = case
+    g = torch.Generator().manual_seed(8)
+    held = torch.randn(B, Hq, Sq, Sk + 3, generator=g).to(DEV)
+    for bias in (held[:, :, :, 1:-2], held[:, :1, :, 3:], held[:1, :, :1, :-3].expand(B, Hq, Sq, Sk), held[:1, 1:2, :, 2:-1]):
+        assert bias.shape[-1] == Sk
+        x = Operands(*case, seed=9, bias=bias.cpu())
+        x.more["bias"] = bias
+        got = x.call(m)
+        x.more["bias"] = bias.expand(B, Hq, Sq, Sk).contiguous()
+        for a, b in zip(got, x.call(m)):
+            assert torch.equal(a, b)
+        x.more["bias"] = bias.cpu()
+        check(got, x.expected())
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_a_bias_of_extreme_values(m, D):
+    """Where the mask hides a key the bias may hold anything; the type's lowest value hides like -inf, in rows that see nothing too; a row that sees
+    nothing but keys at -1e9, whose lse has no bits left for its scores, keeps probabilities of at most one."""
+    case = (1, 2, 1, 96, 160, D, 64, True)
+    Sq, Sk = case[3:5]
+    g = torch.Generator().manual_seed(10)
+    hidden = torch.arange(Sk)[None, :] > torch.arange(Sq)[:, None] + Sk - Sq
+    bias = torch.randn(1, 2, Sq, Sk, generator=g).masked_fill(torch.rand(1, 2, Sq, Sk, generator=g) < 0.3, float("-inf"))
+    bias[:, :, 5] = bias[:, 1, 40:] = float("-inf")
+    bias[:, 0, :, 0] = 0.0
+    bias[:, 0, 5] = float("-inf")
+    x = Operands(*case, seed=12, bias=bias)
+    want = x.call(m)
+    check(want, x.expected())
+    assert bool((want[0][:, :, 5] == 0).all()) and bool((want[0][:, 1, 40:] == 0).all())
+    for fill in (float("nan"), float("inf"), torch.finfo(torch.float32).max):
+        x.more["bias"] = bias.masked_fill(hidden, fill)
+        for a, b in zip(x.call(m), want):
+            assert torch.equal(a, b)
+    x.more["bias"] = bias.masked_fill(bias == float("-inf"), torch.finfo(torch.float32).min)
+    for a, b in zip(x.call(m), want):
+        assert torch.equal(a, b)
+    bias[:, :, 7] = -1e9
+    y = Operands(*case, seed=12, bias=bias)
+    dq, dk, dv = y.call(m)
+    assert all(bool(t.isfinite().all()) for t in (dq, dk, dv))
+    limit = y.go.double().abs().sum((1, 2))   # (of the key's only head: every probability at most 1, and half a step of bf16 at it and at the result)
+    assert bool((dv.cpu().double().abs().amax((1, 2)) <= limit * (1 + 2.0 ** -7)).all())
+
+
 @pytest.mark.parametrize("causal", [True, False])
 def test_packed_sequences_are_the_sequences_alone(m, causal):
     """Lengths of one tile, of odd numbers of tiles and of more than a workgroup's block; each sequence's gradients bit for bit those of its own call."""
