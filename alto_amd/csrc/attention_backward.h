@@ -236,16 +236,23 @@ struct BwdSmall {
     offset = takes_codes ? CodeTile<NK>::source(64 * wave + lane) : 16 * lane;
     at = takes_codes ? 1024 * wave : 0;
   }
-  __device__ __forceinline__ void operator()(const uint8_t* to_codes, const uint8_t* to_record, const BwdPlace& p, int lane) const {
-    load_piece(buffer(from + (int64_t)p.at * bytes, bytes), (takes_codes ? to_codes : to_record) + at, offset, 0);
-    if constexpr (LOADS == 2) load_piece(buffer(records + (int64_t)p.at * RECORD, RECORD), to_record, 16 * lane, 0);
+  // of `n` tiles from `first` on
+  __device__ __forceinline__ __amdgpu_buffer_rsrc_t source(int64_t first, int n) const { return buffer(from + first * bytes, (int64_t)n * bytes); }
+  __device__ __forceinline__ __amdgpu_buffer_rsrc_t second(int64_t first, int n) const { return buffer(records + first * RECORD, (int64_t)n * RECORD); }
+  // tile `t` of these
+  __device__ __forceinline__ void operator()(__amdgpu_buffer_rsrc_t source, __amdgpu_buffer_rsrc_t second, int t, const uint8_t* to_codes, const uint8_t* to_record, int lane) const {
+    load_piece(source, (takes_codes ? to_codes : to_record) + at, offset, t * bytes);
+    if constexpr (LOADS == 2) load_piece(second, to_record, 16 * lane, t * RECORD);
   }
 };
-// Load `l` of a tile of bf16 rows (as many of each wave as it is wide / 64)
+// Load `l` of tile `t` of bf16 rows (as many of each wave as it is wide / 64)
 template <int W>
-__device__ __forceinline__ void load_rows(const uint8_t* tiles, uint8_t* to, const BwdPlace& p, int l, int wave, int lane) {
-  const int piece = BWD_WAVES * l + wave;
-  load_piece(buffer(tiles + (int64_t)p.at * RowTile<W>::BYTES, RowTile<W>::BYTES), to + 1024 * piece, lane * 16 + 1024 * wave, 1024 * BWD_WAVES * l);
+__device__ __forceinline__ void load_rows(__amdgpu_buffer_rsrc_t source, const uint8_t* to, int t, int l, int wave, int lane) {
+  load_piece(source, to + 1024 * (BWD_WAVES * l + wave), lane * 16 + 1024 * wave, t * RowTile<W>::BYTES + 1024 * BWD_WAVES * l);
+}
+template <int W>
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_source(const __bf16* tiles, int64_t first, int n) {
+  return buffer(reinterpret_cast<const uint8_t*>(tiles) + first * RowTile<W>::BYTES, (int64_t)n * RowTile<W>::BYTES);
 }
 template <int N>   // loads that may stay under way
 __device__ __forceinline__ void wait_all_but() { __builtin_amdgcn_s_waitcnt(0x0070 | 0x0F00 | (N & 15) | (N >> 4) << 14); }
@@ -361,7 +368,6 @@ __device__ __forceinline__ void attn_bwd_keys_body(const AttnBwdArgs& a, const A
     };
     const Small small(a.q, a.q_records, wave, lane);
     auto record = [&](int i) { return reinterpret_cast<const QRecord*>(lds + L::O_RECORD + (i & 3) * 1024); };
-    const uint8_t* const grads = reinterpret_cast<const uint8_t*>(a.g_tiles);
     const int code_base = lane * 16, row_base[2] = {VT::row_base(lane, 0), VT::row_base(lane, 1)}, column_base[2] = {VT::column_base(lane, 0), VT::column_base(lane, 1)};
     const float c2 = a.sm_scale * ATTN_RCP_LN2, inverse_scale = 1.0f / a.sm_scale;
     // The additive terms of tile `i`
@@ -384,27 +390,27 @@ __device__ __forceinline__ void attn_bwd_keys_body(const AttnBwdArgs& a, const A
         S[4 * g + e] = ADD == ADD_BIAS ? __builtin_fmaf(S[4 * g + e], inverse_scale, x) : x;
       }
     };
-    // Eight columns of one row of tile `i`'s values, from its codes: dword `j` of row tid % 32, j = tid / 32 + 8 u
+    // Eight columns of one row of tile `i`'s values, from its codes: dword j = 2 wave + h + 8 u of row r
     uint32_t eight = 0, eight_scales = 0;
+    const int eight_from = 16 * r + 4 * h, eight_to = tile_piece(r, 2 * wave + h) * 16;
     auto read_codes = [&](int i, int u) {
-      const int row = tid & 31, j = (tid >> 5) + 8 * u, block = j >> 2;
-      eight = *reinterpret_cast<const uint32_t*>(lds + (i & 3) * T::CODES + (block * 32 + row) * 16 + 4 * (j & 3));
-      eight_scales = reinterpret_cast<const uint32_t*>(record(i)->scales)[block & 1];
+      eight = *reinterpret_cast<const uint32_t*>(lds + (i & 3) * T::CODES + ((wave >> 1) + 2 * u) * 512 + 8 * (wave & 1) + eight_from);
+      eight_scales = reinterpret_cast<const uint32_t*>(record(i)->scales)[wave >> 1];
     };
     auto write_values = [&](int i, int u) {
-      const int row = tid & 31, j = (tid >> 5) + 8 * u;
-      *reinterpret_cast<v4i_t*>(lds + L::O_D + (i & 1) * T::ROWS_D + tile_piece(row, j) * 16) = decode8(eight, e8m0_value((eight_scales >> (8 * (j >> 3))) & 0xFFu));
+      *reinterpret_cast<v4i_t*>(lds + L::O_D + (i & 1) * T::ROWS_D + 4096 * u + eight_to) = decode8(eight, e8m0_value((eight_scales >> (8 * u)) & 0xFFu));
     };
-    auto load_small = [&](const BwdPlace& p, int i) { small(lds + (i & 3) * T::CODES, lds + L::O_RECORD + (i & 3) * 1024, p, lane); };
+    auto load_small = [&](const BwdPlace& p, int i) { small(small.source(p.at, 1), small.second(p.at, 1), 0, lds + (i & 3) * T::CODES, lds + L::O_RECORD + (i & 3) * 1024, lane); };
+    auto load_grads = [&](const BwdPlace& p, int l, int slot) { load_rows<64 * NV>(rows_source<64 * NV>(a.g_tiles, p.at, 1), lds + L::O_V + slot * T::ROWS_V, 0, l, wave, lane); };
 
     BwdPlace p0 = next(), p1 = next(), p2 = next();
     if constexpr (ADD == ADD_BIAS) load_bias(p0);
     load_small(p0, 0);
     load_small(p1, 1);
 #pragma unroll
-    for (int l = 0; l < NV; ++l) load_rows<64 * NV>(grads, lds + L::O_V, p0, l, wave, lane);
+    for (int l = 0; l < NV; ++l) load_grads(p0, l, 0);
 #pragma unroll
-    for (int l = 0; l < NV; ++l) load_rows<64 * NV>(grads, lds + L::O_V + T::ROWS_V, p1, l, wave, lane);
+    for (int l = 0; l < NV; ++l) load_grads(p1, l, 1);
     load_small(p2, 2);
     wait_all_but<NV + Small::LOADS>();
     asm volatile("s_barrier" ::: "memory");
@@ -524,7 +530,7 @@ __device__ __forceinline__ void attn_bwd_keys_body(const AttnBwdArgs& a, const A
         if constexpr (i >= NS + NI + NF) {   // the loads for later tiles, the next one's values
           constexpr int j = i - NS - NI - NF;
           if constexpr (j == 0) load_small(p3, t + 3);
-          if constexpr (j >= 1 && j <= NV) load_rows<64 * NV>(grads, lds + L::O_V + two_on * T::ROWS_V, p2, j - 1, wave, lane);
+          if constexpr (j >= 1 && j <= NV) load_grads(p2, j - 1, two_on);
           if constexpr (j % 4 == 0) read_codes(t + 1, j / 4);
           if constexpr (j % 4 == 3) write_values(t + 1, j / 4);
           if constexpr (ADD == ADD_BIAS && j < 2) {
@@ -648,7 +654,10 @@ __device__ __forceinline__ void attn_bwd_rows_body(const AttnBwdArgs& a, const A
 
   const Small small(a.k, a.k_records, wave, lane);
   const int code_base = lane * 16, row_base[2] = {VT::row_base(lane, 0), VT::row_base(lane, 1)}, column_base[2] = {DT::column_base(lane, 0), DT::column_base(lane, 1)};
-  auto place = [&](int t) { t = t < total ? t : total - 1; return BwdPlace{t, first_at + t}; };   // (past the end: the last tile again)
+  auto tile = [&](int t) { return t < total ? t : total - 1; };   // (past the end: the last tile again)
+  // (a head's rows take less than 4 GB)
+  const __amdgpu_buffer_rsrc_t small_source = small.source(first_at, total), second_source = small.second(first_at, total);
+  const __amdgpu_buffer_rsrc_t v_source = rows_source<64 * NV>(a.v_tiles, first_at, total), k_source = rows_source<64 * NK>(a.k_tiles, first_at, total);
 
   // Which keys of the tile the lane's row sees, in the bits of the packed pairs: most tiles are seen whole (state 2), the diagonal's in part (1), a
   // tile behind it not at all (0: another wave of the workgroup needs it).
@@ -680,7 +689,7 @@ __device__ __forceinline__ void attn_bwd_rows_body(const AttnBwdArgs& a, const A
   // The additive terms of tile `i`, in the registers where its scores will be
   uint8_t* const at_bias = lds + L::O_BIAS + wave * Bias::BYTES;
   auto load_bias = [&](int i) {
-    Bias::load(a.bias + b * a.bias_sb + hq * a.bias_sh + (int64_t)(live ? row0 : 0) * a.bias_sm + 32 * place(i).tile, a.bias_sm, at_bias, lane);
+    Bias::load(a.bias + b * a.bias_sb + hq * a.bias_sh + (int64_t)(live ? row0 : 0) * a.bias_sm + 32 * tile(i), a.bias_sm, at_bias, lane);
   };
   auto add = [&](int i, int g, v16f_t& S) {
     const float away = (float)(row0 + r + shift - 32 * i - 4 * h);
@@ -781,14 +790,15 @@ __device__ __forceinline__ void attn_bwd_rows_body(const AttnBwdArgs& a, const A
   // Loads go out two steps before they are used: a step starts those of the scores of t + 3 and the factor of t + 1, and ends with a wait for
   // everything that earlier steps started.
   auto load_scores = [&](int i, int slot) {
-    const BwdPlace p = place(i);
-    small(lds + slot * T::CODES, lds + L::O_RECORD + (i & 3) * 1024, p, lane);
+    const int t = tile(i);
+    small(small_source, second_source, t, lds + slot * T::CODES, lds + L::O_RECORD + (i & 3) * 1024, lane);
 #pragma unroll
-    for (int l = 0; l < NV; ++l) load_rows<64 * NV>(reinterpret_cast<const uint8_t*>(a.v_tiles), lds + L::O_V + slot * T::ROWS_V, p, l, wave, lane);
+    for (int l = 0; l < NV; ++l) load_rows<64 * NV>(v_source, lds + L::O_V + slot * T::ROWS_V, t, l, wave, lane);
   };
   auto load_factor = [&](int i, int slot) {
+    const int t = tile(i);
 #pragma unroll
-    for (int l = 0; l < NK; ++l) load_rows<64 * NK>(reinterpret_cast<const uint8_t*>(a.k_tiles), lds + L::O_D + slot * T::ROWS_D, place(i), l, wave, lane);
+    for (int l = 0; l < NK; ++l) load_rows<64 * NK>(k_source, lds + L::O_D + slot * T::ROWS_D, t, l, wave, lane);
   };
   Scores x, y;
   if constexpr (ADD == ADD_BIAS) {
