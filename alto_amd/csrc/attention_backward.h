@@ -241,14 +241,14 @@ struct BwdSmall {
   __device__ __forceinline__ __amdgpu_buffer_rsrc_t second(int64_t first, int n) const { return buffer(records + first * RECORD, (int64_t)n * RECORD); }
   // tile `t` of these
   __device__ __forceinline__ void operator()(__amdgpu_buffer_rsrc_t source, __amdgpu_buffer_rsrc_t second, int t, const uint8_t* to_codes, const uint8_t* to_record, int lane) const {
-    load_piece(source, (takes_codes ? to_codes : to_record) + at, offset, t * bytes);
-    if constexpr (LOADS == 2) load_piece(second, to_record, 16 * lane, t * RECORD);
+    load_piece(source, (takes_codes ? to_codes : to_record) + at, offset, (int)((uint32_t)t * bytes));
+    if constexpr (LOADS == 2) load_piece(second, to_record, 16 * lane, (int)((uint32_t)t * RECORD));
   }
 };
 // Load `l` of tile `t` of bf16 rows (as many of each wave as it is wide / 64)
 template <int W>
 __device__ __forceinline__ void load_rows(__amdgpu_buffer_rsrc_t source, const uint8_t* to, int t, int l, int wave, int lane) {
-  load_piece(source, to + 1024 * (BWD_WAVES * l + wave), lane * 16 + 1024 * wave, t * RowTile<W>::BYTES + 1024 * BWD_WAVES * l);
+  load_piece(source, to + 1024 * (BWD_WAVES * l + wave), lane * 16 + 1024 * wave, (int)((uint32_t)t * RowTile<W>::BYTES + 1024 * BWD_WAVES * l));
 }
 template <int W>
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_source(const __bf16* tiles, int64_t first, int n) {

@@ -70,9 +70,11 @@ __global__ __launch_bounds__(256) void attn_bwd_prepare_kernel(const PrepareArgs
     if (tid == 0) a.q_records[tile].slope = a.alibi ? -a.alibi[b * a.alibi_sb + h * a.alibi_sh] / a.sm_scale : 0.0f;
     const v4i_t* go = reinterpret_cast<const v4i_t*>(a.dout + b * a.do_sb + h * a.do_sh + i * a.do_ss);
     const v4i_t* o = reinterpret_cast<const v4i_t*>(a.out + b * a.o_sb + h * a.o_sh + i * a.o_ss);
+    const float l = a.lse[b * a.l_sb + h * a.l_sh + i * a.l_ss];
+    const bool none = l == -__builtin_inff();   // a row that sees no key: it gives nothing, whatever the forward left in O and whatever dO holds
     float d = 0.0f;
     for (int p = c; p < a.Dv / 8; p += 8) {
-      const v4i_t x = go[p], y = o[p];
+      const v4i_t x = none ? v4i_t{0, 0, 0, 0} : go[p], y = o[p];
       grad[tile_piece(r, p)] = x;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -83,8 +85,6 @@ __global__ __launch_bounds__(256) void attn_bwd_prepare_kernel(const PrepareArgs
 #pragma unroll
     for (int m = 1; m < 8; m <<= 1) d += __shfl_xor(d, m, 64);
     if (c == 0) {
-      const float l = a.lse[b * a.l_sb + h * a.l_sh + i * a.l_ss];
-      const bool none = l == -__builtin_inff();   // a row that sees no key: its probabilities are zeros, whatever the forward left in O
       a.q_records[tile].lse2[r] = none ? __builtin_inff() : l * ATTN_RCP_LN2;
       a.q_records[tile].minus_d[r] = none ? 0.0f : -d;
     }

@@ -134,6 +134,9 @@ def test_a_bias_of_extreme_values(m, D):
         x.more["bias"] = bias.masked_fill(hidden, fill)
         for a, b in zip(x.call(m), want):
             assert torch.equal(a, b)
+    x.go[:, :, 5] = x.out[:, :, 5] = float("nan")   # nor does what a row holds that sees nothing
+    for a, b in zip(x.call(m), want):
+        assert torch.equal(a, b)
     x.more["bias"] = bias.masked_fill(bias == float("-inf"), torch.finfo(torch.float32).min)
     for a, b in zip(x.call(m), want):
         assert torch.equal(a, b)
@@ -219,3 +222,27 @@ def test_results_do_not_change_from_run_to_run(m):
     for _ in range(3):
         for a, b in zip(x.call(m), first):
             assert torch.equal(a, b)
+
+
+def test_a_head_of_more_than_2_gb(m):
+    """Keys whose rows of 512 bytes lie behind 2^31 bytes: all keys but the first and the last are zeros, which change no sum, so that the gradients
+    are those of the two alone."""
+    edge, Sk, D, Dv = 64, (1 << 22) + 128, 256, 64
+    x = Operands(1, 1, 1, 32, 2 * edge, D, Dv, False, seed=13)
+    want = x.call(m)
+    y = Operands.__new__(Operands)
+    y.more, y.go, y.out, y.lse, y.q, y.qs = x.more, x.go, x.out, x.lse, x.q, x.qs
+
+    def spread(t, dim, edge):
+        size = list(t.shape)
+        size[dim] = size[dim] // 2 * (Sk // 64)
+        big = torch.zeros(size, dtype=t.dtype, device=DEV)
+        big.narrow(dim, 0, edge).copy_(t.narrow(dim, 0, edge))
+        big.narrow(dim, size[dim] - edge, edge).copy_(t.narrow(dim, edge, edge))
+        return big
+
+    y.k, y.ks, y.v, y.vs = spread(x.k, 2, edge), spread(x.ks, 2, edge // 32), spread(x.v, 3, edge // 2), spread(x.vs, 2, edge // 32)
+    dq, dk, dv = y.call(m)
+    assert dk.shape[2] == Sk and torch.equal(dq, want[0])
+    for got, exact in ((dk, want[1]), (dv, want[2])):
+        assert torch.equal(got[:, :, :edge], exact[:, :, :edge]) and torch.equal(got[:, :, -edge:], exact[:, :, edge:])
