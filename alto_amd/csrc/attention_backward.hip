@@ -142,11 +142,14 @@ Cuts cut(const alto_mxfp4_attention_bwd_t& p) {
   } else {
     sum = count_tiles(p.Sq, p.Sk_used, block, p.causal, heads, longest);
   }
-  // A tile of dQ takes about .62 of one of dK and dV (products: 18 to 26 with D = Dv = 128).  The compute units hold 512 workgroups; a list longer than
-  // an equal share of the whole would end alone.
-  const int64_t share = (int64_t)(0.85 * 1.62 * (double)(sum * p.B * p.Hk) / 512.0);
+  // A tile of dQ takes about .62 of one of dK and dV (products: 18 to 26 with D = Dv = 128), and the compute units hold 512 workgroups: a list much longer
+  // than an equal share of the whole would end alone.  Pieces of 1.7 / 1.62 of that share (1.9 and 1.4: 3 % and 1.5 % more over 13 shapes), of 24 tiles
+  // at least (16 and 32: 80.9 and 73.6 us for 72.2, 6 packed sequences of 16 / 4 heads of 128).  The parts' sums go through memory and take a kernel, so
+  // a list stays whole that is little longer than a piece: 2048 tokens of 128, 32 heads, 64 tiles for pieces of 58, 124 us for 134 in two parts; 20 heads,
+  // 64 for 36, 94 for 102; but not: 12 heads, 64 for 24, 82 for 77; 3 x 64 / 8 heads, 512 for 346, 691 for 655.
+  const int64_t share = (int64_t)(1.7 * (double)(sum * p.B * p.Hk) / 512.0);
   int64_t chunk = share < 24 ? 24 : share;
-  int64_t parts = (longest + chunk - 1) / chunk;
+  int64_t parts = 4 * longest <= 5 * chunk || longest <= chunk + 30 ? 1 : (longest + chunk - 1) / chunk;
   parts = parts < 1 ? 1 : (parts > 16 ? 16 : parts);
   if (parts == 16) chunk = (longest + 15) / 16;
   return {(int)parts, (int)(chunk < (1 << 30) ? chunk : 1 << 30)};
