@@ -45,13 +45,17 @@ struct AttnBwdSeqs {
 };
 
 // How a launch is cut into workgroups, first those of dK and dV, then those of dQ.  A block of keys walks the tiles of 32 rows that see it, of
-// all query heads on its key head; lists longer than `chunk` are dealt out to up to `parts` workgroups, whose fp32 sums meet in a kernel of
-// their own (`partial`: one set of accumulators for each part and block).
+// all query heads on its key head, a block of rows the tiles of 32 keys that it sees; lists longer than `chunk` are dealt out to up to `parts`
+// workgroups, whose fp32 sums meet in a kernel of their own (`partial`: one set of accumulators for each part and block).
+struct AttnBwdCut {
+  int parts, chunk;
+  float* partial;
+};
 struct AttnBwdPlan {
   int q_blocks, k_blocks;       // over all sequences
-  int parts, chunk;
+  AttnBwdCut keys, rows;
   int key_groups, row_groups;   // workgroups of either kind (those of the keys: a multiple of 8)
-  float* partial;
+  int key_sums, row_sums;       // workgroups of the kernel that adds the parts
 };
 // Waves of a workgroup, each with 32 keys or query rows; two workgroups share a compute unit where 256 registers a lane do.  (One of 8 waves reads each
 // tile half as often, but its two waves on a SIMD keep step and wait together: 4 x 2048 tokens, 64 / 8 heads of 128, 988 us for 889.)
@@ -185,12 +189,22 @@ __device__ __forceinline__ HeadItem head_item(int item, int heads) {
   return {heads % 8 == 0 ? (o & 7) * (heads >> 3) + (o >> 3) : o, item / heads};
 }
 
-// The list of a block of keys: tiles first .. all of each of the group's heads.
-struct KeyList {
-  int first, each, total, parts;
+// Part `part` of a list of `total` tiles: tiles begin .. + count of it, of `parts` in all (none behind these).
+struct BwdPart {
+  int begin, count, parts;
 };
-__device__ __forceinline__ KeyList key_list(const AttnBwdArgs& a, const AttnBwdBlock& w, const AttnBwdPlan& plan) {
-  KeyList l{0, 0, 0, 1};
+__device__ __forceinline__ BwdPart part_of(int total, int part, const AttnBwdCut& cut) {
+  int parts = (total + cut.chunk - 1) / cut.chunk;
+  parts = parts < 1 ? 1 : (parts > cut.parts ? cut.parts : parts);
+  const int begin = (int)((int64_t)total * part / parts);
+  return {begin, (int)((int64_t)total * (part + 1) / parts) - begin, parts};
+}
+// The list of a block of keys: tiles first .. + each of every head of the group.
+struct KeyList {
+  int first, each, total;
+};
+__device__ __forceinline__ KeyList key_list(const AttnBwdArgs& a, const AttnBwdBlock& w) {
+  KeyList l{0, 0, 0};
   const int all = w.qn / 32;
   if (a.causal) {
     l.first = (w.block * BWD_BLOCK - (w.kn - w.qn)) / 32;
@@ -198,9 +212,16 @@ __device__ __forceinline__ KeyList key_list(const AttnBwdArgs& a, const AttnBwdB
   }
   l.each = l.first < all && w.block * BWD_BLOCK < w.kn ? all - l.first : 0;
   l.total = l.each * (a.Hq / a.Hk);
-  l.parts = (l.total + plan.chunk - 1) / plan.chunk;
-  l.parts = l.parts < 1 ? 1 : (l.parts > plan.parts ? plan.parts : l.parts);
   return l;
+}
+// Block `z` of rows in the order of dispatch (the longest lists first), and the length of its list.
+__device__ __forceinline__ AttnBwdBlock row_block(const AttnBwdArgs& a, const AttnBwdSeqs& seqs, const AttnBwdPlan& plan, int z) {
+  return attn_bwd_block<false>(a, seqs, a.causal && !seqs.n ? plan.q_blocks - 1 - z : z);
+}
+__device__ __forceinline__ int row_list(const AttnBwdArgs& a, const AttnBwdBlock& w) {
+  if (!a.causal) return w.kn / 32;
+  const int end = (w.block + 1) * BWD_BLOCK < w.qn ? (w.block + 1) * BWD_BLOCK : w.qn;
+  return (end + w.kn - w.qn) / 32;
 }
 
 // What the two kinds of workgroup share.  A wave holds 32 rows of its own side (keys for dK and dV, query rows for dQ) and walks tiles of 32 rows of
@@ -213,7 +234,11 @@ template <int NK, int NV>
 struct BwdShape {
   static constexpr int CODES = CodeTile<NK>::BYTES, ROWS_D = RowTile<64 * NK>::BYTES, ROWS_V = RowTile<64 * NV>::BYTES;
   static constexpr int ACC = 2 * NK + 2 * NV;                                 // accumulators of 32 keys
-  static constexpr int64_t PARTIAL = (int64_t)BWD_WAVES * ACC * 16 * 64;      // floats of a workgroup's sums
+  // Sums of part `part` of block z of head `bh`: of every wave its accumulators, four registers of all lanes after the other
+  template <int N>
+  __device__ static __forceinline__ v4f_t* sums(const AttnBwdCut& cut, int z, int part, int heads, int bh, int wave, int lane) {
+    return reinterpret_cast<v4f_t*>(cut.partial) + ((((int64_t)z * cut.parts + part) * heads + bh) * BWD_WAVES + wave) * (N * 4 * 64) + lane;
+  }
 };
 
 struct BwdPlace {
@@ -312,7 +337,7 @@ struct KeysLds {
 // One step: S and dP of a tile, its probabilities, and its part of the sums.  P is taken from S behind the products of dP, dS behind those of dV.
 template <int NK, int NV, int ADD>
 __device__ __forceinline__ void attn_bwd_keys_body(const AttnBwdArgs& a, const AttnBwdSeqs& seqs, const AttnBwdPlan& plan, int item, __bf16* __restrict__ dk_out,
-                                                   __bf16* __restrict__ dv_out, float* __restrict__ partial, uint8_t* lds) {
+                                                   __bf16* __restrict__ dv_out, uint8_t* lds) {
   using T = BwdShape<NK, NV>;
   using VT = RowTile<64 * NV>;
   using DT = RowTile<64 * NK>;
@@ -323,12 +348,13 @@ __device__ __forceinline__ void attn_bwd_keys_body(const AttnBwdArgs& a, const A
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 31, h = lane >> 5;
   const int heads = a.B * a.Hk, group = a.Hq / a.Hk;
   const HeadItem it = head_item(item, heads);
-  const int bh = it.head, part = it.index % plan.parts, z = it.index / plan.parts;
+  const int bh = it.head, part = it.index % plan.keys.parts, z = it.index / plan.keys.parts;
   if (z >= plan.k_blocks) return;   // (the last few of a number that is no multiple of 8)
   const AttnBwdBlock w = attn_bwd_block<true>(a, seqs, z);
-  const KeyList list = key_list(a, w, plan);
-  if (part >= list.parts) return;
-  const int begin = (int)((int64_t)list.total * part / list.parts), total = (int)((int64_t)list.total * (part + 1) / list.parts) - begin;
+  const KeyList list = key_list(a, w);
+  const BwdPart mine = part_of(list.total, part, plan.keys);
+  if (part >= mine.parts) return;
+  const int begin = mine.begin, total = mine.count;
   const int b = bh / a.Hk, hk = bh % a.Hk;
   const int shift = w.kn - w.qn, key0 = w.block * BWD_BLOCK + wave * 32;
   const bool live = key0 < w.kn;
@@ -555,8 +581,8 @@ __device__ __forceinline__ void attn_bwd_keys_body(const AttnBwdArgs& a, const A
     wait_all_but<0>();   // (the last loads into the LDS, which nobody reads, before it is given back)
   }
 
-  if (list.parts > 1) {
-    v4f_t* to = reinterpret_cast<v4f_t*>(partial + (((int64_t)z * plan.parts + part) * heads + bh) * T::PARTIAL) + wave * (T::ACC * 4 * 64) + lane;
+  if (mine.parts > 1) {
+    v4f_t* to = T::template sums<T::ACC>(plan.keys, z, part, heads, bh, wave, lane);
 #pragma unroll
     for (int n = 0; n < T::ACC; ++n)
 #pragma unroll
@@ -574,22 +600,16 @@ __device__ __forceinline__ void attn_bwd_keys_body(const AttnBwdArgs& a, const A
   store_rows<64 * NV>(dv, 1.0f, live, own, dv_out + b * a.dv_sb + hk * a.dv_sh + at * a.dv_ss, a.dv_ss, lane);
 }
 
-// Sums of the parts, in their order.  Grid: (key blocks by heads, blocks of 32 columns of dK, then of dV).
+// Sums of the parts, in their order.  A workgroup: 32 columns of one block's gradients (dK, then dV; those of dQ behind them).
 template <int NK, int NV>
 __global__ __launch_bounds__(64 * BWD_WAVES) void attn_bwd_sum_kernel(AttnBwdArgs a, AttnBwdSeqs seqs, AttnBwdPlan plan) {
   using T = BwdShape<NK, NV>;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 31, h = lane >> 5;
-  const int heads = a.B * a.Hk, bh = blockIdx.x % heads, z = blockIdx.x / heads, n = blockIdx.y;
-  const AttnBwdBlock w = attn_bwd_block<true>(a, seqs, z);
-  const KeyList list = key_list(a, w, plan);
-  const int key = w.block * BWD_BLOCK + wave * 32;
-  if (list.parts == 1 || key >= (seqs.n ? w.kn : a.Sk)) return;
-  const int hk = bh % a.Hk, b = bh / a.Hk;
-  v16f_t sum = zeros();
-  if (key < w.kn) {
+  auto sum_of = [&](auto count, const AttnBwdCut& cut, int parts, int z, int heads, int bh, int n) {
+    v16f_t sum = zeros();
 #pragma unroll 4
-    for (int part = 0; part < list.parts; ++part) {   // (the loads of four parts at a time under way)
-      const v4f_t* from = reinterpret_cast<const v4f_t*>(plan.partial + (((int64_t)z * plan.parts + part) * heads + bh) * T::PARTIAL) + (wave * T::ACC + n) * 4 * 64 + lane;
+    for (int part = 0; part < parts; ++part) {   // (the loads of four parts at a time under way)
+      const v4f_t* from = T::template sums<decltype(count)::value>(cut, z, part, heads, bh, wave, lane) + n * 4 * 64;
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         const v4f_t x = from[g * 64];
@@ -597,10 +617,28 @@ __global__ __launch_bounds__(64 * BWD_WAVES) void attn_bwd_sum_kernel(AttnBwdArg
         for (int i = 0; i < 4; ++i) sum[4 * g + i] += x[i];
       }
     }
+    return sum;
+  };
+  int item = blockIdx.x;
+  if (item < plan.key_sums) {
+    const int heads = a.B * a.Hk, n = item % T::ACC, bh = item / T::ACC % heads, z = item / T::ACC / heads;
+    const AttnBwdBlock w = attn_bwd_block<true>(a, seqs, z);
+    const int parts = part_of(key_list(a, w).total, 0, plan.keys).parts, key = w.block * BWD_BLOCK + wave * 32;
+    if (parts == 1 || key >= (seqs.n ? w.kn : a.Sk)) return;
+    const v16f_t sum = sum_of(std::integral_constant<int, T::ACC>{}, plan.keys, key < w.kn ? parts : 0, z, heads, bh, n);
+    const int hk = bh % a.Hk, b = bh / a.Hk;
+    const int64_t at = w.k_first + key + r;
+    if (n < 2 * NK) store_columns(reinterpret_cast<__bf16*>(a.dk) + b * a.dk_sb + hk * a.dk_sh + at * a.dk_ss, sum, a.sm_scale, n, h);
+    else store_columns(reinterpret_cast<__bf16*>(a.dv) + b * a.dv_sb + hk * a.dv_sh + at * a.dv_ss, sum, 1.0f, n - 2 * NK, h);
+    return;
   }
-  const int64_t at = w.k_first + key + r;
-  if (n < 2 * NK) store_columns(reinterpret_cast<__bf16*>(a.dk) + b * a.dk_sb + hk * a.dk_sh + at * a.dk_ss, sum, a.sm_scale, n, h);
-  else store_columns(reinterpret_cast<__bf16*>(a.dv) + b * a.dv_sb + hk * a.dv_sh + at * a.dv_ss, sum, 1.0f, n - 2 * NK, h);
+  item -= plan.key_sums;
+  const int heads = a.B * a.Hq, n = item % (2 * NK), bh = item / (2 * NK) % heads, z = item / (2 * NK) / heads;
+  const AttnBwdBlock w = row_block(a, seqs, plan, z);
+  const int parts = part_of(row_list(a, w), 0, plan.rows).parts, row = w.block * BWD_BLOCK + wave * 32;
+  if (parts == 1 || row >= w.qn) return;
+  const v16f_t sum = sum_of(std::integral_constant<int, 2 * NK>{}, plan.rows, parts, z, heads, bh, n);
+  store_columns(reinterpret_cast<__bf16*>(a.dq) + (bh / a.Hq) * a.dq_sb + (bh % a.Hq) * a.dq_sh + (int64_t)(w.q_first + row + r) * a.dq_ss, sum, a.sm_scale, n, h);
 }
 
 // ---------------------------------------------------------------------------------------------------------------------- dQ
@@ -623,15 +661,13 @@ __device__ __forceinline__ void attn_bwd_rows_body(const AttnBwdArgs& a, const A
   const int heads = a.B * a.Hq;
   const HeadItem it = head_item(item, heads);
   const int bh = it.head, b = bh / a.Hq, hq = bh % a.Hq, hk = hq / (a.Hq / a.Hk);
-  const AttnBwdBlock w = attn_bwd_block<false>(a, seqs, a.causal && !seqs.n ? plan.q_blocks - 1 - it.index : it.index);
-  const int shift = w.kn - w.qn, row0 = w.block * BWD_BLOCK + wave * 32;
+  const int part = it.index % plan.rows.parts, z = it.index / plan.rows.parts;
+  const AttnBwdBlock w = row_block(a, seqs, plan, z);
+  const BwdPart mine = part_of(row_list(a, w), part, plan.rows);
+  if (part >= mine.parts) return;
+  const int shift = w.kn - w.qn, row0 = w.block * BWD_BLOCK + wave * 32, begin = mine.begin, total = mine.count;   // tile t of this part: begin + t
   const bool live = row0 < w.qn;
-  int total = w.kn / 32;
-  if (a.causal) {
-    const int end = (w.block + 1) * BWD_BLOCK < w.qn ? (w.block + 1) * BWD_BLOCK : w.qn;
-    total = (end + shift) / 32;
-  }
-  const int own_tile = bh * (a.Sq / 32) + w.q_first / 32 + (live ? row0 / 32 : 0), first_at = (b * a.Hk + hk) * (a.Sk / 32) + w.k_first / 32;
+  const int own_tile = bh * (a.Sq / 32) + w.q_first / 32 + (live ? row0 / 32 : 0), first_at = (b * a.Hk + hk) * (a.Sk / 32) + w.k_first / 32 + begin;
 
   v16f_t acc[2 * NK];
 #pragma unroll
@@ -667,7 +703,7 @@ __device__ __forceinline__ void attn_bwd_rows_body(const AttnBwdArgs& a, const A
   int state = 2;
   auto look = [&](int tile) {
     if (!a.causal) return;
-    const int away = row0 + shift - 32 * tile;   // a multiple of 32
+    const int away = row0 + shift - 32 * (begin + tile);   // a multiple of 32
     const int now = away > 0 ? 2 : (away == 0 ? 1 : 0);
     if (now == state) return;
     state = now;
@@ -689,10 +725,10 @@ __device__ __forceinline__ void attn_bwd_rows_body(const AttnBwdArgs& a, const A
   // The additive terms of tile `i`, in the registers where its scores will be
   uint8_t* const at_bias = lds + L::O_BIAS + wave * Bias::BYTES;
   auto load_bias = [&](int i) {
-    Bias::load(a.bias + b * a.bias_sb + hq * a.bias_sh + (int64_t)(live ? row0 : 0) * a.bias_sm + 32 * tile(i), a.bias_sm, at_bias, lane);
+    Bias::load(a.bias + b * a.bias_sb + hq * a.bias_sh + (int64_t)(live ? row0 : 0) * a.bias_sm + 32 * (begin + tile(i)), a.bias_sm, at_bias, lane);
   };
   auto add = [&](int i, int g, v16f_t& S) {
-    const float away = (float)(row0 + r + shift - 32 * i - 4 * h);
+    const float away = (float)(row0 + r + shift - 32 * (begin + i) - 4 * h);
     v4f_t x;
     if constexpr (ADD == ADD_BIAS) x = Bias::read(at_bias, lane, g);
 #pragma unroll
@@ -865,6 +901,15 @@ __device__ __forceinline__ void attn_bwd_rows_body(const AttnBwdArgs& a, const A
       for (int n = 0; n < 2 * NK; ++n) acc[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(DT::column_frag(at + column_base[0], at + column_base[1], n, c), f[c], acc[n], 0, 0, 0);
   }
   wait_all_but<0>();   // (the last loads into the LDS, which nobody reads, before it is given back)
+  if (mine.parts > 1) {
+    if (!live) return;
+    v4f_t* to = T::template sums<2 * NK>(plan.rows, z, part, heads, bh, wave, lane);
+#pragma unroll
+    for (int n = 0; n < 2 * NK; ++n)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) to[(n * 4 + g) * 64] = v4f_t{acc[n][4 * g], acc[n][4 * g + 1], acc[n][4 * g + 2], acc[n][4 * g + 3]};
+    return;
+  }
   asm volatile("s_barrier" ::: "memory");   // (no wave's loads or reads are under way any more)
   if (!live) return;
   store_rows<64 * NK>(acc, a.sm_scale, true, lds + wave * (64 * 64 * NK), dq_out + b * a.dq_sb + hq * a.dq_sh + (int64_t)(w.q_first + row0) * a.dq_ss, a.dq_ss, lane);
@@ -874,7 +919,7 @@ template <int NK, int NV, int ADD>
 __global__ __launch_bounds__(64 * BWD_WAVES, NK > 2 ? 1 : 2) void attn_bwd_kernel(AttnBwdArgs a, AttnBwdSeqs seqs, AttnBwdPlan plan) {
   extern __shared__ __attribute__((aligned(256))) uint8_t lds[];
   const int item = (int)blockIdx.x;
-  if (item < plan.key_groups) attn_bwd_keys_body<NK, NV, ADD>(a, seqs, plan, item, reinterpret_cast<__bf16*>(a.dk), reinterpret_cast<__bf16*>(a.dv), plan.partial, lds);
+  if (item < plan.key_groups) attn_bwd_keys_body<NK, NV, ADD>(a, seqs, plan, item, reinterpret_cast<__bf16*>(a.dk), reinterpret_cast<__bf16*>(a.dv), lds);
   else attn_bwd_rows_body<NK, NV, ADD>(a, seqs, plan, item - plan.key_groups, reinterpret_cast<__bf16*>(a.dq), lds);
 }
 
@@ -886,8 +931,11 @@ int launch_one(const AttnBwdArgs& a, const AttnBwdSeqs& seqs, const AttnBwdPlan&
   if (const int rc = limit.raise((const void*)attn_bwd_kernel<NK, NV, ADD>, lds, "attention_bwd")) return rc;
   hipLaunchKernelGGL((attn_bwd_kernel<NK, NV, ADD>), dim3((unsigned)(plan.key_groups + plan.row_groups)), dim3(64 * BWD_WAVES), lds, st, a, seqs, plan);
   if (const int rc = check_launch("attention_bwd")) return rc;
-  if (!a.dk || plan.parts == 1) return ALTO_MXFP4_OK;
-  hipLaunchKernelGGL((attn_bwd_sum_kernel<NK, NV>), dim3((unsigned)(a.B * a.Hk * plan.k_blocks), T::ACC), dim3(64 * BWD_WAVES), 0, st, a, seqs, plan);
+  AttnBwdPlan sums = plan;
+  sums.key_sums *= T::ACC;
+  sums.row_sums *= 2 * NK;
+  if (sums.key_sums + sums.row_sums == 0) return ALTO_MXFP4_OK;
+  hipLaunchKernelGGL((attn_bwd_sum_kernel<NK, NV>), dim3((unsigned)(sums.key_sums + sums.row_sums)), dim3(64 * BWD_WAVES), 0, st, a, seqs, sums);
   return check_launch("attention_bwd");
 }
 

@@ -118,45 +118,75 @@ __global__ __launch_bounds__(256) void attn_bwd_prepare_kernel(const PrepareArgs
   }
 }
 
-// Cuts of the key blocks' lists (see AttnBwdPlan), counted in a workgroup's tiles of 32 rows.
-struct Cuts {
-  int parts, chunk;
+// Lists of tiles (see AttnBwdPlan) of one head: how many, of all together, the longest.
+struct Lists {
+  int64_t blocks, sum, longest;
 };
-int64_t count_tiles(int64_t qn, int64_t kn, int64_t block_keys, int causal, int64_t heads, int64_t& longest) {   // of one key head
-  const int64_t blocks = (kn + block_keys - 1) / block_keys, tiles = qn / 32;
-  int64_t sum = 0;
-  for (int64_t b = 0; b < blocks; ++b) {
-    int64_t first = causal ? (b * block_keys - (kn - qn)) / 32 : 0;
-    first = first < 0 ? 0 : first;
-    const int64_t n = first < tiles ? (tiles - first) * heads : 0;
-    sum += n;
-    longest = n > longest ? n : longest;
+void count_tiles(Lists& keys, Lists& rows, int64_t qn, int64_t kn, int causal) {
+  const int64_t shift = kn - qn;
+  auto add = [](Lists& l, int64_t n) {
+    l.blocks += 1;
+    l.sum += n;
+    l.longest = n > l.longest ? n : l.longest;
+  };
+  for (int64_t at = 0; at < kn; at += BWD_BLOCK) {
+    const int64_t first = causal && at > shift ? (at - shift) / 32 : 0;
+    add(keys, first < qn / 32 ? qn / 32 - first : 0);
   }
-  return sum;
+  for (int64_t at = 0; at < qn; at += BWD_BLOCK) {
+    const int64_t end = at + BWD_BLOCK < qn ? at + BWD_BLOCK : qn;
+    add(rows, (causal ? end + shift : kn) / 32);
+  }
+}
+// How long lists are cut.
+struct Cuts {
+  AttnBwdCut keys, rows;
+};
+AttnBwdCut cut_lists(bool cut, int64_t longest, int64_t piece, int most) {
+  if (!cut) return {1, 1 << 30, nullptr};
+  int64_t parts = (longest + piece - 1) / piece;
+  if (parts > most) {
+    parts = most;
+    piece = (longest + most - 1) / most;
+  }
+  return {(int)parts, (int)(piece < (1 << 30) ? piece : 1 << 30), nullptr};
 }
 Cuts cut(const alto_mxfp4_attention_bwd_t& p) {
-  const int64_t block = BWD_BLOCK, heads = p.Hq / p.Hk;
-  int64_t longest = 0, sum = 0;
+  const int64_t group = p.Hq / p.Hk;
+  Lists keys{}, rows{};
   if (p.n_seqs > 0) {
-    for (int i = 0; i < p.n_seqs; ++i) sum += count_tiles(p.cu_q[i + 1] - p.cu_q[i], p.cu_k[i + 1] - p.cu_k[i], block, p.causal, heads, longest);
+    for (int i = 0; i < p.n_seqs; ++i) count_tiles(keys, rows, p.cu_q[i + 1] - p.cu_q[i], p.cu_k[i + 1] - p.cu_k[i], p.causal);
   } else {
-    sum = count_tiles(p.Sq, p.Sk_used, block, p.causal, heads, longest);
+    count_tiles(keys, rows, p.Sq, p.Sk_used, p.causal);
   }
-  // A tile of dQ takes about .62 of one of dK and dV (products: 18 to 26 with D = Dv = 128), and the compute units hold 512 workgroups: a list much longer
-  // than an equal share of the whole would end alone.  Pieces of 1.7 / 1.62 of that share (1.9 and 1.4: 3 % and 1.5 % more over 13 shapes), of 24 tiles
-  // at least (16 and 32: 80.9 and 73.6 us for 72.2, 6 packed sequences of 16 / 4 heads of 128).  The parts' sums go through memory and take a kernel, so
-  // a list stays whole that is little longer than a piece: 2048 tokens of 128, 32 heads, 64 tiles for pieces of 58, 124 us for 134 in two parts; 20 heads,
-  // 64 for 36, 94 for 102; but not: 12 heads, 64 for 24, 82 for 77; 3 x 64 / 8 heads, 512 for 346, 691 for 655.
-  const int64_t share = (int64_t)(1.7 * (double)(sum * p.B * p.Hk) / 512.0);
-  int64_t chunk = share < 24 ? 24 : share;
-  int64_t parts = 4 * longest <= 5 * chunk || longest <= chunk + 30 ? 1 : (longest + chunk - 1) / chunk;
-  parts = parts < 1 ? 1 : (parts > 16 ? 16 : parts);
-  if (parts == 16) chunk = (longest + 15) / 16;
-  return {(int)parts, (int)(chunk < (1 << 30) ? chunk : 1 << 30)};
+  // Counted in tiles of dK and dV; one of dQ takes about .62 of one (products: 18 to 26 with D = Dv = 128).  The compute units hold 512 workgroups, and a
+  // list much longer than an equal share of the whole ends alone.  Pieces have 1.05 of that share (1.17 and 0.85: 3 % and 1.5 % more over 13 shapes) and
+  // 24 tiles at least (16 and 32: 80.9 and 73.6 us for 72.2, 6 packed sequences of 16 / 4 heads of 128).  Parts cost a kernel, 5 tiles' time, and their
+  // sums' way through memory.  So whichever of the two kinds is cut by what the launch would take: both, where few rows or heads leave all but some
+  // units idle (3 x 6 / 3 heads, 64 rows, 4736 keys of 128 / 64: 32 us, 84 whole; 2048 tokens of 128, 4 heads 45, 57 whole), neither at 2048 tokens of
+  // 20 heads (94 us, 102 with dK and dV cut) or 32 (124, 134), dK and dV at 12 (77, 82 whole) and 3 x 64 / 8 (655, 691 whole).
+  const double B = (double)p.B, share = 1.05 * B * p.Hq * ((double)keys.sum + 0.62 * (double)rows.sum) / 512.0;
+  const double key_piece = std::max(share, 24.0), row_piece = std::max(share / 0.62, 24.0);
+  const double key_whole = (double)(keys.longest * group), row_whole = (double)rows.longest;
+  const double key_cost = 0.042 * B * ((double)keys.sum * p.Hq / key_piece + (double)keys.blocks * p.Hk / 2) * (double)(p.D + p.Dv) / 256;
+  const double row_cost = 0.04 * B * p.Hq * ((double)rows.sum / row_piece + (double)rows.blocks / 2) * (double)p.D / 128;
+  bool best_keys = false, best_rows = false;
+  double best = 0;
+  for (int c = 0; c < 4; ++c) {
+    const bool k = c & 1, r = c & 2;
+    if ((k && key_whole <= 1.25 * key_piece) || (r && row_whole <= 1.25 * row_piece)) continue;
+    const double time = std::max(share, std::max(k ? key_piece : key_whole, 0.62 * (r ? row_piece : row_whole))) + (c ? 5.0 : 0.0) + (k ? key_cost : 0.0) + (r ? row_cost : 0.0);
+    if (c == 0 || time < best) {
+      best = time;
+      best_keys = k;
+      best_rows = r;
+    }
+  }
+  return {cut_lists(best_keys, keys.longest * group, (int64_t)key_piece, 16), cut_lists(best_rows, rows.longest, (int64_t)row_piece, 32)};
 }
 
 struct Workspace {
-  int64_t q_records, k_records, k_rows, v_rows, g_rows, partial, total;
+  int64_t q_records, k_records, k_rows, v_rows, g_rows, key_sums, row_sums, total;
 };
 Workspace workspace(const alto_mxfp4_attention_bwd_t& p, const Cuts& cuts) {
   const int64_t B = p.B, Hq = p.Hq, Hk = p.Hk, Sq = p.Sq, Sk = p.Sk, D = p.D, Dv = p.Dv;
@@ -168,8 +198,9 @@ Workspace workspace(const alto_mxfp4_attention_bwd_t& p, const Cuts& cuts) {
   take(w.k_rows, B * Hk * Sk * D * 2);
   take(w.v_rows, B * Hk * Sk * Dv * 2);
   take(w.g_rows, B * Hq * Sq * Dv * 2);
-  const int64_t block = BWD_BLOCK, blocks = Sk / block + (p.n_seqs > 0 ? (p.n_seqs < ATTN_MAX_SEQS ? p.n_seqs : ATTN_MAX_SEQS) : 1);   // (at least those of any launch)
-  take(w.partial, cuts.parts > 1 ? B * Hk * blocks * cuts.parts * block * (D + Dv) * 4 : 0);
+  const int64_t more = p.n_seqs > 0 ? (p.n_seqs < ATTN_MAX_SEQS ? p.n_seqs : ATTN_MAX_SEQS) : 1;   // (blocks: at least those of any launch)
+  take(w.key_sums, cuts.keys.parts > 1 ? B * Hk * (Sk / BWD_BLOCK + more) * cuts.keys.parts * BWD_BLOCK * (D + Dv) * 4 : 0);
+  take(w.row_sums, cuts.rows.parts > 1 ? B * Hq * (Sq / BWD_BLOCK + more) * cuts.rows.parts * BWD_BLOCK * D * 4 : 0);
   w.total = at;
   return w;
 }
@@ -252,11 +283,17 @@ static int attention_bwd(const alto_mxfp4_attention_bwd_t& p, hipStream_t st) {
   a.bias = p.bias; a.bias_sb = p.bias_sb; a.bias_sh = p.bias_sh; a.bias_sm = p.bias_sm; a.distances = p.alibi_slopes != nullptr;
   const int row_block = BWD_BLOCK, key_block = row_block;
   auto go = [&](const AttnBwdSeqs& s, int q_blocks, int k_blocks) {
-    AttnBwdPlan plan{q_blocks, k_blocks, cuts.parts, cuts.chunk, 0, 0, (float*)(ws + w.partial)};
-    const int64_t keys = p.dk ? (p.B * p.Hk * cuts.parts * k_blocks + 7) / 8 * 8 : 0, rows = p.dq ? p.B * p.Hq * q_blocks : 0;
-    ALTO_REQUIRE(keys + rows < (1ll << 31), "attention_bwd: too many workgroups");
-    plan.key_groups = (int)keys;
-    plan.row_groups = (int)rows;
+    AttnBwdPlan plan{q_blocks, k_blocks, cuts.keys, cuts.rows, 0, 0, 0, 0};
+    plan.keys.partial = (float*)(ws + w.key_sums);
+    plan.rows.partial = (float*)(ws + w.row_sums);
+    const int64_t key_blocks = p.dk ? p.B * p.Hk * k_blocks : 0, row_blocks = p.dq ? p.B * p.Hq * q_blocks : 0;
+    const int64_t key_groups = (key_blocks * cuts.keys.parts + 7) / 8 * 8, row_groups = row_blocks * cuts.rows.parts;
+    const int64_t key_sums = cuts.keys.parts > 1 ? key_blocks : 0, row_sums = cuts.rows.parts > 1 ? row_blocks : 0;
+    ALTO_REQUIRE(key_groups + row_groups < (1ll << 31) && (key_sums + row_sums) * 12 < (1ll << 31), "attention_bwd: too many workgroups");
+    plan.key_groups = (int)key_groups;
+    plan.row_groups = (int)row_groups;
+    plan.key_sums = (int)key_sums;
+    plan.row_sums = (int)row_sums;
     switch (p.D) {
       case 64: return launch_attn_bwd<1>(a, s, plan, p.Dv, st);
       case 128: return launch_attn_bwd<2>(a, s, plan, p.Dv, st);

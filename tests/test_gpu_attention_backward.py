@@ -67,6 +67,11 @@ CASES = [
     (1, 3, 3, 160, 320, 192, 64, True),
     (1, 2, 1, 64, 192, 256, 128, False),
     (1, 5, 5, 288, 288, 256, 64, True),
+    (1, 2, 1, 64, 2080, 64, 64, False),        # few rows: their lists of keys in several parts
+    (2, 1, 1, 96, 1504, 128, 128, True),
+    (1, 1, 1, 32, 3200, 192, 64, True),
+    (1, 4, 1, 1280, 96, 64, 128, False),       # few keys: their lists of rows in several parts
+    (1, 2, 1, 1312, 1344, 256, 128, True),     # both, of blocks that differ
 ]
 
 
@@ -76,7 +81,7 @@ def test_gradients_match_the_formula(m, case):
     check(x.call(m), x.expected())
 
 
-@pytest.mark.parametrize("case", [(2, 4, 2, 96, 160, 128, 128, False), (2, 2, 2, 64, 64, 64, 64, True), (1, 2, 1, 64, 96, 192, 128, False), (1, 2, 1, 32, 64, 256, 64, True)],
+@pytest.mark.parametrize("case", [(2, 4, 2, 96, 160, 128, 128, False), (2, 2, 2, 64, 64, 64, 64, True), (1, 2, 1, 64, 96, 192, 128, False), (1, 2, 1, 32, 64, 256, 64, True), (1, 1, 1, 96, 1600, 128, 64, True)],
                          ids=lambda c: "x".join(map(str, c)))
 @pytest.mark.parametrize("extra", ["bias", "alibi", "both"])
 def test_additive_terms(m, case, extra):
@@ -96,7 +101,8 @@ def test_additive_terms(m, case, extra):
         assert bool((got[0][-1, :, 0] == 0).all())
 
 
-@pytest.mark.parametrize("case", [(2, 4, 2, 96, 160, 128, 64, True), (2, 2, 2, 160, 192, 192, 128, False)], ids=lambda c: "x".join(map(str, c)))
+@pytest.mark.parametrize("case", [(2, 4, 2, 96, 160, 128, 64, True), (2, 2, 2, 160, 192, 192, 128, False), (1, 2, 1, 64, 1280, 64, 64, True)],
+                         ids=lambda c: "x".join(map(str, c)))
 def test_a_bias_of_any_layout(m, case):
     """Broadcast rows, batches and heads, a part of something larger at an odd place with rows an odd number of elements apart: the bits of its dense copy."""
     B, Hq, _, Sq, Sk, *_ = case
@@ -152,7 +158,7 @@ def test_a_bias_of_extreme_values(m, D):
 def test_packed_sequences_are_the_sequences_alone(m, causal):
     """Lengths of one tile, of odd numbers of tiles and of more than a workgroup's block; each sequence's gradients bit for bit those of its own call."""
     Hq, Hk, D, Dv = 4, 2, 128, 64
-    lens_q, lens_k = [32, 96, 288, 160], [32, 96, 288, 224] if causal else [64, 32, 96, 160]
+    lens_q, lens_k = [32, 96, 288, 160, 64], [32, 96, 288, 224, 1600] if causal else [64, 32, 96, 160, 1600]
     parts = [Operands(1, Hq, Hk, a, b, D, Dv, causal, seed=a + b) for a, b in zip(lens_q, lens_k)]
     cat = lambda name, dim: torch.cat([getattr(p, name) for p in parts], dim).contiguous()  # noqa: E731
     whole = Operands.__new__(Operands)
@@ -166,8 +172,9 @@ def test_packed_sequences_are_the_sequences_alone(m, causal):
         rows, keys = slice(cu_q[i], cu_q[i + 1]), slice(cu_k[i], cu_k[i + 1])
         mine = got[0][:, :, rows], got[1][:, :, keys], got[2][:, :, keys]
         check(mine, p.expected(), f"sequence {i}")
-        for a, b in zip(mine, p.call(m)):
-            assert torch.equal(a, b)
+        if max(lens_k[i] // 32, lens_q[i] // 32 * Hq // Hk) <= 24:   # (longer lists of tiles are cut as the whole call asks for it)
+            for a, b in zip(mine, p.call(m)):
+                assert torch.equal(a, b)
 
 
 def test_more_sequences_than_one_launch_takes(m):

@@ -62,7 +62,7 @@ def test_attention_operands(changes, text):
 
 
 def test_attention_workspace():
-    """It holds the tiles, and parts of dK and dV only where lists are cut."""
+    """It holds the tiles, and parts of sums only where lists are cut."""
     size = _lib.load().alto_mxfp4_attention_bwd_workspace_bytes
 
     def up(n):
@@ -75,6 +75,9 @@ def test_attention_workspace():
     # one head with one block of keys and 1024 tiles of rows: 16 parts
     long = dict(Hq=1, Hk=1, Sq=32768, causal=0)
     assert size(ctypes.byref(attention(**long))) == up(1024 * 272) + up(4 * 16) + 128 * 192 * 2 + 32768 * 64 * 2 + 2 * 16 * 128 * 192 * 4
+    # one block of rows with 1024 tiles of keys: 32 parts
+    few = dict(Hq=1, Hk=1, Sq=32, Sk=32768, Sk_used=32768)
+    assert size(ctypes.byref(attention(**few))) == up(272) + up(1024 * 16) + 32768 * 192 * 2 + 32 * 64 * 2 + 32 * 128 * 128 * 4
 
 
 @pytest.mark.parametrize("changes,text", [
