@@ -237,11 +237,11 @@ def _attend_quantized(operands, sm_scale: float, causal: bool, out: torch.Tensor
 @torch.compiler.allow_in_graph
 class MXFP4AttentionFunction(torch.autograd.Function):
     """The attention of :func:`_attend` (or with a ``bias``, of :func:`attention_mxfp4_forward`) on [B, H, S, D] views, with its backward.  Kept from
-    one to the other: Q, K and V as codes and scales, the output and the log-sum-exp."""
+    one to the other: Q, K and V as codes and scales, the output and the log-sum-exp.  What only the backward refuses (a scale that is not positive, the
+    gradient of a bias) it refuses when it runs."""
 
     @staticmethod
     def forward(ctx, q, k, v, sm_scale, causal, rows_outer, bias, alibi_slopes, cu_q, cu_k):
-        torch._check(0.0 < sm_scale < float("inf"), lambda: f"sm_scale {sm_scale}: the backward needs a positive one")
         (B, Hq, Sq, D), (_, Hk, Sk, Dv) = q.shape, v.shape
         ctx.dtypes, ctx.keys = (q.dtype, k.dtype, v.dtype), Sk
         pad = 32 if bias is not None and Sk % 64 == 32 else 0   # (as in _fixed_length)
@@ -264,6 +264,8 @@ class MXFP4AttentionFunction(torch.autograd.Function):
     def backward(ctx, grad_out, _):
         qq, qs, kq, ks, vq, vs, out, lse, b4, sl = ctx.saved_tensors
         sm_scale, causal, rows_outer, cu_q, cu_k = ctx.more
+        if ctx.needs_input_grad[6]:
+            raise NotImplementedError("the gradient of a bias is not implemented: detach it")
         want_q, want_kv = ctx.needs_input_grad[0], ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
         dq, dk, dv = _gradients(grad_out, (qq, qs, kq, ks, vq, vs), out, lse, sm_scale, causal, ctx.keys, b4, sl, cu_q, cu_k, rows_outer, want_q, want_kv)
         grads = [None if g is None or not need else g[:, :, :n].to(dt) for g, need, n, dt in
@@ -349,8 +351,6 @@ def _fixed_length(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, alibi_slope
     if sm_scale is None:
         sm_scale = q.shape[-1] ** -0.5
     if _differentiated(q, k, v):
-        if bias is not None and bias.requires_grad:
-            raise NotImplementedError("a bias that requires a gradient is not implemented: detach it")
         out, lse = MXFP4AttentionFunction.apply(q, k, v, float(sm_scale), bool(causal), rows_outer, bias, alibi_slopes, None, None)
     elif bias is None:
         out, lse = _results(q, v.shape[3], rows_outer, False)

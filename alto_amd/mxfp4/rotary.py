@@ -148,6 +148,7 @@ def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], inv_freq: torch.Ten
     batch, head, row = _DIMS[layout]
     rt.dtype_code(q.dtype)
     assert q.dim() == dims and (k is None or (k.dim() == dims and k.dtype == q.dtype)), f"layout {layout!r}: q and k of {dims} dims and one type"
+    assert q.shape[head] > 0, "q has no heads"
     assert k is None or all(k.shape[d] == q.shape[d] for d in range(dims) if d != head), f"q of shape {tuple(q.shape)} and k of {tuple(k.shape)}"
     assert inv_freq.dim() == 1 and inv_freq.dtype == torch.float64 and inv_freq.is_contiguous(), "inv_freq: fp64, one frequency for each pair"
     assert 1 <= inv_freq.shape[0] <= 1024 and 2 * inv_freq.shape[0] <= q.shape[-1], f"{inv_freq.shape[0]} frequencies for heads of {q.shape[-1]}"
@@ -155,6 +156,8 @@ def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], inv_freq: torch.Ten
         assert positions.dtype in (torch.int32, torch.int64), f"positions of type {positions.dtype}: int32 or int64"
         fits = positions.shape == (q.shape[row],) or (batch is not None and positions.dim() == 2 and positions.shape[0] in (1, q.shape[batch]) and positions.shape[1] == q.shape[row])
         assert fits, f"positions of shape {tuple(positions.shape)} for q of {tuple(q.shape)}, layout {layout!r}"
+    if inv_freq.requires_grad and torch.is_grad_enabled():
+        raise NotImplementedError("the gradient of the frequencies is not implemented: detach them")
     for t in (k, inv_freq, positions):
         assert t is None or t.device == q.device, f"tensors on {q.device} and {t.device}"
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):

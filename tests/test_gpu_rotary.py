@@ -204,6 +204,21 @@ def test_refusals(m):
         m.apply_rotary(q, None, freq, layout="sbhd")
     with pytest.raises(RuntimeError):
         m.apply_rotary(q, None, freq.cpu())
+    with pytest.raises(AssertionError):
+        m.apply_rotary(q[:, :0], q, freq)
+    with pytest.raises(NotImplementedError):
+        m.apply_rotary(q, q, freq.clone().requires_grad_(True))
+
+
+def test_nothing_to_rotate(m):
+    """No tokens, no sequences, no heads of K: as empty as they came."""
+    freq = m.rotary_frequencies(8)[0].to(DEV)
+    q = torch.randn(2, 3, 5, 8, dtype=torch.bfloat16, device=DEV)
+    for a, b in ((q[:0], q[:0]), (q[:, :, :0], q[:, :1, :0])):
+        got = m.apply_rotary(a, b, freq)
+        assert got[0].shape == a.shape and got[1].shape == b.shape
+    got = m.apply_rotary(q, q[:, :0], freq)
+    assert torch.equal(got[0], m.apply_rotary(q, None, freq)) and got[1].numel() == 0
 
 
 def test_native_call_and_python_function_are_the_same(m, monkeypatch):
