@@ -44,7 +44,7 @@ struct AttnBwdSeqs {
   int zq[ATTN_MAX_SEQS + 1], zk[ATTN_MAX_SEQS + 1], q0[ATTN_MAX_SEQS], qn[ATTN_MAX_SEQS], k0[ATTN_MAX_SEQS], kn[ATTN_MAX_SEQS];
 };
 
-// How a launch is cut into workgroups, first those of dK and dV, then those of dQ.  A block of keys walks the tiles of 32 rows that see it, of
+// How a launch is cut into workgroups, those of dK and dV and those of dQ, the longer ones first.  A block of keys walks the tiles of 32 rows that see it, of
 // all query heads on its key head, a block of rows the tiles of 32 keys that it sees; lists longer than `chunk` are dealt out to up to `parts`
 // workgroups, whose fp32 sums meet in a kernel of their own (`partial`: one set of accumulators for each part and block).
 struct AttnBwdCut {
@@ -54,7 +54,8 @@ struct AttnBwdCut {
 struct AttnBwdPlan {
   int q_blocks, k_blocks;       // over all sequences
   AttnBwdCut keys, rows;
-  int key_groups, row_groups;   // workgroups of either kind (those of the keys: a multiple of 8)
+  int key_groups, row_groups;   // workgroups of either kind (multiples of 8: the last few may have nothing)
+  int rows_first;
   int key_sums, row_sums;       // workgroups of the kernel that adds the parts
 };
 // Waves of a workgroup, each with 32 keys or query rows; two workgroups share a compute unit where 256 registers a lane do.  (One of 8 waves reads each
@@ -662,6 +663,7 @@ __device__ __forceinline__ void attn_bwd_rows_body(const AttnBwdArgs& a, const A
   const HeadItem it = head_item(item, heads);
   const int bh = it.head, b = bh / a.Hq, hq = bh % a.Hq, hk = hq / (a.Hq / a.Hk);
   const int part = it.index % plan.rows.parts, z = it.index / plan.rows.parts;
+  if (z >= plan.q_blocks) return;
   const AttnBwdBlock w = row_block(a, seqs, plan, z);
   const BwdPart mine = part_of(row_list(a, w), part, plan.rows);
   if (part >= mine.parts) return;
@@ -925,9 +927,11 @@ __device__ __forceinline__ void attn_bwd_rows_body(const AttnBwdArgs& a, const A
 template <int NK, int NV, int ADD>
 __global__ __launch_bounds__(64 * BWD_WAVES, NK > 2 ? 1 : 2) void attn_bwd_kernel(AttnBwdArgs a, AttnBwdSeqs seqs, AttnBwdPlan plan) {
   extern __shared__ __attribute__((aligned(256))) uint8_t lds[];
-  const int item = (int)blockIdx.x;
-  if (item < plan.key_groups) attn_bwd_keys_body<NK, NV, ADD>(a, seqs, plan, item, reinterpret_cast<__bf16*>(a.dk), reinterpret_cast<__bf16*>(a.dv), lds);
-  else attn_bwd_rows_body<NK, NV, ADD>(a, seqs, plan, item - plan.key_groups, reinterpret_cast<__bf16*>(a.dq), lds);
+  const int at = (int)blockIdx.x;
+  const bool rows = plan.rows_first ? at < plan.row_groups : at >= plan.key_groups;
+  const int item = rows == (plan.rows_first != 0) ? at : at - (rows ? plan.key_groups : plan.row_groups);
+  if (!rows) attn_bwd_keys_body<NK, NV, ADD>(a, seqs, plan, item, reinterpret_cast<__bf16*>(a.dk), reinterpret_cast<__bf16*>(a.dv), lds);
+  else attn_bwd_rows_body<NK, NV, ADD>(a, seqs, plan, item, reinterpret_cast<__bf16*>(a.dq), lds);
 }
 
 template <int NK, int NV, int ADD>

@@ -141,6 +141,7 @@ void count_tiles(Lists& keys, Lists& rows, int64_t qn, int64_t kn, int causal) {
 // How long lists are cut.
 struct Cuts {
   AttnBwdCut keys, rows;
+  int rows_first;
 };
 AttnBwdCut cut_lists(bool cut, int64_t longest, int64_t piece, int most) {
   if (!cut) return {1, 1 << 30, nullptr};
@@ -182,7 +183,10 @@ Cuts cut(const alto_mxfp4_attention_bwd_t& p) {
       best_rows = r;
     }
   }
-  return {cut_lists(best_keys, keys.longest * group, (int64_t)key_piece, 16), cut_lists(best_rows, rows.longest, (int64_t)row_piece, 32)};
+  // The kind with the longer lists starts first: dQ's at 3 x 8 heads, 480 rows, 1056 keys of 192 / 128 with a bias (83 us, 89 last) or 4 x 16 heads, 256
+  // rows, 4096 keys of 128 (161, 170); not where they are about as long (6 packed sequences of 16 / 4 heads of 64: 54, 50 last).
+  const bool rows_first = 0.62 * (best_rows ? row_piece : row_whole) > 1.25 * (best_keys ? key_piece : key_whole);
+  return {cut_lists(best_keys, keys.longest * group, (int64_t)key_piece, 16), cut_lists(best_rows, rows.longest, (int64_t)row_piece, 32), rows_first};
 }
 
 struct Workspace {
@@ -283,11 +287,11 @@ static int attention_bwd(const alto_mxfp4_attention_bwd_t& p, hipStream_t st) {
   a.bias = p.bias; a.bias_sb = p.bias_sb; a.bias_sh = p.bias_sh; a.bias_sm = p.bias_sm; a.distances = p.alibi_slopes != nullptr;
   const int row_block = BWD_BLOCK, key_block = row_block;
   auto go = [&](const AttnBwdSeqs& s, int q_blocks, int k_blocks) {
-    AttnBwdPlan plan{q_blocks, k_blocks, cuts.keys, cuts.rows, 0, 0, 0, 0};
+    AttnBwdPlan plan{q_blocks, k_blocks, cuts.keys, cuts.rows, 0, 0, cuts.rows_first, 0, 0};
     plan.keys.partial = (float*)(ws + w.key_sums);
     plan.rows.partial = (float*)(ws + w.row_sums);
     const int64_t key_blocks = p.dk ? p.B * p.Hk * k_blocks : 0, row_blocks = p.dq ? p.B * p.Hq * q_blocks : 0;
-    const int64_t key_groups = (key_blocks * cuts.keys.parts + 7) / 8 * 8, row_groups = row_blocks * cuts.rows.parts;
+    const int64_t key_groups = (key_blocks * cuts.keys.parts + 7) / 8 * 8, row_groups = (row_blocks * cuts.rows.parts + 7) / 8 * 8;
     const int64_t key_sums = cuts.keys.parts > 1 ? key_blocks : 0, row_sums = cuts.rows.parts > 1 ? row_blocks : 0;
     ALTO_REQUIRE(key_groups + row_groups < (1ll << 31) && (key_sums + row_sums) * 12 < (1ll << 31), "attention_bwd: too many workgroups");
     plan.key_groups = (int)key_groups;
