@@ -132,6 +132,15 @@ __device__ __forceinline__ void store_columns(__bf16* row, const v16f_t& acc, fl
   }
 }
 
+// All of these in accumulation registers at one time.  Where they do not fit the other half of the register file, the compiler has been seen to give
+// scores the place of sums and to move these out and back in every step, with half of the accumulation registers free.
+#define ALTO_A2(x, i) "+a"(x[i]), "+a"(x[i + 1])
+__device__ __forceinline__ void at_once(v16f_t& s, v16f_t (&v)[2], v16f_t (&k)[6]) { asm volatile("" : "+a"(s), ALTO_A2(v, 0), ALTO_A2(k, 0), ALTO_A2(k, 2), ALTO_A2(k, 4)); }
+__device__ __forceinline__ void at_once(v16f_t& s, v16f_t (&v)[4], v16f_t (&k)[6]) { asm volatile("" : "+a"(s), ALTO_A2(v, 0), ALTO_A2(v, 2), ALTO_A2(k, 0), ALTO_A2(k, 2), ALTO_A2(k, 4)); }
+__device__ __forceinline__ void at_once(v16f_t& s, v16f_t (&v)[2], v16f_t (&k)[8]) { asm volatile("" : "+a"(s), ALTO_A2(v, 0), ALTO_A2(k, 0), ALTO_A2(k, 2), ALTO_A2(k, 4), ALTO_A2(k, 6)); }
+__device__ __forceinline__ void at_once(v16f_t& s, v16f_t (&v)[4], v16f_t (&k)[8]) { asm volatile("" : "+a"(s), ALTO_A2(v, 0), ALTO_A2(v, 2), ALTO_A2(k, 0), ALTO_A2(k, 2), ALTO_A2(k, 4), ALTO_A2(k, 6)); }
+#undef ALTO_A2
+
 // A wave's 32 rows of W columns of transposed accumulators as bf16 to memory, by way of `lds` (64 W bytes of the wave's own, idle): written straight from
 // the registers they would be 16 bytes a row and store, and a store passes one line of the cache at a time.  The 16-byte pieces of a row change
 // places with the row, so that the writes of 32 rows meet all banks.
@@ -532,6 +541,10 @@ __device__ __forceinline__ void attn_bwd_keys_body(const AttnBwdArgs& a, const A
         if constexpr (ADD == ADD_BIAS && i == NS + NI + NF) wait_all_but<0>();   // the last step's loads, the bias of the next tile among them
         product(ic);
         if constexpr (i == NS - 1) {
+          if constexpr (NK > 2) {
+            at_once(S, dv, dk);
+            asm volatile("" : "+v"(S));
+          }
           if (a.causal && 32 * p0.tile + shift <= key0) {   // the diagonal's tile, or one before it, that another wave of the workgroup needs
             asm volatile("" ::: "memory");   // keep this a branch: most tiles skip it
             const int hidden = key0 + r - 32 * p0.tile - shift;
