@@ -135,10 +135,18 @@ __device__ __forceinline__ void store_columns(__bf16* row, const v16f_t& acc, fl
 // All of these in accumulation registers at one time.  Where they do not fit the other half of the register file, the compiler has been seen to give
 // scores the place of sums and to move these out and back in every step, with half of the accumulation registers free.
 #define ALTO_A2(x, i) "+a"(x[i]), "+a"(x[i + 1])
-__device__ __forceinline__ void at_once(v16f_t& s, v16f_t (&v)[2], v16f_t (&k)[6]) { asm volatile("" : "+a"(s), ALTO_A2(v, 0), ALTO_A2(k, 0), ALTO_A2(k, 2), ALTO_A2(k, 4)); }
-__device__ __forceinline__ void at_once(v16f_t& s, v16f_t (&v)[4], v16f_t (&k)[6]) { asm volatile("" : "+a"(s), ALTO_A2(v, 0), ALTO_A2(v, 2), ALTO_A2(k, 0), ALTO_A2(k, 2), ALTO_A2(k, 4)); }
-__device__ __forceinline__ void at_once(v16f_t& s, v16f_t (&v)[2], v16f_t (&k)[8]) { asm volatile("" : "+a"(s), ALTO_A2(v, 0), ALTO_A2(k, 0), ALTO_A2(k, 2), ALTO_A2(k, 4), ALTO_A2(k, 6)); }
-__device__ __forceinline__ void at_once(v16f_t& s, v16f_t (&v)[4], v16f_t (&k)[8]) { asm volatile("" : "+a"(s), ALTO_A2(v, 0), ALTO_A2(v, 2), ALTO_A2(k, 0), ALTO_A2(k, 2), ALTO_A2(k, 4), ALTO_A2(k, 6)); }
+template <int NK>
+__device__ __forceinline__ void at_once(v16f_t& s, v16f_t (&k)[NK]) {
+  if constexpr (NK == 6) asm volatile("" : "+a"(s), ALTO_A2(k, 0), ALTO_A2(k, 2), ALTO_A2(k, 4));
+  if constexpr (NK == 8) asm volatile("" : "+a"(s), ALTO_A2(k, 0), ALTO_A2(k, 2), ALTO_A2(k, 4), ALTO_A2(k, 6));
+}
+template <int NV, int NK>
+__device__ __forceinline__ void at_once(v16f_t& s, v16f_t (&v)[NV], v16f_t (&k)[NK]) {
+  if constexpr (NV == 2 && NK == 6) asm volatile("" : "+a"(s), ALTO_A2(v, 0), ALTO_A2(k, 0), ALTO_A2(k, 2), ALTO_A2(k, 4));
+  if constexpr (NV == 4 && NK == 6) asm volatile("" : "+a"(s), ALTO_A2(v, 0), ALTO_A2(v, 2), ALTO_A2(k, 0), ALTO_A2(k, 2), ALTO_A2(k, 4));
+  if constexpr (NV == 2 && NK == 8) asm volatile("" : "+a"(s), ALTO_A2(v, 0), ALTO_A2(k, 0), ALTO_A2(k, 2), ALTO_A2(k, 4), ALTO_A2(k, 6));
+  if constexpr (NV == 4 && NK == 8) asm volatile("" : "+a"(s), ALTO_A2(v, 0), ALTO_A2(v, 2), ALTO_A2(k, 0), ALTO_A2(k, 2), ALTO_A2(k, 4), ALTO_A2(k, 6));
+}
 #undef ALTO_A2
 
 // A wave's 32 rows of W columns of transposed accumulators as bf16 to memory, by way of `lds` (64 W bytes of the wave's own, idle): written straight from
@@ -826,6 +834,7 @@ __device__ __forceinline__ void attn_bwd_rows_body(const AttnBwdArgs& a, const A
       constexpr int i = decltype(ic)::value;
       read(std::integral_constant<int, i + AHEAD>{});
       product(ic);
+      if constexpr (NK > 2 && RUN && i == NS - 1) at_once(to.S, acc);
       if constexpr (RUN) {
         constexpr int u0 = HALVES * i / N, u1 = HALVES * (i + 1) / N;
         static_for<u1 - u0>([&](auto uc) { half(std::integral_constant<int, u0 + decltype(uc)::value>{}); });
