@@ -103,7 +103,7 @@ void mutate(alto_mxfp4_rotary_t& a) {
 struct Count {
   long calls = 0, ok = 0, launches = 0;
 };
-bool judge(Count& c, int64_t rc, const char* what) {
+bool looked_at(Count& c, int64_t rc, const char* what) {
   ++c.calls;
   if (rc >= 0) { ++c.ok; return true; }
   const char* msg = alto_mxfp4_last_error();
@@ -125,10 +125,10 @@ int main(int argc, char** argv) {
     const unsigned which = next_u64() % (2 * sizeof(g_bounds) / sizeof(g_bounds[0]));
     alto_mxfp4_attention_bwd_t a = attention(which < sizeof(g_bounds) / sizeof(g_bounds[0]) ? &g_bounds[which] : nullptr);
     for (int c = (int)(next_u64() % 4); c > 0; --c) mutate(a);
-    if (!judge(bwd, alto_mxfp4_attention_bwd(&a, nullptr), "attention_bwd") || !judge(size, alto_mxfp4_attention_bwd_workspace_bytes(&a), "attention_bwd_workspace_bytes")) return 2;
+    if (!looked_at(bwd, alto_mxfp4_attention_bwd(&a, nullptr), "attention_bwd") || !looked_at(size, alto_mxfp4_attention_bwd_workspace_bytes(&a), "attention_bwd_workspace_bytes")) return 2;
     alto_mxfp4_rotary_t r = rotary();
     for (int c = (int)(next_u64() % 4); c > 0; --c) mutate(r);
-    if (!judge(rot, alto_mxfp4_rotary(&r, nullptr), "rotary")) return 2;
+    if (!looked_at(rot, alto_mxfp4_rotary(&r, nullptr), "rotary")) return 2;
   }
   if (alto_mxfp4_attention_bwd(nullptr, nullptr) != -1 || alto_mxfp4_attention_bwd_workspace_bytes(nullptr) != -1 || alto_mxfp4_rotary(nullptr, nullptr) != -1) return 3;
   alto_mxfp4_attention_bwd_t a = attention(&g_bounds[0]);

@@ -92,3 +92,14 @@ def test_rotary_arguments(changes, text):
 def test_rotary_of_no_tokens():
     lib = _lib.load()
     assert lib.alto_mxfp4_rotary(ctypes.byref(rotary(S=0, q=None, q_out=None, k=None, k_out=None)), None) == 0
+
+
+def test_no_cpu_fallback():
+    import torch
+
+    import alto_amd.mxfp4 as mx
+    codes, scales, rows = torch.zeros(1, 1, 32, 32, dtype=torch.uint8), torch.zeros(1, 1, 1, 2, dtype=torch.uint8), torch.zeros(1, 1, 32, 64, dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError):
+        mx.attention_mxfp4_backward(rows, codes, codes, codes.reshape(1, 1, 64, 16), scales, scales, scales, rows, torch.zeros(1, 1, 32), 0.125, True)
+    with pytest.raises(RuntimeError):
+        mx.apply_rotary(rows, rows, mx.rotary_frequencies(64)[0])
