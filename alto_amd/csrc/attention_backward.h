@@ -272,21 +272,24 @@ struct BwdSmall {
   const uint8_t *codes, *records, *from;
   int bytes, offset;      // of what this wave loads first: a tile's, and this lane's in it
   bool takes_codes;
-  int at;
-  __device__ __forceinline__ BwdSmall(const uint8_t* codes, const void* all_records, int wave, int lane) : codes(codes), records(reinterpret_cast<const uint8_t*>(all_records)) {
+  int to, slot_bytes, second_to;   // slots of this wave's in the LDS
+  __device__ __forceinline__ BwdSmall(const uint8_t* codes, const void* all_records, int wave, int lane, int lds_codes, int lds_records)
+      : codes(codes), records(reinterpret_cast<const uint8_t*>(all_records)) {
     takes_codes = wave < NK;
     from = takes_codes ? codes : records;
     bytes = takes_codes ? CODES : RECORD;
     offset = takes_codes ? CodeTile<NK>::source(64 * wave + lane) : 16 * lane;
-    at = takes_codes ? 1024 * wave : 0;
+    to = takes_codes ? lds_codes + 1024 * wave : lds_records;
+    slot_bytes = takes_codes ? CODES : 1024;
+    second_to = lds_records;
   }
   // of `n` tiles from `first` on
   __device__ __forceinline__ __amdgpu_buffer_rsrc_t source(int64_t first, int n) const { return buffer(from + first * bytes, (int64_t)n * bytes); }
   __device__ __forceinline__ __amdgpu_buffer_rsrc_t second(int64_t first, int n) const { return buffer(records + first * RECORD, (int64_t)n * RECORD); }
-  // tile `t` of these
-  __device__ __forceinline__ void operator()(__amdgpu_buffer_rsrc_t source, __amdgpu_buffer_rsrc_t second, int t, const uint8_t* to_codes, const uint8_t* to_record, int lane) const {
-    load_piece(source, (takes_codes ? to_codes : to_record) + at, offset, (int)((uint32_t)t * bytes));
-    if constexpr (LOADS == 2) load_piece(second, to_record, 16 * lane, (int)((uint32_t)t * RECORD));
+  // tile `t` of these, to these slots
+  __device__ __forceinline__ void operator()(__amdgpu_buffer_rsrc_t source, __amdgpu_buffer_rsrc_t second, int t, const uint8_t* lds, int code_slot, int record_slot, int lane) const {
+    load_piece(source, lds + to + (takes_codes ? code_slot : record_slot) * slot_bytes, offset, (int)((uint32_t)t * bytes));
+    if constexpr (LOADS == 2) load_piece(second, lds + second_to + record_slot * 1024, 16 * lane, (int)((uint32_t)t * RECORD));
   }
 };
 // Load `l` of tile `t` of bf16 rows (as many of each wave as it is wide / 64)
@@ -403,7 +406,7 @@ __device__ __forceinline__ void attn_bwd_keys_body(const AttnBwdArgs& a, const A
     }
     auto next = [&]() {   // (past the end: the last tile again)
       const BwdPlace p{next_tile, next_base + next_tile};
-      const int more = left > 1 ? 1 : 0;
+      const int more = left - 1 < 1 ? left - 1 : 1;
       left -= more;
       next_tile += more;
       const int wrap = next_tile == last ? -1 : 0;
@@ -411,7 +414,7 @@ __device__ __forceinline__ void attn_bwd_keys_body(const AttnBwdArgs& a, const A
       next_base += wrap & tiles;
       return p;
     };
-    const Small small(a.q, a.q_records, wave, lane);
+    const Small small(a.q, a.q_records, wave, lane, 0, L::O_RECORD);
     auto record = [&](int i) { return reinterpret_cast<const QRecord*>(lds + L::O_RECORD + (i & 3) * 1024); };
     const int code_base = lane * 16, row_base[2] = {VT::row_base(lane, 0), VT::row_base(lane, 1)}, column_base[2] = {VT::column_base(lane, 0), VT::column_base(lane, 1)};
     const float c2 = a.sm_scale * ATTN_RCP_LN2, inverse_scale = 1.0f / a.sm_scale;
@@ -445,7 +448,7 @@ __device__ __forceinline__ void attn_bwd_keys_body(const AttnBwdArgs& a, const A
     auto write_values = [&](int i, int u) {
       *reinterpret_cast<v4i_t*>(lds + L::O_D + (i & 1) * T::ROWS_D + 4096 * u + eight_to) = decode8(eight, e8m0_value((eight_scales >> (8 * u)) & 0xFFu));
     };
-    auto load_small = [&](const BwdPlace& p, int i) { small(small.source(p.at, 1), small.second(p.at, 1), 0, lds + (i & 3) * T::CODES, lds + L::O_RECORD + (i & 3) * 1024, lane); };
+    auto load_small = [&](const BwdPlace& p, int i) { small(small.source(p.at, 1), small.second(p.at, 1), 0, lds, i & 3, i & 3, lane); };
     auto load_grads = [&](const BwdPlace& p, int l, int slot) { load_rows<64 * NV>(rows_source<64 * NV>(a.g_tiles, p.at, 1), lds + L::O_V + slot * T::ROWS_V, 0, l, wave, lane); };
 
     BwdPlace p0 = next(), p1 = next(), p2 = next();
@@ -712,7 +715,7 @@ __device__ __forceinline__ void attn_bwd_rows_body(const AttnBwdArgs& a, const A
   const float c2 = a.sm_scale * ATTN_RCP_LN2, inverse_scale = 1.0f / a.sm_scale;
   const float slope = ADD == ADD_NOTHING ? 0.0f : own_record->slope;
 
-  const Small small(a.k, a.k_records, wave, lane);
+  const Small small(a.k, a.k_records, wave, lane, 0, L::O_RECORD);
   const int code_base = lane * 16, row_base[2] = {VT::row_base(lane, 0), VT::row_base(lane, 1)}, column_base[2] = {DT::column_base(lane, 0), DT::column_base(lane, 1)};
   auto tile = [&](int t) { return t < total ? t : total - 1; };   // (past the end: the last tile again)
   // (a head's rows take less than 4 GB)
@@ -852,7 +855,7 @@ __device__ __forceinline__ void attn_bwd_rows_body(const AttnBwdArgs& a, const A
   // everything that earlier steps started.
   auto load_scores = [&](int i, int slot) {
     const int t = tile(i);
-    small(small_source, second_source, t, lds + slot * T::CODES, lds + L::O_RECORD + (i & 3) * 1024, lane);
+    small(small_source, second_source, t, lds, slot, i & 3, lane);
 #pragma unroll
     for (int l = 0; l < NV; ++l) load_rows<64 * NV>(v_source, lds + L::O_V + slot * T::ROWS_V, t, l, wave, lane);
   };
