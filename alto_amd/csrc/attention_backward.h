@@ -604,7 +604,7 @@ __device__ __forceinline__ void attn_bwd_keys_body(const AttnBwdArgs& a, const A
       wait_lds_and_all_but<Small::LOADS + NV + (ADD == ADD_BIAS ? Bias::LOADS : 0)>();   // all but this step's loads; the values are written
       asm volatile("s_barrier" ::: "memory");
     }
-    wait_all_but<0>();   // (the last loads into the LDS, which nobody reads, before it is given back)
+    wait_lds_and_all_but<0>();   // (the last loads into the LDS, which nobody reads, before it is used otherwise)
   }
 
   if (mine.parts > 1) {
@@ -928,7 +928,7 @@ __device__ __forceinline__ void attn_bwd_rows_body(const AttnBwdArgs& a, const A
 #pragma unroll
       for (int n = 0; n < 2 * NK; ++n) acc[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(DT::column_frag(at + column_base[0], at + column_base[1], n, c), f[c], acc[n], 0, 0, 0);
   }
-  wait_all_but<0>();   // (the last loads into the LDS, which nobody reads, before it is given back)
+  wait_lds_and_all_but<0>();   // (this wave's reads; the last loads into the LDS, which nobody reads, before it is used otherwise)
   if (mine.parts > 1) {
     if (!live) return;
     v4f_t* to = T::template sums<2 * NK>(plan.rows, z, part, heads, bh, wave, lane);
