@@ -896,6 +896,7 @@ __device__ __forceinline__ void attn_bwd_rows_body(const AttnBwdArgs& a, const A
   bf16x8_t f[2], g[2];
   f[0] = f[1] = __builtin_bit_cast(bf16x8_t, v4i_t{0, 0, 0, 0});
   step(std::false_type{}, -1, 2, x, f, x, f);
+  asm volatile("s_barrier" ::: "memory");   // (every wave has read tile 0, whose slot the next step's loads go to)
   int slot = 0;   // of tile t
   auto whole_step = [&](int t, Scores& from, const bf16x8_t (&f_now)[2], Scores& to, bf16x8_t (&f_next)[2]) {
     const int after = slot == 2 ? 0 : slot + 1;

@@ -120,6 +120,16 @@ def test_a_bias_of_any_layout(m, case):
         check(got, x.expected())
 
 
+@pytest.mark.parametrize("Sk,biased", [(64, True), (64, False), (96, True), (32, False)])
+def test_many_workgroups_of_short_lists(m, Sk, biased):
+    """Several workgroups after one another on every unit, whose waves drift apart from the first tile on."""
+    g = torch.Generator().manual_seed(15)
+    x = Operands(2, 16, 4, 1024, Sk, 128, 128, False, seed=14, bias=torch.randn(2, 1, 1024, Sk, generator=g) if biased else None)
+    ref = x.expected()
+    for _ in range(4):
+        check(x.call(m), ref)
+
+
 @pytest.mark.parametrize("D", [64, 128, 256])
 def test_a_bias_of_extreme_values(m, D):
     """Where the mask hides a key the bias may hold anything; the type's lowest value hides like -inf, in rows that see nothing too; a row that sees
