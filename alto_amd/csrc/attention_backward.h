@@ -344,9 +344,10 @@ __device__ __forceinline__ float probability_of(float x, std::integral_constant<
   return ADD == ADD_BIAS ? __builtin_amdgcn_fmed3f(p, 0.0f, 1.0f) : p;
 }
 
-// The products of a step are issued in a fixed order (sched_barrier): the read of an operand runs BWD_AHEAD products before its use, vector work lies
-// behind each product.  Left to itself the compiler puts every read right in front of its product and waits there.
-constexpr int BWD_AHEAD = 2;
+// The products of a step are issued in a fixed order (sched_barrier): the read of an operand runs AHEAD products before its use, vector work lies
+// behind each product.  Left to itself the compiler puts every read right in front of its product and waits there.  Four products where the registers
+// allow it (2 x 1024 tokens, 16 heads of 64 with slopes 41.1 us, two 42.4; 8192 tokens, 16 / 2 heads of 256 / 128 1246, 1261), two with D = 128.
+constexpr int bwd_ahead(int nk) { return nk == 2 ? 2 : 4; }
 
 // ---------------------------------------------------------------------------------------------------------------- dK and dV
 // Four slots of codes, statistics and scales, three of dO, two of Q's values, which the workgroup makes from the codes one step ahead (a quarter of the
@@ -478,7 +479,7 @@ __device__ __forceinline__ void attn_bwd_keys_body(const AttnBwdArgs& a, const A
     asm volatile("s_barrier" ::: "memory");
     if constexpr (ADD == ADD_BIAS) load_bias(p1);
 
-    constexpr int NS = NK, NI = 4 * NV, NF = 4 * NV, NG = 4 * NK, N = NS + NI + NF + NG, AHEAD = BWD_AHEAD;
+    constexpr int NS = NK, NI = 4 * NV, NF = 4 * NV, NG = 4 * NK, N = NS + NI + NF + NG, AHEAD = bwd_ahead(NK);
     int slot = 0;
     for (int t = 0; t < total; ++t) {
       const int two_on = slot == 0 ? 2 : slot - 1;
@@ -742,7 +743,7 @@ __device__ __forceinline__ void attn_bwd_rows_body(const AttnBwdArgs& a, const A
   };
 
   // The products in order: those of the scores, then by turns one of dP and one of the sums.
-  constexpr int NS = NK, NI = 4 * NV, NF = 4 * NK, AHEAD = BWD_AHEAD, HALVES = 16, STEP_LOADS = Small::LOADS + NV + NK;
+  constexpr int NS = NK, NI = 4 * NV, NF = 4 * NK, AHEAD = bwd_ahead(NK), HALVES = 16, STEP_LOADS = Small::LOADS + NV + NK;
   struct Op {
     int kind, j;   // 0: S, 1: dP, 2: sums
   };
