@@ -234,7 +234,6 @@ def _attend_quantized(operands, sm_scale: float, causal: bool, out: torch.Tensor
         "alto_mxfp4_attention_fwd_strided")
 
 
-@torch.compiler.allow_in_graph
 class MXFP4AttentionFunction(torch.autograd.Function):
     """The attention of :func:`_attend` (or with a ``bias``, of :func:`attention_mxfp4_forward`) on [B, H, S, D] views, with its backward.  Kept from
     one to the other: Q, K and V as codes and scales, the output and the log-sum-exp.  What only the backward refuses (a scale that is not positive, the
@@ -298,6 +297,11 @@ def triton_attention_mxfp4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, al
 
     ``use_exp2`` is accepted either way: both settings evaluate exp(x) as exp2(x * log2 e) on the GPU's exp unit.
     """
+    return (_attention_between_graphs if torch.compiler.is_compiling() else _attention)(
+        q, k, v, alibi_slopes, bias, sm_scale, dropout_p, cu_seqlens_q, cu_seqlens_k, max_seqlens_q, max_seqlens_k, causal, return_scores, layout)
+
+
+def _attention(q, k, v, alibi_slopes, bias, sm_scale, dropout_p, cu_seqlens_q, cu_seqlens_k, max_seqlens_q, max_seqlens_k, causal, return_scores, layout):
     if layout == "bshd":
         # [B, S, H, D] tensors: the same attention on the permuted views, result back in [B, S, H, D].  (The reference's
         # wrapper has no consistent behaviour to reproduce here: it takes 2D blocks over (heads, head dim) of the tensor as
@@ -338,6 +342,9 @@ def triton_attention_mxfp4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, al
     if layout != "bhsd":
         raise NotImplementedError(f"layout {layout!r}: 'bhsd', 'bshd' and 'thd' are implemented")
     return _fixed_length(q, k, v, alibi_slopes, bias, sm_scale, dropout_p, max_seqlens_q, max_seqlens_k, causal, return_scores, rows_outer=False)
+
+
+_attention_between_graphs = torch.compiler.disable(_attention)   # (nothing of it can be traced: a compiled caller breaks its graph here and runs the same call)
 
 
 def _fixed_length(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, alibi_slopes, bias, sm_scale, dropout_p, max_seqlens_q, max_seqlens_k, causal,

@@ -109,7 +109,6 @@ def _rotate(q: torch.Tensor, k: Optional[torch.Tensor], inv_freq: torch.Tensor, 
     return out
 
 
-@torch.compiler.allow_in_graph
 class RotaryFunction(torch.autograd.Function):
     """(q, k) rotated; the backward rotates their gradients back with the same kernel and keeps neither Q nor K."""
 
@@ -137,9 +136,13 @@ def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], inv_freq: torch.Ten
     (i, i + R/2), or (2i, 2i + 1) with ``interleaved``, the others pass.  ``positions``: int32 or int64 [S] or [B, S] ([T] with ``"thd"``) of any
     sign, None for 0, 1, ...  ``factor`` multiplies cosines and sines.  Angles, cosines and sines are taken in 64 bits.
     """
+    return (_apply_between_graphs if torch.compiler.is_compiling() else _apply)(q, k, inv_freq, positions, interleaved, factor, layout)
+
+
+def _apply(q, k, inv_freq, positions, interleaved, factor, layout):
     if layout not in _DIMS:
         raise NotImplementedError(f"layout {layout!r}: 'bhsd', 'bshd' and 'thd' are implemented")
-    if k is not None and q.is_cuda and not torch.compiler.is_compiling():   # one native call; what it declines goes on here
+    if k is not None and q.is_cuda:   # one native call; what it declines goes on here
         out = rt.host().rotary(q, k, inv_freq, positions, bool(interleaved), float(factor), _NATIVE[layout])
         if out is not None:
             return out
@@ -164,3 +167,6 @@ def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], inv_freq: torch.Ten
         return RotaryFunction.apply(q, k, inv_freq, positions, bool(interleaved), float(factor), layout, False)
     out = _rotate(q, k, inv_freq, positions, bool(interleaved), float(factor), layout, False)
     return tuple(out) if k is not None else out[0]
+
+
+_apply_between_graphs = torch.compiler.disable(_apply)   # (nothing of it can be traced: a compiled caller breaks its graph here and runs the same call)

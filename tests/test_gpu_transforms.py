@@ -1,0 +1,44 @@
+"""Attention and rotary positions under torch's transforms: what they serve gives the bits of an eager call, what they do not they refuse."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+@pytest.fixture(scope="module")
+def m():
+    import alto_amd.mxfp4 as mod
+    return mod
+
+
+def leaves(B, S, Hq, Hk, D, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    return [torch.randn(B, S, h, D, generator=g).bfloat16().to(DEV) for h in (Hq, Hk, Hk, Hq)]
+
+
+def test_a_compiled_step_has_the_bits_of_an_eager_one(m):
+    """Rotation and attention of a compiled block (the graphs around them without a code generator), forward and backward, twice."""
+    q, k, v, go = leaves(2, 96, 4, 2, 64)
+    freq = m.rotary_frequencies(64)[0].to(DEV)
+    attention = m.LPScaledDotProductAttention(m.TrainingOpConfig())
+
+    def block(q, k, v):
+        a, b = m.apply_rotary(q * 2, k, freq, layout="bshd")
+        a = m.apply_rotary(a, None, freq, layout="bshd")
+        return attention(a, b, v, is_causal=True, rotary=m.Rotary(freq)) + q
+
+    def step(fn):
+        x = [t.clone().requires_grad_(True) for t in (q, k, v)]
+        y = fn(*x)
+        return y.detach(), *torch.autograd.grad(y, x, go)
+
+    want = step(block)
+    torch._dynamo.reset()
+    compiled = torch.compile(block, backend="aot_eager")
+    for _ in range(2):
+        for a, b in zip(step(compiled), want):
+            assert torch.equal(a, b)
+    with torch.no_grad():
+        assert torch.equal(compiled(q, k, v), want[0])
+    torch._dynamo.reset()

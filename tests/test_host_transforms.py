@@ -1,0 +1,101 @@
+"""Attention and rotary positions under torch's transforms, without a GPU: the native calls are stood in for by plain ones."""
+import pytest
+import torch
+
+import alto_amd.mxfp4 as mx
+from alto_amd.mxfp4 import _runtime as rt
+from alto_amd.mxfp4 import rotary as R
+
+FREQ = torch.ones(16, dtype=torch.float64)
+
+
+class Host:
+    """Native calls that leave a trace of their operands: the attention's output is Q's first rows, its gradients are 2, 3 and 4."""
+
+    def attend(self, q, k, v, sm_scale, causal, out, lse, *more):
+        out.copy_(q[..., :out.shape[-1]])
+        lse.zero_()
+        return True
+
+    def attention_gradients(self, go, q, qs, k, ks, v, vs, out, lse, sm_scale, causal, keys, bias, slopes, cu_q, cu_k, rows_outer, want_q, want_kv):
+        def full(value, heads, rows, columns):
+            return torch.full((q.shape[0], rows, heads, columns), value, dtype=torch.bfloat16).transpose(1, 2)
+
+        return full(2.0, q.shape[1], q.shape[2], 2 * q.shape[3]), full(3.0, k.shape[1], k.shape[2], 2 * q.shape[3]), full(4.0, k.shape[1], k.shape[2], v.shape[2])
+
+    def rotary(self, *args):
+        return None
+
+
+class Lib:
+    def __getattr__(self, name):
+        return lambda *args: 0
+
+
+@pytest.fixture
+def stand_in(monkeypatch):
+    monkeypatch.setattr(rt, "require_gpu", lambda *tensors: None)
+    monkeypatch.setattr(rt, "host", Host)
+    monkeypatch.setattr(rt, "lib", Lib)
+    monkeypatch.setattr(rt, "stream_ptr", lambda device: 0)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: None)
+    torch._dynamo.reset()
+    yield
+    torch._dynamo.reset()
+
+
+@pytest.fixture
+def plain_rotation(monkeypatch):
+    """Twice x, or half of it back: a rotation as far as its callers can tell (a launch takes addresses, which only tensors of real memory have)."""
+
+    def rotate(q, k, freq, positions, interleaved, factor, layout, inverse):
+        return [None if t is None or t.data_ptr() == 0 else t * (0.5 if inverse else 2) for t in (q, k)]
+
+    monkeypatch.setattr(R, "_rotate", rotate)
+
+
+def tensors(requires_grad):
+    g = torch.Generator().manual_seed(0)
+    return [torch.randn(1, 2, 64, 64, generator=g).bfloat16().requires_grad_(requires_grad) for _ in range(3)]
+
+
+def compiled(fn):
+    return torch.compile(fn, backend="aot_eager")
+
+
+@pytest.mark.parametrize("layout", ["bhsd", "bshd", "thd"])
+def test_a_compiled_training_step_of_the_attention(stand_in, layout):
+    """The caller's graph breaks at the attention, which runs as in an eager step, its gradients too."""
+    x = tensors(True)
+    if layout == "thd":
+        x = [t.detach()[0].transpose(0, 1).contiguous().requires_grad_(True) for t in x]
+    more = dict(cu_seqlens_q=[0, 64], cu_seqlens_k=[0, 64]) if layout == "thd" else {}
+    fn = compiled(lambda q, k, v: mx.triton_attention_mxfp4(q * 2, k, v, causal=True, layout=layout, **more)[0] * 3)
+    for _ in range(2):
+        y = fn(*x)
+        grads = torch.autograd.grad(y.sum(), x)
+        assert [float(t.float().amin()) for t in grads] == [4.0, 3.0, 4.0] == [float(t.float().amax()) for t in grads]
+    with torch.no_grad():
+        assert fn(*x).shape == y.shape
+
+
+def test_a_compiled_training_step_of_the_rotation(stand_in, plain_rotation):
+    q, k, _ = tensors(True)
+    fn = compiled(lambda q, k: [t + 1 for t in mx.apply_rotary(q, k, FREQ)])
+    for _ in range(2):
+        a, b = fn(q, k)
+        assert torch.equal(a, 2 * q + 1) and torch.equal(b, 2 * k + 1)
+        assert all(bool((t == 0.5).all()) for t in torch.autograd.grad(a.sum() + b.sum(), (q, k)))
+    alone = compiled(lambda q: mx.apply_rotary(q, None, FREQ) + 1)
+    assert all(bool((t == 0.5).all()) for t in torch.autograd.grad(alone(q).sum(), (q,)))
+    with torch.no_grad():
+        assert torch.equal(fn(q, k)[0], 2 * q + 1)
+
+
+def test_a_compiled_module_with_rotated_positions(stand_in, plain_rotation):
+    x = [t.detach().transpose(1, 2).contiguous().requires_grad_(True) for t in tensors(True)]
+    attention = mx.LPScaledDotProductAttention(mx.TrainingOpConfig())
+    fn = compiled(lambda q, k, v: attention(q, k, v, rotary=mx.Rotary(FREQ)).float().square())
+    y = fn(*x)
+    grads = torch.autograd.grad(y.sum(), x)
+    assert [float(t.float().amax()) for t in grads] == [1.0, 1.5, 4.0]
