@@ -30,6 +30,15 @@ def require_gpu(*tensors: torch.Tensor) -> None:
                 f"'{t.device}'. There is no CPU fallback for the HIP kernels.")
 
 
+def refuse_transforms(what: str) -> None:
+    """Ends a call whose launches torch would not see: ``torch.jit.trace`` would record the allocation of its outputs and nothing that fills them,
+    and a functorch transform hands in tensors without memory."""
+    if torch.jit.is_tracing():
+        raise NotImplementedError(f"{what} under torch.jit.trace: none of its launches would be recorded")
+    if torch._C._are_functorch_transforms_active():
+        raise NotImplementedError(f"{what} under a functorch transform is not implemented")
+
+
 def ptr(t: Optional[torch.Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 

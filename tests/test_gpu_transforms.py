@@ -42,3 +42,18 @@ def test_a_compiled_step_has_the_bits_of_an_eager_one(m):
     with torch.no_grad():
         assert torch.equal(compiled(q, k, v), want[0])
     torch._dynamo.reset()
+
+
+@pytest.mark.filterwarnings("ignore:`torch.jit")
+@pytest.mark.filterwarnings("ignore::torch.jit.TracerWarning")
+def test_a_traced_rotation_is_refused(m):
+    q, k, _, _ = leaves(1, 32, 2, 2, 64)
+    freq = m.rotary_frequencies(64)[0].to(DEV)
+    for grad in (False, True):
+        q.requires_grad_(grad)
+        for fn, x in ((lambda q, k: m.apply_rotary(q, k, freq, layout="bshd"), (q, k)), (lambda q: m.apply_rotary(q, None, freq, layout="bshd"), (q,))):
+            with pytest.raises(NotImplementedError, match="torch.jit.trace"):
+                torch.jit.trace(fn, x, check_trace=False)
+            fn(*x)
+            with pytest.raises(NotImplementedError, match="functorch"):
+                torch.func.jvp(lambda q: fn(q, *x[1:]), (q.detach(),), (q.detach(),))

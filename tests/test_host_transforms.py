@@ -99,3 +99,25 @@ def test_a_compiled_module_with_rotated_positions(stand_in, plain_rotation):
     y = fn(*x)
     grads = torch.autograd.grad(y.sum(), x)
     assert [float(t.float().amax()) for t in grads] == [1.0, 1.5, 4.0]
+
+
+@pytest.mark.parametrize("requires_grad", [False, True])
+@pytest.mark.filterwarnings("ignore:`torch.jit")
+@pytest.mark.filterwarnings("ignore::torch.jit.TracerWarning")
+def test_a_traced_rotation_is_refused(stand_in, requires_grad):
+    """(its trace would hold the outputs' allocation alone)"""
+    q, k, _ = tensors(requires_grad)
+    for fn, x in ((lambda q, k: mx.apply_rotary(q, k, FREQ), (q, k)), (lambda q: mx.apply_rotary(q, None, FREQ), (q,))):
+        with pytest.raises(NotImplementedError, match="torch.jit.trace"):
+            torch.jit.trace(fn, x, check_trace=False)
+
+
+def test_a_rotation_under_functorch_is_refused(stand_in):
+    q, k, _ = tensors(False)
+    for fn in (lambda q: mx.apply_rotary(q, None, FREQ), lambda q: mx.apply_rotary(q, k, FREQ)[0]):
+        with pytest.raises(NotImplementedError, match="functorch"):
+            torch.func.jvp(fn, (q,), (q,))
+        with pytest.raises(NotImplementedError, match="functorch"):
+            torch.func.grad(lambda q: fn(q).float().sum())(q)
+    with pytest.raises(NotImplementedError, match="functorch"):
+        torch.func.vmap(lambda q: mx.apply_rotary(q, None, FREQ, layout="thd"))(q)
