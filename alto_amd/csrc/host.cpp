@@ -526,6 +526,11 @@ void raise_in_engine(const Failure& f) {
 }
 // (a module that is loaded: a lookup)
 py::object python_function(const char* module, const char* name) { return py::module_::import(module).attr(name); }
+// Forward-mode tangents of what comes into a node's backward would be lost there
+void refuse_tangents(const char* what, const std::vector<Tensor>& grads) {
+  for (const Tensor& g : grads)
+    if (g.defined() && g._fw_grad(0).defined()) with_interpreter([&] { python_function("alto_amd.mxfp4._runtime", "refuse_transforms")(what, g); });
+}
 bool host_keyed_hardware_rounding() {
   return with_interpreter([] { return python_function("alto_amd.mxfp4._runtime", "host_keyed_hardware_rounding")().cast<bool>(); });
 }
@@ -879,6 +884,7 @@ struct RotaryNode : torch::autograd::Function<RotaryNode> {
     return out;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    refuse_tangents("apply_rotary", grads);
     const variable_list saved = ctx->get_saved_variables();
     RotaryOperands op;
     op.inv_freq = saved[0];
@@ -916,7 +922,7 @@ py::object rotary(const Tensor& q, const Tensor& k, const Tensor& inv_freq, cons
   if (q.scalar_type() != k.scalar_type() || q.numel() == 0 || k.numel() == 0) return py::none();
   for (int64_t d = 0; d < dims; ++d)
     if (d != op.head() && q.size(d) != k.size(d)) return py::none();
-  if (!on_current_device(inv_freq) || inv_freq.scalar_type() != at::kDouble || inv_freq.dim() != 1 || !inv_freq.is_contiguous() || inv_freq.requires_grad()) return py::none();
+  if (!on_current_device(inv_freq) || inv_freq.scalar_type() != at::kDouble || inv_freq.dim() != 1 || !inv_freq.is_contiguous() || inv_freq.requires_grad() || inv_freq._fw_grad(0).defined()) return py::none();
   if (inv_freq.size(0) < 1 || inv_freq.size(0) > 1024 || 2 * inv_freq.size(0) > q.size(-1)) return py::none();
   if (positions.has_value()) {
     const Tensor& p = *positions;

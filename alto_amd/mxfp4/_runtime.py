@@ -5,6 +5,7 @@ import os
 from typing import Callable, Optional
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 
 from .. import _lib
 
@@ -30,13 +31,15 @@ def require_gpu(*tensors: torch.Tensor) -> None:
                 f"'{t.device}'. There is no CPU fallback for the HIP kernels.")
 
 
-def refuse_transforms(what: str) -> None:
+def refuse_transforms(what: str, *tensors: Optional[torch.Tensor]) -> None:
     """Ends a call whose launches torch would not see: ``torch.jit.trace`` would record the allocation of its outputs and nothing that fills them,
-    and a functorch transform hands in tensors without memory."""
+    a functorch transform hands in tensors without memory, and the forward-mode tangents of ``tensors`` would be lost."""
     if torch.jit.is_tracing():
         raise NotImplementedError(f"{what} under torch.jit.trace: none of its launches would be recorded")
     if torch._C._are_functorch_transforms_active():
         raise NotImplementedError(f"{what} under a functorch transform is not implemented")
+    if any(t is not None and unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{what}: forward-mode derivatives are not implemented")
 
 
 def ptr(t: Optional[torch.Tensor]) -> Optional[int]:

@@ -146,7 +146,7 @@ def _apply(q, k, inv_freq, positions, interleaved, factor, layout):
         out = rt.host().rotary(q, k, inv_freq, positions, bool(interleaved), float(factor), _NATIVE[layout])
         if out is not None:
             return out
-    rt.refuse_transforms("apply_rotary")
+    rt.refuse_transforms("apply_rotary", q, k, inv_freq)
     rt.require_gpu(q, k, inv_freq, positions)
     dims = 3 if layout == "thd" else 4
     batch, head, row = _DIMS[layout]

@@ -1,6 +1,7 @@
 """Attention and rotary positions under torch's transforms: what they serve gives the bits of an eager call, what they do not they refuse."""
 import pytest
 import torch
+from torch.autograd.forward_ad import dual_level, make_dual
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -57,3 +58,21 @@ def test_a_traced_rotation_is_refused(m):
             fn(*x)
             with pytest.raises(NotImplementedError, match="functorch"):
                 torch.func.jvp(lambda q: fn(q, *x[1:]), (q.detach(),), (q.detach(),))
+
+def test_a_rotation_with_forward_mode_tangents_is_refused(m):
+    q, k, _, _ = leaves(1, 32, 2, 2, 64)
+    freq = m.rotary_frequencies(64)[0].to(DEV)
+    want = m.apply_rotary(q, k, freq, layout="bshd")
+    with dual_level():
+        dual = make_dual(q, torch.ones_like(q))
+        for call in (lambda: m.apply_rotary(dual, None, freq, layout="bshd"), lambda: m.apply_rotary(dual, k, freq, layout="bshd"),
+                     lambda: m.apply_rotary(k, dual, freq, layout="bshd"), lambda: m.apply_rotary(q, k, make_dual(freq, torch.ones_like(freq)), layout="bshd")):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+        for a, b in zip(m.apply_rotary(q, k, freq, layout="bshd"), want):
+            assert torch.equal(a, b)
+        for x in ((q.clone().requires_grad_(True), k), (q.clone().requires_grad_(True), None)):
+            y = m.apply_rotary(*x, freq, layout="bshd")
+            y = y if x[1] is None else y[0]
+            with pytest.raises(NotImplementedError):
+                y.backward(make_dual(torch.ones_like(y), torch.ones_like(y)))   # (nor of a gradient)

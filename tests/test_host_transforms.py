@@ -1,6 +1,7 @@
 """Attention and rotary positions under torch's transforms, without a GPU: the native calls are stood in for by plain ones."""
 import pytest
 import torch
+from torch.autograd.forward_ad import dual_level, make_dual
 
 import alto_amd.mxfp4 as mx
 from alto_amd.mxfp4 import _runtime as rt
@@ -121,3 +122,18 @@ def test_a_rotation_under_functorch_is_refused(stand_in):
             torch.func.grad(lambda q: fn(q).float().sum())(q)
     with pytest.raises(NotImplementedError, match="functorch"):
         torch.func.vmap(lambda q: mx.apply_rotary(q, None, FREQ, layout="thd"))(q)
+
+@pytest.mark.parametrize("requires_grad", [False, True])
+def test_a_rotation_with_forward_mode_tangents_is_refused(stand_in, plain_rotation, requires_grad):
+    """(they would be lost: the launches see no tangent)"""
+    q, k, _ = tensors(requires_grad)
+    with dual_level():
+        dual = make_dual(q, torch.ones_like(q))
+        for call in (lambda: mx.apply_rotary(dual, None, FREQ), lambda: mx.apply_rotary(dual, k, FREQ), lambda: mx.apply_rotary(k, dual, FREQ),
+                     lambda: mx.apply_rotary(q, None, make_dual(FREQ, torch.ones_like(FREQ)))):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+        assert mx.apply_rotary(q, None, FREQ).shape == q.shape   # (no tangent: nothing to lose)
+        y = mx.apply_rotary(q.detach().requires_grad_(True), None, FREQ)
+        with pytest.raises(NotImplementedError):
+            y.backward(make_dual(torch.ones_like(y), torch.ones_like(y)))   # (nor of a gradient)
