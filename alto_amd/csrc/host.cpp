@@ -108,6 +108,15 @@ bool aligned16(const Tensor& t) { return (reinterpret_cast<uintptr_t>(t.data_ptr
 int64_t stride_of(const Tensor& t, int64_t d) { return t.size(d) == 1 ? 0 : t.stride(d); }   // a dim of one is never stepped over: its stride may be anything
 int64_t div_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+// (torch.jit.trace would record the outputs' allocation and none of the launches: the general functions end in an error there)
+bool being_traced() { return c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::Tracer); }
+// A call that a node may serve: not under torch.jit.trace, a functorch transform or forward-mode differentiation, which the general
+// functions refuse
+bool node_serves(const Tensor& x, const Tensor& weight) {
+  return !being_traced() && !c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::FuncTorchDynamicLayerFrontMode) && !x._fw_grad(0).defined() &&
+         !weight._fw_grad(0).defined();
+}
+
 struct Alloc {
   at::TensorOptions u8;
   explicit Alloc(const Tensor& like) : u8(at::TensorOptions().dtype(at::kByte).device(like.device())) {}
@@ -261,6 +270,7 @@ py::object grouped_dw_packed(const Tensor& go, const Tensor& go_ps, const Tensor
 // kernel quantizes Q itself)
 bool attend(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in, double sm_scale, bool causal, const Tensor& out, const Tensor& lse,
             const std::vector<int32_t>& cu_q, const std::vector<int32_t>& cu_k, uintptr_t stream) {
+  if (!node_serves(q_in, k_in) || v_in._fw_grad(0).defined()) return false;
   Tensor q = q_in, k = k_in, v = v_in;
   for (Tensor* t : {&q, &k, &v}) {
     if (!on_gpu(*t) || !is_float(*t) || t->dim() != 4 || t->scalar_type() != q_in.scalar_type()) return false;
@@ -382,9 +392,6 @@ struct Failure {
   }
 };
 
-// (torch.jit.trace would record the outputs' allocation and none of the launches: the general functions end in an error there)
-bool being_traced() { return c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::Tracer); }
-
 int64_t pitch128(int64_t n) { return div_up(n, 128) * 128; }
 int64_t up256(int64_t n) { return div_up(n, 256) * 256; }
 int64_t packed_bytes(int64_t K, int64_t rows) { return div_up(K / 32, 16) * rows * 16; }
@@ -495,12 +502,6 @@ struct LinearCopies {
   }
 };
 
-// A call that a node may serve: not under torch.jit.trace, a functorch transform or forward-mode differentiation, which the general
-// functions refuse
-bool node_serves(const Tensor& x, const Tensor& weight) {
-  return !being_traced() && !c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::FuncTorchDynamicLayerFrontMode) && !x._fw_grad(0).defined() &&
-         !weight._fw_grad(0).defined();
-}
 void* current_stream(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
 
 // A refused launch on its way out of a node

@@ -56,6 +56,7 @@ def attention_mxfp4_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q
     ``bias`` (broadcastable to [B, Hq, Sq, seqlen_k]) is added to the scaled scores, ``alibi_slopes`` ([Hq] or [B, Hq]) give
     the ALiBi term ``-slope * |row + Sk - Sq - key|`` (:135-164,288-299).
     """
+    rt.refuse_transforms("attention_mxfp4_forward", bias, alibi_slopes)
     rt.require_gpu(q, k, v, q_scale, k_scale, v_scale)
     for t in (q, k, v, q_scale, k_scale, v_scale):
         assert t.is_contiguous() and t.dtype == torch.uint8
@@ -154,6 +155,7 @@ def attention_mxfp4_backward(grad_out: torch.Tensor, q: torch.Tensor, k: torch.T
     ``cu_seqlens_q`` / ``cu_seqlens_k``: boundaries (multiples of 32, both or neither) of sequences packed along the tokens, with B = 1 and no bias.
     Equal inputs give equal bits.
     """
+    rt.refuse_transforms("attention_mxfp4_backward", grad_out, out, lse, bias, alibi_slopes)
     rt.require_gpu(grad_out, q, k, v, q_scale, k_scale, v_scale, out, lse)
     for t in (q, k, v, q_scale, k_scale, v_scale):
         assert t.is_contiguous() and t.dtype == torch.uint8
@@ -189,6 +191,7 @@ def _readable(t: torch.Tensor) -> torch.Tensor:
 def quantize_qkv(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor):
     """bf16/fp32 [B,H,S,D] tensors (any batch, head and row strides) -> (q, q_scale, k, k_scale, v packed along keys, v_scale)
     in one launch."""
+    rt.refuse_transforms("attention", q, k, v)
     rt.require_gpu(q, k, v)
     if not q.dtype == k.dtype == v.dtype:   # (widening changes neither codes nor scales)
         q, k, v = q.float(), k.float(), v.float()
@@ -217,6 +220,7 @@ def _attend(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, sm_scale: float, 
     caller's results in whatever layout they have.  ``cu_q`` / ``cu_k``: boundaries (host ints) of sequences packed along S."""
     if alibi_slopes is None and rt.host().attend(q, k, v, sm_scale, bool(causal), out, lse, cu_q or [], cu_k or [], rt.stream_ptr(q.device)):
         return
+    rt.refuse_transforms("attention", q, k, v, alibi_slopes)
     operands = quantize_qkv(q, k, v)
     _attend_quantized(operands, sm_scale, causal, out, lse, _additive(None, alibi_slopes, q.shape[0], q.shape[1], q.shape[2], k.shape[2])[1], cu_q, cu_k)
 
@@ -265,6 +269,7 @@ class MXFP4AttentionFunction(torch.autograd.Function):
         sm_scale, causal, rows_outer, cu_q, cu_k = ctx.more
         if ctx.needs_input_grad[6]:
             raise NotImplementedError("the gradient of a bias is not implemented: detach it")
+        rt.refuse_transforms("attention", grad_out)
         want_q, want_kv = ctx.needs_input_grad[0], ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
         dq, dk, dv = _gradients(grad_out, (qq, qs, kq, ks, vq, vs), out, lse, sm_scale, causal, ctx.keys, b4, sl, cu_q, cu_k, rows_outer, want_q, want_kv)
         grads = [None if g is None or not need else g[:, :, :n].to(dt) for g, need, n, dt in
@@ -317,6 +322,7 @@ def _attention(q, k, v, alibi_slopes, bias, sm_scale, dropout_p, cu_seqlens_q, c
         # boundaries must be multiples of 32 (no block may belong to two sequences), and a causal mask is aligned to the
         # bottom-right corner of each sequence's own score matrix.  One quantizer launch over all tokens (no 32 x 32 block
         # spans two sequences) and one attention launch over all sequences.
+        rt.refuse_transforms("attention")   # (a trace would make tensors of the sizes checked here)
         cq = [int(c) for c in (cu_seqlens_q.tolist() if isinstance(cu_seqlens_q, torch.Tensor) else cu_seqlens_q)]
         ck = [int(c) for c in (cu_seqlens_k.tolist() if isinstance(cu_seqlens_k, torch.Tensor) else cu_seqlens_k)]
         torch._check(q.dim() == 3 and k.dim() == 3 and v.dim() == 3, lambda: "layout 'thd' takes [tokens, heads, head dim] tensors")
@@ -331,6 +337,7 @@ def _attention(q, k, v, alibi_slopes, bias, sm_scale, dropout_p, cu_seqlens_q, c
         _check_options(dropout_p, return_scores)
         rt.require_gpu(q, k, v)
         if _differentiated(q, k, v):
+            rt.refuse_transforms("attention", q, k, v, alibi_slopes)
             q4, k4, v4 = (t.transpose(0, 1).unsqueeze(0) for t in (q, k, v))
             out, lse = MXFP4AttentionFunction.apply(q4, k4, v4, q.shape[-1] ** -0.5 if sm_scale is None else float(sm_scale), bool(causal), True, None, alibi_slopes, cq, ck)
             return out.squeeze(0).transpose(0, 1), lse.squeeze(0).transpose(0, 1), torch.empty([], device=q.device, dtype=torch.float32)
@@ -358,6 +365,7 @@ def _fixed_length(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, alibi_slope
     if sm_scale is None:
         sm_scale = q.shape[-1] ** -0.5
     if _differentiated(q, k, v):
+        rt.refuse_transforms("attention", q, k, v, bias, alibi_slopes)
         out, lse = MXFP4AttentionFunction.apply(q, k, v, float(sm_scale), bool(causal), rows_outer, bias, alibi_slopes, None, None)
     elif bias is None:
         out, lse = _results(q, v.shape[3], rows_outer, False)

@@ -76,3 +76,28 @@ def test_a_rotation_with_forward_mode_tangents_is_refused(m):
             y = y if x[1] is None else y[0]
             with pytest.raises(NotImplementedError):
                 y.backward(make_dual(torch.ones_like(y), torch.ones_like(y)))   # (nor of a gradient)
+
+
+@pytest.mark.parametrize("requires_grad", [False, True])
+@pytest.mark.filterwarnings("ignore:`torch.jit")
+@pytest.mark.filterwarnings("ignore::torch.jit.TracerWarning")
+def test_attention_under_transforms_is_refused(m, requires_grad):
+    x = leaves(1, 64, 2, 2, 64)[:3]
+    want = m.triton_attention_mxfp4(*x, causal=True, layout="bshd")[0]
+    x = [t.requires_grad_(requires_grad) for t in x]
+    fn = lambda q, k, v: m.triton_attention_mxfp4(q, k, v, causal=True, layout="bshd")[0]  # noqa: E731
+    with pytest.raises(NotImplementedError, match="torch.jit.trace"):
+        torch.jit.trace(fn, tuple(x), check_trace=False)
+    with pytest.raises(NotImplementedError, match="functorch"):
+        torch.func.vmap(lambda q: fn(q, *x[1:]))(x[0].detach()[None])
+    with dual_level():
+        for i in range(3):
+            y = list(x)
+            y[i] = make_dual(x[i], torch.ones_like(x[i]))
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                fn(*y)
+        y = fn(*x)
+        assert torch.equal(y, want)
+        if requires_grad:
+            with pytest.raises(NotImplementedError):
+                y.backward(make_dual(torch.ones_like(y), torch.ones_like(y)))

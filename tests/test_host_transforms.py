@@ -1,7 +1,7 @@
 """Attention and rotary positions under torch's transforms, without a GPU: the native calls are stood in for by plain ones."""
 import pytest
 import torch
-from torch.autograd.forward_ad import dual_level, make_dual
+from torch.autograd.forward_ad import dual_level, make_dual, unpack_dual
 
 import alto_amd.mxfp4 as mx
 from alto_amd.mxfp4 import _runtime as rt
@@ -14,6 +14,8 @@ class Host:
     """Native calls that leave a trace of their operands: the attention's output is Q's first rows, its gradients are 2, 3 and 4."""
 
     def attend(self, q, k, v, sm_scale, causal, out, lse, *more):
+        if torch.jit.is_tracing() or torch._C._are_functorch_transforms_active() or any(unpack_dual(t).tangent is not None for t in (q, k, v)):
+            return False   # (as the native call does)
         out.copy_(q[..., :out.shape[-1]])
         lse.zero_()
         return True
@@ -137,3 +139,58 @@ def test_a_rotation_with_forward_mode_tangents_is_refused(stand_in, plain_rotati
         y = mx.apply_rotary(q.detach().requires_grad_(True), None, FREQ)
         with pytest.raises(NotImplementedError):
             y.backward(make_dual(torch.ones_like(y), torch.ones_like(y)))   # (nor of a gradient)
+
+
+ATTENTION = [dict(), dict(bias=torch.zeros(1, 1, 64, 64)), dict(alibi_slopes=torch.ones(2))]
+
+
+@pytest.mark.parametrize("requires_grad", [False, True])
+@pytest.mark.parametrize("more", ATTENTION, ids=["plain", "bias", "slopes"])
+@pytest.mark.filterwarnings("ignore:`torch.jit")
+@pytest.mark.filterwarnings("ignore::torch.jit.TracerWarning")
+def test_attention_under_transforms_is_refused(stand_in, requires_grad, more):
+    """A trace of it would hold the outputs' allocation alone, its tangents would be lost."""
+    x = tensors(requires_grad)
+    call = lambda q, k, v: mx.triton_attention_mxfp4(q, k, v, causal=True, **more)[0]  # noqa: E731
+    packed = lambda q, k, v: mx.triton_attention_mxfp4(*(t[0].transpose(0, 1) for t in (q, k, v)), causal=True, layout="thd", cu_seqlens_q=[0, 64], cu_seqlens_k=[0, 64])[0]  # noqa: E731
+    for fn in (call, packed):
+        with pytest.raises(NotImplementedError, match="torch.jit.trace"):
+            torch.jit.trace(fn, tuple(x), check_trace=False)
+        with pytest.raises(NotImplementedError, match="functorch"):
+            torch.func.grad(lambda q: fn(q, *x[1:]).float().sum())(x[0].detach())
+        with dual_level():
+            for i in range(3):
+                y = list(x)
+                y[i] = make_dual(x[i], torch.ones_like(x[i]))
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    fn(*y)
+    with dual_level():
+        for name, t in more.items():
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                mx.triton_attention_mxfp4(*x, causal=True, **{name: make_dual(t, torch.ones_like(t))})
+        if requires_grad:
+            y = call(*x)
+            with pytest.raises(NotImplementedError):
+                y.backward(make_dual(torch.ones_like(y), torch.ones_like(y)))
+
+
+@pytest.mark.filterwarnings("ignore:`torch.jit")
+@pytest.mark.filterwarnings("ignore::torch.jit.TracerWarning")
+def test_the_entry_points_on_codes_under_transforms_are_refused(stand_in):
+    codes, scales, rows = torch.zeros(1, 2, 64, 32, dtype=torch.uint8), torch.zeros(1, 2, 2, 2, dtype=torch.uint8), tensors(False)[0]
+    lse, bias = torch.zeros(1, 2, 64), torch.zeros(1, 1, 64, 64)
+    operands = codes, codes, codes, scales, scales, scales
+    with pytest.raises(NotImplementedError, match="torch.jit.trace"):
+        torch.jit.trace(lambda go: mx.attention_mxfp4_backward(go, *operands, rows, lse, 0.1, True), rows, check_trace=False)
+    with pytest.raises(NotImplementedError, match="torch.jit.trace"):
+        torch.jit.trace(lambda bias: mx.attention_mxfp4_forward(*operands, 0.1, True, bias=bias), bias, check_trace=False)
+    with pytest.raises(NotImplementedError, match="torch.jit.trace"):
+        torch.jit.trace(lambda q: mx.quantize_qkv(q, rows, rows)[:2], rows, check_trace=False)
+    with dual_level():
+        for go, out in ((make_dual(rows, rows), rows), (rows, make_dual(rows, rows))):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                mx.attention_mxfp4_backward(go, *operands, out, lse, 0.1, True)
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            mx.attention_mxfp4_forward(*operands, 0.1, True, bias=make_dual(bias, bias))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            mx.quantize_qkv(rows, rows, make_dual(rows, rows))
