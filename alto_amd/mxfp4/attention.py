@@ -151,7 +151,7 @@ def attention_mxfp4_backward(grad_out: torch.Tensor, q: torch.Tensor, k: torch.T
 
         P = exp(S - lse),  dV = P^T dO,  dS = P * (dO V^T - rowsum(dO * O)),  dQ = sm_scale dS K,  dK = sm_scale dS^T Q
 
-    Rows that see no key (``lse`` = -inf) give nothing to any gradient; keys from ``seqlen_k`` on get zeros.  ``bias`` gets no gradient.
+    Rows that see no key (``lse`` = -inf) give nothing to any gradient; keys from ``seqlen_k`` on get zeros.  ``bias`` and ``alibi_slopes`` get no gradient.
     ``cu_seqlens_q`` / ``cu_seqlens_k``: boundaries (multiples of 32, both or neither) of sequences packed along the tokens, with B = 1 and no bias.
     Equal inputs give equal bits.
     """
@@ -241,7 +241,7 @@ def _attend_quantized(operands, sm_scale: float, causal: bool, out: torch.Tensor
 class MXFP4AttentionFunction(torch.autograd.Function):
     """The attention of :func:`_attend` (or with a ``bias``, of :func:`attention_mxfp4_forward`) on [B, H, S, D] views, with its backward.  Kept from
     one to the other: Q, K and V as codes and scales, the output and the log-sum-exp.  What only the backward refuses (a scale that is not positive, the
-    gradient of a bias) it refuses when it runs."""
+    gradient of a bias or of slopes) it refuses when it runs."""
 
     @staticmethod
     def forward(ctx, q, k, v, sm_scale, causal, rows_outer, bias, alibi_slopes, cu_q, cu_k):
@@ -267,8 +267,9 @@ class MXFP4AttentionFunction(torch.autograd.Function):
     def backward(ctx, grad_out, _):
         qq, qs, kq, ks, vq, vs, out, lse, b4, sl = ctx.saved_tensors
         sm_scale, causal, rows_outer, cu_q, cu_k = ctx.more
-        if ctx.needs_input_grad[6]:
-            raise NotImplementedError("the gradient of a bias is not implemented: detach it")
+        for i, name in ((6, "a bias"), (7, "ALiBi slopes")):
+            if ctx.needs_input_grad[i]:
+                raise NotImplementedError(f"the gradient of {name} is not implemented: detach it")
         rt.refuse_transforms("attention", grad_out)
         want_q, want_kv = ctx.needs_input_grad[0], ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
         dq, dk, dv = _gradients(grad_out, (qq, qs, kq, ks, vq, vs), out, lse, sm_scale, causal, ctx.keys, b4, sl, cu_q, cu_k, rows_outer, want_q, want_kv)
@@ -289,8 +290,8 @@ def _results(q: torch.Tensor, Dv: int, rows_outer: bool, lse_rows_outer: bool) -
     return out, torch.empty((B, Hq, Sq), dtype=torch.float32, device=q.device)
 
 
-def _differentiated(*tensors: torch.Tensor) -> bool:
-    return torch.is_grad_enabled() and any(t.requires_grad for t in tensors)
+def _differentiated(*tensors: Optional[torch.Tensor]) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
 def triton_attention_mxfp4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, alibi_slopes: Optional[torch.Tensor] = None,
@@ -300,6 +301,7 @@ def triton_attention_mxfp4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, al
     """(q, k, v) [B,H,S,D] (or [B,S,H,D] with ``layout="bshd"``, or packed [T,H,D] with ``layout="thd"`` and ``cu_seqlens_*``)
     -> (out bf16 in the layout of q, softmax_lse fp32 [B,H,S] ([T,H] for 'thd'), exp_scores placeholder), as :1206-1239.
 
+    Differentiable in q, k and v; where a bias or slopes require a gradient, the backward raises.
     ``use_exp2`` is accepted either way: both settings evaluate exp(x) as exp2(x * log2 e) on the GPU's exp unit.
     """
     return (_attention_between_graphs if torch.compiler.is_compiling() else _attention)(
@@ -336,7 +338,7 @@ def _attention(q, k, v, alibi_slopes, bias, sm_scale, dropout_p, cu_seqlens_q, c
         torch._check(all(a < b for a, b in zip(cq, cq[1:])) and all(a < b for a, b in zip(ck, ck[1:])), lambda: "empty sequences are not supported")
         _check_options(dropout_p, return_scores)
         rt.require_gpu(q, k, v)
-        if _differentiated(q, k, v):
+        if _differentiated(q, k, v, alibi_slopes):
             rt.refuse_transforms("attention", q, k, v, alibi_slopes)
             q4, k4, v4 = (t.transpose(0, 1).unsqueeze(0) for t in (q, k, v))
             out, lse = MXFP4AttentionFunction.apply(q4, k4, v4, q.shape[-1] ** -0.5 if sm_scale is None else float(sm_scale), bool(causal), True, None, alibi_slopes, cq, ck)
@@ -364,7 +366,7 @@ def _fixed_length(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, alibi_slope
     assert max_seqlens_q in (None, q.shape[2]) and max_seqlens_k in (None, k.shape[2]), "variable lengths are not implemented"
     if sm_scale is None:
         sm_scale = q.shape[-1] ** -0.5
-    if _differentiated(q, k, v):
+    if _differentiated(q, k, v, bias, alibi_slopes):
         rt.refuse_transforms("attention", q, k, v, bias, alibi_slopes)
         out, lse = MXFP4AttentionFunction.apply(q, k, v, float(sm_scale), bool(causal), rows_outer, bias, alibi_slopes, None, None)
     elif bias is None:

@@ -540,7 +540,7 @@ int alto_mxfp4_attention_rows_per_workgroup(int64_t B, int64_t Hq, int64_t Sq, i
  * the gradients are bf16 with element strides of batch, head and row (multiples of 8), unit stride along the head dim, 16-byte
  * aligned.  sm_scale is positive, with a bias or slopes at least 2^-64; rows of the bias are less than 2^24 elements apart.  Keys from Sk_used on get zero gradients
  * and those of a row with lse = -inf are zero.  n_seqs > 0: packed sequences as in alto_mxfp4_attention_fwd_strided (cu_q / cu_k on the host,
- * no bias).  dq, or dk and dv together, may be NULL: not wanted.  bias: element (b, h, m, n) at b bias_sb + h bias_sh + m bias_sm + n, NULL: none; it gets no gradient.
+ * no bias).  dq, or dk and dv together, may be NULL: not wanted.  bias: element (b, h, m, n) at b bias_sb + h bias_sh + m bias_sm + n, NULL: none; neither it nor the slopes get a gradient.
  * workspace: alto_mxfp4_attention_bwd_workspace_bytes() bytes (sizes, the mask and the boundaries count, pointers do not), 256-byte aligned, of this call until it is done.
  * The results of equal inputs are equal bit for bit.
  */

@@ -101,3 +101,15 @@ def test_attention_under_transforms_is_refused(m, requires_grad):
         if requires_grad:
             with pytest.raises(NotImplementedError):
                 y.backward(make_dual(torch.ones_like(y), torch.ones_like(y)))
+
+
+@pytest.mark.parametrize("of_q", [True, False])
+def test_the_gradient_of_an_additive_term_is_refused(m, of_q):
+    """Also where nothing else requires one; the forward gives the bits that it gives without a graph."""
+    q, k, v, go = leaves(1, 64, 2, 2, 64)
+    for name, term in (("bias", torch.randn(1, 1, 64, 64, device=DEV)), ("alibi_slopes", torch.rand(2, device=DEV))):
+        want = m.triton_attention_mxfp4(q, k, v, causal=True, layout="bshd", **{name: term})[0]
+        y = m.triton_attention_mxfp4(q.detach().requires_grad_(of_q), k, v, causal=True, layout="bshd", **{name: term.clone().requires_grad_(True)})[0]
+        assert torch.equal(y, want)
+        with pytest.raises(NotImplementedError, match="detach"):
+            y.backward(go)

@@ -194,3 +194,28 @@ def test_the_entry_points_on_codes_under_transforms_are_refused(stand_in):
             mx.attention_mxfp4_forward(*operands, 0.1, True, bias=make_dual(bias, bias))
         with pytest.raises(NotImplementedError, match="forward-mode"):
             mx.quantize_qkv(rows, rows, make_dual(rows, rows))
+
+
+@pytest.mark.parametrize("of_q", [True, False])
+@pytest.mark.parametrize("name", ["bias", "alibi_slopes"])
+def test_the_gradient_of_an_additive_term_is_refused(stand_in, name, of_q):
+    """Also where nothing else requires one: no result without a graph, no gradient left out."""
+    x = tensors(False)
+    x[0].requires_grad_(of_q)
+    term = (torch.zeros(1, 1, 64, 64) if name == "bias" else torch.ones(2)).requires_grad_(True)
+    y = mx.triton_attention_mxfp4(*x, causal=True, **{name: term})[0]
+    with pytest.raises(NotImplementedError, match="detach"):
+        y.sum().backward()
+    with torch.no_grad():
+        assert not mx.triton_attention_mxfp4(*x, causal=True, **{name: term})[0].requires_grad
+    if of_q:
+        y = mx.triton_attention_mxfp4(*x, causal=True, **{name: term.detach()})[0]
+        assert bool((torch.autograd.grad(y.sum(), x[0])[0] == 2).all())
+
+
+def test_the_gradient_of_slopes_is_refused_for_packed_sequences(stand_in):
+    x = [t[0].transpose(0, 1) for t in tensors(False)]
+    slopes = torch.ones(2, requires_grad=True)
+    y = mx.triton_attention_mxfp4(*x, causal=True, alibi_slopes=slopes, layout="thd", cu_seqlens_q=[0, 64], cu_seqlens_k=[0, 64])[0]
+    with pytest.raises(NotImplementedError, match="detach"):
+        y.sum().backward()
