@@ -337,11 +337,12 @@ struct BiasBlock {
   }
 };
 
-// A probability.  None is above 1; where the bias is so large that lse has no bits left for the scores, a rounding could say so.
+// A probability.  None is above 1; where the bias is so large that lse has no bits left for the scores, a rounding could say so.  NaN stays NaN
+// (v_minimum3_f32; v_med3_f32 would make 0 of it, and a NaN of the bias or of lse would not be seen in dV).
 template <int ADD>
 __device__ __forceinline__ float probability_of(float x, std::integral_constant<int, ADD>) {
   const float p = __builtin_amdgcn_exp2f(x);
-  return ADD == ADD_BIAS ? __builtin_amdgcn_fmed3f(p, 0.0f, 1.0f) : p;
+  return ADD == ADD_BIAS ? __builtin_elementwise_minimum(p, 1.0f) : p;
 }
 
 // The products of a step are issued in a fixed order (sched_barrier): the read of an operand runs AHEAD products before its use, vector work lies

@@ -85,7 +85,9 @@ __global__ __launch_bounds__(256) void attn_bwd_prepare_kernel(const PrepareArgs
 #pragma unroll
     for (int m = 1; m < 8; m <<= 1) d += __shfl_xor(d, m, 64);
     if (c == 0) {
-      a.q_records[tile].lse2[r] = none ? __builtin_inff() : l * ATTN_RCP_LN2;
+      // (a finite one stays finite in base 2, where a score that overflows with it is then -inf or +inf over it and not NaN: P = 0 or 1)
+      const float l2 = l * ATTN_RCP_LN2, most = 0x1.fffffep127f;
+      a.q_records[tile].lse2[r] = none ? __builtin_inff() : (__builtin_fabsf(l) <= most ? __builtin_amdgcn_fmed3f(l2, -most, most) : l2);
       a.q_records[tile].minus_d[r] = none ? 0.0f : -d;
     }
     __syncthreads();
