@@ -279,15 +279,12 @@ class MXFP4AttentionFunction(torch.autograd.Function):
 
 
 def _results(q: torch.Tensor, Dv: int, rows_outer: bool, lse_rows_outer: bool) -> Tuple[torch.Tensor, torch.Tensor]:
-    """Room for [B, Hq, Sq, Dv] and [B, Hq, Sq]; ``rows_outer``: as views of memory with the rows outside the heads."""
+    """Room for [B, Hq, Sq, Dv] and [B, Hq, Sq]; ``rows_outer``: in memory with the rows outside the heads (no views: autograd lets a caller change
+    a function's result in place, not a view made inside the function)."""
     B, Hq, Sq = q.shape[:3]
-    if rows_outer:
-        out = torch.empty((B, Sq, Hq, Dv), dtype=torch.bfloat16, device=q.device).transpose(1, 2)
-    else:
-        out = torch.empty((B, Hq, Sq, Dv), dtype=torch.bfloat16, device=q.device)
-    if lse_rows_outer:
-        return out, torch.empty((B, Sq, Hq), dtype=torch.float32, device=q.device).transpose(1, 2)
-    return out, torch.empty((B, Hq, Sq), dtype=torch.float32, device=q.device)
+    out = torch.empty_strided((B, Hq, Sq, Dv), (Hq * Sq * Dv, Dv, Hq * Dv, 1) if rows_outer else (Hq * Sq * Dv, Sq * Dv, Dv, 1), dtype=torch.bfloat16, device=q.device)
+    lse = torch.empty_strided((B, Hq, Sq), (Hq * Sq, 1, Hq) if lse_rows_outer else (Hq * Sq, Sq, 1), dtype=torch.float32, device=q.device)
+    return out, lse
 
 
 def _differentiated(*tensors: Optional[torch.Tensor]) -> bool:

@@ -113,3 +113,21 @@ def test_the_gradient_of_an_additive_term_is_refused(m, of_q):
         assert torch.equal(y, want)
         with pytest.raises(NotImplementedError, match="detach"):
             y.backward(go)
+
+
+@pytest.mark.parametrize("layout", ["bhsd", "bshd", "thd"])
+def test_a_result_is_changed_in_place(m, layout):
+    """A gate on the attention's result, where no gradient is asked for; where one is, autograd says that the backward needs the result that was."""
+    q, k, v, _ = leaves(1, 64, 4, 2, 64)
+    more = {}
+    if layout == "bhsd":
+        q, k, v = (t.transpose(1, 2) for t in (q, k, v))
+    if layout == "thd":
+        (q, k, v), more = (t[0] for t in (q, k, v)), dict(cu_seqlens_q=[0, 32, 64], cu_seqlens_k=[0, 32, 64])
+    want = m.triton_attention_mxfp4(q, k, v, causal=True, layout=layout, **more)
+    x = [t.detach().requires_grad_(True) for t in (q, k, v)]
+    y, lse, _ = m.triton_attention_mxfp4(*x, causal=True, layout=layout, **more)
+    assert torch.equal(y, want[0]) and torch.equal(lse, want[1]) and y.stride() == want[0].stride() and lse.stride() == want[1].stride()
+    assert torch.equal(y.mul_(2), want[0] * 2)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()

@@ -219,3 +219,21 @@ def test_the_gradient_of_slopes_is_refused_for_packed_sequences(stand_in):
     y = mx.triton_attention_mxfp4(*x, causal=True, alibi_slopes=slopes, layout="thd", cu_seqlens_q=[0, 64], cu_seqlens_k=[0, 64])[0]
     with pytest.raises(NotImplementedError, match="detach"):
         y.sum().backward()
+
+
+@pytest.mark.parametrize("layout", ["bhsd", "bshd", "thd"])
+def test_a_result_is_changed_in_place(stand_in, layout):
+    """With a graph behind it as without one; a backward, which needs the output that was, then says so."""
+    for requires_grad in (False, True):
+        x = tensors(requires_grad)
+        if layout == "thd":
+            x = [t[0].transpose(0, 1) for t in x]
+        more = dict(cu_seqlens_q=[0, 64], cu_seqlens_k=[0, 64]) if layout == "thd" else {}
+        y = mx.triton_attention_mxfp4(*x, causal=True, layout=layout, **more)[0]
+        assert y.is_contiguous()
+        before = y.detach().clone()
+        y.mul_(2)
+        assert torch.equal(y, before * 2)
+        if requires_grad:
+            with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                y.sum().backward()
