@@ -219,7 +219,8 @@ int check_sizes(const alto_mxfp4_attention_bwd_t& p) {
   ALTO_REQUIRE(Dv == 64 || Dv == 128, "attention_bwd: value dim Dv=%lld must be 64 or 128", Dv);
   ALTO_REQUIRE(B <= 65535 && Hq < (1ll << 31) && Sq <= 65535ll * 128 && Sk <= 65535ll * 128, "attention_bwd: B, Sq / 128 and Sk / 128 must stay below 65536");
   ALTO_REQUIRE(product_below(1ll << 40, B * Sq, Hq, D > Dv ? D : Dv) && product_below(1ll << 40, B * Sk, Hk, D > Dv ? D : Dv), "attention_bwd: tensor too large");
-  ALTO_REQUIRE(product_below(1ll << 31, B, Hq, Sq / 32 + Sk / 32 + 1), "attention_bwd: tensor too large");
+  // (a launch's threads, 256 a workgroup, are counted in 32 bits)
+  ALTO_REQUIRE(B * Hq * (Sq / 32) + B * Hk * (Sk / 32) < (1ll << 24), "attention_bwd: tensor too large: 2^24 tiles of 32 rows or more");
   ALTO_REQUIRE(p.Sk_used > 0 && p.Sk_used <= p.Sk && p.Sk_used % 32 == 0, "attention_bwd: Sk_used=%lld must be a multiple of 32 in (0, Sk]", (long long)p.Sk_used);
   ALTO_REQUIRE(p.n_seqs >= 0, "attention_bwd: negative number of sequences");
   ALTO_REQUIRE(p.causal == 0 || p.n_seqs > 0 || p.Sq <= p.Sk_used, "attention_bwd: causal attention needs Sq <= Sk (got %lld > %lld)", (long long)p.Sq, (long long)p.Sk_used);
@@ -295,7 +296,7 @@ static int attention_bwd(const alto_mxfp4_attention_bwd_t& p, hipStream_t st) {
     const int64_t key_blocks = p.dk ? p.B * p.Hk * k_blocks : 0, row_blocks = p.dq ? p.B * p.Hq * q_blocks : 0;
     const int64_t key_groups = (key_blocks * cuts.keys.parts + 7) / 8 * 8, row_groups = (row_blocks * cuts.rows.parts + 7) / 8 * 8;
     const int64_t key_sums = cuts.keys.parts > 1 ? key_blocks : 0, row_sums = cuts.rows.parts > 1 ? row_blocks : 0;
-    ALTO_REQUIRE(key_groups + row_groups < (1ll << 31) && (key_sums + row_sums) * 12 < (1ll << 31), "attention_bwd: too many workgroups");
+    ALTO_REQUIRE(key_groups + row_groups < (1ll << 24) && (key_sums + row_sums) * 12 < (1ll << 24), "attention_bwd: too many workgroups");
     plan.key_groups = (int)key_groups;
     plan.row_groups = (int)row_groups;
     plan.key_sums = (int)key_sums;

@@ -223,7 +223,7 @@ static int rotary(const alto_mxfp4_rotary_t& p, hipStream_t st) {
   while (split * a.tokens < 256 && units > 256 * split && split < p.Hq + p.Hk) split *= 2;
   a.heads_each = (int)((p.Hq + p.Hk + split - 1) / split);
   const int64_t groups = (a.tokens + a.per_group - 1) / a.per_group;
-  ALTO_REQUIRE(groups < (1ll << 31), "rotary: too many tokens");
+  ALTO_REQUIRE(groups < (1ll << 24), "rotary: too many tokens for one launch");   // (its threads, 256 a workgroup, are counted in 32 bits)
   const dim3 grid((unsigned)groups, (unsigned)((p.Hq + p.Hk + a.heads_each - 1) / a.heads_each));
   const size_t lds = (size_t)a.per_group * p.R * 4;
   if (p.dtype == ALTO_DT_BF16) p.interleaved ? launch<__bf16, true>(a, (int)vec, grid, lds, st) : launch<__bf16, false>(a, (int)vec, grid, lds, st);

@@ -542,7 +542,7 @@ int alto_mxfp4_attention_rows_per_workgroup(int64_t B, int64_t Hq, int64_t Sq, i
  * and those of a row with lse = -inf are zero.  n_seqs > 0: packed sequences as in alto_mxfp4_attention_fwd_strided (cu_q / cu_k on the host,
  * no bias).  dq, or dk and dv together, may be NULL: not wanted.  bias: element (b, h, m, n) at b bias_sb + h bias_sh + m bias_sm + n, NULL: none; neither it nor the slopes get a gradient.
  * workspace: alto_mxfp4_attention_bwd_workspace_bytes() bytes (sizes, the mask and the boundaries count, pointers do not), 256-byte aligned, of this call until it is done.
- * The results of equal inputs are equal bit for bit.
+ * Q and K have fewer than 2^24 tiles of 32 rows together, all heads counted.  The results of equal inputs are equal bit for bit.
  */
 typedef struct {
   const void *q_codes, *q_scales, *k_codes, *k_scales, *vt_codes, *v_scales, *dout, *out;
@@ -565,7 +565,7 @@ int alto_mxfp4_attention_bwd(const alto_mxfp4_attention_bwd_t* args, void* strea
  * back (the transpose: its backward).  q [B][S][Hq][D] and k [B][S][Hk][D] (Hk = 0: none) at element strides of batch, head and row, unit
  * stride along D, bf16 or f32, outputs alike; an output is no input.  inv_freq: R/2 doubles on the device; angles, cosines and sines are taken
  * in 64 bits, products in 32, rounded once.  positions: int64 (or int32 with positions_are_32), element (b, s) at b pos_sb + s pos_ss, any
- * sign; NULL: s.  R even, at most 2048.
+ * sign; NULL: s.  R even, at most 2048; fewer than 2^24 tokens, up to 8 times as many where a token's heads have little work.
  */
 typedef struct {
   const void *q, *k;
