@@ -231,9 +231,8 @@ def test_a_result_is_changed_in_place(stand_in, layout):
         more = dict(cu_seqlens_q=[0, 64], cu_seqlens_k=[0, 64]) if layout == "thd" else {}
         y = mx.triton_attention_mxfp4(*x, causal=True, layout=layout, **more)[0]
         assert y.is_contiguous()
-        before = y.detach().clone()
-        y.mul_(2)
-        assert torch.equal(y, before * 2)
+        y.zero_().add_(2)   # (what stands in for the launch leaves memory as it was: anything)
+        assert bool((y == 2).all())
         if requires_grad:
             with pytest.raises(RuntimeError, match="modified by an inplace operation"):
                 y.sum().backward()
