@@ -17,6 +17,7 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_cpp_function.h>
 
 #include <algorithm>
@@ -310,66 +311,7 @@ bool attend(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in, double s
   return true;
 }
 
-// attention.py:attention_mxfp4_backward on dense operands -> (dq, dk, dv)
 bool on_current_device(const Tensor& t) { return on_gpu(t) && t.get_device() == c10::hip::current_device(); }
-py::object attention_gradients(const Tensor& go_in, const Tensor& q, const Tensor& q_scale, const Tensor& k, const Tensor& k_scale, const Tensor& v, const Tensor& v_scale,
-                               const Tensor& out_in, const Tensor& lse, double sm_scale, bool causal, int64_t seqlen_k, const OptTensor& bias, const OptTensor& slopes,
-                               const std::vector<int32_t>& cu_q, const std::vector<int32_t>& cu_k, bool rows_outer, bool want_q, bool want_kv) {
-  for (const Tensor* t : {&q, &q_scale, &k, &k_scale, &v, &v_scale})
-    if (!on_current_device(*t) || t->scalar_type() != at::kByte || t->dim() != 4 || !t->is_contiguous()) return py::none();
-  for (const Tensor* t : {&go_in, &out_in})
-    if (!on_current_device(*t) || t->scalar_type() != at::kBFloat16 || t->dim() != 4) return py::none();
-  const int64_t B = q.size(0), Hq = q.size(1), Sq = q.size(2), D = 2 * q.size(3), Hk = k.size(1), Sk = k.size(2), Dv = v.size(2);
-  auto is = [](const Tensor& t, at::IntArrayRef size) { return t.sizes() == size; };
-  if (!is(k, {B, Hk, Sk, D / 2}) || !is(v, {B, Hk, Dv, Sk / 2}) || !is(q_scale, {B, Hq, Sq / 32, D / 32}) || !is(k_scale, {B, Hk, Sk / 32, D / 32}) ||
-      !is(v_scale, {B, Hk, Sk / 32, Dv / 32}) || !is(go_in, {B, Hq, Sq, Dv}) || !is(out_in, {B, Hq, Sq, Dv}))
-    return py::none();
-  if (!on_current_device(lse) || lse.scalar_type() != at::kFloat || !is(lse, {B, Hq, Sq}) || cu_q.size() != cu_k.size() || cu_q.size() == 1) return py::none();
-  for (const OptTensor* t : {&bias, &slopes})   // (as _additive gives them)
-    if (t->has_value() && (!on_current_device(**t) || (*t)->scalar_type() != at::kFloat)) return py::none();
-  auto readable = [](const Tensor& t) {
-    return t.stride(3) == 1 && aligned16(t) && stride_of(t, 0) % 8 == 0 && stride_of(t, 1) % 8 == 0 && stride_of(t, 2) % 8 == 0 ? t : t.contiguous();
-  };
-  const Tensor go = readable(go_in), out = readable(out_in);
-  const auto opts = at::TensorOptions().dtype(at::kBFloat16).device(q.device());
-  auto grad = [&](bool want, int64_t H, int64_t S, int64_t n) {
-    if (!want) return Tensor();
-    return rows_outer ? at::empty({B, S, H, n}, opts).transpose(1, 2) : at::empty({B, H, S, n}, opts);
-  };
-  const Tensor dq = grad(want_q, Hq, Sq, D), dk = grad(want_kv, Hk, Sk, D), dv = grad(want_kv, Hk, Sk, Dv);
-  alto_mxfp4_attention_bwd_t a{};
-  a.q_codes = bytes(q); a.q_scales = bytes(q_scale); a.k_codes = bytes(k); a.k_scales = bytes(k_scale); a.vt_codes = bytes(v); a.v_scales = bytes(v_scale);
-  a.dout = bytes(go); a.out = bytes(out); a.lse = static_cast<const float*>(lse.data_ptr());
-  a.dq = bytes(dq); a.dk = bytes(dk); a.dv = bytes(dv);
-  a.B = B; a.Hq = Hq; a.Hk = Hk; a.Sq = Sq; a.Sk = Sk; a.Sk_used = seqlen_k; a.D = D; a.Dv = Dv;
-  auto strides = [](const Tensor& t, int64_t& sb, int64_t& sh, int64_t& ss) {
-    if (!t.defined()) return;
-    sb = stride_of(t, 0); sh = stride_of(t, 1); ss = stride_of(t, 2);
-  };
-  strides(go, a.dout_sb, a.dout_sh, a.dout_ss);
-  strides(out, a.out_sb, a.out_sh, a.out_ss);
-  strides(lse, a.lse_sb, a.lse_sh, a.lse_ss);
-  strides(dq, a.dq_sb, a.dq_sh, a.dq_ss);
-  strides(dk, a.dk_sb, a.dk_sh, a.dk_ss);
-  strides(dv, a.dv_sb, a.dv_sh, a.dv_ss);
-  if (bias.has_value()) {
-    a.bias = static_cast<const float*>(bias->data_ptr());
-    a.bias_sb = stride_of(*bias, 0); a.bias_sh = stride_of(*bias, 1); a.bias_sm = bias->stride(2);
-  }
-  if (slopes.has_value()) {
-    a.alibi_slopes = static_cast<const float*>(slopes->data_ptr());
-    a.alibi_sb = stride_of(*slopes, 0); a.alibi_sh = slopes->stride(1);
-  }
-  if (!cu_q.empty()) { a.cu_q = cu_q.data(); a.cu_k = cu_k.data(); a.n_seqs = (int)cu_q.size() - 1; }
-  a.causal = causal; a.sm_scale = (float)sm_scale;
-  a.workspace_bytes = api.attention_bwd_workspace_bytes(&a);
-  if (a.workspace_bytes < 0) return py::none();   // (the general path words the error)
-  const Tensor ws = Alloc(q).dense({a.workspace_bytes});
-  a.workspace = ws.data_ptr();
-  call("alto_mxfp4_attention_bwd", api.attention_bwd, &a, c10::hip::getCurrentHIPStream(q.device().index()).stream());
-  auto opt = [](const Tensor& t) -> py::object { return t.defined() ? py::cast(t) : py::none(); };
-  return py::make_tuple(opt(dq), opt(dk), opt(dv));
-}
 
 // ------------------------------------------------------------------------------------------------- whole training directions
 // A layer's step as an autograd node of its own, one native call per direction: outputs, quantizers and products, the interpreter
@@ -826,6 +768,221 @@ py::tuple draw_hadamard(const std::optional<at::Generator>& gen, at::ScalarType 
   return py::make_tuple(signs, perm);
 }
 
+// -------------------------------------------------------------------------------------------------- attention and its gradients
+// What the backward takes beside the gradient of the output: quantized operands, the forward's results, the additive terms as _additive gives them
+struct AttentionKept {
+  Tensor q, q_scale, k, k_scale, v, v_scale, out, lse;
+  OptTensor bias, slopes;
+  double sm_scale = 0;
+  bool causal = false, rows_outer = false;
+  int64_t keys = 0;
+  std::vector<int32_t> cu_q, cu_k;
+};
+
+// attention.py:_gradients -> {dq, dk, dv} (undefined: not wanted), or false: declined
+bool attention_gradients(Failure& f, const Tensor& go_in, const AttentionKept& x, bool want_q, bool want_kv, variable_list& grads) {
+  const Tensor &q = x.q, &k = x.k, &v = x.v;
+  for (const Tensor* t : {&q, &x.q_scale, &k, &x.k_scale, &v, &x.v_scale})
+    if (!on_current_device(*t) || t->scalar_type() != at::kByte || t->dim() != 4 || !t->is_contiguous()) return false;
+  for (const Tensor* t : {&go_in, &x.out})
+    if (!on_current_device(*t) || t->scalar_type() != at::kBFloat16 || t->dim() != 4) return false;
+  const int64_t B = q.size(0), Hq = q.size(1), Sq = q.size(2), D = 2 * q.size(3), Hk = k.size(1), Sk = k.size(2), Dv = v.size(2);
+  auto is = [](const Tensor& t, at::IntArrayRef size) { return t.sizes() == size; };
+  if (!is(k, {B, Hk, Sk, D / 2}) || !is(v, {B, Hk, Dv, Sk / 2}) || !is(x.q_scale, {B, Hq, Sq / 32, D / 32}) || !is(x.k_scale, {B, Hk, Sk / 32, D / 32}) ||
+      !is(x.v_scale, {B, Hk, Sk / 32, Dv / 32}) || !is(go_in, {B, Hq, Sq, Dv}) || !is(x.out, {B, Hq, Sq, Dv}))
+    return false;
+  if (!on_current_device(x.lse) || x.lse.scalar_type() != at::kFloat || !is(x.lse, {B, Hq, Sq}) || x.cu_q.size() != x.cu_k.size() || x.cu_q.size() == 1) return false;
+  for (const OptTensor* t : {&x.bias, &x.slopes})
+    if (t->has_value() && (!on_current_device(**t) || (*t)->scalar_type() != at::kFloat)) return false;
+  auto readable = [](const Tensor& t) {
+    return t.stride(3) == 1 && aligned16(t) && stride_of(t, 0) % 8 == 0 && stride_of(t, 1) % 8 == 0 && stride_of(t, 2) % 8 == 0 ? t : t.contiguous();
+  };
+  const Tensor go = readable(go_in), out = readable(x.out);
+  const auto opts = at::TensorOptions().dtype(at::kBFloat16).device(q.device());
+  auto grad = [&](bool want, int64_t H, int64_t S, int64_t n) {
+    if (!want) return Tensor();
+    return x.rows_outer ? at::empty({B, S, H, n}, opts).transpose(1, 2) : at::empty({B, H, S, n}, opts);
+  };
+  const Tensor dq = grad(want_q, Hq, Sq, D), dk = grad(want_kv, Hk, Sk, D), dv = grad(want_kv, Hk, Sk, Dv);
+  alto_mxfp4_attention_bwd_t a{};
+  a.q_codes = bytes(q); a.q_scales = bytes(x.q_scale); a.k_codes = bytes(k); a.k_scales = bytes(x.k_scale); a.vt_codes = bytes(v); a.v_scales = bytes(x.v_scale);
+  a.dout = bytes(go); a.out = bytes(out); a.lse = static_cast<const float*>(x.lse.data_ptr());
+  a.dq = bytes(dq); a.dk = bytes(dk); a.dv = bytes(dv);
+  a.B = B; a.Hq = Hq; a.Hk = Hk; a.Sq = Sq; a.Sk = Sk; a.Sk_used = x.keys; a.D = D; a.Dv = Dv;
+  auto strides = [](const Tensor& t, int64_t& sb, int64_t& sh, int64_t& ss) {
+    if (!t.defined()) return;
+    sb = stride_of(t, 0); sh = stride_of(t, 1); ss = stride_of(t, 2);
+  };
+  strides(go, a.dout_sb, a.dout_sh, a.dout_ss);
+  strides(out, a.out_sb, a.out_sh, a.out_ss);
+  strides(x.lse, a.lse_sb, a.lse_sh, a.lse_ss);
+  strides(dq, a.dq_sb, a.dq_sh, a.dq_ss);
+  strides(dk, a.dk_sb, a.dk_sh, a.dk_ss);
+  strides(dv, a.dv_sb, a.dv_sh, a.dv_ss);
+  if (x.bias.has_value()) {
+    a.bias = static_cast<const float*>(x.bias->data_ptr());
+    a.bias_sb = stride_of(*x.bias, 0); a.bias_sh = stride_of(*x.bias, 1); a.bias_sm = x.bias->stride(2);
+  }
+  if (x.slopes.has_value()) {
+    a.alibi_slopes = static_cast<const float*>(x.slopes->data_ptr());
+    a.alibi_sb = stride_of(*x.slopes, 0); a.alibi_sh = x.slopes->stride(1);
+  }
+  if (!x.cu_q.empty()) { a.cu_q = x.cu_q.data(); a.cu_k = x.cu_k.data(); a.n_seqs = (int)x.cu_q.size() - 1; }
+  a.causal = x.causal; a.sm_scale = (float)x.sm_scale;
+  a.workspace_bytes = api.attention_bwd_workspace_bytes(&a);
+  if (a.workspace_bytes < 0) return false;   // (the general path words the error)
+  const Tensor ws = Alloc(q).dense({a.workspace_bytes});
+  a.workspace = ws.data_ptr();
+  f.ok("alto_mxfp4_attention_bwd", api.attention_bwd(&a, current_stream(q)));
+  grads = {dq, dk, dv};
+  return true;
+}
+py::object opt(const Tensor& t) { return t.defined() ? py::cast(t) : py::none(); }
+py::object attention_gradients_py(const Tensor& go, const Tensor& q, const Tensor& q_scale, const Tensor& k, const Tensor& k_scale, const Tensor& v, const Tensor& v_scale,
+                                  const Tensor& out, const Tensor& lse, double sm_scale, bool causal, int64_t seqlen_k, const OptTensor& bias, const OptTensor& slopes,
+                                  const std::vector<int32_t>& cu_q, const std::vector<int32_t>& cu_k, bool rows_outer, bool want_q, bool want_kv) {
+  Failure f;
+  variable_list grads;
+  {
+    py::gil_scoped_release nogil;
+    if (!attention_gradients(f, go, {q, q_scale, k, k_scale, v, v_scale, out, lse, bias, slopes, sm_scale, causal, rows_outer, seqlen_k, cu_q, cu_k}, want_q, want_kv, grads))
+      grads.clear();
+  }
+  f.raise();
+  return grads.empty() ? py::none() : py::object(py::make_tuple(opt(grads[0]), opt(grads[1]), opt(grads[2])));
+}
+
+// attention.py:MXFP4AttentionFunction without additive terms, as one native call a direction: as a Python function a forward of small sizes with a graph
+// took 44 us, here 18 (without one 16).  Q is quantized ahead of the attention kernel, because the backward needs its codes, and not in it: 2048 tokens of
+// 32 / 8 heads of 128 take 43 us for 40, 4 x 2048 of 64 / 8 185 for 173, 8192 of 16 / 2 145.5 for 146.3.
+struct AttentionShape {
+  int64_t B, Hq, Hk, Sq, Sk, D, Dv;
+  double sm_scale;
+  bool causal, rows_outer;
+  // of the kept buffer: codes and scales of Q, K and V, 16 bytes of room behind each (the attention kernel reads scale bytes in whole dwords)
+  int64_t bytes_of(int i) const {
+    const int64_t n[6] = {B * Hq * Sq * D / 2, B * Hq * (Sq / 32) * (D / 32), B * Hk * Sk * D / 2, B * Hk * (Sk / 32) * (D / 32), B * Hk * Sk * Dv / 2, B * Hk * (Sk / 32) * (Dv / 32)};
+    return n[i];
+  }
+  int64_t start(int i) const {
+    int64_t at = 0;
+    for (int j = 0; j < i; ++j) at += div_up(bytes_of(j) + 16, 256) * 256;
+    return at;
+  }
+};
+static_assert(std::is_trivially_copyable<AttentionShape>::value, "kept as bytes");
+template <typename T>
+std::string bytes_text(const T* p, size_t n) { return std::string(reinterpret_cast<const char*>(p), n * sizeof(T)); }
+
+struct AttentionOperands {
+  AttentionShape shape;
+  bool lse_rows_outer;
+  std::vector<int32_t> cu_q, cu_k;
+};
+
+struct AttentionNode : torch::autograd::Function<AttentionNode> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& q_in, const Tensor& k_in, const Tensor& v_in, const AttentionOperands& op) {
+    const AttentionShape& x = op.shape;
+    Tensor q = q_in, k = k_in, v = v_in;
+    const int64_t vec = q.scalar_type() == at::kBFloat16 ? 8 : 4;
+    for (Tensor* t : {&q, &k, &v})
+      if (t->stride(3) != 1 || !aligned16(*t) || stride_of(*t, 0) % vec != 0 || stride_of(*t, 1) % vec != 0 || stride_of(*t, 2) % vec != 0) *t = t->contiguous();
+    const int64_t out_rows = x.rows_outer ? x.Hq * x.Dv : x.Dv, out_heads = x.rows_outer ? x.Dv : x.Sq * x.Dv;
+    const Tensor buf = Alloc(q).dense({x.start(6)});
+    const Tensor out = at::empty_strided({x.B, x.Hq, x.Sq, x.Dv}, {x.Hq * x.Sq * x.Dv, out_heads, out_rows, 1}, buf.options().dtype(at::kBFloat16));
+    const Tensor lse = at::empty_strided({x.B, x.Hq, x.Sq}, {x.Hq * x.Sq, op.lse_rows_outer ? 1 : x.Sq, op.lse_rows_outer ? x.Hq : 1}, buf.options().dtype(at::kFloat));
+    uint8_t* p[6];
+    for (int i = 0; i < 6; ++i) p[i] = bytes(buf) + x.start(i);
+    void* s = current_stream(q);
+    const int n = op.cu_q.empty() ? 0 : (int)op.cu_q.size() - 1;
+    Failure f;
+    f.ok("alto_mxfp4_attention_quantize",
+         api.attention_quantize(q.data_ptr(), k.data_ptr(), v.data_ptr(), dtype_code(q.scalar_type()), x.B, x.Hq, x.Hk, x.Sq, x.Sk, x.D, x.Dv, stride_of(q, 0), stride_of(q, 1),
+                                stride_of(q, 2), stride_of(k, 0), stride_of(k, 1), stride_of(k, 2), stride_of(v, 0), stride_of(v, 1), stride_of(v, 2), p[0], p[1], p[2], p[3],
+                                p[4], p[5], s)) &&
+        f.ok("alto_mxfp4_attention_fwd_strided",
+             api.attention_fwd_strided(p[0], p[1], p[2], p[3], p[4], p[5], out.data_ptr(), static_cast<float*>(lse.data_ptr()), x.B, x.Hq, x.Hk, x.Sq, x.Sk, x.D, x.Dv,
+                                       out.stride(0), out.stride(1), out.stride(2), lse.stride(0), lse.stride(1), lse.stride(2), n, n ? op.cu_q.data() : nullptr,
+                                       n ? op.cu_k.data() : nullptr, (float)x.sm_scale, (int)x.causal, nullptr, 0, 0, s));
+    if (f.rc != 0) throw Refused{f};
+    ctx->save_for_backward({buf, out, lse});
+    ctx->saved_data["shape"] = bytes_text(&x, 1);
+    ctx->saved_data["cu_q"] = bytes_text(op.cu_q.data(), op.cu_q.size());
+    ctx->saved_data["cu_k"] = bytes_text(op.cu_k.data(), op.cu_k.size());
+    ctx->saved_data["dtype"] = (int64_t)q.scalar_type();
+    ctx->mark_non_differentiable({lse});
+    return {out, lse};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    refuse_tangents("attention", {grads[0]});
+    const bool again = at::GradMode::is_enabled() && grads[0].requires_grad();
+    const at::NoGradGuard guard;
+    const variable_list saved = ctx->get_saved_variables();
+    AttentionShape x;
+    std::memcpy(&x, ctx->saved_data["shape"].toStringRef().data(), sizeof x);
+    auto boundaries = [&](const char* name) {
+      const std::string& text = ctx->saved_data[name].toStringRef();
+      std::vector<int32_t> c(text.size() / sizeof(int32_t));
+      if (!c.empty()) std::memcpy(c.data(), text.data(), text.size());
+      return c;
+    };
+    const Tensor buf = whole_aligned(saved[0]);
+    auto part = [&](int i, at::IntArrayRef size) { return buf.narrow(0, x.start(i), x.bytes_of(i)).view(size); };
+    const AttentionKept kept{part(0, {x.B, x.Hq, x.Sq, x.D / 2}),       part(1, {x.B, x.Hq, x.Sq / 32, x.D / 32}), part(2, {x.B, x.Hk, x.Sk, x.D / 2}),
+                             part(3, {x.B, x.Hk, x.Sk / 32, x.D / 32}), part(4, {x.B, x.Hk, x.Dv, x.Sk / 2}),      part(5, {x.B, x.Hk, x.Sk / 32, x.Dv / 32}),
+                             saved[1], saved[2], std::nullopt, std::nullopt, x.sm_scale, x.causal, x.rows_outer, x.Sk, boundaries("cu_q"), boundaries("cu_k")};
+    const bool need[3] = {ctx->needs_input_grad(0), ctx->needs_input_grad(1), ctx->needs_input_grad(2)};
+    variable_list out;
+    Failure f;
+    if (!attention_gradients(f, grads[0], kept, need[0], need[1] || need[2], out))
+      with_interpreter([&] {   // (what the native form declines: the general form serves it, or words the error)
+        const py::tuple operands = py::make_tuple(kept.q, kept.q_scale, kept.k, kept.k_scale, kept.v, kept.v_scale);
+        const py::tuple g = python_function("alto_amd.mxfp4.attention", "_gradients")(grads[0], operands, kept.out, kept.lse, kept.sm_scale, kept.causal, kept.keys, py::none(),
+                                                                                     py::none(), kept.cu_q, kept.cu_k, kept.rows_outer, need[0], need[1] || need[2]);
+        out.resize(3);
+        for (int i = 0; i < 3; ++i)
+          if (!g[i].is_none()) out[i] = g[i].cast<Tensor>();
+      });
+    raise_in_engine(f);
+    const at::ScalarType dtype = (at::ScalarType)ctx->saved_data["dtype"].toInt();
+    for (int i = 0; i < 3; ++i) {
+      if (!need[i]) out[i] = Tensor();
+      else if (out[i].scalar_type() != dtype) out[i] = out[i].to(dtype);
+    }
+    if (again) {   // (the gradients have none of their own: a second derivative ends in an error, as of a function marked once_differentiable)
+      for (Tensor& g : out)
+        if (g.defined()) g = g.detach().set_requires_grad(true);
+      const at::AutoGradMode on(true);
+      out = std::make_shared<torch::autograd::DelayedError>("the gradients of attention are not differentiable", 3)->apply(std::move(out));
+    }
+    out.emplace_back();   // (the operands)
+    return out;
+  }
+};
+
+// Attention of everyday calls whose Q, K or V require a gradient -> (out, lse) with their graph, or None
+py::object attention_step(const Tensor& q, const Tensor& k, const Tensor& v, double sm_scale, bool causal, bool rows_outer, bool lse_rows_outer, const std::vector<int32_t>& cu_q,
+                          const std::vector<int32_t>& cu_k) {
+  for (const Tensor* t : {&q, &k, &v})
+    if (!on_current_device(*t) || !is_float(*t) || t->dim() != 4 || t->scalar_type() != q.scalar_type() || t->numel() == 0) return py::none();
+  if (!node_serves(q, k) || v._fw_grad(0).defined() || cu_q.size() != cu_k.size()) return py::none();
+  const AttentionShape x{q.size(0), q.size(1), v.size(1), q.size(2), v.size(2), q.size(3), v.size(3), sm_scale, causal, rows_outer};
+  if (k.size(0) != x.B || v.size(0) != x.B || k.size(1) != x.Hk || k.size(2) != x.Sk || k.size(3) != x.D) return py::none();
+  if (x.Sq % 32 != 0 || x.Sk % 32 != 0 || x.D % 32 != 0 || x.Dv % 32 != 0) return py::none();
+  variable_list out;
+  Failure f;
+  {
+    py::gil_scoped_release nogil;
+    try {
+      out = AttentionNode::apply(q, k, v, AttentionOperands{x, lse_rows_outer, cu_q, cu_k});
+    } catch (const Refused& r) {
+      f = r.failure;
+    }
+  }
+  f.raise();
+  return py::make_tuple(out[0], out[1]);
+}
+
 // ------------------------------------------------------------------------------------------------------------ rotary positions
 // rotary.py:apply_rotary and its backward.  As Python functions around one native call each a forward took 21 us and a training step 145
 // (5.8 and 33 to 60 here: torch's engine and its thread).
@@ -982,6 +1139,7 @@ void introduce_node(const char* name) {
 PYBIND11_MODULE(alto_mxfp4_host, m) {
   introduce_node<LinearNode>("MXFP4LinearStepBackward");
   introduce_node<GroupedNode>("MXFP4GroupedStepBackward");
+  introduce_node<AttentionNode>("MXFP4AttentionFunctionBackward");
   introduce_node<RotaryNode>("RotaryBackward");
   m.def("bind", &bind);
   m.def("quantize", &quantize);
@@ -991,7 +1149,8 @@ PYBIND11_MODULE(alto_mxfp4_host, m) {
   m.def("grouped_packed", &grouped_packed);
   m.def("grouped_dw_packed", &grouped_dw_packed);
   m.def("attend", &attend);
-  m.def("attention_gradients", &attention_gradients);
+  m.def("attention_gradients", &attention_gradients_py);
+  m.def("attention_step", &attention_step);
   m.def("rotary", &rotary);
   m.def("linear_step", &linear_step);
   m.def("linear_saved", &linear_saved);

@@ -278,6 +278,16 @@ class MXFP4AttentionFunction(torch.autograd.Function):
         return (*grads, None, None, None, None, None, None, None)
 
 
+def _attend_with_graph(q, k, v, sm_scale, causal, rows_outer, bias, alibi_slopes, cu_q, cu_k):
+    """(out, lse) of [B, H, S, D] views, differentiable in q, k and v: a native node where it serves the call."""
+    if bias is None and alibi_slopes is None:
+        both = rt.host().attention_step(q, k, v, float(sm_scale), bool(causal), rows_outer, cu_q is not None, cu_q or [], cu_k or [])
+        if both is not None:
+            return both
+    rt.refuse_transforms("attention", q, k, v, bias, alibi_slopes)
+    return MXFP4AttentionFunction.apply(q, k, v, float(sm_scale), bool(causal), rows_outer, bias, alibi_slopes, cu_q, cu_k)
+
+
 def _results(q: torch.Tensor, Dv: int, rows_outer: bool, lse_rows_outer: bool) -> Tuple[torch.Tensor, torch.Tensor]:
     """Room for [B, Hq, Sq, Dv] and [B, Hq, Sq]; ``rows_outer``: in memory with the rows outside the heads (no views: autograd lets a caller change
     a function's result in place, not a view made inside the function)."""
@@ -336,9 +346,8 @@ def _attention(q, k, v, alibi_slopes, bias, sm_scale, dropout_p, cu_seqlens_q, c
         _check_options(dropout_p, return_scores)
         rt.require_gpu(q, k, v)
         if _differentiated(q, k, v, alibi_slopes):
-            rt.refuse_transforms("attention", q, k, v, alibi_slopes)
             q4, k4, v4 = (t.transpose(0, 1).unsqueeze(0) for t in (q, k, v))
-            out, lse = MXFP4AttentionFunction.apply(q4, k4, v4, q.shape[-1] ** -0.5 if sm_scale is None else float(sm_scale), bool(causal), True, None, alibi_slopes, cq, ck)
+            out, lse = _attend_with_graph(q4, k4, v4, q.shape[-1] ** -0.5 if sm_scale is None else sm_scale, causal, True, None, alibi_slopes, cq, ck)
             return out.squeeze(0).transpose(0, 1), lse.squeeze(0).transpose(0, 1), torch.empty([], device=q.device, dtype=torch.float32)
         out = torch.empty((q.shape[0], q.shape[1], v.shape[2]), dtype=torch.bfloat16, device=q.device)
         lse = torch.empty((q.shape[0], q.shape[1]), dtype=torch.float32, device=q.device)
@@ -364,8 +373,7 @@ def _fixed_length(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, alibi_slope
     if sm_scale is None:
         sm_scale = q.shape[-1] ** -0.5
     if _differentiated(q, k, v, bias, alibi_slopes):
-        rt.refuse_transforms("attention", q, k, v, bias, alibi_slopes)
-        out, lse = MXFP4AttentionFunction.apply(q, k, v, float(sm_scale), bool(causal), rows_outer, bias, alibi_slopes, None, None)
+        out, lse = _attend_with_graph(q, k, v, sm_scale, causal, rows_outer, bias, alibi_slopes, None, None)
     elif bias is None:
         out, lse = _results(q, v.shape[3], rows_outer, False)
         _attend(q, k, v, sm_scale, causal, out, lse, alibi_slopes)

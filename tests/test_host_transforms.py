@@ -26,6 +26,9 @@ class Host:
 
         return full(2.0, q.shape[1], q.shape[2], 2 * q.shape[3]), full(3.0, k.shape[1], k.shape[2], 2 * q.shape[3]), full(4.0, k.shape[1], k.shape[2], v.shape[2])
 
+    def attention_step(self, *args):
+        return None
+
     def rotary(self, *args):
         return None
 
