@@ -108,6 +108,11 @@ uint8_t* bytes(const Tensor& t) { return t.defined() ? static_cast<uint8_t*>(t.d
 bool aligned16(const Tensor& t) { return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0; }
 int64_t stride_of(const Tensor& t, int64_t d) { return t.size(d) == 1 ? 0 : t.stride(d); }   // a dim of one is never stepped over: its stride may be anything
 int64_t div_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
+// attention.py:_readable.  (contiguous() would hand back a dense tensor at an odd address as it is)
+Tensor readable_rows(const Tensor& t) {
+  const int64_t vec = 16 / t.element_size();
+  return t.stride(3) == 1 && aligned16(t) && stride_of(t, 0) % vec == 0 && stride_of(t, 1) % vec == 0 && stride_of(t, 2) % vec == 0 ? t : t.clone(at::MemoryFormat::Contiguous);
+}
 
 // (torch.jit.trace would record the outputs' allocation and none of the launches: the general functions end in an error there)
 bool being_traced() { return c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::Tracer); }
@@ -275,8 +280,7 @@ bool attend(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in, double s
   Tensor q = q_in, k = k_in, v = v_in;
   for (Tensor* t : {&q, &k, &v}) {
     if (!on_gpu(*t) || !is_float(*t) || t->dim() != 4 || t->scalar_type() != q_in.scalar_type()) return false;
-    const int64_t vec = t->scalar_type() == at::kBFloat16 ? 8 : 4;
-    if (t->stride(3) != 1 || !aligned16(*t) || stride_of(*t, 0) % vec != 0 || stride_of(*t, 1) % vec != 0 || stride_of(*t, 2) % vec != 0) *t = t->contiguous();
+    *t = readable_rows(*t);
   }
   const int64_t B = q.size(0), Hq = q.size(1), Sq = q.size(2), D = q.size(3), Hk = v.size(1), Sk = v.size(2), Dv = v.size(3);
   if (k.size(0) != v.size(0) || k.size(1) != Hk || k.size(2) != Sk || B != k.size(0) || k.size(3) != D) return false;
@@ -794,10 +798,7 @@ bool attention_gradients(Failure& f, const Tensor& go_in, const AttentionKept& x
   if (!on_current_device(x.lse) || x.lse.scalar_type() != at::kFloat || !is(x.lse, {B, Hq, Sq}) || x.cu_q.size() != x.cu_k.size() || x.cu_q.size() == 1) return false;
   for (const OptTensor* t : {&x.bias, &x.slopes})
     if (t->has_value() && (!on_current_device(**t) || (*t)->scalar_type() != at::kFloat)) return false;
-  auto readable = [](const Tensor& t) {
-    return t.stride(3) == 1 && aligned16(t) && stride_of(t, 0) % 8 == 0 && stride_of(t, 1) % 8 == 0 && stride_of(t, 2) % 8 == 0 ? t : t.contiguous();
-  };
-  const Tensor go = readable(go_in), out = readable(x.out);
+  const Tensor go = readable_rows(go_in), out = readable_rows(x.out);
   const auto opts = at::TensorOptions().dtype(at::kBFloat16).device(q.device());
   auto grad = [&](bool want, int64_t H, int64_t S, int64_t n) {
     if (!want) return Tensor();
@@ -883,10 +884,7 @@ struct AttentionOperands {
 struct AttentionNode : torch::autograd::Function<AttentionNode> {
   static variable_list forward(AutogradContext* ctx, const Tensor& q_in, const Tensor& k_in, const Tensor& v_in, const AttentionOperands& op) {
     const AttentionShape& x = op.shape;
-    Tensor q = q_in, k = k_in, v = v_in;
-    const int64_t vec = q.scalar_type() == at::kBFloat16 ? 8 : 4;
-    for (Tensor* t : {&q, &k, &v})
-      if (t->stride(3) != 1 || !aligned16(*t) || stride_of(*t, 0) % vec != 0 || stride_of(*t, 1) % vec != 0 || stride_of(*t, 2) % vec != 0) *t = t->contiguous();
+    const Tensor q = readable_rows(q_in), k = readable_rows(k_in), v = readable_rows(v_in);
     const int64_t out_rows = x.rows_outer ? x.Hq * x.Dv : x.Dv, out_heads = x.rows_outer ? x.Dv : x.Sq * x.Dv;
     const Tensor buf = Alloc(q).dense({x.start(6)});
     const Tensor out = at::empty_strided({x.B, x.Hq, x.Sq, x.Dv}, {x.Hq * x.Sq * x.Dv, out_heads, out_rows, 1}, buf.options().dtype(at::kBFloat16));

@@ -33,7 +33,7 @@ def _additive(bias: Optional[torch.Tensor], alibi_slopes: Optional[torch.Tensor]
         torch._check(b4.shape[-2] == Sq and b4.shape[-1] == Sk and b4.shape[0] in (1, B) and b4.shape[1] in (1, Hq),
                      lambda: f"bias of shape {tuple(bias.shape)} does not broadcast to {(B, Hq, Sq, Sk)}")
         if b4.stride(3) != 1 or b4.stride(2) % 4 or b4.stride(2) >= 1 << 24 or b4.data_ptr() % 16 or (b4.shape[0] > 1 and b4.stride(0) < 0) or (b4.shape[1] > 1 and b4.stride(1) < 0):
-            b4 = b4.contiguous()
+            b4 = b4.clone(memory_format=torch.contiguous_format)
     if alibi_slopes is not None:
         rt.require_gpu(alibi_slopes)
         sl = alibi_slopes.to(torch.float32)
@@ -182,10 +182,10 @@ def _strides(t: torch.Tensor) -> list:
 
 def _readable(t: torch.Tensor) -> torch.Tensor:
     """``t`` [B, H, S, D] as the operand quantizer reads it: any strides of the first three dims in whole 16-byte units, unit
-    stride along D.  Anything else is copied."""
+    stride along D.  Anything else is copied (``contiguous`` would hand back a dense tensor at an odd address as it is)."""
     vec = 8 if t.dtype == torch.bfloat16 else 4
     ok = t.stride(3) == 1 and t.data_ptr() % 16 == 0 and all(s % vec == 0 for s in _strides(t))
-    return t if ok else t.contiguous()
+    return t if ok else t.clone(memory_format=torch.contiguous_format)
 
 
 def quantize_qkv(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor):
