@@ -786,6 +786,9 @@ struct AttentionKept {
 // attention.py:_gradients -> {dq, dk, dv} (undefined: not wanted), or false: declined
 bool attention_gradients(Failure& f, const Tensor& go_in, const AttentionKept& x, bool want_q, bool want_kv, variable_list& grads) {
   const Tensor &q = x.q, &k = x.k, &v = x.v;
+  if (!node_serves(go_in, x.out) || x.lse._fw_grad(0).defined()) return false;
+  for (const OptTensor* t : {&x.bias, &x.slopes})
+    if (t->has_value() && (*t)->_fw_grad(0).defined()) return false;
   for (const Tensor* t : {&q, &x.q_scale, &k, &x.k_scale, &v, &x.v_scale})
     if (!on_current_device(*t) || t->scalar_type() != at::kByte || t->dim() != 4 || !t->is_contiguous()) return false;
   for (const Tensor* t : {&go_in, &x.out})

@@ -5,7 +5,7 @@ import os
 from typing import Callable, Optional
 
 import torch
-from torch.autograd.forward_ad import unpack_dual
+from torch.autograd import forward_ad
 
 from .. import _lib
 
@@ -38,7 +38,7 @@ def refuse_transforms(what: str, *tensors: Optional[torch.Tensor]) -> None:
         raise NotImplementedError(f"{what} under torch.jit.trace: none of its launches would be recorded")
     if torch._C._are_functorch_transforms_active():
         raise NotImplementedError(f"{what} under a functorch transform is not implemented")
-    if any(t is not None and unpack_dual(t).tangent is not None for t in tensors):
+    if getattr(forward_ad, "_current_level", 0) >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
         raise NotImplementedError(f"{what}: forward-mode derivatives are not implemented")
 
 

@@ -104,6 +104,7 @@ def _gradients(grad_out, operands, out, lse, sm_scale, causal, seqlen_k, b4, sl,
                                            want_q, want_kv)
     if native is not None:
         return native
+    rt.refuse_transforms("attention_mxfp4_backward", grad_out, out, lse, b4, sl)
     (B, Hq, Sq), (Hk, Sk), D, Dv = q.shape[:3], k.shape[1:3], 2 * q.shape[3], v.shape[2]
 
     def empty(want, heads, rows, columns):
@@ -155,7 +156,6 @@ def attention_mxfp4_backward(grad_out: torch.Tensor, q: torch.Tensor, k: torch.T
     ``cu_seqlens_q`` / ``cu_seqlens_k``: boundaries (multiples of 32, both or neither) of sequences packed along the tokens, with B = 1 and no bias.
     Equal inputs give equal bits.
     """
-    rt.refuse_transforms("attention_mxfp4_backward", grad_out, out, lse, bias, alibi_slopes)
     rt.require_gpu(grad_out, q, k, v, q_scale, k_scale, v_scale, out, lse)
     for t in (q, k, v, q_scale, k_scale, v_scale):
         assert t.is_contiguous() and t.dtype == torch.uint8

@@ -136,16 +136,18 @@ def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], inv_freq: torch.Ten
     (i, i + R/2), or (2i, 2i + 1) with ``interleaved``, the others pass.  ``positions``: int32 or int64 [S] or [B, S] ([T] with ``"thd"``) of any
     sign, None for 0, 1, ...  ``factor`` multiplies cosines and sines.  Angles, cosines and sines are taken in 64 bits.
     """
-    return (_apply_between_graphs if torch.compiler.is_compiling() else _apply)(q, k, inv_freq, positions, interleaved, factor, layout)
+    if torch.compiler.is_compiling():
+        return _apply_between_graphs(q, k, inv_freq, positions, interleaved, factor, layout)
+    if k is not None and q.is_cuda and layout in _NATIVE:   # one native call; what it declines takes the general way
+        out = rt.host().rotary(q, k, inv_freq, positions, bool(interleaved), float(factor), _NATIVE[layout])
+        if out is not None:
+            return out
+    return _apply(q, k, inv_freq, positions, interleaved, factor, layout)
 
 
 def _apply(q, k, inv_freq, positions, interleaved, factor, layout):
     if layout not in _DIMS:
         raise NotImplementedError(f"layout {layout!r}: 'bhsd', 'bshd' and 'thd' are implemented")
-    if k is not None and q.is_cuda:   # one native call; what it declines goes on here
-        out = rt.host().rotary(q, k, inv_freq, positions, bool(interleaved), float(factor), _NATIVE[layout])
-        if out is not None:
-            return out
     rt.refuse_transforms("apply_rotary", q, k, inv_freq)
     rt.require_gpu(q, k, inv_freq, positions)
     dims = 3 if layout == "thd" else 4
@@ -170,4 +172,8 @@ def _apply(q, k, inv_freq, positions, interleaved, factor, layout):
     return tuple(out) if k is not None else out[0]
 
 
-_apply_between_graphs = torch.compiler.disable(_apply)   # (nothing of it can be traced: a compiled caller breaks its graph here and runs the same call)
+@torch.compiler.disable
+def _apply_between_graphs(q, k, inv_freq, positions, interleaved, factor, layout):
+    """(nothing of the call can be traced: a compiled caller breaks its graph here)"""
+    out = rt.host().rotary(q, k, inv_freq, positions, bool(interleaved), float(factor), _NATIVE[layout]) if k is not None and q.is_cuda and layout in _NATIVE else None
+    return out if out is not None else _apply(q, k, inv_freq, positions, interleaved, factor, layout)

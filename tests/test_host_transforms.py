@@ -10,17 +10,25 @@ from alto_amd.mxfp4 import rotary as R
 FREQ = torch.ones(16, dtype=torch.float64)
 
 
+def declined(*tensors):
+    """(what the native calls leave to the general ones)"""
+    return torch.jit.is_tracing() or torch._C._are_functorch_transforms_active() or any(t is not None and unpack_dual(t).tangent is not None for t in tensors)
+
+
 class Host:
     """Native calls that leave a trace of their operands: the attention's output is Q's first rows, its gradients are 2, 3 and 4."""
 
     def attend(self, q, k, v, sm_scale, causal, out, lse, *more):
-        if torch.jit.is_tracing() or torch._C._are_functorch_transforms_active() or any(unpack_dual(t).tangent is not None for t in (q, k, v)):
-            return False   # (as the native call does)
+        if declined(q, k, v):
+            return False
         out.copy_(q[..., :out.shape[-1]])
         lse.zero_()
         return True
 
     def attention_gradients(self, go, q, qs, k, ks, v, vs, out, lse, sm_scale, causal, keys, bias, slopes, cu_q, cu_k, rows_outer, want_q, want_kv):
+        if declined(go, out, lse, bias, slopes):
+            return None
+
         def full(value, heads, rows, columns):
             return torch.full((q.shape[0], rows, heads, columns), value, dtype=torch.bfloat16).transpose(1, 2)
 
