@@ -338,7 +338,8 @@ struct BiasBlock {
 };
 
 // A probability.  None is above 1; where the bias is so large that lse has no bits left for the scores, a rounding could say so.  NaN stays NaN
-// (v_minimum3_f32; v_med3_f32 would make 0 of it, and a NaN of the bias or of lse would not be seen in dV).
+// (v_minimum3_f32: 72 us for 3 x 8 heads, 480 rows, 1056 keys of 192 / 128; the clamp that v_exp_f32 has for nothing, 70 us, makes 0 of it, and dV would
+// not see a NaN of the bias or of lse).
 template <int ADD>
 __device__ __forceinline__ float probability_of(float x, std::integral_constant<int, ADD>) {
   const float p = __builtin_amdgcn_exp2f(x);
@@ -948,10 +949,10 @@ __device__ __forceinline__ void attn_bwd_rows_body(const AttnBwdArgs& a, const A
 
 // All three gradients in one launch, so that the workgroups of dQ fill the units while the last ones of dK and dV end.
 //
-// What bounds it with D = 128 is the board's power.  4 x 2048 tokens, 64 / 8 heads, causal: 730 to 800 us for 687 GFLOP (five products over the pairs that
-// the mask leaves), 0.9 PFLOP/s; it issues 44 products of 32 cycles for every 32 x 32 scores of either side (26 for dK and dV, 18 for dQ, four of them on
-// codes), matrix pipes busy 61 % of the cycles, vector pipes 45 %, some instruction issued in 89 %, at a clock of 1.7 GHz that is 2.1 when fewer products are
-// busy.  So it is not only the waits that count but what a step spends: K's, V's and Q's tiles are read as codes or once for four waves, nothing is spilled.  With D = 64 the
+// 4 x 2048 tokens of 128, 64 / 8 heads, causal: 730 to 800 us for 687 GFLOP (five products over the pairs that the mask leaves), 0.9 PFLOP/s; it issues 44
+// products of 32 cycles for every 32 x 32 scores of either side (26 for dK and dV, 18 for dQ, four of them on codes), matrix pipes busy 61 % of the cycles,
+// vector pipes 45 %, some instruction issued in 89 %, at a clock of 1.7 GHz that is 2.1 when fewer products are busy: the clock and the waits bound it
+// together, which of them more has not been told apart.  K's, V's and Q's tiles are read as codes or once for four waves, nothing is spilled.  With D = 64 the
 // issue of instructions is the bound (99 % of the cycles), with D > 128 one wave a SIMD waits for itself (54 %).
 template <int NK, int NV, int ADD>
 __global__ __launch_bounds__(64 * BWD_WAVES, NK > 2 ? 1 : 2) void attn_bwd_kernel(AttnBwdArgs a, AttnBwdSeqs seqs, AttnBwdPlan plan) {

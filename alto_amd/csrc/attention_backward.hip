@@ -3,10 +3,12 @@
 // With S_ij = sm_scale Q_i . K_j + bias_ij - slope |i + Sk - Sq - j| on the values that the codes stand for, and the forward's log-sum-exp:
 //   P_ij = exp(S_ij - lse_i)   (0 where the mask hides j, and in a row that sees no key),   D_i = dO_i . O_i,
 //   dV_j = sum_i P_ij dO_i,   dS_ij = P_ij (dO_i . V_j - D_i),   dQ_i = sm_scale sum_j dS_ij K_j,   dK_j = sm_scale sum_i dS_ij Q_i.
-// The roundings of Q, K, V and P to FP4 are passed straight through.  The scores are recomputed on the FP4 pipe from the forward's codes;
+// The roundings of Q, K, V and P to FP4 are passed straight through; lse and O are the forward's, which sums quantized probabilities: P sums to one
+// and D is the mean of dO . V only up to their rounding.  The scores are recomputed on the FP4 pipe from the forward's codes;
 // the other products have a factor that is not on the FP4 grid (P, dS, dO) and run in bf16, in which the codes' values are exact.  P and
-// dS are rounded to bf16 as factors (half a step, 2^-8 of a value at most, independent from element to element: the sums have at most the
-// relative error of one rounding of their terms); scores, probabilities, dS before that, D and all sums are fp32.
+// dS are rounded to bf16 as factors: half a step, 2^-8 of a value at most, so that a sum is off by at most 2^-8 of the sum of its terms' magnitudes
+// (of the sum itself, which may cancel, by more; all gradients together by 2.4e-3 of their size, their own rounding alone 1.7e-3).  Scores,
+// probabilities, dS before that, D and all sums are fp32.
 //
 // Two launches, or three.  This file's preparation reads every operand once and writes what the main kernel's many workgroups read over and
 // over in the order in which they read it: D and lse, the scale bytes, and tiles of K's and V's values and of dO in bf16.  (A copy of dO costs 2
@@ -162,8 +164,9 @@ Cuts cut(const alto_mxfp4_attention_bwd_t& p) {
   } else {
     count_tiles(keys, rows, p.Sq, p.Sk_used, p.causal);
   }
-  // Counted in tiles of dK and dV; one of dQ takes about .62 of one (products: 18 to 26 with D = Dv = 128).  The compute units hold 512 workgroups, and a
-  // list much longer than an equal share of the whole ends alone.  Pieces have 1.05 of that share (1.17 and 0.85: 3 % and 1.5 % more over 13 shapes) and
+  // Counted in tiles of dK and dV; one of dQ takes about .62 of one (products: 18 to 26 with D = Dv = 128).  The compute units hold 512 workgroups up to
+  // D = 128 (above, 256; a share of 256 there was faster for one sequence of 192 / 64 on a few key heads, 238 -> 175 us, and slower for packed ones of 192,
+  // 95 -> 117: 512 for all), and a list much longer than an equal share of the whole ends alone.  Pieces have 1.05 of that share (1.17 and 0.85: 3 % and 1.5 % more over 13 shapes) and
   // 24 tiles at least (16 and 32: 80.9 and 73.6 us for 72.2, 6 packed sequences of 16 / 4 heads of 128).  Parts cost a kernel, 5 tiles' time, and their
   // sums' way through memory.  So whichever of the two kinds is cut by what the launch would take: both, where few rows or heads leave all but some
   // units idle (3 x 6 / 3 heads, 64 rows, 4736 keys of 128 / 64: 32 us, 84 whole; 2048 tokens of 128, 4 heads 45, 57 whole), neither at 2048 tokens of

@@ -1,12 +1,13 @@
-"""MXFP4 flash-attention forward, named as in ``alto/kernels/fp4/mxfp4/triton_flash_attention_mxfp4.py``.
+"""MXFP4 flash attention, named as in ``alto/kernels/fp4/mxfp4/triton_flash_attention_mxfp4.py``, and its gradients.
 
 ``triton_attention_mxfp4`` keeps the reference's name and argument list (:1206-1239) so that
 ``alto/kernels/dispatch/attention.py:22`` can point at it; here it quantises K and V with one launch (2D blocks along the
 head dim, :1105-1107; V packed along the keys), read in the layout they come in, and runs one HIP kernel, which quantises
-a bf16 Q itself (an fp32 one goes through that launch as well).
+a bf16 Q itself (an fp32 one goes through that launch as well, and so does any whose codes are kept for a backward).
 The reference has no backward (:1143-1145); here Q, K and V that require a gradient get one: ``attention_mxfp4_backward`` recomputes the
-probabilities from the quantized operands, which is all that is kept of them (half a byte an element).  Options outside the path ALTO's dispatch layer uses
-(``alto/kernels/dispatch/attention.py:61-77``: layout "bhsd", no bias, no alibi, no dropout, fixed lengths) raise.
+probabilities from the quantized operands, which is all that is kept of them (half a byte an element).  Dropout, ``return_scores``, a bias with
+layout "thd", gradients of a bias or of slopes, ``torch.jit.trace``, functorch transforms and forward-mode tangents raise; a caller
+under ``torch.compile`` breaks its graph here.
 """
 from __future__ import annotations
 
@@ -152,7 +153,10 @@ def attention_mxfp4_backward(grad_out: torch.Tensor, q: torch.Tensor, k: torch.T
 
         P = exp(S - lse),  dV = P^T dO,  dS = P * (dO V^T - rowsum(dO * O)),  dQ = sm_scale dS K,  dK = sm_scale dS^T Q
 
-    Rows that see no key (``lse`` = -inf) give nothing to any gradient; keys from ``seqlen_k`` on get zeros.  ``bias`` and ``alibi_slopes`` get no gradient.
+    ``out`` and ``lse`` come from quantized probabilities, so the rows of dS sum to zero only up to their rounding.
+    Rows that see no key (``lse`` = -inf) give nothing to any gradient, nor do rows whose keys all carry the type's lowest value; keys from ``seqlen_k`` on
+    get zeros.  A finite bias of -M on all keys of a row leaves ``lse`` without the bits of its scores (M 2^-24): its probabilities are then at most one and
+    otherwise unspecified.  NaN in a bias or in ``lse`` stays NaN.  ``bias`` and ``alibi_slopes`` get no gradient.
     ``cu_seqlens_q`` / ``cu_seqlens_k``: boundaries (multiples of 32, both or neither) of sequences packed along the tokens, with B = 1 and no bias.
     Equal inputs give equal bits.
     """

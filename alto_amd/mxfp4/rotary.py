@@ -34,7 +34,9 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional
     * ``"ntk"``: the base becomes ``base * f ** (rotary_dim / (rotary_dim - 2))``: the highest frequency stays, the lowest is divided by f.
     * ``"yarn"``: a pair that turns ``"beta_fast"`` (32) times or more over ``"original_length"`` positions keeps its frequency, one that turns
       ``"beta_slow"`` (1) times or less has it divided by f, and between them the two are blended linearly in the turns; cosines and
-      sines are multiplied with ``0.1 ln f + 1`` (or ``"attention_factor"``).
+      sines are multiplied with ``0.1 ln f + 1`` (or ``"attention_factor"``).  (The blend is linear in the turns, as the method's formula has it.  Models
+      trained with a ramp over the pairs' numbers, between the two pairs with those turns, have other frequencies in between: give theirs to
+      :func:`apply_rotary` as they are.)
     * ``"wavelength"``: the same blend between ``"high"`` (4) and ``"low"`` (1) wavelengths in ``"original_length"``, factor 1.
     """
     if rotary_dim <= 0 or rotary_dim % 2:
@@ -132,7 +134,7 @@ def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], inv_freq: torch.Ten
     """``q`` and ``k`` with their heads rotated by their tokens' positions, as new tensors (``k`` None: only ``q``); differentiable.
 
     bf16 or fp32, [B, H, S, D], [B, S, H, D] with ``layout="bshd"`` or [T, H, D] with ``"thd"``, of any strides.  ``inv_freq`` (fp64, on their device,
-    :func:`rotary_frequencies`): radians a position of each pair; twice as many columns, from the first on, are rotated in the pairs
+    :func:`rotary_frequencies`, or a model's own in fp64): radians a position of each pair; twice as many columns, from the first on, are rotated in the pairs
     (i, i + R/2), or (2i, 2i + 1) with ``interleaved``, the others pass.  ``positions``: int32 or int64 [S] or [B, S] ([T] with ``"thd"``) of any
     sign, None for 0, 1, ...  ``factor`` multiplies cosines and sines.  Angles, cosines and sines are taken in 64 bits.
     """

@@ -534,8 +534,8 @@ int alto_mxfp4_attention_rows_per_workgroup(int64_t B, int64_t Hq, int64_t Sq, i
 /*
  * Gradients of the attention forward with respect to Q, K and V, recomputing the probabilities: with the codes' values,
  *   P = exp(S - lse),  dV = P^T dO,  dS = P * (dO V^T - rowsum(dO * O)),  dQ = sm_scale dS K,  dK = sm_scale dS^T Q,
- * S and its additive terms as in alto_mxfp4_attention_fwd_ex, lse and out as that forward left them; the roundings of Q, K, V and P to
- * MXFP4 are passed straight through.  (The reference's attention has no backward, triton_flash_attention_mxfp4.py:1143-1145.)
+ * S and its additive terms as in alto_mxfp4_attention_fwd_ex, lse and out as that forward left them (of quantized probabilities: the rows of
+ * dS sum to zero up to their rounding); the roundings of Q, K, V and P to MXFP4 are passed straight through.  (The reference's attention has no backward, triton_flash_attention_mxfp4.py:1143-1145.)
  * Codes and scales dense, as alto_mxfp4_attention_fwd takes them (Sq and Sk any multiples of 32, nothing is read behind them).  dout, out and
  * the gradients are bf16 with element strides of batch, head and row (multiples of 8), unit stride along the head dim, 16-byte
  * aligned.  sm_scale is positive, with a bias or slopes at least 2^-64; rows of the bias are less than 2^24 elements apart.  Keys from Sk_used on get zero gradients
