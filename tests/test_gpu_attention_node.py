@@ -162,3 +162,41 @@ def test_checkpointed(m, no_python_function):
     y.backward(tensors[3])
     for a, b in zip(x, want[2]):
         assert torch.equal(a.grad, b)
+
+
+@pytest.mark.parametrize("needed", [(True, False, False), (False, True, False), (False, False, True)])
+def test_a_second_derivative_of_some_of_the_gradients_is_an_error(m, no_python_function, needed):
+    q, k, v, go = leaves(1, 2, 2, 32, 32, 64, 64)
+    x = [t.requires_grad_(n) for t, n in zip((q, k, v), needed)]
+    u = go.clone().requires_grad_(True)
+    (grad,) = torch.autograd.grad(m.triton_attention_mxfp4(*x, causal=True)[0], [t for t in x if t.requires_grad], u, create_graph=True)
+    assert grad.requires_grad
+    with pytest.raises(RuntimeError, match="not differentiable"):
+        grad.float().sum().backward()
+
+
+def test_two_streams(m, no_python_function):
+    """Steps in flight on two streams, each with the bits that it has alone."""
+    both = [leaves(1, 8, 2, 256, 256, 128, 128, seed=s) for s in (1, 2)]
+    want = [step(m, "bshd", t, (True, True, True)) for t in both]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], []
+    for _ in range(3):
+        for t, s in zip(both, streams):
+            with torch.cuda.stream(s):
+                got.append(step(m, "bshd", t, (True, True, True)))
+    torch.cuda.synchronize()
+    for i, g in enumerate(got):
+        assert torch.equal(g[0], want[i % 2][0]) and all(torch.equal(a, b) for a, b in zip(g[2], want[i % 2][2]))
+
+
+@pytest.mark.parametrize("q_is_k", [True, False])
+def test_one_tensor_for_two_operands(m, no_python_function, q_is_k):
+    """The same leaf as Q and K, or as K and V: its gradient is the sum of theirs."""
+    q, k, v, go = leaves(1, 2, 2, 64, 64, 64, 64)
+    a = q.clone().requires_grad_(True)
+    y = m.triton_attention_mxfp4(a, a, v, causal=True)[0] if q_is_k else m.triton_attention_mxfp4(k, a, a, causal=True)[0]
+    (got,) = torch.autograd.grad(y, a, go)
+    x = [t.clone().requires_grad_(True) for t in ((q, q, v) if q_is_k else (k, q, q))]
+    grads = torch.autograd.grad(m.triton_attention_mxfp4(*x, causal=True)[0], x, go)
+    assert torch.equal(got, grads[0] + grads[1] if q_is_k else grads[1] + grads[2])
