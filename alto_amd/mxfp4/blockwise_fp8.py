@@ -417,6 +417,14 @@ def _quantized_weight(owner: torch.Tensor, w: torch.Tensor, want_transposed: boo
     return cached_weight_quantisation(owner, ("blockwise_fp8", tuple(w.shape), tuple(w.stride())), make)
 
 
+def _check_reductions(want_dx: bool, want_dw: bool, N: int, M: int, groups: int = 0) -> None:
+    """What only a backward's products would refuse, ahead of the forward: their reductions run over the columns of y and over its rows (each group's in whole blocks)."""
+    assert not want_dx or N <= _LONGEST, f"{N} columns: an input's gradient sums over {_LONGEST} at most"
+    if want_dw and groups:
+        assert M + 127 * (groups + 2) < 2 ** 22, f"{M} rows in {groups} groups: weight gradients by group take 2^22 - 1 - 127 (groups + 2) at most"
+    assert not want_dw or M <= _LONGEST, f"{M} rows: a weight's gradient sums over {_LONGEST} at most"
+
+
 class BlockwiseFP8LinearFunction(torch.autograd.Function):
     """y = x W^T, dX = dY W and dW = dY^T X, each on operands quantized along its reduction; x [M, K], W [N, K]."""
 
@@ -424,6 +432,7 @@ class BlockwiseFP8LinearFunction(torch.autograd.Function):
     def forward(ctx, x, weight, grad_dtype, training):
         w = unwrap_weight_wrapper(weight)
         want_dx, want_dw = (training and n for n in ctx.needs_input_grad[:2])   # (those say what requires gradients under no_grad as well)
+        _check_reductions(want_dx and x.numel() > 0, want_dw and w.numel() > 0, w.shape[0], x.shape[0])
         xq, xs, xt, xts = _copies(x, True, want_dw, False, torch.float8_e4m3fn)
         wq, ws, wt = _quantized_weight(weight, w, want_dx)
         ctx.save_for_backward(xt, xts, wt if want_dx else None, ws if want_dx else None)
@@ -455,8 +464,8 @@ def blockwise_fp8_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[t
     """``x @ weight.T (+ bias)`` with 8-bit operands in all three products of a training step; x [..., K], weight [N, K], bf16 or fp32, of any sizes.
 
     x and the gradient are quantized in blocks of 1 x 128 along each product's reduction (the gradient to ``grad_dtype``, E4M3 or E5M2), the weight in blocks
-    of 128 x 128.  The result has x's type (with a bias of another, what torch's sum of them has), each gradient its tensor's.  Without a graph to build only the forward product's operands are made.  A training step takes
-    at most 2^22 - 16 rows and columns.
+    of 128 x 128.  The result has x's type (with a bias of another, what torch's sum of them has), each gradient its tensor's.  Without a graph to build only the forward product's operands are made.  Each
+    product's reduction is at most 2^22 - 16 long: K, N where x requires a gradient, and x's rows where the weight does.
     """
     if torch.compiler.is_compiling():
         return _between_graphs(_linear, x, weight, bias, grad_dtype)
@@ -479,6 +488,7 @@ class BlockwiseFP8GroupedFunction(torch.autograd.Function):
         w = unwrap_weight_wrapper(weight)
         w = w if trans_weights else w.transpose(1, 2)
         want_dx, want_dw = (training and n for n in ctx.needs_input_grad[:2])
+        _check_reductions(want_dx and x.numel() > 0, want_dw and w.numel() > 0, w.shape[1], x.shape[0], w.shape[0])
         xq, xs, xt, xts = _copies(x, True, want_dw, False, torch.float8_e4m3fn, offsets if want_dw else None)
         wq, ws, wt = _quantized_weight(weight, w, want_dx)
         ctx.save_for_backward(xt, xts, wt if want_dx else None, ws if want_dx else None, offsets)
@@ -508,7 +518,7 @@ def blockwise_fp8_grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets:
     ``offsets[e] <= m < offsets[e + 1]`` meet weight[e].
 
     ``offsets``: int32 [E + 1] on the device, non-decreasing, at most M; groups of any size, E at most 65535.  Rows of no expert, and their gradients, are zero.  The blocks of the weight
-    gradients' operands start anew with each group.
+    gradients' operands start anew with each group: where the weight requires a gradient, M + 127 (E + 2) is below 2^22.
     """
     if torch.compiler.is_compiling():
         return _between_graphs(_grouped_linear, x, weight, offsets, grad_dtype, trans_weights)
