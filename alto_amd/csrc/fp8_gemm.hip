@@ -57,11 +57,14 @@ __global__ __launch_bounds__(W::THREADS, 2) void fp8_gemm_kernel(const Fp8GemmAr
 // 155.5 -> 133.2).  Of 9 to 16 tiles, two such rounds, nothing is gained: 6400 x 6400 x 2048 89.5 -> 91.6.
 int whole_tiles(int per_xcd) { return per_xcd > 32 && per_xcd % 32 <= 8 ? per_xcd / 32 * 32 : per_xcd; }
 
+template <class W>
+bool fits(int64_t M, int64_t N) { return product_below(FP8_MOST_TILES<W>, (M + W::TM - 1) / W::TM, (N + W::TN - 1) / W::TN); }
+
 template <class W, int CODE_A, bool B1D, typename OutT>
 int launch(Fp8GemmArgs& a, hipStream_t st) {
+  ALTO_REQUIRE(fits<W>(a.M, a.N), "fp8_gemm: too many tiles for one launch");
   a.tiles_m = (int)((a.M + W::TM - 1) / W::TM);
   a.tiles_n = (int)((a.N + W::TN - 1) / W::TN);
-  ALTO_REQUIRE(product_below(1ll << 22, a.tiles_m, a.tiles_n), "fp8_gemm: too many tiles for one launch");   // (its threads are counted in 32 bits)
   static LdsLimit limit;
   const int rc = limit.raise(reinterpret_cast<const void*>(&fp8_gemm_kernel<W, CODE_A, B1D, OutT>), W::LDS, "fp8_gemm");
   if (rc != ALTO_MXFP4_OK) return rc;
@@ -132,7 +135,8 @@ static int fp8_gemm(const alto_mxfp4_fp8_gemm_t& p, hipStream_t st) {
   const double of_large = (double)((whole + 31) / 32) * (7.5 + kb * (1.2 + 0.25 * share)) + (per_xcd == whole ? 0.0 : 4.0 + 0.575 * kb);
   const double rest = (double)(small % 512) / 512, rounds = (double)(small / 512) + (rest > 0.0 && rest < 0.55 ? 0.55 : rest);
   const double of_small = small <= 512 ? 7.0 + kb * (small > 458 ? 0.95 * (double)small / 512 : 0.85) : 3.0 + rounds * (2.5 + 1.11 * kb);
-  if (of_large <= of_small) return p.a_code == ALTO_FP8_E4M3 ? launch_types<Large, ALTO_FP8_E4M3>(a, b1d, f32, st) : launch_types<Large, ALTO_FP8_E5M2>(a, b1d, f32, st);
+  // (more of the second than one launch takes are no choice)
+  if (of_large <= of_small || !fits<Small>(p.M, p.N)) return p.a_code == ALTO_FP8_E4M3 ? launch_types<Large, ALTO_FP8_E4M3>(a, b1d, f32, st) : launch_types<Large, ALTO_FP8_E5M2>(a, b1d, f32, st);
   if (small <= 256) {
     // Few tiles: 128 x 128 with K in halves, 64 x 64 with K in quarters, or the kernel for few rows, by what each was measured to take (us; within 20 % over 1 to 768 rows, N
     // and K from 512 to 14336).  The first: 4, and 0.9 to 1.15 for each 256 of K.  The second: 3.2 and 1.06 for each 512 of K and 256 tiles, and no less than 3 and the operands at

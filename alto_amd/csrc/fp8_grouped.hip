@@ -46,11 +46,14 @@ __global__ __launch_bounds__(W::THREADS, 2) void fp8_grouped_kernel(const Fp8Gro
   fp8_tile_product<W, CODE_A, B1D>(t, reinterpret_cast<OutT*>(p.c) + seg.lo * p.ldc + n0, p.ldc, p.vec, smem);
 }
 
+template <class W>
+bool fits(const Fp8GroupedArgs& a) { return product_below(FP8_MOST_TILES<W>, used_pieces(a, W::TM), (a.N + W::TN - 1) / W::TN); }
+
 template <class W, int CODE_A, bool B1D, typename OutT>
 int launch(Fp8GroupedArgs& a, hipStream_t st) {
+  ALTO_REQUIRE(fits<W>(a), "fp8_grouped_gemm: too many tiles for one launch");
   const int64_t tiles_m = used_pieces(a, W::TM);
   a.tiles_n = (int)((a.N + W::TN - 1) / W::TN);
-  ALTO_REQUIRE(product_below(1ll << 22, tiles_m, a.tiles_n), "fp8_grouped_gemm: too many tiles for one launch");   // (its threads are counted in 32 bits)
   static LdsLimit limit;
   const int rc = limit.raise(reinterpret_cast<const void*>(&fp8_grouped_kernel<W, CODE_A, B1D, OutT>), W::LDS, "fp8_grouped_gemm");
   if (rc != ALTO_MXFP4_OK) return rc;
@@ -119,7 +122,7 @@ template <class W, int CODE_A, typename OutT>
 int launch_weights(Fp8WeightsArgs& a, hipStream_t st) {
   a.tiles_n = (int)((a.N + W::TM - 1) / W::TM);
   a.tiles_k = (int)((a.K + W::TN - 1) / W::TN);
-  ALTO_REQUIRE(product_below(1ll << 22, a.tiles_n, a.tiles_k), "fp8_grouped_gemm_weights: too many tiles for one launch");   // (its threads are counted in 32 bits)
+  ALTO_REQUIRE(product_below(FP8_MOST_TILES<W>, a.tiles_n, a.tiles_k), "fp8_grouped_gemm_weights: too many tiles for one launch");
   static LdsLimit limit;
   const int rc = limit.raise(reinterpret_cast<const void*>(&fp8_grouped_weights_kernel<W, CODE_A, OutT>), W::LDS, "fp8_grouped_gemm_weights");
   if (rc != ALTO_MXFP4_OK) return rc;
@@ -157,8 +160,10 @@ static int fp8_grouped_gemm(const alto_mxfp4_fp8_grouped_gemm_t& p, hipStream_t 
   // Few rows a group: 16 rows at a time, K split over the waves, the longer K is the more rows (16 rows, 128 x 128, us: 32 experts of 5760 x 2880, 64 rows 98.8, 102.4, 96 rows
   // 111, 106; of 2880 x 5760, 128 rows 108.6, 120.4, 256 rows 125, 120.5; 64 of 512 x 2048, 64 rows 11.5, 18.2; 8 of 4096 x 1024, 8 rows 9.9, 9.1).
   if (p.M * 1024 < (int64_t)p.groups * (p.K < 8192 ? p.K : 8192) && product_below(1ll << 23, used_pieces(a, 16), (p.N + 31) / 32)) return p.a_code == ALTO_FP8_E4M3 ? launch_rows_types<1, 2, ALTO_FP8_E4M3>(a, b1d, f32, st) : launch_rows_types<1, 2, ALTO_FP8_E5M2>(a, b1d, f32, st);
-  // (256 x 256, 128 x 128, us: 32 experts of 5760 x 2880, 4096 rows 183, 163, 8192 rows 232, 232, 16384 rows 341, 396; 8 of 4096 x 1024, 1024 rows 18.0, 13.5, 2048 rows 18.7, 22.0)
-  if (p.M >= 256ll * p.groups && p.N > 128) return p.a_code == ALTO_FP8_E4M3 ? launch_types<Large, ALTO_FP8_E4M3>(a, b1d, f32, st) : launch_types<Large, ALTO_FP8_E5M2>(a, b1d, f32, st);
+  // (256 x 256, 128 x 128, us: 32 experts of 5760 x 2880, 4096 rows 183, 163, 8192 rows 232, 232, 16384 rows 341, 396; 8 of 4096 x 1024, 1024 rows 18.0, 13.5, 2048 rows 18.7, 22.0;
+  // more of either than one launch takes are no choice)
+  const bool large = p.M >= 256ll * p.groups && p.N > 128 ? fits<Large>(a) || !fits<Small>(a) : !fits<Small>(a);
+  if (large) return p.a_code == ALTO_FP8_E4M3 ? launch_types<Large, ALTO_FP8_E4M3>(a, b1d, f32, st) : launch_types<Large, ALTO_FP8_E5M2>(a, b1d, f32, st);
   return p.a_code == ALTO_FP8_E4M3 ? launch_types<Small, ALTO_FP8_E4M3>(a, b1d, f32, st) : launch_types<Small, ALTO_FP8_E5M2>(a, b1d, f32, st);
 }
 

@@ -43,6 +43,10 @@ struct Fp8Tile {
   static_assert(LOADS_A * 8 * WAVES == TM && LOADS * 8 * WAVES == TM + TN && TM % 64 == 0 && TN % 64 == 0 && (KS - 1) * TM * TN * 4 <= LDS, "");
 };
 
+// Tiles that one launch takes: its threads are counted in 32 bits (512 workgroups are left for what whole parts for each XCD and tiles in quarters add).
+template <class W>
+constexpr int64_t FP8_MOST_TILES = (1ll << 32) / W::THREADS - 512;
+
 struct Fp8Operand {
   const uint8_t* codes;   // of the tile's first row, at the reduction's first element
   const float* scales;    // its first row's (or block of rows'), first block
