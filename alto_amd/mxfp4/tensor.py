@@ -153,30 +153,39 @@ class MXFP4TrainingWeightWrapperTensor(TrainingWeightWrapperBaseTensor):
             return func(*args, **kwargs)
 
 
+_PARAMETERS = {"linear": ("input", "weight", "bias"), "mm": ("input", "mat2"), "matmul": ("input", "other"), "addmm": ("input", "mat1", "mat2"),
+               "_grouped_mm": ("input", "mat2", "offs", "bias", "out_dtype")}
+
+
 class BlockwiseFP8TrainingWeightWrapperTensor(TrainingWeightWrapperBaseTensor):
-    """Routes ``_grouped_mm`` and the linear-like ops on a wrapped weight to :func:`blockwise_fp8_grouped_linear` and :func:`blockwise_fp8_linear`."""
+    """Routes ``_grouped_mm`` and the linear-like ops on a wrapped weight to :func:`blockwise_fp8_grouped_linear` and :func:`blockwise_fp8_linear`.
+
+    Results have the first operand's type: another ``out_dtype`` is refused, and so are ``out`` and factors other than 1 of ``addmm``."""
 
     @classmethod
     def __torch_function__(cls, func, types, args=(), kwargs=None):
         kwargs = kwargs or {}
         name = getattr(func, "__name__", "")
-        if name == "_grouped_mm":
-            A, B, offs = args[0], args[1], kwargs.get("offs", None)
-            assert not isinstance(A, cls) and isinstance(B, cls), f"the second operand, and it alone, should be a {cls.__name__}"
+        if name != "_grouped_mm" and name not in gemm_ops:
+            with torch._C.DisableTorchFunctionSubclass():
+                return func(*args, **kwargs)
+        op = name.removesuffix(".default")
+        parameters = _PARAMETERS[op]
+        assert len(args) <= len(parameters), f"{op}: arguments {parameters} are supported by position"
+        given = dict(zip(parameters, args), **{"input" if k == "self" else k: v for k, v in kwargs.items()})   # (aten's name for it)
+        A, B = (given.pop(p, None) for p in (parameters[1:3] if op == "addmm" else parameters[:2]))
+        assert isinstance(A, torch.Tensor) and not isinstance(A, cls) and isinstance(B, cls), f"the second operand of {op}, and it alone, should be a {cls.__name__}"
+        bias, offs, out_dtype = given.pop("input" if op == "addmm" else "bias", None), given.pop("offs", None), given.pop("out_dtype", None)
+        assert out_dtype is None or out_dtype == A.dtype, f"out_dtype {out_dtype} of operands of type {A.dtype} is not supported"
+        if op == "addmm":
+            assert given.pop("beta", 1) == 1 and given.pop("alpha", 1) == 1, "addmm with beta and alpha of 1 is supported"
+        for k, v in given.items():
+            assert v is None, f"{k} of {op} is not supported"
+        if op == "_grouped_mm":
             assert A.ndim == 2 and B.ndim == 3 and offs is not None, "Only 2d x 3d with offsets is supported for now"
-            assert kwargs.get("bias", None) is None, "Bias is not supported for now"
+            assert bias is None, "Bias is not supported for now"
             return blockwise_fp8_grouped_linear(A, B, offsets_from_ends(offs), trans_weights=False)
-        if name in gemm_ops:
-            if name.startswith("addmm"):
-                assert kwargs.get("beta", 1) == 1 and kwargs.get("alpha", 1) == 1, "addmm with beta and alpha of 1 is supported"
-                bias, A, B = args[0], args[1], args[2]
-            else:
-                A, B = args[0], args[1]
-                bias = args[2] if len(args) > 2 else kwargs.get("bias", None)
-            assert not isinstance(A, cls) and isinstance(B, cls), f"the second operand of {name}, and it alone, should be a {cls.__name__}"
-            return blockwise_fp8_linear(A, B if name == "linear" else B.transpose(0, 1), bias)
-        with torch._C.DisableTorchFunctionSubclass():
-            return func(*args, **kwargs)
+        return blockwise_fp8_linear(A, B if op == "linear" else B.transpose(0, 1), bias)
 
 
 _WRAPPERS = {"mxfp4": MXFP4TrainingWeightWrapperTensor, "blockwise_fp8": BlockwiseFP8TrainingWeightWrapperTensor}
