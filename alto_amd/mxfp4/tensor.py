@@ -199,6 +199,8 @@ def swap_params(module: nn.Module, *, module_filter_fn: Optional[Callable[[nn.Mo
     """
     if config is None:
         raise ValueError("training op config is required")
+    if config.precision not in _WRAPPERS:
+        raise ValueError(f"Unsupported training op config: {config}")
     tensor_cls = _WRAPPERS[config.precision]
 
     if isinstance(module, nn.Parameter):
