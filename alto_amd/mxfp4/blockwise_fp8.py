@@ -234,8 +234,9 @@ def _convert_from(codes, scales, axis, is_2d, output_dtype):
     if C > 1 and q.stride(2) != 1:
         q = q.contiguous()
     out = torch.empty((B, R, C), dtype=output_dtype, device=codes.device)
-    if out.numel():
-        a = _Dequantize(codes=q.data_ptr(), scales=s.data_ptr(), out=out.data_ptr(), B=B, R=R, C=C, codes_sb=_stride(q, 0), ld=_stride(q, 1), s_sb=_stride(s, 0), s_r=_stride(s, 1),
+    for b in range(0, B if out.numel() else 0, 65535):   # (as many matrices as a launch takes)
+        qb, sb, ob = (t[b:b + 65535] for t in (q, s, out))
+        a = _Dequantize(codes=qb.data_ptr(), scales=sb.data_ptr(), out=ob.data_ptr(), B=qb.shape[0], R=R, C=C, codes_sb=_stride(q, 0), ld=_stride(q, 1), s_sb=_stride(s, 0), s_r=_stride(s, 1),
                         s_c=_stride(s, 2), out_sb=out.stride(0), ldo=out.stride(1), code=code, is_2d=int(bool(is_2d)), out_dtype=out_code)
         _call("alto_mxfp4_fp8_dequantize", a, codes.device)
     out = out if last else out.transpose(1, 2)
