@@ -129,7 +129,8 @@ static int fp8_gemm(const alto_mxfp4_fp8_gemm_t& p, hipStream_t st) {
   // 256 x 256 or 128 x 128, by what either was measured to take (us).  A round of at most 256 of the first: 7.5 and 1.2 to 1.45 for each 128 of K, and the quarters of a last
   // one.  The second, 512 at a time: 7 and 0.95 for each 128 of K, then 3, and 2.5 and 1.11 for each 128 of K and round, the last one no less than 0.55 of one.  Within 12 %
   // over these (first, second): 1500 x 4096 x 4096 46.5, 33.0; 2304 x 4096 x 2048 27.7, 33.5; 3000 x 4096 x 2048 29.4, 34.6; 2048 x 4096 x 4096 46.1, 36.5; 5000 x 5000 x
-  // 1024 40.0, 45.0; 8192 x 8192 x 256 42.5, 40.9; 2048 x 14336 x 4096 113, 137.
+  // 1024 40.0, 45.0; 8192 x 8192 x 256 42.5, 40.9; 2048 x 14336 x 4096 113, 137.  (All with scales of B for 128 x 128.  With one for each of its rows stages take longer on either side, 1.75
+  // to 1.97 of the first: the same rule serves, its pairs are not measured.)
   const double kb = (double)((p.K + 127) / 128), share = large < 256 ? (double)large / 256 : 1.0;
   const int per_xcd = (int)((large + 7) / 8 < 1 << 20 ? (large + 7) / 8 : 1 << 20), whole = whole_tiles(per_xcd);
   const double of_large = (double)((whole + 31) / 32) * (7.5 + kb * (1.2 + 0.25 * share)) + (per_xcd == whole ? 0.0 : 4.0 + 0.575 * kb);
@@ -138,7 +139,7 @@ static int fp8_gemm(const alto_mxfp4_fp8_gemm_t& p, hipStream_t st) {
   // (more of the second than one launch takes are no choice)
   if (of_large <= of_small || !fits<Small>(p.M, p.N)) return p.a_code == ALTO_FP8_E4M3 ? launch_types<Large, ALTO_FP8_E4M3>(a, b1d, f32, st) : launch_types<Large, ALTO_FP8_E5M2>(a, b1d, f32, st);
   if (small <= 256) {
-    // Few tiles: 128 x 128 with K in halves, 64 x 64 with K in quarters, or the kernel for few rows, by what each was measured to take (us; within 20 % over 1 to 768 rows, N
+    // Few tiles (of more, as a row by more than 32768 columns makes, none of these was measured): 128 x 128 with K in halves, 64 x 64 with K in quarters, or the kernel for few rows, by what each was measured to take (us; within 20 % over 1 to 768 rows, N
     // and K from 512 to 14336).  The first: 4, and 0.9 to 1.15 for each 256 of K.  The second: 3.2 and 1.06 for each 512 of K and 256 tiles, and no less than 3 and the operands at
     // 4.2 TB/s.  The third: 2.5 and, 256 workgroups at a time, their reads at 31 GB/s x 1000 each, no less than the operands at 6.3 TB/s.  (First, second, third: 32 x 4096 x 4096 17.1,
     // 10.7, 8.2; 32 x 14336 x 4096 22.4, 17.3, 19.9; 64 x 14336 x 4096 22.8, 17.9, 22.6; 128 x 4096 x 4096 17.7, 11.2, 14.7; 256 x 4096 x 4096 22.0, 11.5, -; 128 x 14336 x 4096 23.3, 28.5, -; 256 x 1024 x 14336

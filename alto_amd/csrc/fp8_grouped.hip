@@ -160,7 +160,8 @@ static int fp8_grouped_gemm(const alto_mxfp4_fp8_grouped_gemm_t& p, hipStream_t 
   // Few rows a group: 16 rows at a time, K split over the waves, the longer K is the more rows (16 rows, 128 x 128, us: 32 experts of 5760 x 2880, 64 rows 98.8, 102.4, 96 rows
   // 111, 106; of 2880 x 5760, 128 rows 108.6, 120.4, 256 rows 125, 120.5; 64 of 512 x 2048, 64 rows 11.5, 18.2; 8 of 4096 x 1024, 8 rows 9.9, 9.1).
   if (p.M * 1024 < (int64_t)p.groups * (p.K < 8192 ? p.K : 8192) && product_below(1ll << 23, used_pieces(a, 16), (p.N + 31) / 32)) return p.a_code == ALTO_FP8_E4M3 ? launch_rows_types<1, 2, ALTO_FP8_E4M3>(a, b1d, f32, st) : launch_rows_types<1, 2, ALTO_FP8_E5M2>(a, b1d, f32, st);
-  // (256 x 256, 128 x 128, us: 32 experts of 5760 x 2880, 4096 rows 183, 163, 8192 rows 232, 232, 16384 rows 341, 396; 8 of 4096 x 1024, 1024 rows 18.0, 13.5, 2048 rows 18.7, 22.0;
+  // (256 x 256, 128 x 128, us: 32 experts of 5760 x 2880, 4096 rows 183, 163, 8192 rows 232, 232, 16384 rows 341, 396; 8 of 4096 x 1024, 1024 rows 18.0, 13.5, 2048 rows 18.7, 22.0; fewer than 8
+  // groups are not measured, and tiles whose waves share K, which one weight's products of few tiles have, are not built by group;
   // more of either than one launch takes are no choice)
   const bool large = p.M >= 256ll * p.groups && p.N > 128 ? fits<Large>(a) || !fits<Small>(a) : !fits<Small>(a);
   if (large) return p.a_code == ALTO_FP8_E4M3 ? launch_types<Large, ALTO_FP8_E4M3>(a, b1d, f32, st) : launch_types<Large, ALTO_FP8_E5M2>(a, b1d, f32, st);

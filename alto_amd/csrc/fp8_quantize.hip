@@ -7,7 +7,8 @@
 // code = RNE(x L / amax) is meant exactly.  With L = 0.875 2^k:  t = 0.875 x  and  a = amax 2^-k  (no overflow, and for bf16 data both are exact), r = RN(1 / a),
 //   q = t r,   e = q a - t,   q - e r
 // is t / a rounded correctly (Markstein), so a quotient of bf16 numbers that lies halfway between two codes is that midpoint in fp32 too and
-// goes to the even code; q alone is a rounding off, and one code in 300 of Gaussian bf16 data was the other neighbour.
+// goes to the even code; q alone is a rounding off, and one code in 300 of Gaussian bf16 data was the other neighbour.  Of fp32 data t and the quotient are rounded to fp32
+// ahead of the code: one within 2^-22 of a midpoint may take the other neighbour.
 //
 // What bounds it is HBM: 4096 x 14336 of a weight, both copies, 49.6 us in a stream of such calls (4.7 TB/s; 38 us, 6.2 TB/s, where x is still cached), 32 experts of 5760 x 2880 411 us
 // (5.2 TB/s, what a large copy reaches); 8192 x 4096 of activations, both copies, 28.8.  Below 2000 tiles all loads, then all stores, are under way at once and

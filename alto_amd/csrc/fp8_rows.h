@@ -102,7 +102,8 @@ __device__ __forceinline__ void fp8_rows_product(const Fp8RowsOperand& A, const 
         for (int i = 0; i < 4; ++i) acc[t][u][i] = __builtin_fmaf(part[i], x.sa[t] * x.sb[B1D ? 4 * u + i : 0], acc[t][u][i]);
       }
   };
-  constexpr int AHEAD = MT * NT >= (B1D ? 4 : 8) ? 2 : 4;   // blocks under way, as registers allow (64 x 4096 x 4096 with a scale for each row of both: 15.3 us with 4, which spilled, 10.9 with 2)
+  constexpr int AHEAD = MT * NT >= (B1D ? 4 : 8) ? 2 : 4;   // blocks under way, as registers allow (64 x 4096 x 4096 with a scale for each row of both: 15.3 us with 4, which spilled, 10.9 with 2, where this
+  // form of MT = 4 still keeps 11 registers in 48 bytes of scratch, eight of them read back each time round; no other form does)
   Block x[AHEAD];
   int k = wave;
 #pragma unroll

@@ -20,7 +20,8 @@
 //
 // Measured: 8192 x 14336 x 4096, 128 x 128 scales of B, 400 us warm (2400 TFLOP/s; a library's product of the same codes with one scale for all 393): matrix pipes busy 59 % at the
 // 1.8 GHz that its power leaves of 2.4.  A stage takes 1.45 us there (1.2 with half of the chip idle), a tile 7.5 more for its first loads, its stores and its launch.
-// 4096 x 14336 x 8192 with a scale for each row of both 475 (2026): the vector instructions bound it, 80 % of their issue slots are taken, a stage is 1.75 to 1.97 us.
+// 4096 x 14336 x 8192 with a scale for each row of both 475 (2026): neither side alone bounds it, vector instructions take 56 % of their issue slots
+// (0.139 a SIMD and clock, 4 clocks each), the matrix pipes are busy 46 %, and the two waves of a SIMD cover only a part of each other's; a stage is 1.75 to 1.97 us.
 // What did not help: see-through changes of this loop's order (one or three MFMAs of lag, more of A ahead, priorities) within 1 %; two barriers a stage, half stages,
 // waves half a stage apart; prefetches into the L2; 256 x 128; results stored from registers in pieces of 64 bytes; one workgroup a unit taking tile after tile with
 // the next one's loads ahead of the stores: 1.3 % of this product, 2.7 % by expert, but 12 % lost on weight gradients of uneven groups, dealt out in advance.

@@ -7,8 +7,9 @@ For the layers of a model that do not stand 4 bits, next to the MXFP4 path and i
 
     scale = amax / L,   code = x L / amax to the nearest code, ties to even;
 
-a block with NaN or an infinity in it stands for NaN.  Activations and gradients have blocks of 1 x 128 along a product's reduction, weights blocks of
-128 x 128, whose codes serve the forward product and, stored transposed, the input gradient's.
+a block with NaN or an infinity in it stands for NaN.  (Of bf16 data that is exact; of fp32 data a quotient within 2^-22 of halfway between two codes may go to
+either.)  Activations and gradients have blocks of 1 x 128 along a product's reduction, weights blocks of 128 x 128, whose codes serve the forward product and,
+stored transposed, the input gradient's.
 
 The reference has such a path beside its MXFP4 one (``alto/kernels/blockwise_fp8/``).
 """
@@ -465,7 +466,8 @@ def blockwise_fp8_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[t
     """``x @ weight.T (+ bias)`` with 8-bit operands in all three products of a training step; x [..., K], weight [N, K], bf16 or fp32, of any sizes.
 
     x and the gradient are quantized in blocks of 1 x 128 along each product's reduction (the gradient to ``grad_dtype``, E4M3 or E5M2), the weight in blocks
-    of 128 x 128.  The result has x's type (with a bias of another, what torch's sum of them has), each gradient its tensor's.  Without a graph to build only the forward product's operands are made.  Each
+    of 128 x 128.  The result has x's type (with a bias of another, what torch's sum of them has), each gradient its tensor's; of fp32 tensors too
+    the products hold what :func:`blockwise_fp8_gemm` says.  Without a graph to build only the forward product's operands are made.  Each
     product's reduction is at most 2^22 - 16 long: K, N where x requires a gradient, and x's rows where the weight does.
     """
     if torch.compiler.is_compiling():

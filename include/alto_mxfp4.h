@@ -582,7 +582,7 @@ int alto_mxfp4_rotary(const alto_mxfp4_rotary_t* args, void* stream);
 /*
  * 8-bit floating point with one fp32 scale for each block of 128 (blocks 1 x 128 along one dim, or 128 x 128).
  * Codes are OCP E4M3 or E5M2, one byte each; L is the largest: 448 or 57344.  With a block's largest magnitude amax, at least 2^-100 L:
- *   scale = amax / L (fp32),   code = x L / amax to nearest even.
+ *   scale = amax / L (fp32),   code = x L / amax to nearest even (of f32 data the quotient is rounded to fp32 first).
  * A block that holds NaN or an infinity stands for NaN throughout.  Blocks at the ends of M and C are shorter.
  */
 #define ALTO_FP8_E4M3 0
