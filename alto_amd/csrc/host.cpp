@@ -1199,6 +1199,7 @@ bool fp8_readable(const Tensor& t, int64_t row, int64_t k) {
   }
   return K % 16 == 0 || end <= (int64_t)t.storage().nbytes();
 }
+constexpr int64_t fp8_longest = (1 << 22) - 16;   // reduction of a native product; longer ones are taken in parts there
 bool fp8_scales(const Tensor& s, int64_t row) { return s.scalar_type() == at::kFloat && stride_of(s, row) < (1 << 21); }
 Tensor fp8_result(at::IntArrayRef size, const Tensor& like, at::ScalarType dtype) { return at::empty(size, at::TensorOptions().dtype(dtype).device(like.device())); }
 
@@ -1207,7 +1208,7 @@ Tensor fp8_gemm_call(Failure& f, const Tensor& a, const Tensor& as, const Tensor
   if (a.dim() != 2 || b.dim() != 2 || as.dim() != 2 || bs.dim() != 2 || !is_fp8(a) || b.scalar_type() != at::kFloat8_e4m3fn) return Tensor();
   const int ar = trans_a ? 1 : 0, ak = 1 - ar, br = trans_b ? 0 : 1, bk = 1 - br;
   const int64_t M = a.size(ar), K = a.size(ak), N = b.size(br), KB = div_up(K, 128);
-  if (M == 0 || N == 0 || K == 0 || b.size(bk) != K || as.size(ar) != (a_2d ? div_up(M, 128) : M) || as.size(ak) != KB || bs.size(br) != (b_2d ? div_up(N, 128) : N) || bs.size(bk) != KB)
+  if (M == 0 || N == 0 || K == 0 || K > fp8_longest || b.size(bk) != K || as.size(ar) != (a_2d ? div_up(M, 128) : M) || as.size(ak) != KB || bs.size(br) != (b_2d ? div_up(N, 128) : N) || bs.size(bk) != KB)
     return Tensor();
   if (!fp8_readable(a, ar, ak) || !fp8_readable(b, br, bk) || !fp8_scales(as, ar) || !fp8_scales(bs, br)) return Tensor();
   const Tensor c = fp8_result({M, N}, a, dtype);
@@ -1224,7 +1225,7 @@ Tensor fp8_grouped_call(Failure& f, const Tensor& a, const Tensor& as, const Ten
   if (a.dim() != 2 || w.dim() != 3 || as.dim() != 2 || ws.dim() != 3 || !is_fp8(a) || w.scalar_type() != at::kFloat8_e4m3fn) return Tensor();
   const int wr = trans_weights ? 1 : 2, wk = 3 - wr;
   const int64_t M = a.size(0), K = a.size(1), E = w.size(0), N = w.size(wr), KB = div_up(K, 128);
-  if (M == 0 || N == 0 || K == 0 || w.size(wk) != K || offs.size(0) != E + 1 || as.size(0) != M || as.size(1) != KB || ws.size(0) != E || ws.size(wr) != (w_2d ? div_up(N, 128) : N) || ws.size(wk) != KB)
+  if (M == 0 || N == 0 || K == 0 || K > fp8_longest || w.size(wk) != K || offs.size(0) != E + 1 || as.size(0) != M || as.size(1) != KB || ws.size(0) != E || ws.size(wr) != (w_2d ? div_up(N, 128) : N) || ws.size(wk) != KB)
     return Tensor();
   if (!fp8_readable(a, 0, 1) || !fp8_readable(w, wr, wk) || !fp8_scales(as, 0) || !fp8_scales(ws, wr)) return Tensor();
   const Tensor c = fp8_result({M, N}, a, dtype);
@@ -1241,7 +1242,7 @@ Tensor fp8_grouped_call(Failure& f, const Tensor& a, const Tensor& as, const Ten
 Tensor fp8_grouped_weights_call(Failure& f, const Tensor& go, const Tensor& gs, const Tensor& x, const Tensor& xs, const Tensor& offs, at::ScalarType dtype) {
   if (go.dim() != 2 || x.dim() != 2 || gs.dim() != 2 || xs.dim() != 2 || !is_fp8(go) || x.scalar_type() != at::kFloat8_e4m3fn) return Tensor();
   const int64_t P = go.size(0), N = go.size(1), K = x.size(1), E = offs.size(0) - 1;
-  if (P == 0 || N == 0 || K == 0 || P % 128 != 0 || x.size(0) != P || gs.size(0) != P / 128 || gs.size(1) != N || xs.size(0) != P / 128 || xs.size(1) != K) return Tensor();
+  if (P == 0 || N == 0 || K == 0 || P > fp8_longest || P % 128 != 0 || x.size(0) != P || gs.size(0) != P / 128 || gs.size(1) != N || xs.size(0) != P / 128 || xs.size(1) != K) return Tensor();
   if (!fp8_readable(go, 1, 0) || !fp8_readable(x, 1, 0) || gs.scalar_type() != at::kFloat || xs.scalar_type() != at::kFloat || (N != 1 && gs.stride(1) != 1) || (K != 1 && xs.stride(1) != 1)) return Tensor();
   const Tensor dw = fp8_result({E, N, K}, go, dtype);
   alto_mxfp4_fp8_grouped_gemm_weights_t p{};

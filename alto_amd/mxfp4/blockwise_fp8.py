@@ -27,7 +27,8 @@ from .linear import cached_weight_quantisation, unwrap_weight_wrapper, weight_ca
 
 FP8_BLOCK_SIZE = 128
 
-_LONGEST = 2 ** 22 - 16   # codes of a row, and bytes from row to row, that a product takes
+_LONGEST = 2 ** 22 - 16   # codes of a row, and bytes from row to row, that a native product takes
+_PART = 2 ** 22 - 128     # whole blocks of them: longer reductions are taken in parts of this length
 
 _CODES = {torch.float8_e4m3fn: 0, torch.float8_e5m2: 1}
 
@@ -266,6 +267,15 @@ def _scales(s: torch.Tensor) -> torch.Tensor:
     return s if all(0 <= _stride(s, d) for d in range(s.dim())) and _stride(s, -2) < 2 ** 21 else s.transpose(-1, -2).contiguous().transpose(-1, -2)
 
 
+def _in_parts(K: int, product, dtype: torch.dtype) -> torch.Tensor:
+    """A reduction longer than a native product's: ``product(lo, hi)`` over each part in fp32, summed in fp32 in their order and rounded once."""
+    total = None
+    for lo in range(0, K, _PART):
+        part = product(lo, min(lo + _PART, K))
+        total = part if total is None else total.add_(part)
+    return total.to(dtype)
+
+
 def _check_scales(name: str, s: torch.Tensor, expected) -> None:
     assert s.dtype == torch.float32, f"{name}: scales of type {s.dtype}, float32 is taken"
     assert tuple(s.shape) == tuple(expected), f"{name} has shape {tuple(s.shape)}, but {tuple(expected)} is expected."
@@ -278,7 +288,8 @@ def blockwise_fp8_gemm(a: torch.Tensor, a_s: torch.Tensor, b: torch.Tensor, b_s:
     ``a`` [M, K] ([K, M] with ``trans_a``) of ``float8_e4m3fn`` or ``float8_e5m2``, ``b`` [K, N] ([N, K] with ``trans_b``) of ``float8_e4m3fn``; ``a_s``, ``b_s`` in the same
     orientation: one scale for each row (column) and 128 of K, or with ``use_2dblock_*`` for each 128 x 128.  Any sizes and strides: operands
     with unit stride along K and rows at multiples of 16 bytes (what the quantizers return) are read as they are, others are copied first, and so is
-    what lies 2^22 bytes or more from row to row (the quantizers' copies of more than 2^22 - 128).  K is at most 2^22 - 16.
+    what lies 2^22 bytes or more from row to row (the quantizers' copies of more than 2^22 - 128).  K above 2^22 - 16 is taken in parts, whose sums are added
+    in fp32.
 
     The matrix pipe adds the products of 8 neighbouring k aligned to the largest of them and cut at 2^-13 of it, whatever instruction or library asks: of Gaussian
     data an fp32 result is off by 3e-5 of the results' norm, a hundredth of a bf16 rounding.  The product of two scales is taken in fp32, whose normal range has to hold it.
@@ -304,6 +315,9 @@ def _gemm(a, a_s, b, b_s, a_2d, b_2d, trans_a, trans_b, output_dtype):
     assert b.dtype == torch.float8_e4m3fn, f"B of type {b.dtype}: torch.float8_e4m3fn"
     _check_scales("A scale", asv, (_blocks(M) if a_2d else M, _blocks(K)))
     _check_scales("B scale", bsv, (_blocks(N) if b_2d else N, _blocks(K)))
+    if K > _LONGEST:
+        blocks = lambda s, lo, hi: s[:, lo // FP8_BLOCK_SIZE:_blocks(hi)]  # noqa: E731
+        return _in_parts(K, lambda lo, hi: _gemm(av[:, lo:hi], blocks(asv, lo, hi), bv[:, lo:hi], blocks(bsv, lo, hi), a_2d, b_2d, False, True, torch.float32), output_dtype)
     c = torch.empty((M, N), dtype=output_dtype, device=a.device)
     if K == 0:
         return c.zero_()
@@ -346,6 +360,9 @@ def _grouped(a, a_s, w, w_s, offsets, w_2d, trans_weights, output_dtype):
     assert w.dtype == torch.float8_e4m3fn, f"w of type {w.dtype}: torch.float8_e4m3fn"
     _check_scales("a scale", a_s, (M, _blocks(K)))
     _check_scales("w scale", wsv, (E, _blocks(N) if w_2d else N, _blocks(K)))
+    if K > _LONGEST:
+        blocks = lambda s, lo, hi: s[..., lo // FP8_BLOCK_SIZE:_blocks(hi)]  # noqa: E731
+        return _in_parts(K, lambda lo, hi: _grouped(a[:, lo:hi], blocks(a_s, lo, hi), wv[..., lo:hi], blocks(wsv, lo, hi), offsets, w_2d, True, torch.float32), output_dtype)
     out = torch.empty((M, N), dtype=output_dtype, device=a.device)
     if K == 0:
         return out.zero_()
@@ -363,7 +380,7 @@ def blockwise_fp8_grouped_gemm_weights(grad_output: torch.Tensor, go_s: torch.Te
     """Weight gradients by group, [E, N, K]: dW[e] = dY_e^T X_e over the rows of each group e (zeros for a group without rows).
 
     ``grad_output`` [P, N] and ``inputs`` [P, K] with scales [P/128, N] and [P/128, K] are the second pairs that :func:`quantize_blockwise_fp8_rowcol` returns with the
-    same ``offsets``; the gradient may be ``float8_e5m2``.  P is below 2^22.
+    same ``offsets``; the gradient may be ``float8_e5m2``.  P of 2^22 and more is taken in parts, whose sums are added in fp32.
     """
     if torch.compiler.is_compiling():
         return _between_graphs(_grouped_weights, grad_output, go_s, inputs, x_s, offsets, output_dtype)
@@ -385,6 +402,12 @@ def _grouped_weights(go, go_s, x, x_s, offsets, output_dtype):
     assert x.dtype == torch.float8_e4m3fn, f"inputs of type {x.dtype}: torch.float8_e4m3fn"
     _check_scales("grad_output scale", go_s, (P // FP8_BLOCK_SIZE, N))
     _check_scales("input scale", x_s, (P // FP8_BLOCK_SIZE, K))
+    if P > _PART:
+        # the groups' tokens lie in whole blocks, one group's behind another's: a part's boundaries are theirs, cut off at its ends
+        ends = torch.cummax(offsets.clamp(min=0).long(), 0).values
+        padded = torch.cat([ends[:1], ends.diff()]).add_(FP8_BLOCK_SIZE - 1).div_(FP8_BLOCK_SIZE, rounding_mode="floor").cumsum(0).mul_(FP8_BLOCK_SIZE)
+        blocks = lambda s, lo, hi: s[lo // FP8_BLOCK_SIZE:hi // FP8_BLOCK_SIZE]  # noqa: E731
+        return _in_parts(P, lambda lo, hi: _grouped_weights(go[lo:hi], blocks(go_s, lo, hi), x[lo:hi], blocks(x_s, lo, hi), (padded - lo).clamp_(0, hi - lo).int(), torch.float32), output_dtype)
     dw = torch.empty((E, N, K), dtype=output_dtype, device=go.device)
     if P == 0:
         return dw.zero_()
@@ -419,14 +442,6 @@ def _quantized_weight(owner: torch.Tensor, w: torch.Tensor, want_transposed: boo
     return cached_weight_quantisation(owner, ("blockwise_fp8", tuple(w.shape), tuple(w.stride())), make)
 
 
-def _check_reductions(want_dx: bool, want_dw: bool, N: int, M: int, groups: int = 0) -> None:
-    """What only a backward's products would refuse, ahead of the forward: their reductions run over the columns of y and over its rows (each group's in whole blocks)."""
-    assert not want_dx or N <= _LONGEST, f"{N} columns: an input's gradient sums over {_LONGEST} at most"
-    if want_dw and groups:
-        assert M + 127 * (groups + 2) < 2 ** 22, f"{M} rows in {groups} groups: weight gradients by group take 2^22 - 1 - 127 (groups + 2) at most"
-    assert not want_dw or M <= _LONGEST, f"{M} rows: a weight's gradient sums over {_LONGEST} at most"
-
-
 class BlockwiseFP8LinearFunction(torch.autograd.Function):
     """y = x W^T, dX = dY W and dW = dY^T X, each on operands quantized along its reduction; x [M, K], W [N, K]."""
 
@@ -434,7 +449,6 @@ class BlockwiseFP8LinearFunction(torch.autograd.Function):
     def forward(ctx, x, weight, grad_dtype, training):
         w = unwrap_weight_wrapper(weight)
         want_dx, want_dw = (training and n for n in ctx.needs_input_grad[:2])   # (those say what requires gradients under no_grad as well)
-        _check_reductions(want_dx and x.numel() > 0, want_dw and w.numel() > 0, w.shape[0], x.shape[0])
         xq, xs, xt, xts = _copies(x, True, want_dw, False, torch.float8_e4m3fn)
         wq, ws, wt = _quantized_weight(weight, w, want_dx)
         ctx.save_for_backward(xt, xts, wt if want_dx else None, ws if want_dx else None)
@@ -467,8 +481,7 @@ def blockwise_fp8_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[t
 
     x and the gradient are quantized in blocks of 1 x 128 along each product's reduction (the gradient to ``grad_dtype``, E4M3 or E5M2), the weight in blocks
     of 128 x 128.  The result has x's type (with a bias of another, what torch's sum of them has), each gradient its tensor's; of fp32 tensors too
-    the products hold what :func:`blockwise_fp8_gemm` says.  Without a graph to build only the forward product's operands are made.  Each
-    product's reduction is at most 2^22 - 16 long: K, N where x requires a gradient, and x's rows where the weight does.
+    the products hold what :func:`blockwise_fp8_gemm` says.  Without a graph to build only the forward product's operands are made.
     """
     if torch.compiler.is_compiling():
         return _between_graphs(_linear, x, weight, bias, grad_dtype)
@@ -491,7 +504,6 @@ class BlockwiseFP8GroupedFunction(torch.autograd.Function):
         w = unwrap_weight_wrapper(weight)
         w = w if trans_weights else w.transpose(1, 2)
         want_dx, want_dw = (training and n for n in ctx.needs_input_grad[:2])
-        _check_reductions(want_dx and x.numel() > 0, want_dw and w.numel() > 0, w.shape[1], x.shape[0], w.shape[0])
         xq, xs, xt, xts = _copies(x, True, want_dw, False, torch.float8_e4m3fn, offsets if want_dw else None)
         wq, ws, wt = _quantized_weight(weight, w, want_dx)
         ctx.save_for_backward(xt, xts, wt if want_dx else None, ws if want_dx else None, offsets)
@@ -521,7 +533,7 @@ def blockwise_fp8_grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets:
     ``offsets[e] <= m < offsets[e + 1]`` meet weight[e].
 
     ``offsets``: int32 [E + 1] on the device, non-decreasing, at most M; groups of any size, E at most 65535.  Rows of no expert, and their gradients, are zero.  The blocks of the weight
-    gradients' operands start anew with each group: where the weight requires a gradient, M + 127 (E + 2) is below 2^22.
+    gradients' operands start anew with each group.
     """
     if torch.compiler.is_compiling():
         return _between_graphs(_grouped_linear, x, weight, offsets, grad_dtype, trans_weights)

@@ -41,47 +41,50 @@ def stand_in(monkeypatch):
     monkeypatch.setattr(torch.cuda, "current_device", lambda: None)
 
 
-def test_steps_of_more_rows_are_refused_ahead_of_the_forward(stand_in):
-    """(they ran their forward and failed in a product of the backward)"""
-    w, wide = torch.zeros(1, 1).bfloat16().requires_grad_(), torch.zeros(LONGEST + 1, 1).bfloat16()
-    rows = lambda n: torch.zeros(1, 1).bfloat16().expand(n, 1)  # noqa: E731
-    assert mx.blockwise_fp8_linear(rows(LONGEST), w).requires_grad
-    with pytest.raises(AssertionError, match="4194289 rows"):
-        mx.blockwise_fp8_linear(rows(LONGEST + 1), w)
-    with torch.no_grad():
-        assert mx.blockwise_fp8_linear(rows(LONGEST + 1), w).shape == (LONGEST + 1, 1)
-    x = rows(3).clone().requires_grad_()   # the input's gradient sums over the columns
-    with pytest.raises(AssertionError, match="4194289 columns"):
-        mx.blockwise_fp8_linear(x, wide)
-    assert mx.blockwise_fp8_linear(x, wide[:LONGEST]).requires_grad
-    assert mx.blockwise_fp8_linear(rows(LONGEST + 1), w.detach().clone()).shape == (LONGEST + 1, 1)   # (no gradient of either is asked for)
+PART = 2 ** 22 - 128
 
 
-@pytest.mark.parametrize("E,most", [(1, 2 ** 22 - 1 - 127 * 3), (30, 2 ** 22 - 1 - 127 * 32)])
-def test_grouped_steps_of_more_rows_are_refused_ahead_of_the_forward(stand_in, E, most):
-    w, offsets = torch.zeros(E, 1, 1).bfloat16().requires_grad_(), torch.zeros(E + 1, dtype=torch.int32)
-    rows = lambda n: torch.zeros(1, 1).bfloat16().expand(n, 1)  # noqa: E731
-    assert mx.blockwise_fp8_grouped_linear(rows(most), w, offsets).requires_grad
-    with pytest.raises(AssertionError, match=f"{most + 1} rows"):
-        mx.blockwise_fp8_grouped_linear(rows(most + 1), w, offsets)
-    assert mx.blockwise_fp8_grouped_linear(rows(most + 1).requires_grad_(), w.detach(), offsets).requires_grad   # (no weight gradient)
-    with torch.no_grad():
-        assert mx.blockwise_fp8_grouped_linear(rows(most + 1), w, offsets).shape == (most + 1, 1)
-    x = rows(3).clone().requires_grad_()
-    with pytest.raises(AssertionError, match="4194289 columns"):
-        mx.blockwise_fp8_grouped_linear(x, torch.zeros(E, 1, 1).bfloat16().expand(E, LONGEST + 1, 1), offsets)
+def test_longer_reductions_are_taken_in_parts(stand_in, monkeypatch):
+    """Each part ends with a whole block, the last one with the reduction; what a native product would be handed is recorded."""
+    made, whole = [], F._gemm
+
+    def gemm(a, a_s, b, b_s, a_2d, b_2d, trans_a, trans_b, out):
+        if (a.shape[0] if trans_a else a.shape[1]) > LONGEST:
+            return whole(a, a_s, b, b_s, a_2d, b_2d, trans_a, trans_b, out)
+        made.append((a.shape, a_s.shape, b.shape, b_s.shape, float(a_s[0, 0]), out))
+        return torch.full((a.shape[0], b.shape[0]), 2.0 ** (8 * len(made)), dtype=out)
+    monkeypatch.setattr(F, "_gemm", gemm)
+    K = 2 * PART + 300
+    a, b, KB = torch.zeros(1, K, dtype=torch.uint8).view(torch.float8_e4m3fn), torch.zeros(K, 2, dtype=torch.uint8).view(torch.float8_e4m3fn), -(-K // 128)
+    scales = torch.arange(float(KB))
+    got = mx.blockwise_fp8_gemm(a, scales.view(1, KB), b, scales.view(KB, 1), use_2dblock_b=True)
+    n = PART // 128
+    assert made == [((1, w), (1, s), (2, w), (1, s), at, torch.float32) for w, s, at in ((PART, n, 0), (PART, n, n), (300, 3, 2 * n))]
+    assert got.dtype == torch.bfloat16 and bool((got == torch.tensor(2.0 ** 8 + 2.0 ** 16 + 2.0 ** 24).bfloat16()).all())
 
 
-def test_many_groups_have_no_weight_gradients(stand_in):
-    w, offsets, x = torch.zeros(1, 1, 1).bfloat16().expand(33024, 1, 1).requires_grad_(), torch.zeros(33025, dtype=torch.int32), torch.zeros(2, 1).bfloat16()
-    with pytest.raises(AssertionError, match="33024 groups"):
-        mx.blockwise_fp8_grouped_linear(x, w, offsets)
-    with torch.no_grad():
-        assert mx.blockwise_fp8_grouped_linear(x, w, offsets).shape == (2, 1)
+@pytest.mark.parametrize("offsets", [[0, 5, 5, 700], [3, 2, 1000, 900], [-7, 0, 128, 256], [0, 2 ** 31 - 1, 5, 6], [0, PART, PART, PART + 129], [0, 100, PART, 2 * PART + 1], [PART + 1, 2 * PART, 2 * PART, 2 * PART + 50]])
+def test_boundaries_of_the_parts_of_weight_gradients(stand_in, monkeypatch, offsets):
+    """Every block of tokens of every group is in one part and in that group there, and no other is."""
+    made, whole = [], F._grouped_weights
 
-
-def test_empty_gradients_of_long_reductions(stand_in):
-    x, w = torch.zeros(LONGEST + 1, 0).bfloat16(), torch.zeros(2, 0).bfloat16().requires_grad_()
-    assert torch.autograd.grad(mx.blockwise_fp8_linear(x, w).sum(), w)[0].shape == (2, 0)
-    x, w = torch.zeros(0, 1).bfloat16().requires_grad_(), torch.zeros(1, 1).bfloat16().expand(LONGEST + 1, 1)
-    assert torch.autograd.grad(mx.blockwise_fp8_linear(x, w).sum(), x)[0].shape == (0, 1)
+    def weights(go, go_s, x, x_s, offs, out):
+        if go.shape[0] > PART:
+            return whole(go, go_s, x, x_s, offs, out)
+        assert go.shape[0] == x.shape[0] == 128 * go_s.shape[0] == 128 * x_s.shape[0] and offs.dtype == torch.int32
+        made.append((int(go_s[0, 0]), go.shape[0] // 128, offs.tolist()))
+        return torch.ones(3, 1, 1, dtype=out)
+    monkeypatch.setattr(F, "_grouped_weights", weights)
+    P = 2 * PART + 128 * 9
+    codes, scales = torch.zeros(1, P, dtype=torch.uint8).t().view(torch.float8_e4m3fn), torch.arange(float(P // 128)).view(-1, 1)
+    got = mx.blockwise_fp8_grouped_gemm_weights(codes, scales, codes, scales, torch.tensor(offsets, dtype=torch.int32))
+    assert got.shape == (3, 1, 1) and bool((got == 3).all()) and [m[:2] for m in made] == [(0, PART // 128), (PART // 128, PART // 128), (2 * PART // 128, 9)]
+    last, at, want = 0, 0, []
+    for o in offsets:   # the segments in whole blocks, as the quantizer lays them out
+        size = max(last, o) - last
+        last += size
+        at += -(-size // 128)
+        want.append(min(at, P // 128))
+    for first, n, offs in made:
+        assert all(o % 128 == 0 for o in offs)
+        assert [o // 128 for o in offs] == [min(max(w - first, 0), n) for w in want]
