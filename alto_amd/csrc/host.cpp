@@ -1199,7 +1199,7 @@ bool fp8_readable(const Tensor& t, int64_t row, int64_t k) {
   }
   return K % 16 == 0 || end <= (int64_t)t.storage().nbytes();
 }
-constexpr int64_t fp8_longest = (1 << 22) - 16;   // reduction of a native product; longer ones are taken in parts there
+constexpr int64_t fp8_longest = (1 << 22) - 16;   // reduction of a native product; blockwise_fp8.py takes longer ones in parts
 bool fp8_scales(const Tensor& s, int64_t row) { return s.scalar_type() == at::kFloat && stride_of(s, row) < (1 << 21); }
 Tensor fp8_result(at::IntArrayRef size, const Tensor& like, at::ScalarType dtype) { return at::empty(size, at::TensorOptions().dtype(dtype).device(like.device())); }
 
